@@ -363,6 +363,127 @@ exl3_status exl3_hip_iface_matmul(unsigned bits, unsigned codebook, size_t k, si
                                   const uint16_t *packed, const uint16_t *suh, const uint16_t *svh, const float *x,
                                   float *y, void *workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* ---- the attention block between the q/k/v layers and the o layer --------
+ * The reference leaves these operators to llama.cpp's graph; none of the entry
+ * points below has a counterpart in it.  Together they take the rows that the q, k
+ * and v layers wrote to the rows that the o layer reads:
+ *   exl3_hip_qk_norm_rope      norms and positions of the queries and keys
+ *   exl3_hip_attention_prompt  attention of packed prompts over their own keys
+ *   exl3_hip_kv_cache_write    new keys and values into the quantised cache
+ *   exl3_hip_attention_cached  attention of the next token(s) over that cache
+ *   exl3_hip_kv_cache_read     cached rows back as F16/F32 (a prompt that continues them)
+ * Heads are grouped: with g = q heads / kv heads (a whole number), q head h reads kv
+ * head h / g. */
+
+/* Rows of heads: element i of head h of token t is at data[t * token_stride + h *
+ * head_stride + i] (strides in elements, the head's elements dense), so a slice of a
+ * fused q/k/v buffer is a view.  Outputs: no two heads overlap. */
+typedef struct exl3_head_view {
+    void *data;          /* device */
+    size_t heads;
+    size_t token_stride;
+    size_t head_stride;
+} exl3_head_view;
+
+/* RMS norm of each head and rotation by position, of queries and keys in one launch:
+ *   z = x / sqrt(mean(x^2) + eps) * weight              (weight NULL: z = x)
+ *   (a, b) -> rope_scale (a cos t - b sin t, b cos t + a sin t),  t = positions[token] inv_freq[p]
+ * for the pairs p < rot_dim / 2 of z's first rot_dim elements, (z[p], z[p + rot_dim /
+ * 2]) or with `interleaved` (z[2p], z[2p + 1]); the other elements stay z.  The scaling
+ * of long contexts is the caller's inv_freq and rope_scale.  Computed in fp32 and
+ * rounded once; t is reduced to a turn with two fp32 words per frequency, so sin and cos
+ * hold to about 1e-6 at any position (|position| < 2^24).
+ *   q, k       xt rows; k and k_out may both be NULL; q_out / k_out have their heads and
+ *              are the same view as q / k (xt = yt: in place) or disjoint from both
+ *   head_dim   multiple of 8 up to 256
+ *   q_weight, k_weight   device fp32[head_dim] or NULL
+ *   positions  device int32[tokens]; inv_freq device fp32[rot_dim / 2]; either may be
+ *              NULL when rot_dim is 0
+ *   rot_dim    multiple of 16 up to head_dim, or 0
+ * tokens = 0 is a no-op. */
+exl3_status exl3_hip_qk_norm_rope(const exl3_head_view *q, const exl3_head_view *k, exl3_dtype xt, size_t tokens,
+                                  size_t head_dim, const float *q_weight, const float *k_weight, float eps,
+                                  const int32_t *positions, const float *inv_freq, size_t rot_dim, int interleaved,
+                                  float rope_scale, const exl3_head_view *q_out, const exl3_head_view *k_out,
+                                  exl3_dtype yt, hipStream_t stream);
+
+/* The cache: page_count pages of page_tokens (P) tokens, each with every kv head's keys
+ * and values at `bits` = 4 or 8.  Token slot s = page * P + offset.  32 consecutive
+ * elements of a head form a group: the group is rotated by the orthonormal
+ * Walsh-Hadamard matrix H32 (which spreads a large channel over the group), ext is its
+ * element of largest magnitude (the negative one of two equal), scale = fp16(-ext /
+ * 2^(bits-1)) with its magnitude rounded up to 12 - bits significant bits (a zero is +0), and code =
+ * clamp(rint(y / scale), -2^(bits-1), 2^(bits-1) - 1): every scale * code is an fp16
+ * number, so attention reads the cache without a further rounding.  A group with a
+ * non-finite element, or beyond fp16's range, reads back as NaN.
+ * A page is, for each kv head, four runs:
+ *   keys    [P][head_dim * bits / 8]          code + 2^(bits-1); 4 bits: the even element low
+ *   values  [P/4][16][4][head_dim * bits / 128]  blocks of 4 tokens: 16 slices of a row, each
+ *                                               with its 4 tokens next to each other
+ *   key scales    fp16 [P][head_dim / 32]
+ *   value scales  fp16 [P/4][head_dim / 32][4]
+ * Bytes of a page; 0 unless bits is 4 or 8, head_dim 64, 128 or 256, page_tokens a
+ * nonzero multiple of 16 up to 65536 and 1 <= kv_heads <= 1024. */
+size_t exl3_hip_kv_page_bytes(unsigned bits, size_t kv_heads, size_t head_dim, size_t page_tokens);
+
+/* Quantises `tokens` rows of keys and values (k->heads = v->heads = kv heads) into
+ * their slots.  slots: device int64[tokens], no slot twice; a negative one is skipped (a
+ * padded place of a batch), one beyond the cache is skipped and sets *bad_slots
+ * (optional device int) to 1.  pages: 16-byte aligned, page_count *
+ * exl3_hip_kv_page_bytes() bytes, its unwritten slots of any contents. */
+exl3_status exl3_hip_kv_cache_write(void *pages, size_t page_count, unsigned bits, size_t page_tokens, size_t head_dim,
+                                    const exl3_head_view *k, const exl3_head_view *v, exl3_dtype xt, size_t tokens,
+                                    const int64_t *slots, int *bad_slots, hipStream_t stream);
+
+/* The rows of some slots as the cache holds them, rotated back, rounded once to yt.  A
+ * slot outside the cache gives NaN rows and sets *bad_slots (optional). */
+exl3_status exl3_hip_kv_cache_read(const void *pages, size_t page_count, unsigned bits, size_t page_tokens,
+                                   size_t head_dim, const int64_t *slots, size_t tokens, const exl3_head_view *k_out,
+                                   const exl3_head_view *v_out, exl3_dtype yt, int *bad_slots, hipStream_t stream);
+
+/* Attention of the last q_len tokens of each sequence over the cache:
+ *   out[i] = sum_n softmax_n(scale q[i] . K[n]) V[n]
+ * where row s * q_len + j of q (F16) is token j of sequence s's last q_len, and sees the
+ * keys n < kv_lens[s] - (q_len - 1 - j); a row that sees none is zero.  Token n of
+ * sequence s is at offset n % P of page page_table[s * table_stride + n / P].
+ *   page_table  device int32[sequences * table_stride]; an entry outside the cache makes
+ *               the rows of its sequence that read it NaN
+ *   kv_lens     device int32[sequences], the cached tokens of each sequence with the
+ *               q_len new ones (written before the call); beyond table_stride * P it
+ *               counts as that, negative as 0
+ *   out         F16, disjoint from q
+ *   workspace   device, 256-byte aligned, >= exl3_hip_attention_cached_workspace_bytes(),
+ *               zero-filled before first use (exl3_hip_workspace_init); it may be one
+ *               that exl3_hip_mul_mat uses too.  NULL: the internal one of this stream
+ * head_dim 64, 128 or 256; q heads a multiple of kv_heads, up to 64 of them per kv head;
+ * q_len 1..65536.  Scores, softmax statistics and sums in fp32; q as an fp16 pair (high
+ * and low part), weights rounded to fp16.  The same inputs give the same bits on every
+ * call.  sequences = 0 is a no-op. */
+exl3_status exl3_hip_attention_cached(const exl3_head_view *q, const exl3_head_view *out, size_t head_dim,
+                                      const void *pages, size_t page_count, unsigned bits, size_t page_tokens,
+                                      size_t kv_heads, const int32_t *page_table, size_t table_stride,
+                                      const int32_t *kv_lens, size_t sequences, size_t q_len, float scale,
+                                      void *workspace, size_t workspace_bytes, hipStream_t stream);
+/* 0 for arguments that exl3_hip_attention_cached refuses */
+size_t exl3_hip_attention_cached_workspace_bytes(size_t q_heads, size_t kv_heads, size_t head_dim, size_t sequences,
+                                                 size_t q_len);
+
+/* Attention of packed sequences: sequence s has the query rows q_starts[s] ..
+ * q_starts[s + 1] - 1 and the key and value rows kv_starts[s] .. kv_starts[s + 1] - 1
+ * (device int32[sequences + 1] each, ascending from 0).  With `causal` query i of nq
+ * sees the first nk - (nq - 1 - i) of its nk keys (the sequences' ends aligned: keys
+ * ahead of the queries are a prefix), else all; a row that sees none is zero.  q, k, v
+ * and out are F16, out disjoint from the inputs; head_dim 64, 128 or 256; q heads a
+ * multiple of kv heads.  q_tokens and kv_tokens are the rows of the views (no row
+ * outside them is read or written, whatever the starts hold; a query row that no
+ * sequence has is not written).  Scores, softmax statistics and sums in fp32, weights
+ * rounded to fp16.  The same inputs give the same bits on every call.  sequences = 0 or
+ * q_tokens = 0 is a no-op. */
+exl3_status exl3_hip_attention_prompt(const exl3_head_view *q, const exl3_head_view *k, const exl3_head_view *v,
+                                      const exl3_head_view *out, size_t head_dim, const int32_t *q_starts,
+                                      const int32_t *kv_starts, size_t sequences, size_t q_tokens, size_t kv_tokens,
+                                      float scale, int causal, hipStream_t stream);
+
 /* *result (device int) = 1 when every su/sv value of every record is finite,
  * 0 otherwise; EXL3_INVAL_PARAMS when nbytes is not a whole number of records. */
 exl3_status exl3_hip_validate_records(const void *records, size_t nbytes, unsigned bits, int *result,

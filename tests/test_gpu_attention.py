@@ -1,0 +1,355 @@
+"""Attention over the cache and over packed prompts against the formula in 64 bits, element by element within
+attention_ref.attention_bound (derived from the roundings that the entry points state)."""
+import numpy as np
+import pytest
+
+import attention_ref as ref
+import synth
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(seed, *shape, sigma=1.0):
+    return synth.normal(seed, int(np.prod(shape)), sigma).reshape(shape).astype(np.float16)
+
+
+# ------------------------------------------------------------------ prompts
+def prompt_reference(q, k, v, qs, ks, causal, scale):
+    """(want, bound, which rows belong to a sequence)"""
+    want, bound = np.zeros(q.shape), np.zeros(q.shape)
+    used = np.zeros(q.shape[0], bool)
+    per = q.shape[1] // k.shape[1]
+    d = q.shape[2]
+    q, k, v = (a.astype(np.float64) for a in (q, k, v))
+    for s in range(len(qs) - 1):
+        nq, nk = qs[s + 1] - qs[s], ks[s + 1] - ks[s]
+        i = np.arange(nq)
+        ends = nk - (nq - 1 - i) if causal else np.full(nq, nk)
+        used[qs[s]:qs[s + 1]] = True
+        for h in range(q.shape[1]):
+            kk, vv = k[ks[s]:ks[s + 1], h // per], v[ks[s]:ks[s + 1], h // per]
+            o, mass, dots, total = ref.attend(q[qs[s]:qs[s + 1], h], kk, vv, ends, scale)
+            want[qs[s]:qs[s + 1], h] = o
+            top = np.abs(vv).max(initial=0.0)
+            bound[qs[s]:qs[s + 1], h] = ref.attention_bound(o, mass, dots, total, top, nk, d)
+    return want, bound, used
+
+
+def run_prompt(amd, q, k, v, qs, ks, causal, scale=None, **kw):
+    import torch
+    to = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    return amd.attention_prompt(to(q), to(k), to(v), to(np.asarray(qs, np.int32)), to(np.asarray(ks, np.int32)),
+                                causal=causal, scale=scale, **kw).cpu().numpy()
+
+
+def starts(lens):
+    return [0] + [int(x) for x in np.cumsum(lens)]
+
+
+PROMPTS = [  # query lengths, key lengths, hq, hk, d, causal
+    ([1], [1], 1, 1, 64, True),
+    ([1], [1000], 4, 2, 128, True),
+    ([37], [37], 8, 2, 256, True),
+    ([65], [65], 3, 1, 64, False),
+    ([1, 0, 5, 64, 33], [1, 0, 5, 64, 33], 6, 2, 128, True),
+    ([130, 7, 256], [131, 300, 256], 4, 4, 64, True),
+    ([70, 9], [20, 4], 2, 1, 128, True),          # more queries than keys: the first rows see nothing
+    ([12, 40], [0, 3], 2, 2, 64, False),          # a sequence without keys
+    ([129, 64], [257, 1], 5, 1, 256, False),
+    ([300], [300], 2, 1, 256, True),
+    ([513], [700], 2, 2, 128, True),
+]
+
+
+@pytest.mark.parametrize("case", PROMPTS, ids=str)
+def test_prompt_matches_formula(amd, case):
+    lq, lk, hq, hk, d, causal = case
+    print("  attention_prompt", case, flush=True)
+    qs, ks = starts(lq), starts(lk)
+    q, k, v = rows(70, qs[-1], hq, d, sigma=2.0), rows(71, max(1, ks[-1]), hk, d), rows(72, max(1, ks[-1]), hk, d)
+    want, bound, used = prompt_reference(q, k, v, qs, ks, causal, d ** -0.5)
+    got = run_prompt(amd, q, k, v, qs, ks, causal).astype(np.float64)
+    assert np.isfinite(got).all()
+    assert np.all(np.abs(got - want) <= bound), float((np.abs(got - want) / np.maximum(bound, 1e-30)).max())
+
+
+@pytest.mark.parametrize("sigma,scale", [(30.0, None), (0.01, None), (1.0, -0.2), (1.0, 0.0), (8.0, 1.0)])
+def test_prompt_score_ranges(amd, sigma, scale):
+    """scores from almost equal to hundreds apart, a negative scale and a zero one"""
+    lens, d = [200, 61], 128
+    qs = starts(lens)
+    q, k, v = rows(80, qs[-1], 2, d, sigma=sigma), rows(81, qs[-1], 1, d), rows(82, qs[-1], 1, d, sigma=0.5)
+    v += np.float16(2.0)
+    want, bound, _ = prompt_reference(q, k, v, qs, qs, True, d ** -0.5 if scale is None else scale)
+    got = run_prompt(amd, q, k, v, qs, qs, True, scale).astype(np.float64)
+    assert np.all(np.abs(got - want) <= bound)
+
+
+def test_prompt_rising_scores(amd):
+    """the running maximum grows with every key, and falls with every key"""
+    n, d = 333, 64
+    ramp = (np.arange(n) * 0.06).astype(np.float16)
+    for k_of in (ramp, ramp[::-1]):
+        q, k, v = np.ones((n, 1, d), np.float16), np.zeros((n, 1, d), np.float16), rows(84, n, 1, d)
+        k[:, 0, :] = k_of[:, None]
+        want, bound, _ = prompt_reference(q, k, v, [0, n], [0, n], True, 1.0)
+        got = run_prompt(amd, q, k, v, [0, n], [0, n], True, 1.0).astype(np.float64)
+        assert np.all(np.abs(got - want) <= bound)
+
+
+@pytest.mark.parametrize("poison", [np.nan, np.inf, -np.inf, 65504.0])
+def test_prompt_masked_places_do_not_reach_a_row(amd, poison):
+    """keys and values that a row does not see (after its end, of other sequences, of none) hold anything"""
+    import torch
+    lens, d = [50, 20], 128
+    qs = starts(lens)
+    q, k, v = rows(90, 80, 2, d), rows(91, 80, 1, d), rows(92, 80, 1, d)
+    clean = run_prompt(amd, q, k, v, qs, qs, True)
+    for at in (49, 69, 75):  # the last key of each sequence, a row of no sequence
+        kk, vv = k.copy(), v.copy()
+        kk[at], vv[at] = poison, poison
+        got = run_prompt(amd, q, kk, vv, qs, qs, True, out=torch.zeros((80, 2, d), dtype=torch.float16, device="cuda"))
+        keep = np.ones(80, bool)
+        keep[at] = keep[70:] = False
+        assert np.array_equal(got[keep], clean[keep]), at
+
+
+def test_prompt_leaves_other_rows_and_views(amd):
+    """head-major, sliced and unaligned views; rows of no sequence keep what they held"""
+    import torch
+    lens, hq, hk, d = [40, 25], 4, 2, 64
+    qs = starts(lens)
+    n = qs[-1] + 6
+    q, k, v = rows(95, n, hq, d), rows(96, n, hk, d), rows(97, n, hk, d)
+    want = run_prompt(amd, q, k, v, qs, qs, True)[:qs[-1]]
+    width = (hq + 2 * hk) * d + 3
+    buf = torch.zeros(n * width + 1, dtype=torch.float16, device="cuda")
+    view = buf[1:].view(n, width)
+    parts = []
+    at = 0
+    for a, h in ((q, hq), (k, hk), (v, hk)):
+        piece = view[:, at:at + h * d].unflatten(1, (h, d))
+        piece.copy_(torch.from_numpy(a))
+        parts.append(piece)
+        at += h * d
+    st = torch.tensor(qs, dtype=torch.int32, device="cuda")
+    out = torch.full((hq, n, d), 9.0, dtype=torch.float16, device="cuda")
+    amd.attention_prompt(*parts, st, out=out.transpose(0, 1))
+    got = out.transpose(0, 1).cpu().numpy()
+    assert np.array_equal(got[:qs[-1]], want) and np.all(got[qs[-1]:] == 9.0)
+
+
+def test_prompt_starts_beyond_the_rows(amd):
+    """starts that do not fit the views: nothing outside them is read or written"""
+    import torch
+    d = 64
+    q = rows(98, 30, 1, d)
+    for qs, ks in (([0, 30], [0, 4000]), ([0, 4000], [0, 30]), ([-5, 30], [-9, 30]), ([20, 10], [0, 30]),
+                   ([0, 30], [25, 5])):
+        out = run_prompt(amd, q, q, q, qs, ks, True, out=torch.zeros((30, 1, d), dtype=torch.float16, device="cuda"))
+        assert out.shape == (30, 1, d)
+
+
+# ------------------------------------------------------------------ the cache
+def make_cache(amd, lens, heads, d, bits, p, width=None, seed=100, spare=3):
+    """(pages, table, rotated keys and values of each sequence) with random rows in shuffled pages; the rest of the
+    pages is filled with bytes that read as NaN and infinities"""
+    import torch
+    need = [-(-n // p) for n in lens]
+    width = max([1] + need) if width is None else width
+    count = sum(need) + spare
+    size = amd.kv_page_bytes(heads, d, bits, p)
+    pages = np.full((count, size), 0xFF, np.uint8)
+    order = np.argsort(synth.splitmix64(seed, count))
+    table = np.full((len(lens), width), int(order[-1]), np.int32)  # unused places point at a page of NaN
+    kept, at = [], 0
+    for s, n in enumerate(lens):
+        k, v = rows(seed + 2 * s, max(n, 1), heads, d), rows(seed + 2 * s + 1, max(n, 1), heads, d, sigma=0.6)
+        (kc, ks), (vc, vs) = ref.quantise(k, bits), ref.quantise(v, bits)
+        for j in range(need[s]):
+            page = int(order[at + j])
+            table[s, j] = page
+            parts = [a.copy() for a in ref.page_parts(pages[page], bits, heads, d, p)]
+            m = min(p, n - j * p)
+            for part, src in zip(parts, (kc, vc, ks, vs)):
+                part[:, :m] = src[j * p:j * p + m].transpose(1, 0, 2)
+            pages[page] = ref.pack_page(*parts, bits)
+        kept.append((ref.values(kc, ks, bits)[:n], ref.values(vc, vs, bits)[:n]))
+        at += need[s]
+    return torch.from_numpy(pages).cuda(), torch.from_numpy(table).cuda(), kept
+
+
+def cached_reference(q, kept, q_len, heads, scale):
+    want, bound = np.zeros(q.shape), np.zeros(q.shape)
+    per, d = q.shape[1] // heads, q.shape[2]
+    qr = ref.rotate(q.astype(np.float64))
+    for s, (k, v) in enumerate(kept):
+        n = len(k)
+        ends = n - (q_len - 1 - np.arange(q_len))
+        for h in range(q.shape[1]):
+            at = slice(s * q_len, (s + 1) * q_len)
+            kk, vv = k[:, h // per], v[:, h // per]
+            o, mass, dots, total = ref.attend(qr[at, h], kk, vv, ends, scale)
+            # the bound of the rotated row; rotating back sums 32 elements of it with +-1/sqrt(32), in binary32
+            b = ref.attention_bound(o, mass, dots, total, np.abs(vv).max(initial=0.0), n, d)
+            b = b.reshape(q_len, -1, 32)
+            o32 = np.abs(o).reshape(q_len, -1, 32)
+            both = (b.sum(-1, keepdims=True) + 6 * 2.0 ** -24 * o32.sum(-1, keepdims=True)) / np.sqrt(32)
+            want[at, h] = ref.rotate(o)
+            bound[at, h] = np.broadcast_to(both, b.shape).reshape(q_len, d) + ref.U16 * np.abs(want[at, h]) + 2.0 ** -25
+    return want, bound
+
+
+def run_cached(amd, q, pages, table, lens, heads, bits, p, q_len, **kw):
+    import torch
+    return amd.attention_cached(torch.from_numpy(q).cuda(), pages, table,
+                                torch.tensor(lens, dtype=torch.int32, device="cuda"), heads, bits=bits, page_tokens=p,
+                                q_len=q_len, **kw).cpu().numpy()
+
+
+CACHED = [  # lengths, hq, hk, d, bits, page, q_len
+    ([1], 1, 1, 64, 4, 16, 1),
+    ([17], 8, 2, 256, 4, 16, 1),
+    ([1000], 8, 2, 256, 4, 16, 1),
+    ([31, 0, 33, 400], 4, 4, 128, 4, 32, 1),
+    ([500, 64, 3], 12, 4, 64, 8, 64, 4),
+    ([700, 2], 5, 1, 128, 8, 48, 3),           # a sequence shorter than its new tokens: rows that see nothing
+    ([129, 255, 1000, 5, 77], 6, 2, 128, 4, 256, 1),
+    ([333], 40, 1, 64, 4, 16, 7),              # more rows per kv head than one tile
+    ([260, 90], 16, 2, 256, 8, 16, 2),
+    ([2500], 3, 3, 128, 4, 80, 1),
+    ([64] * 20, 2, 1, 64, 4, 16, 1),
+]
+
+
+@pytest.mark.parametrize("case", CACHED, ids=str)
+def test_cached_matches_formula(amd, case):
+    lens, hq, hk, d, bits, p, q_len = case
+    print("  attention_cached", case, flush=True)
+    pages, table, kept = make_cache(amd, lens, hk, d, bits, p)
+    q = rows(120, len(lens) * q_len, hq, d, sigma=2.0)
+    want, bound = cached_reference(q, kept, q_len, hk, d ** -0.5)
+    got = run_cached(amd, q, pages, table, lens, hk, bits, p, q_len).astype(np.float64)
+    assert np.isfinite(got).all()
+    assert np.all(np.abs(got - want) <= bound), float((np.abs(got - want) / np.maximum(bound, 1e-30)).max())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_cached_long(amd, bits):
+    """one long sequence beside short ones; the table is wider than any of them"""
+    lens, hq, hk, d, p = [9001, 3, 700], 4, 2, 128, 64
+    pages, table, kept = make_cache(amd, lens, hk, d, bits, p, width=160)
+    q = rows(130, 3, hq, d, sigma=3.0)
+    want, bound = cached_reference(q, kept, 1, hk, 0.11)
+    got = run_cached(amd, q, pages, table, lens, hk, bits, p, 1, scale=0.11).astype(np.float64)
+    assert np.all(np.abs(got - want) <= bound)
+
+
+def test_cached_workspaces_streams_and_repeats(amd):
+    """the caller's workspace (which mul_mat may share), the internal one, another stream: the same bits"""
+    import torch
+    lens, hq, hk, d, bits, p = [800, 90, 0], 8, 2, 128, 4, 16
+    pages, table, _ = make_cache(amd, lens, hk, d, bits, p)
+    q = rows(140, 3, hq, d)
+    first = run_cached(amd, q, pages, table, lens, hk, bits, p, 1)
+    nbytes = amd.attention_cached_workspace_bytes(hq, hk, d, 3)
+    ws = amd.new_workspace(128, 128, 1, nbytes=nbytes)
+    for _ in range(3):
+        assert np.array_equal(run_cached(amd, q, pages, table, lens, hk, bits, p, 1, workspace=ws), first)
+    assert not amd.workspace_faulted(ws)
+    with pytest.raises(amd.Exl3Error) as e:
+        run_cached(amd, q, pages, table, lens, hk, bits, p, 1, workspace=ws[:nbytes - 1])
+    assert e.value.status == amd.WORKSPACE_TOO_SMALL
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = run_cached(amd, q, pages, table, lens, hk, bits, p, 1)
+    assert np.array_equal(other, first)
+
+
+def test_cached_bad_pages_and_lengths(amd):
+    """an entry outside the cache makes its sequence's rows NaN and no other's; lengths are held to the table"""
+    import torch
+    lens, hq, hk, d, bits, p = [100, 100, 40], 4, 2, 64, 4, 16
+    pages, table, _ = make_cache(amd, lens, hk, d, bits, p)
+    q = rows(150, 3, hq, d)
+    clean = run_cached(amd, q, pages, table, lens, hk, bits, p, 1)
+    for entry in (-1, pages.shape[0], 2 ** 31 - 1, -(2 ** 31)):
+        t = table.clone()
+        t[1, 2] = entry
+        got = run_cached(amd, q, pages, t, lens, hk, bits, p, 1)
+        assert np.isnan(got[1]).all() and np.array_equal(got[[0, 2]], clean[[0, 2]])
+        t = table.clone()
+        t[2, 4:] = entry  # places that nothing reads
+        assert np.array_equal(run_cached(amd, q, pages, t, lens, hk, bits, p, 1), clean)
+    capped = run_cached(amd, q, pages, table, [2 ** 31 - 1, 100, -7], hk, bits, p, 1)
+    full = run_cached(amd, q, pages, table, [table.shape[1] * p, 100, 0], hk, bits, p, 1)
+    assert np.array_equal(capped, full, equal_nan=True) and np.all(capped[2] == 0)
+
+
+def test_cached_views_and_far_pages(amd):
+    """head-major and unaligned rows, and a cache beyond 4 GiB"""
+    import torch
+    lens, hq, hk, d, bits, p = [75], 4, 2, 64, 4, 16
+    pages, table, _ = make_cache(amd, lens, hk, d, bits, p)
+    q = rows(160, 1, hq, d)
+    want = run_cached(amd, q, pages, table, lens, hk, bits, p, 1)
+    far = torch.zeros(((1 << 32) // pages.shape[1] + 40, pages.shape[1]), dtype=torch.uint8, device="cuda")
+    off = far.shape[0] - pages.shape[0]
+    far[off:] = pages
+    buf = torch.zeros(hq * (d + 3) + 1, dtype=torch.float16, device="cuda")
+    qv = buf[1:].view(1, hq, d + 3)[:, :, :d]
+    qv.copy_(torch.from_numpy(q))
+    out = torch.zeros_like(buf)[1:].view(1, hq, d + 3)[:, :, :d]
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    amd.attention_cached(qv, far, table + off, ln, hk, bits=bits, page_tokens=p, out=out)
+    assert np.array_equal(out.cpu().numpy(), want)
+
+
+# ------------------------------------------------------------------ together
+def test_block_in_a_captured_graph(amd):
+    """norm and positions, cache write, attention over cache and prompt in one HIP graph: each replay equals the
+    eager calls, with eager work in between, also after the inputs have changed"""
+    import torch
+    hq, hk, d, bits, p, n = 8, 2, 128, 4, 16, 300
+    g = torch.Generator(device="cuda").manual_seed(5)
+    draw = lambda *s: torch.randn(s, generator=g, device="cuda").half()  # noqa: E731
+    qkv = draw(n, (hq + 2 * hk), d)
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    f = torch.from_numpy((1e4 ** (-np.arange(0, d, 2) / d)).astype(np.float32)).cuda()
+    w = torch.ones(d, device="cuda")
+    pages = amd.new_kv_cache(20, hk, d, bits, p)
+    slots = torch.arange(n, device="cuda")
+    table = torch.arange(19, dtype=torch.int32, device="cuda")[None].contiguous()
+    lens, starts_ = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([n], [0, n]))
+    ws = amd.new_workspace(128, 128, 1, nbytes=amd.attention_cached_workspace_bytes(hq, hk, d, 1))
+
+    def step():
+        q, k = amd.qk_norm_rope(qkv[:, :hq], qkv[:, hq:hq + hk], pos, f, w, w)
+        v = qkv[:, hq + hk:]
+        amd.kv_cache_write(pages, k, v, slots, bits=bits, page_tokens=p)
+        rk, rv = amd.kv_cache_read(pages, slots, hk, d, bits=bits, page_tokens=p)
+        a = amd.attention_prompt(q, rk, rv, starts_)
+        b = amd.attention_cached(q[-1:], pages, table, lens, hk, bits=bits, page_tokens=p, workspace=ws)
+        return a, b
+
+    def eager():
+        out = tuple(t.clone() for t in step())
+        torch.cuda.synchronize()
+        return out
+
+    first = eager()
+    # the last row of the prompt and the cached step see the same keys and values
+    assert (first[0][-1].float() - first[1][0].float()).abs().max() < 0.01
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        a, b = step()
+    for r in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, first[0]) and torch.equal(b, first[1]), r
+        if r == 1:
+            qkv.copy_(draw(n, hq + 2 * hk, d))
+        first = eager()

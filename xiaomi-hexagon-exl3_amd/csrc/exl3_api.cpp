@@ -13,6 +13,7 @@
 #include <utility>
 #include <vector>
 
+#include "exl3_attention.hpp"
 #include "exl3_launch.hpp"
 
 namespace {
@@ -159,6 +160,12 @@ size_t group_need(size_t k, const size_t *n, size_t count, size_t rows, bool fus
 }
 
 }  // namespace
+
+namespace exl3k {
+exl3_status take_workspace(size_t need, hipStream_t stream, void **workspace, size_t *bytes) {
+    return call_workspace(need, stream, workspace, bytes);
+}
+}  // namespace exl3k
 
 extern "C" {
 
