@@ -1,90 +1,577 @@
 // exl3_attention_cached.hip -- attention of each sequence's last tokens over the quantised cache.
-#include "exl3_attention_rows.hpp"
-#include "exl3_launch.hpp"
+//
+// One pass over the cached tokens: 16 query rows (the q heads of one kv head times the new
+// tokens) meet every key, with the running maximum and sum of the softmax.  Bound by the
+// cache's bytes: a token of one kv head is D * bits / 4 + D / 8 bytes and 2 * 16 * 2 D
+// multiply-adds on the matrix cores.
+//
+// A wave takes 32 tokens at a time and computes S^T = K Q^T and O^T = V^T P^T with
+// mfma_f32_16x16x32_f16.  The layout of the page makes each operand one or two wide loads and a
+// few VALU operations per eight codes, with no exchange between lanes and no LDS:
+//   K: lane (m = lane % 16, g = lane / 16) holds a quarter of key m's row, so 16 keys are one
+//      contiguous run; the k index of MFMA j is element g D / 4 + 8 j + e, of the queries too.
+//   S^T leaves lane (row, g) with keys 4 g .. 4 g + 3 of each 16: as the B operand of the second
+//      product these are its k indices 8 g + (0 .. 3) and, from the second 16 keys, 8 g + (4 .. 7).
+//   V: a lane's block of four tokens holds those four keys for its slice of D / 16 elements;
+//      the A operand of O^T tile t is element t of the slice: row m of the tile is element
+//      m D / 16 + t of the head.
+// Every value scale * code is an fp16 number, so dequantising adds no rounding.  The queries are
+// rotated by H32 like the cached rows and kept as an fp16 pair (high and low part: two
+// MFMAs, which the VALU work hides); the result is rotated back at the end.
+#include "exl3_head_rows.hpp"
 
 namespace exl3k {
 
 namespace {
 
+constexpr int kCachedWaves = 4;
+constexpr int kTile = 32;                          // tokens of a wave's step
+constexpr int kUnit = kTile * kCachedWaves;        // tokens by which the work is divided
+constexpr int kRows = 16;                          // query rows of a workgroup
+constexpr int kCachedTarget = 512;                 // workgroups: two on each of 256 CUs
+constexpr float kStart = -1e30f;                   // running maximum before the first key
+constexpr float kSlack = 8.f;                      // scores may pass the running maximum by 2^8
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The tokens of all sequences as one row of units of kUnit tokens, which the workers of a kv
+// head share evenly: worker w of `workers` has units [w U / workers, (w + 1) U / workers).
+// A worker's part of sequence s is partial w + s (one of them grows at each step).
+struct Share {
+    const int32_t *lens;
+    long most;  // tokens that the page table can name
+    int sequences;
+    __device__ __forceinline__ int len(int s) const {
+        const int n = lens[s];
+        return n < 0 ? 0 : (n > most ? (int)most : n);
+    }
+    __device__ __forceinline__ int units(int s) const { return s < sequences ? (len(s) + kUnit - 1) / kUnit : 0; }
+};
+__device__ __forceinline__ int wave_sum(int v) {
+    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    return v;
+}
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(v, d);
+        v += lane >= d ? o : 0;
+    }
+    return v;
+}
+__device__ __forceinline__ long total_units(const Share &sh, int lane) {
+    long all = 0;
+    for (int s0 = 0; s0 < sh.sequences; s0 += 64) all += wave_sum(sh.units(s0 + lane));
+    return all;
+}
+// the sequence that holds unit u (u < the total), and its first unit
+__device__ __forceinline__ int find_unit(const Share &sh, long u, int lane, long &first) {
+    long before = 0;
+    for (int s0 = 0;; s0 += 64) {
+        const int n = sh.units(s0 + lane);
+        const int end = wave_scan(n, lane);
+        const unsigned long long hit = __ballot(u < before + end);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            first = before + __shfl(end - n, l);
+            return s0 + l;
+        }
+        before += __shfl(end, 63);
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[N]) {
+    if constexpr (N == 2) {
+        const u2 t = *(const u2 *)p;
+        w[0] = t.x;
+        w[1] = t.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const u4 t = ((const u4 *)p)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[4 * i + e] = t[e];
+        }
+    }
+}
+
+// Two 4-bit codes in the low halves' bits 0..3, or 4..7, as fp16 values -8 .. 7: or-ing them into
+// 1024 (spacing 1) or 1024 at spacing 16 gives 1024 + c and 1024 + 16 c exactly.
+__device__ __forceinline__ h2 low_codes(uint32_t w) {
+    const h2 t = bitcast<h2>((w & 0x000f000fu) | 0x64006400u);
+    return t + (h2){(_Float16)-1032.f, (_Float16)-1032.f};
+}
+__device__ __forceinline__ h2 high_codes(uint32_t w) {
+    const h2 t = bitcast<h2>((w & 0x00f000f0u) | 0x64006400u);
+    return __builtin_elementwise_fma(t, (h2){(_Float16)0.0625f, (_Float16)0.0625f},
+                                     (h2){(_Float16)-72.f, (_Float16)-72.f});
+}
+__device__ __forceinline__ h2 byte_codes(uint32_t w) {  // 8 bits: -128 .. 127
+    return bitcast<h2>(w | 0x64006400u) + (h2){(_Float16)-1152.f, (_Float16)-1152.f};
+}
+
 template <int D, int BITS>
-struct CachedRows {
-    const uint8_t *pages;
-    const int32_t *table;
-    size_t page_count;
-    KvLayout l;
-    int head;
-    __device__ const uint8_t *at(int n) const {
-        const int page = table[n / l.page_tokens];
-        if (page < 0 || (size_t)page >= page_count) return nullptr;
-        return pages + (size_t)page * l.page_bytes + (size_t)head * l.region;
+struct Cached {
+    static constexpr int RUN = D * BITS / 8;   // bytes of a row's codes
+    static constexpr int NW = RUN / 16;        // words of a lane's share of 16 keys, or of 4 tokens' slices
+    static constexpr int G = D / kKvGroup;     // scale groups of a row
+    static constexpr int NJ = D / 32;          // MFMAs over the elements
+    static constexpr int NT = D / 16;          // O^T tiles
+
+    struct Half {  // one lane's part of 16 tokens
+        uint32_t k[NW], v[NW], ks;
+        u2 vs;
+    };
+
+    // base: the head's region of the page; off: the first token's place in it
+    static __device__ __forceinline__ void load(const uint8_t *base, int off, const KvLayout &l, int m, int g, Half &h) {
+        load_words<NW>(base + (size_t)(off + m) * RUN + g * (RUN / 4), h.k);
+        load_words<NW>(base + l.v_off + (size_t)((off >> 2) + g) * (4 * RUN) + m * (RUN / 4), h.v);
+        const uint8_t *ks = base + l.ks_off + (size_t)(off + m) * (2 * G);
+        if constexpr (G == 8) h.ks = *(const uint32_t *)(ks + 4 * g);
+        else h.ks = *(const uint16_t *)(ks + 2 * (G == 4 ? g : g >> 1));
+        h.vs = *(const u2 *)(base + l.vs_off + (size_t)((off >> 2) + g) * (8 * G) + 8 * (m * G / 16));
     }
-    __device__ static float code(uint8_t b, int i) {
-        return BITS == 8 ? (float)((int)b - 128) : (float)((int)((i & 1) ? b >> 4 : b & 15) - 8);
+
+    // Fragment j of a lane's key: elements 8 j .. 8 j + 7 of its quarter row, in the order that
+    // q_order undoes.
+    static __device__ __forceinline__ h8 key(const Half &h, int j) {
+        const uint32_t sw = G == 8 ? (j < 4 ? h.ks & 0xffffu : h.ks >> 16) : h.ks;
+        const _Float16 s = bitcast<_Float16>((uint16_t)sw);
+        const h2 s2 = {s, s};
+        h2 p[4];
+        if constexpr (BITS == 4) {
+            const uint32_t w = h.k[j], w8 = w >> 8;
+            p[0] = low_codes(w);
+            p[1] = high_codes(w);
+            p[2] = low_codes(w8);
+            p[3] = high_codes(w8);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                p[i] = byte_codes(__builtin_amdgcn_perm(0u, h.k[2 * j + i / 2], i & 1 ? 0x0c030c02u : 0x0c010c00u));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = p[i] * s2;
+        return (h8){p[0][0], p[0][1], p[1][0], p[1][1], p[2][0], p[2][1], p[3][0], p[3][1]};
     }
-    __device__ float key(int n, int i) const {
-        const uint8_t *b = at(n);
-        if (!b) return __builtin_nanf("");
-        const int t = n % l.page_tokens;
-        const float s = half_bits_to_float(((const uint16_t *)(b + l.ks_off))[t * (D / 32) + i / 32]);
-        return code(b[(size_t)t * (D * BITS / 8) + i * BITS / 8], i) * s;
+    // eight query elements in natural order, in that order
+    static __device__ __forceinline__ h8 q_order(h8 v) {
+        if constexpr (BITS == 4) return (h8){v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};
+        else return v;
     }
-    __device__ float value(int n, int i) const {
-        const uint8_t *b = at(n);
-        if (!b) return __builtin_nanf("");
-        const int t = n % l.page_tokens;
-        const float s = half_bits_to_float(((const uint16_t *)(b + l.vs_off))[(t / 4 * (D / 32) + i / 32) * 4 + t % 4]);
-        constexpr int PART = D * BITS / 128, W = D / 16;
-        return code(b[l.v_off + (size_t)(t / 4) * (D * BITS / 2) + i / W * (4 * PART) + t % 4 * PART + i % W * BITS / 8], i) * s;
+
+    // element t of the lane's slice for its four tokens (as two pairs)
+    static __device__ __forceinline__ void value(const Half &h, int t, h2 &a, h2 &b) {
+        const h2 s01 = bitcast<h2>(h.vs.x), s23 = bitcast<h2>(h.vs.y);
+        if constexpr (D == 64 && BITS == 4) {  // 2-byte slices: a word holds two tokens
+            const uint32_t x = t < 2 ? h.v[0] : h.v[0] >> 8, y = t < 2 ? h.v[1] : h.v[1] >> 8;
+            a = (t & 1) ? high_codes(x) : low_codes(x);
+            b = (t & 1) ? high_codes(y) : low_codes(y);
+        } else {
+            constexpr int PW = NW / 4;  // words of a token's slice
+            const int byte = BITS == 4 ? (t / 2) % 4 : t % 4, word = BITS == 4 ? t / 8 : t / 4;
+            const uint32_t sel = 0x0c000c00u + (uint32_t)(byte + ((byte + 4) << 16));
+            const uint32_t x = __builtin_amdgcn_perm(h.v[PW + word], h.v[word], sel);
+            const uint32_t y = __builtin_amdgcn_perm(h.v[3 * PW + word], h.v[2 * PW + word], sel);
+            if constexpr (BITS == 4) {
+                a = (t & 1) ? high_codes(x) : low_codes(x);
+                b = (t & 1) ? high_codes(y) : low_codes(y);
+            } else {
+                a = byte_codes(x);
+                b = byte_codes(y);
+            }
+        }
+        a = a * s01;
+        b = b * s23;
     }
 };
 
-// One wave per query row and head.
+__device__ __forceinline__ float over_groups_max(float v) {  // over lanes l ^ 16, l ^ 32
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+    v = fmaxf(__int_as_float(a[0]), __int_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return fmaxf(__int_as_float(b[0]), __int_as_float(b[1]));
+}
+__device__ __forceinline__ float over_groups_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+    v = __int_as_float(a[0]) + __int_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return __int_as_float(b[0]) + __int_as_float(b[1]);
+}
+
+// Partials of one (kv head, row tile): sums [slot][kRows][D], then (maximum, sum) [slot][kRows][2].
+struct Parts {
+    float *sums, *stats;
+};
+__device__ __forceinline__ Parts parts_of(float *ws, int d, size_t slots, size_t y) {
+    Parts p;
+    p.sums = ws + y * slots * (size_t)(kRows * (d + 2));
+    p.stats = p.sums + slots * (size_t)(kRows * d);
+    return p;
+}
+
+// Row r of a workgroup's tile: query token r / group of the sequence, q head r % group of the kv head.
+struct RowAt {
+    size_t q, out;
+    bool on;
+};
+__device__ __forceinline__ RowAt row_at(const CachedArgs &a, int s, int r, int kvh, int group) {
+    RowAt x;
+    x.on = r < a.q_len * group;
+    const int j = x.on ? r / group : 0, h = kvh * group + (x.on ? r % group : 0);
+    const size_t token = (size_t)s * a.q_len + j;
+    x.q = token * a.q.token_stride + h * a.q.head_stride;
+    x.out = token * a.out.token_stride + h * a.out.head_stride;
+    return x;
+}
+
 template <int D, int BITS>
-__global__ __launch_bounds__(64) void attention_cached_kernel(CachedArgs a) {
-    const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-    const int s = row / a.q_len, j = row - s * a.q_len;
-    const long most = (long)a.table_stride * a.l.page_tokens;
-    long n = a.kv_lens[s];
-    n = n > most ? most : n;
-    const int seen = (int)n - (a.q_len - 1 - j);
-    const CachedRows<D, BITS> r{a.pages, a.page_table + (size_t)s * a.table_stride, a.page_count, a.l,
-                                head / (a.q.heads / a.l.kv_heads)};
-    float o[D / 64];
-    const float inv = attend_row<D>((const _Float16 *)a.q.data + (size_t)row * a.q.token_stride + head * a.q.head_stride,
-                                    1, r, seen, a.scale, o);
-    __shared__ float os[D];
-    for (int i = 0; i < D / 64; ++i) os[i * 64 + lane] = o[i] * inv;
-    __syncthreads();
-    if (8 * lane < D) {
-        float x[8];
-        for (int e = 0; e < 8; ++e) x[e] = os[8 * lane + e];
-        h32_run8(x, lane);
-        store_run8<1>(a.out.data, (size_t)row * a.out.token_stride + head * a.out.head_stride + 8 * lane, a.out.vec, x);
+__global__ __launch_bounds__(64 * kCachedWaves) void attention_cached_kernel(CachedArgs a, float *ws, int workers,
+                                                                             size_t slots, int row_tiles) {
+    using C = Cached<D, BITS>;
+    __shared__ __align__(16) float lds[kCachedWaves * kRows * D + 2 * kCachedWaves * kRows];
+    const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kvh = blockIdx.y / row_tiles, row0 = (blockIdx.y - kvh * row_tiles) * kRows;
+    const int group = a.q.heads / a.l.kv_heads;
+    const Share sh{a.kv_lens, (long)a.table_stride * a.l.page_tokens, a.sequences};
+    const long all = total_units(sh, lane);
+    const long active = workers < all ? workers : all;
+    const long w = blockIdx.x;
+    if (w >= active) return;
+    long unit = w * all / active;
+    const long last = (w + 1) * all / active;
+    long first;
+    int s = find_unit(sh, unit, lane, first);
+    const Parts parts = parts_of(ws, D, slots, blockIdx.y);
+    _Float16 *const qhi = (_Float16 *)lds, *const qlo = qhi + kRows * D;
+    float *const stat = lds + kCachedWaves * kRows * D;  // (maximum, sum) of [wave][row]
+    const float c = a.scale * kLog2e;
+
+    while (unit < last && s < a.sequences) {  // one sequence's part at a time
+        const int len = sh.len(s), units = sh.units(s);
+        if (!units) {
+            ++s;
+            continue;
+        }
+        const int u0 = (int)(unit - first), u1 = (int)(last - first < units ? last - first : units);
+        // queries: rotated, split in two fp16 parts
+        __syncthreads();
+#pragma unroll
+        for (int i = tid; i < kRows * (D / 8); i += 64 * kCachedWaves) {
+            const int r = i / (D / 8), l8 = i % (D / 8);
+            const RowAt at = row_at(a, s, row0 + r, kvh, group);
+            float x[8] = {};
+            if (at.on) load_run8<1>(a.q.data, at.q + 8 * l8, a.q.vec, x);
+            h32_run8(x, lane);
+            h8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                hi[e] = (_Float16)x[e];
+                lo[e] = (_Float16)(x[e] - (float)hi[e]);
+            }
+            *(h8 *)(qhi + r * D + 8 * l8) = hi;
+            *(h8 *)(qlo + r * D + 8 * l8) = lo;
+        }
+        __syncthreads();
+        h8 bh[C::NJ], bl[C::NJ];
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j) {
+            bh[j] = C::q_order(*(const h8 *)(qhi + m * D + g * (D / 4) + 8 * j));
+            bl[j] = C::q_order(*(const h8 *)(qlo + m * D + g * (D / 4) + 8 * j));
+        }
+        // keys that this lane's row sees
+        const int limit = len - (a.q_len - 1 - (row0 + m) / group);
+
+        f4 o[C::NT];
+#pragma unroll
+        for (int t = 0; t < C::NT; ++t) o[t] = (f4){0.f, 0.f, 0.f, 0.f};
+        float top = kStart, sum = 0.f;
+        const int tile_end = (int)((long)u1 * kCachedWaves < (len + kTile - 1) / kTile ? u1 * kCachedWaves
+                                                                                      : (len + kTile - 1) / kTile);
+        const int32_t *table = a.page_table + (size_t)s * a.table_stride;
+        const int halves = (len + 15) / 16;  // 16-token pieces that hold tokens
+
+        // lane i holds where the 16-token piece i of the next 64 is: byte offset of its head region, place in
+        // the page, and whether its table entry is outside the cache
+        uint32_t at_lo = 0, at_hi = 0, place = 0;
+        typename C::Half cur[2], nxt[2];
+        bool bad_cur[2] = {false, false}, bad_nxt[2] = {false, false};
+        int piece0 = -64;
+        auto fetch = [&](int tile, int piece_base, typename C::Half (&h)[2], bool (&bad)[2]) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int at = (tile - piece_base) / kCachedWaves * 2 + i;
+                const uint32_t lo = __builtin_amdgcn_readlane(at_lo, at), hi = __builtin_amdgcn_readlane(at_hi, at);
+                const uint32_t pl = __builtin_amdgcn_readlane(place, at);
+                bad[i] = pl >> 31;
+                C::load(a.pages + (((uint64_t)hi << 32) | lo), (int)(pl & 0x7fffffffu), a.l, m, g, h[i]);
+            }
+        };
+        // this wave's tiles are tile0, tile0 + 4, ..; the table is looked up for 32 of them at once
+        auto look_up = [&](int tile0) {
+            const int tile = tile0 + (lane >> 1) * kCachedWaves, piece = tile * 2 + (lane & 1);
+            uint64_t off = 0;
+            uint32_t pl = 0;
+            if (piece < halves) {
+                const int tok = piece * 16, page = tok / a.l.page_tokens;
+                const int id = table[page];
+                pl = tok - page * a.l.page_tokens;
+                if (id >= 0 && (size_t)id < a.page_count) off = (uint64_t)id * a.l.page_bytes;
+                else pl |= 0x80000000u;
+            }
+            off += (uint64_t)kvh * a.l.region;
+            at_lo = (uint32_t)off;
+            at_hi = (uint32_t)(off >> 32);
+            place = pl;
+        };
+        const int tile_first = u0 * kCachedWaves + wave;
+        if (tile_first < tile_end) {
+            piece0 = tile_first;
+            look_up(piece0);
+            fetch(tile_first, piece0, nxt, bad_nxt);
+        }
+        for (int tile = tile_first; tile < tile_end; tile += kCachedWaves) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                cur[i] = nxt[i];
+                bad_cur[i] = bad_nxt[i];
+            }
+            const int ahead = tile + kCachedWaves;
+            if (ahead < tile_end) {
+                if (ahead - piece0 >= 32 * kCachedWaves) {
+                    piece0 = ahead;
+                    look_up(piece0);
+                }
+                fetch(ahead, piece0, nxt, bad_nxt);
+            }
+            const int n0 = tile * kTile;
+            const bool edge = n0 + kTile > len - (a.q_len - 1);  // some row does not see all of the tile
+            if (bad_cur[0] || bad_cur[1]) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (bad_cur[i]) cur[i].ks = 0x7e007e00u;
+            }
+            bool lost = false;  // a value scale that is not finite in a tile with an edge
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t sc[4] = {cur[i].vs.x & 0xffffu, cur[i].vs.x >> 16, cur[i].vs.y & 0xffffu, cur[i].vs.y >> 16};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool in = n0 + 16 * i + 4 * g + e < len, nan = (sc[e] & 0x7c00u) == 0x7c00u;
+                        lost |= in && nan;
+                        if (!in || nan) sc[e] = 0;
+                    }
+                    cur[i].vs = (u2){sc[0] | sc[1] << 16, sc[2] | sc[3] << 16};
+                }
+            }
+            f4 st[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                st[i] = (f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < C::NJ; ++j) {
+                    const h8 k = C::key(cur[i], j);
+                    st[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, bl[j], st[i], 0, 0, 0);
+                    st[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, bh[j], st[i], 0, 0, 0);
+                }
+            }
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = st[e >> 2][e & 3] * c;
+            if (edge) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (n0 + 16 * (e >> 2) + 4 * g + (e & 3) >= limit) x[e] = -INFINITY;
+            }
+            float best = x[0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) best = fmaxf(best, x[e]);
+            if (__ballot(best > top + kSlack)) {
+                const float now = fmaxf(top, over_groups_max(best));
+                const float keep = __builtin_amdgcn_exp2f(top - now);
+                sum *= keep;
+                top = now;
+#pragma unroll
+                for (int t = 0; t < C::NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[t][e] *= keep;
+            }
+            h8 p;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = __builtin_amdgcn_exp2f(x[e] - top);
+                sum += v;
+                p[e] = (_Float16)v;
+            }
+#pragma unroll
+            for (int t = 0; t < C::NT; ++t) {
+                h2 v[4];
+                C::value(cur[0], t, v[0], v[1]);
+                C::value(cur[1], t, v[2], v[3]);
+                const h8 vt = {v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, p, o[t], 0, 0, 0);
+            }
+            if (edge && __ballot(lost)) {  // rare: NaN for the rows that see such a token, in its group's elements
+                for (int n = n0; n < n0 + kTile && n < len; ++n) {
+                    const int page = n / a.l.page_tokens, id = table[page];
+                    if (id < 0 || (size_t)id >= a.page_count) continue;
+                    const int off = n - page * a.l.page_tokens;
+                    const uint16_t *vs = (const uint16_t *)(a.pages + (size_t)id * a.l.page_bytes + (size_t)kvh * a.l.region +
+                                                            a.l.vs_off + (size_t)(off >> 2) * (8 * C::G)) + (off & 3);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint16_t sc = vs[4 * ((4 * g + e) * C::G / 16)];
+                        if ((sc & 0x7c00u) == 0x7c00u && n < limit) {
+#pragma unroll
+                            for (int t = 0; t < C::NT; ++t) o[t][e] = __builtin_nanf("");
+                        }
+                    }
+                }
+            }
+        }
+
+        // the waves' parts together
+        sum = over_groups_sum(sum);
+        __syncthreads();
+        if (g == 0) {
+            stat[(wave * kRows + m) * 2] = top;
+            stat[(wave * kRows + m) * 2 + 1] = sum;
+        }
+        __syncthreads();
+        float whole = kStart;
+#pragma unroll
+        for (int i = 0; i < kCachedWaves; ++i) whole = fmaxf(whole, stat[(i * kRows + m) * 2]);
+        const float part = __builtin_amdgcn_exp2f(top - whole);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float *row = lds + (size_t)(wave * kRows + m) * D + (4 * g + e) * C::NT;
+#pragma unroll
+            for (int t = 0; t < C::NT; ++t) row[t] = o[t][e] * part;
+        }
+        __syncthreads();
+        const bool final = u0 == 0 && u1 == units;
+        const size_t slot = (size_t)(w + s);
+#pragma unroll
+        for (int i = tid; i < kRows * (D / 8); i += 64 * kCachedWaves) {
+            const int r = i / (D / 8), l8 = i % (D / 8);
+            float v[8] = {}, peak = kStart, total = 0.f;
+#pragma unroll
+            for (int k = 0; k < kCachedWaves; ++k) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += lds[(size_t)(k * kRows + r) * D + 8 * l8 + e];
+                peak = fmaxf(peak, stat[(k * kRows + r) * 2]);
+            }
+#pragma unroll
+            for (int k = 0; k < kCachedWaves; ++k)
+                total += stat[(k * kRows + r) * 2 + 1] * __builtin_amdgcn_exp2f(stat[(k * kRows + r) * 2] - peak);
+            if (final) {
+                const RowAt at = row_at(a, s, row0 + r, kvh, group);
+                const bool sees = len > a.q_len - 1 - (row0 + r) / group;
+                const float inv = sees ? 1.0f / total : 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = sees ? v[e] * inv : 0.f;
+                h32_run8(v, lane);
+                if (at.on) store_run8<1>(a.out.data, at.out + 8 * l8, a.out.vec, v);
+            } else {
+                store_run8<0>(parts.sums, (slot * kRows + r) * D + 8 * l8, 1, v);
+                if (l8 == 0) {
+                    parts.stats[(slot * kRows + r) * 2] = peak;
+                    parts.stats[(slot * kRows + r) * 2 + 1] = total;
+                }
+            }
+        }
+        unit = first + units;
+        first = unit;
+        ++s;
     }
+}
+
+// Sums the parts of each sequence that more than one worker had, and writes the rows of sequences
+// that have no tokens.
+template <int D>
+__global__ __launch_bounds__(256) void attention_join_kernel(CachedArgs a, float *ws, int workers, size_t slots,
+                                                             int row_tiles) {
+    const int tid = threadIdx.x, lane = tid & 63, s = blockIdx.x;
+    const int kvh = blockIdx.y / row_tiles, row0 = (blockIdx.y - kvh * row_tiles) * kRows;
+    const int group = a.q.heads / a.l.kv_heads;
+    const Share sh{a.kv_lens, (long)a.table_stride * a.l.page_tokens, a.sequences};
+    const int len = sh.len(s), units = sh.units(s);
+    const long all = total_units(sh, lane);
+    const long active = workers < all ? workers : all;
+    long first = 0;
+    for (int s0 = 0; s0 < s; s0 += 64) first += wave_sum(s0 + lane < s ? sh.units(s0 + lane) : 0);
+    // worker w holds unit u when w = ((u + 1) active - 1) / all
+    long w0 = 0, w1 = -1;
+    if (units) {
+        w0 = ((first + 1) * active - 1) / all;
+        w1 = ((first + units) * active - 1) / all;
+        if (w0 == w1) return;
+    }
+    const Parts parts = parts_of(ws, D, slots, blockIdx.y);
+#pragma unroll
+    for (int i = tid; i < kRows * (D / 8); i += 256) {
+        const int r = i / (D / 8), l8 = i % (D / 8);
+        float peak = kStart;
+        for (long w = w0; w <= w1; ++w) peak = fmaxf(peak, parts.stats[((size_t)(w + s) * kRows + r) * 2]);
+        float v[8] = {}, total = 0.f;
+        for (long w = w0; w <= w1; ++w) {
+            const size_t at = (size_t)(w + s) * kRows + r;
+            const float f = __builtin_amdgcn_exp2f(parts.stats[at * 2] - peak);
+            total += parts.stats[at * 2 + 1] * f;
+            float x[8];
+            load_run8<0>(parts.sums, at * D + 8 * l8, 1, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(x[e], f, v[e]);
+        }
+        const bool sees = len > a.q_len - 1 - (row0 + r) / group;
+        const float inv = sees ? 1.0f / total : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = sees ? v[e] * inv : 0.f;
+        h32_run8(v, lane);
+        const RowAt at = row_at(a, s, row0 + r, kvh, group);
+        if (at.on) store_run8<1>(a.out.data, at.out + 8 * l8, a.out.vec, v);
+    }
+}
+
+struct CachedPlan {
+    int row_tiles, workers;
+    size_t slots;
+};
+CachedPlan cached_plan(size_t q_heads, size_t kv_heads, size_t sequences, size_t q_len) {
+    CachedPlan p;
+    p.row_tiles = (int)((q_heads / kv_heads * q_len + kRows - 1) / kRows);
+    const size_t tiles = kv_heads * p.row_tiles;
+    p.workers = (int)(tiles < kCachedTarget ? (kCachedTarget + tiles - 1) / tiles : 1);
+    p.slots = p.workers + sequences;
+    return p;
+}
+
+template <int D>
+hipError_t launch_d(const CachedArgs &a, float *ws, hipStream_t stream) {
+    const CachedPlan p = cached_plan(a.q.heads, a.l.kv_heads, a.sequences, a.q_len);
+    const dim3 grid(p.workers, a.l.kv_heads * p.row_tiles), join(a.sequences, a.l.kv_heads * p.row_tiles);
+    if (a.l.bits == 4)
+        attention_cached_kernel<D, 4><<<grid, 64 * kCachedWaves, 0, stream>>>(a, ws, p.workers, p.slots, p.row_tiles);
+    else
+        attention_cached_kernel<D, 8><<<grid, 64 * kCachedWaves, 0, stream>>>(a, ws, p.workers, p.slots, p.row_tiles);
+    attention_join_kernel<D><<<join, 256, 0, stream>>>(a, ws, p.workers, p.slots, p.row_tiles);
+    return hipGetLastError();
 }
 
 }  // namespace
 
 size_t attention_cached_bytes(size_t q_heads, size_t kv_heads, size_t head_dim, size_t sequences, size_t q_len) {
-    (void)q_heads, (void)kv_heads, (void)head_dim, (void)sequences, (void)q_len;
-    return kSharedPrefixBytes;
+    const CachedPlan p = cached_plan(q_heads, kv_heads, sequences, q_len);
+    return kSharedPrefixBytes + kv_heads * p.row_tiles * p.slots * kRows * (head_dim + 2) * sizeof(float);
 }
 
 hipError_t launch_attention_cached(const CachedArgs &a, void *workspace, hipStream_t stream) {
-    (void)workspace;
-    const dim3 grid(a.sequences * a.q_len, a.q.heads);
-    const int bits = a.l.bits;
-    if (a.l.head_dim == 64) {
-        if (bits == 4) attention_cached_kernel<64, 4><<<grid, 64, 0, stream>>>(a);
-        else attention_cached_kernel<64, 8><<<grid, 64, 0, stream>>>(a);
-    } else if (a.l.head_dim == 128) {
-        if (bits == 4) attention_cached_kernel<128, 4><<<grid, 64, 0, stream>>>(a);
-        else attention_cached_kernel<128, 8><<<grid, 64, 0, stream>>>(a);
-    } else {
-        if (bits == 4) attention_cached_kernel<256, 4><<<grid, 64, 0, stream>>>(a);
-        else attention_cached_kernel<256, 8><<<grid, 64, 0, stream>>>(a);
-    }
-    return hipGetLastError();
+    float *ws = (float *)((uint8_t *)workspace + kSharedPrefixBytes);
+    if (a.l.head_dim == 64) return launch_d<64>(a, ws, stream);
+    if (a.l.head_dim == 128) return launch_d<128>(a, ws, stream);
+    return launch_d<256>(a, ws, stream);
 }
 
 }  // namespace exl3k
