@@ -458,7 +458,8 @@ exl3_status exl3_hip_kv_cache_read(const void *pages, size_t page_count, unsigne
  * head_dim 64, 128 or 256; q heads a multiple of kv_heads, up to 64 of them per kv head;
  * q_len 1..65536.  Scores, softmax statistics and sums in fp32; q as an fp16 pair (high
  * and low part), weights rounded to fp16.  The same inputs give the same bits on every
- * call.  sequences = 0 is a no-op. */
+ * call.  EXL3_NO_SUPPORT above 65,535 blocks of 16 rows (kv_heads * ceil(group * q_len /
+ * 16)).  sequences = 0 is a no-op. */
 exl3_status exl3_hip_attention_cached(const exl3_head_view *q, const exl3_head_view *out, size_t head_dim,
                                       const void *pages, size_t page_count, unsigned bits, size_t page_tokens,
                                       size_t kv_heads, const int32_t *page_table, size_t table_stride,
@@ -477,8 +478,8 @@ size_t exl3_hip_attention_cached_workspace_bytes(size_t q_heads, size_t kv_heads
  * multiple of kv heads.  q_tokens and kv_tokens are the rows of the views (no row
  * outside them is read or written, whatever the starts hold; a query row that no
  * sequence has is not written).  Scores, softmax statistics and sums in fp32, weights
- * rounded to fp16.  The same inputs give the same bits on every call.  sequences = 0 or
- * q_tokens = 0 is a no-op. */
+ * rounded to fp16.  The same inputs give the same bits on every call.  EXL3_NO_SUPPORT
+ * from 2^31 - 2^7 query rows times heads.  sequences = 0 or q_tokens = 0 is a no-op. */
 exl3_status exl3_hip_attention_prompt(const exl3_head_view *q, const exl3_head_view *k, const exl3_head_view *v,
                                       const exl3_head_view *out, size_t head_dim, const int32_t *q_starts,
                                       const int32_t *kv_starts, size_t sequences, size_t q_tokens, size_t kv_tokens,

@@ -1,52 +1,306 @@
 // exl3_attention_prompt.hip -- attention of packed sequences over their own keys and values.
-#include "exl3_attention_rows.hpp"
+//
+// A workgroup of four waves has 128 query rows of one head, 32 per wave, and walks its
+// sequence's keys in tiles of KT through two LDS buffers, with the running maximum and sum of
+// the softmax: 4 D flops per query and key on mfma_f32_32x32x16_f16, which bounds a long
+// prompt.  Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T: a lane's column is one
+// query row throughout, so the row's statistics and factors are one register and one exchange
+// (lanes l and l ^ 32), and S^T leaves each lane with the weights that it needs as the B
+// operand of O^T: keys 8 b + 4 (l / 32) + i of each 32.  V's A operand for those keys is a column of
+// the tile, read with ds_read_b64_tr_b16: within 16 lanes it hands lane i the i-th of 16 elements of
+// four rows.  16-byte chunks of a row are swizzled so that the rows of one read lie in
+// different banks.
+#include "exl3_head_rows.hpp"
 
 namespace exl3k {
 
 namespace {
 
-struct PromptRows {
-    const _Float16 *k, *v;
-    size_t k_stride, v_stride;
-    __device__ float key(int n, int i) const { return (float)k[n * k_stride + i]; }
-    __device__ float value(int n, int i) const { return (float)v[n * v_stride + i]; }
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
+constexpr int kPromptWaves = 4;
+constexpr int kPromptRows = 32 * kPromptWaves;  // query rows of a workgroup
+constexpr float kStart = -1e30f;                // running maximum before the first key
+constexpr float kSlack = 8.f;                   // scores may pass the running maximum by 2^8
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The query tile of a workgroup: tile t counts ceil(rows / kPromptRows) tiles of each sequence
+// in turn.  starts that are not ascending or not within the rows count as empty.
+struct Span {
+    int q0, nq, k0, nk, row0;  // row0: the tile's first row in the sequence; nq = 0: no such tile
+};
+__device__ __forceinline__ int clamp_to(int v, int top) { return v < 0 ? 0 : (v > top ? top : v); }
+__device__ __forceinline__ int rows_of(const PromptArgs &a, int s) {
+    if (s >= a.sequences) return 0;
+    const int b = clamp_to(a.q_starts[s], a.q_tokens), e = clamp_to(a.q_starts[s + 1], a.q_tokens);
+    return e > b ? e - b : 0;
+}
+__device__ __forceinline__ Span find_tile(const PromptArgs &a, int t, int lane) {
+    Span x{};
+    int before = 0;
+    for (int s0 = 0; s0 < a.sequences; s0 += 64) {
+        const int n = (rows_of(a, s0 + lane) + kPromptRows - 1) / kPromptRows;
+        int end = n;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(end, d);
+            end += lane >= d ? o : 0;
+        }
+        const unsigned long long hit = __ballot(t < before + end);
+        if (hit) {
+            const int l = __builtin_ctzll(hit), s = s0 + l;
+            x.q0 = clamp_to(a.q_starts[s], a.q_tokens);
+            x.nq = rows_of(a, s);
+            x.row0 = (t - before - __shfl(end - n, l)) * kPromptRows;
+            x.k0 = clamp_to(a.kv_starts[s], a.kv_tokens);
+            x.nk = clamp_to(a.kv_starts[s + 1], a.kv_tokens) - x.k0;
+            if (x.nk < 0) x.nk = 0;
+            return x;
+        }
+        before += __shfl(end, 63);
+    }
+    return x;
+}
+
+template <int D>
+struct Prompt {
+    static constexpr int KT = D == 256 ? 32 : 64;  // keys of a tile
+    static constexpr int CH = D / 8;               // 16-byte chunks of a row
+    static constexpr int NS = D / 16;              // MFMA steps over the elements
+    static constexpr int NT = D / 32;              // O^T tiles
+    static constexpr int PER = KT * CH / (64 * kPromptWaves);  // chunks of each matrix per thread
+
+    // place of chunk c of row r in an LDS tile, in chunks
+    static __device__ __forceinline__ int k_at(int r, int c) {
+        return r * CH + (D == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15));
+    }
+    static __device__ __forceinline__ int v_at(int r, int c) {
+        return r * CH + (D == 64 ? c ^ (((r >> 1) & 1) << 2) : c ^ ((r & 3) << 2));
+    }
+
+    // this thread's chunks of the tile at key n0 (keys beyond the last are the last)
+    static __device__ __forceinline__ void fetch(const Heads &m, const _Float16 *base, int n0, int nk, int tid,
+                                                 h8 (&x)[PER]) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int at = tid + i * 64 * kPromptWaves, r = at / CH, c = at % CH;
+            const int n = n0 + r < nk ? n0 + r : nk - 1;
+            const _Float16 *p = base + (size_t)n * m.token_stride + 8 * c;
+            if (m.vec) {
+                x[i] = *(const h8 *)p;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[i][e] = p[e];
+            }
+        }
+    }
 };
 
-// One wave per query row and head.
+__device__ __forceinline__ float other_half(float v) {  // the value of lane l ^ 32
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return __int_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// whether any half of the chunk is infinite or NaN; those become 0
+__device__ __forceinline__ bool drop_non_finite(h8 &v) {
+    u4 w = bitcast<u4>(v);
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if ((w[i] & 0x7c00u) == 0x7c00u) {
+            w[i] &= 0xffff0000u;
+            found = true;
+        }
+        if ((w[i] & 0x7c000000u) == 0x7c000000u) {
+            w[i] &= 0xffffu;
+            found = true;
+        }
+    }
+    v = bitcast<h8>(w);
+    return found;
+}
+
 template <int D>
-__global__ __launch_bounds__(64) void attention_prompt_kernel(PromptArgs a) {
-    const int row = blockIdx.x, head = blockIdx.y;
-    int s = 0;
-    while (s < a.sequences && !(row >= a.q_starts[s] && row < a.q_starts[s + 1])) ++s;
-    if (s == a.sequences) return;
-    const int q0 = a.q_starts[s], q1 = a.q_starts[s + 1];
-    int k0 = a.kv_starts[s], k1 = a.kv_starts[s + 1];
-    k0 = k0 < 0 ? 0 : k0;
-    k1 = k1 > a.kv_tokens ? a.kv_tokens : k1;
-    const int nk = k1 > k0 ? k1 - k0 : 0;
-    const int seen = a.causal ? nk - (q1 - 1 - row) : nk;
+__global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(PromptArgs a, int tiles) {
+    using P = Prompt<D>;
+    constexpr int KT = P::KT;
+    __shared__ __align__(16) _Float16 ks[2][KT * D], vs[2][KT * D];
+    const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int head = blockIdx.x % a.q.heads;
+    const Span sp = find_tile(a, tiles - 1 - (int)(blockIdx.x / a.q.heads), lane);  // a causal sequence's longest first
+    if (!sp.nq) return;
     const int kvh = head / (a.q.heads / a.k.heads);
-    PromptRows r;
-    r.k_stride = a.k.token_stride;
-    r.v_stride = a.v.token_stride;
-    r.k = (const _Float16 *)a.k.data + (size_t)k0 * r.k_stride + kvh * a.k.head_stride;
-    r.v = (const _Float16 *)a.v.data + (size_t)k0 * r.v_stride + kvh * a.v.head_stride;
-    float o[D / 64];
-    const float inv = attend_row<D>((const _Float16 *)a.q.data + (size_t)row * a.q.token_stride + head * a.q.head_stride,
-                                    0, r, seen, a.scale, o);
-    (void)q0;
-    _Float16 *out = (_Float16 *)a.out.data + (size_t)row * a.out.token_stride + head * a.out.head_stride;
-    for (int i = 0; i < D / 64; ++i) out[i * 64 + threadIdx.x] = (_Float16)(o[i] * inv);
+    const _Float16 *kb = (const _Float16 *)a.k.data + (size_t)sp.k0 * a.k.token_stride + kvh * a.k.head_stride;
+    const _Float16 *vb = (const _Float16 *)a.v.data + (size_t)sp.k0 * a.v.token_stride + kvh * a.v.head_stride;
+
+    // keys that this lane's row, the wave's first row and the workgroup's last row see
+    const int row = sp.row0 + 32 * wave + m;
+    const int shift = a.causal ? sp.nk - sp.nq + 1 : 0;
+    auto seen = [&](int r) {
+        const int n = a.causal ? (r < sp.nq ? r : sp.nq - 1) + shift : sp.nk;
+        return n < 0 ? 0 : n;
+    };
+    const int limit = seen(row);
+    const int wave_min = seen(sp.row0 + 32 * wave), wave_max_ = seen(sp.row0 + 32 * wave + 31);
+    const int last = seen(sp.row0 + kPromptRows - 1);
+    const int q_row = row < sp.nq ? row : sp.nq - 1;
+    const _Float16 *qp = (const _Float16 *)a.q.data + (size_t)(sp.q0 + q_row) * a.q.token_stride + head * a.q.head_stride;
+    h8 q[P::NS];
+#pragma unroll
+    for (int s = 0; s < P::NS; ++s) {
+        if (a.q.vec) {
+            q[s] = *(const h8 *)(qp + 16 * s + 8 * h);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[s][e] = qp[16 * s + 8 * h + e];
+        }
+    }
+    f16v o[P::NT];
+#pragma unroll
+    for (int t = 0; t < P::NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
+    float top = kStart, sum = 0.f;
+    const float c = a.scale * kLog2e;
+
+    h8 kx[P::PER], vx[P::PER];
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < P::PER; ++i) {
+            const int at = tid + i * 64 * kPromptWaves, r = at / P::CH, ch = at % P::CH;
+            *(h8 *)(ks[buf] + 8 * P::k_at(r, ch)) = kx[i];
+            *(h8 *)(vs[buf] + 8 * P::v_at(r, ch)) = vx[i];
+        }
+    };
+    const int steps = (last + KT - 1) / KT;
+    const int open = seen(sp.row0);  // tiles that end at or before this key have no masked place
+    if (steps) {
+        P::fetch(a.k, kb, 0, sp.nk, tid, kx);
+        P::fetch(a.v, vb, 0, sp.nk, tid, vx);
+    }
+    for (int step = 0; step < steps; ++step) {
+        const int n0 = step * KT, buf = step & 1;
+        // a masked value must not reach a row: 0 * NaN.  In a tile with masked places non-finite values
+        // are taken out here and added below for the rows that see them.
+        bool odd = false;
+        if (n0 + KT > open) {
+#pragma unroll
+            for (int i = 0; i < P::PER; ++i) odd |= drop_non_finite(vx[i]);
+        }
+        put(buf);
+        if (n0 + KT > open) odd = __syncthreads_or(odd);
+        else __syncthreads();
+        if (step + 1 < steps) {
+            P::fetch(a.k, kb, n0 + KT, sp.nk, tid, kx);
+            P::fetch(a.v, vb, n0 + KT, sp.nk, tid, vx);
+        }
+        if (n0 >= wave_max_) continue;  // no row of this wave sees the tile
+        f16v st[KT / 32];
+#pragma unroll
+        for (int b = 0; b < KT / 32; ++b) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) st[b][e] = 0.f;
+#pragma unroll
+            for (int s = 0; s < P::NS; ++s) {
+                const h8 k = *(const h8 *)(ks[buf] + 8 * P::k_at(32 * b + m, 2 * s + h));
+                st[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[s], st[b], 0, 0, 0);
+            }
+        }
+        float best = -INFINITY;
+        const bool edge = n0 + KT > wave_min;
+#pragma unroll
+        for (int b = 0; b < KT / 32; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float x = st[b][e] * c;
+                if (edge && n0 + 32 * b + 8 * (e >> 2) + 4 * h + (e & 3) >= limit) x = -INFINITY;
+                st[b][e] = x;
+                best = fmaxf(best, x);
+            }
+        if (__ballot(best > top + kSlack)) {
+            const float now = fmaxf(top, fmaxf(best, other_half(best)));
+            const float keep = __builtin_amdgcn_exp2f(top - now);
+            sum *= keep;
+            top = now;
+#pragma unroll
+            for (int t = 0; t < P::NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[t][e] *= keep;
+        }
+        h8 p[KT / 16];
+#pragma unroll
+        for (int b = 0; b < KT / 32; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float v = __builtin_amdgcn_exp2f(st[b][e] - top);
+                sum += v;
+                p[2 * b + e / 8][e % 8] = (_Float16)v;
+            }
+#pragma unroll
+        for (int u = 0; u < KT / 16; ++u) {
+#pragma unroll
+            for (int t = 0; t < P::NT; ++t) {
+                const int i = lane & 15, key = 16 * u + 4 * h + (i >> 2);
+                const int ch = 4 * t + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_s4 *)(vs[buf] + 8 * P::v_at(key, ch) + 4 * (i & 1)));
+                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_s4 *)(vs[buf] + 8 * P::v_at(key + 8, ch) + 4 * (i & 1)));
+                const h4 l4 = bitcast<h4>(lo), u4_ = bitcast<h4>(hi);
+                const h8 v = {l4[0], l4[1], l4[2], l4[3], u4_[0], u4_[1], u4_[2], u4_[3]};
+                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u], o[t], 0, 0, 0);
+            }
+        }
+        if (odd) {  // rare
+            for (int n = n0; n < n0 + KT && n < sp.nk; ++n) {
+                const _Float16 *vr = vb + (size_t)n * a.v.token_stride;
+#pragma unroll
+                for (int t = 0; t < P::NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float x = (float)vr[32 * t + 8 * (e >> 2) + 4 * h + (e & 3)];
+                        if (!__builtin_isfinite(x) && n < limit) o[t][e] += x;
+                    }
+            }
+        }
+    }
+    sum += other_half(sum);
+    if (row >= sp.nq) return;
+    const float inv = limit > 0 ? 1.0f / sum : 0.f;
+    _Float16 *out = (_Float16 *)a.out.data + (size_t)(sp.q0 + row) * a.out.token_stride + head * a.out.head_stride;
+#pragma unroll
+    for (int t = 0; t < P::NT; ++t)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            h4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = (_Float16)(limit > 0 ? o[t][4 * b + e] * inv : 0.f);
+            _Float16 *at = out + 32 * t + 8 * b + 4 * h;
+            if (a.out.vec) {
+                *(h4 *)at = x;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) at[e] = x[e];
+            }
+        }
+}
+
+template <int D>
+hipError_t launch_d(const PromptArgs &a, hipStream_t stream) {
+    // every sequence may end in a part tile
+    const int tiles = a.q_tokens / kPromptRows + a.sequences;
+    attention_prompt_kernel<D><<<dim3((unsigned)tiles * a.q.heads), 64 * kPromptWaves, 0, stream>>>(a, tiles);
+    return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_attention_prompt(const PromptArgs &a, hipStream_t stream) {
-    const dim3 grid(a.q_tokens, a.q.heads);
-    if (a.head_dim == 64) attention_prompt_kernel<64><<<grid, 64, 0, stream>>>(a);
-    else if (a.head_dim == 128) attention_prompt_kernel<128><<<grid, 64, 0, stream>>>(a);
-    else attention_prompt_kernel<256><<<grid, 64, 0, stream>>>(a);
-    return hipGetLastError();
+    if (a.head_dim == 64) return launch_d<64>(a, stream);
+    if (a.head_dim == 128) return launch_d<128>(a, stream);
+    return launch_d<256>(a, stream);
 }
 
 }  // namespace exl3k
