@@ -458,8 +458,9 @@ exl3_status exl3_hip_kv_cache_read(const void *pages, size_t page_count, unsigne
  * head_dim 64, 128 or 256; q heads a multiple of kv_heads, up to 64 of them per kv head;
  * q_len 1..65536.  Scores, softmax statistics and sums in fp32; q as an fp16 pair (high
  * and low part), weights rounded to fp16.  The same inputs give the same bits on every
- * call.  EXL3_NO_SUPPORT above 65,535 blocks of 16 rows (kv_heads * ceil(group * q_len /
- * 16)).  sequences = 0 is a no-op. */
+ * call.  A workspace whose exchange gave up (exl3_hip_workspace_status) gives NaN rows until
+ * it is initialised again.  EXL3_NO_SUPPORT where kv_heads * ceil(group * q_len / 16) is
+ * above 65,535, or times the sequences above 2^22.  sequences = 0 is a no-op. */
 exl3_status exl3_hip_attention_cached(const exl3_head_view *q, const exl3_head_view *out, size_t head_dim,
                                       const void *pages, size_t page_count, unsigned bits, size_t page_tokens,
                                       size_t kv_heads, const int32_t *page_table, size_t table_stride,

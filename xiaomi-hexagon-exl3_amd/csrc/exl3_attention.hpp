@@ -71,6 +71,9 @@ struct CachedArgs {
     int sequences, q_len;
     float scale;
 };
+// whether the grid and the counts of arrived parts (one word per row tile and sequence, in the
+// workspace's exchange) hold the call
+bool attention_cached_fits(size_t q_heads, size_t kv_heads, size_t sequences, size_t q_len);
 size_t attention_cached_bytes(size_t q_heads, size_t kv_heads, size_t head_dim, size_t sequences, size_t q_len);
 hipError_t launch_attention_cached(const CachedArgs &a, void *workspace, hipStream_t stream);
 

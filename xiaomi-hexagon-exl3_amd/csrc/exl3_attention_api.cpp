@@ -13,7 +13,6 @@ constexpr size_t kMaxGroup = 64;                 // q heads per kv head
 constexpr size_t kMaxTokens = (size_t)1 << 30;   // rows of a view: 32-bit row numbers in the kernels
 constexpr size_t kMaxSequences = 65536;
 constexpr size_t kMaxGridX = ((size_t)1 << 24) - 1;  // workgroups of 256: fewer than 2^32 work-items
-constexpr size_t kMaxGridY = 65535;
 constexpr size_t kMaxStride = (size_t)1 << 40;   // elements: row * stride stays within 64 bits
 
 exl3_status from_hip(hipError_t e) { return e == hipSuccess ? EXL3_OK : EXL3_HIP_ERROR; }
@@ -158,7 +157,7 @@ exl3_status exl3_hip_attention_cached(const exl3_head_view *q, const exl3_head_v
         return EXL3_INVAL_PARAMS;
     if (!pages || !aligned(pages, 16) || !page_table || !aligned(page_table, 4) || !kv_lens || !aligned(kv_lens, 4))
         return EXL3_INVAL_PARAMS;
-    if (kv_heads * ((q->heads / kv_heads * q_len + 15) / 16) > kMaxGridY) return EXL3_NO_SUPPORT;
+    if (!exl3k::attention_cached_fits(q->heads, kv_heads, sequences, q_len)) return EXL3_NO_SUPPORT;
     const exl3_status st = exl3k::take_workspace(need, stream, &workspace, &workspace_bytes);
     if (st != EXL3_OK) return st;
     a.pages = (const uint8_t *)pages;

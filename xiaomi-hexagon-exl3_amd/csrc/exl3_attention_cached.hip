@@ -24,18 +24,20 @@ namespace exl3k {
 
 namespace {
 
-constexpr int kCachedWaves = 4;
 constexpr int kTile = 32;                          // tokens of a wave's step
-constexpr int kUnit = kTile * kCachedWaves;        // tokens by which the work is divided
 constexpr int kRows = 16;                          // query rows of a workgroup
-constexpr int kCachedTarget = 512;                 // workgroups: two on each of 256 CUs
+// Waves of a workgroup: as many as the registers of a CU hold (two waves per SIMD, one at head
+// dimension 256), so that a part to be joined covers as many tokens as can be.
+constexpr int cached_waves(int d) { return d == 256 ? 4 : 8; }
+constexpr int kCachedGroups = 256;                 // workgroups: one per CU
 constexpr float kStart = -1e30f;                   // running maximum before the first key
 constexpr float kSlack = 8.f;                      // scores may pass the running maximum by 2^8
 constexpr float kLog2e = 1.4426950408889634f;
 
-// The tokens of all sequences as one row of units of kUnit tokens, which the workers of a kv
-// head share evenly: worker w of `workers` has units [w U / workers, (w + 1) U / workers).
+// The tokens of all sequences as one row of units (a tile for every wave), which the workers of a
+// kv head share evenly: worker w of n has units [w U / n, (w + 1) U / n).
 // A worker's part of sequence s is partial w + s (one of them grows at each step).
+template <int UNIT>
 struct Share {
     const int32_t *lens;
     long most;  // tokens that the page table can name
@@ -44,7 +46,7 @@ struct Share {
         const int n = lens[s];
         return n < 0 ? 0 : (n > most ? (int)most : n);
     }
-    __device__ __forceinline__ int units(int s) const { return s < sequences ? (len(s) + kUnit - 1) / kUnit : 0; }
+    __device__ __forceinline__ int units(int s) const { return s < sequences ? (len(s) + UNIT - 1) / UNIT : 0; }
 };
 __device__ __forceinline__ int wave_sum(int v) {
     for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
@@ -57,13 +59,15 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
     }
     return v;
 }
-__device__ __forceinline__ long total_units(const Share &sh, int lane) {
+template <typename S>
+__device__ __forceinline__ long total_units(const S &sh, int lane) {
     long all = 0;
     for (int s0 = 0; s0 < sh.sequences; s0 += 64) all += wave_sum(sh.units(s0 + lane));
     return all;
 }
 // the sequence that holds unit u (u < the total), and its first unit
-__device__ __forceinline__ int find_unit(const Share &sh, long u, int lane, long &first) {
+template <typename S>
+__device__ __forceinline__ int find_unit(const S &sh, long u, int lane, long &first) {
     long before = 0;
     for (int s0 = 0;; s0 += 64) {
         const int n = sh.units(s0 + lane);
@@ -76,6 +80,12 @@ __device__ __forceinline__ int find_unit(const Share &sh, long u, int lane, long
         }
         before += __shfl(end, 63);
     }
+}
+
+// a b / c for a <= c: 32-bit arithmetic where it holds (a 64-bit division is about 150 instructions)
+__device__ __forceinline__ long mul_div(long a, long b, long c) {
+    if (b * c <= 0xffffffffl) return (uint32_t)(a * b) / (uint32_t)c;
+    return a * b / c;
 }
 
 template <int N>
@@ -199,15 +209,27 @@ __device__ __forceinline__ float over_groups_sum(float v) {
     return __int_as_float(b[0]) + __int_as_float(b[1]);
 }
 
-// Partials of one (kv head, row tile): sums [slot][kRows][D], then (maximum, sum) [slot][kRows][2].
+// Partials of one (kv head, row tile): sums [slot][rows][D], then (maximum, sum) [slot][rows], rows the
+// real rows of a tile.  They cross XCDs, each with its own L2, so they are stored and loaded as
+// relaxed agent-scope atomics (coherent at device scope, no cache maintenance; a release fence writes
+// back a whole L2).
 struct Parts {
-    float *sums, *stats;
+    unsigned long long *sums, *stats;  // pairs of binary32
 };
-__device__ __forceinline__ Parts parts_of(float *ws, int d, size_t slots, size_t y) {
+__device__ __forceinline__ Parts parts_of(void *ws, int d, int rows, size_t slots, size_t y) {
     Parts p;
-    p.sums = ws + y * slots * (size_t)(kRows * (d + 2));
-    p.stats = p.sums + slots * (size_t)(kRows * d);
+    p.sums = (unsigned long long *)ws + y * slots * (size_t)(rows * (d / 2 + 1));
+    p.stats = p.sums + slots * (size_t)(rows * (d / 2));
     return p;
+}
+__device__ __forceinline__ void put_pair(unsigned long long *p, float a, float b) {
+    __hip_atomic_store(p, (unsigned long long)__float_as_uint(b) << 32 | __float_as_uint(a), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void take_pair(const unsigned long long *p, float &a, float &b) {
+    const unsigned long long v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    a = __uint_as_float((uint32_t)v);
+    b = __uint_as_float((uint32_t)(v >> 32));
 }
 
 // Row r of a workgroup's tile: query token r / group of the sequence, q head r % group of the kv head.
@@ -226,26 +248,56 @@ __device__ __forceinline__ RowAt row_at(const CachedArgs &a, int s, int r, int k
 }
 
 template <int D, int BITS>
-__global__ __launch_bounds__(64 * kCachedWaves) void attention_cached_kernel(CachedArgs a, float *ws, int workers,
-                                                                             size_t slots, int row_tiles) {
+__global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(CachedArgs a, void *ws,
+                                                                             uint32_t *counts, const uint32_t *status,
+                                                                             int workers, size_t slots, int row_tiles) {
     using C = Cached<D, BITS>;
-    __shared__ __align__(16) float lds[kCachedWaves * kRows * D + 2 * kCachedWaves * kRows];
+    constexpr int kCachedWaves = cached_waves(D);
+    constexpr int kPitch = D + 4;  // floats of a row of sums in LDS: rows in different banks
+    __shared__ __align__(16) float lds[kCachedWaves * kRows * kPitch + 2 * kCachedWaves * kRows];
+    __shared__ int arrived;
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.y / row_tiles, row0 = (blockIdx.y - kvh * row_tiles) * kRows;
     const int group = a.q.heads / a.l.kv_heads;
-    const Share sh{a.kv_lens, (long)a.table_stride * a.l.page_tokens, a.sequences};
+    const int rows = min(kRows, a.q_len * group - row0);  // rows of this tile
+    constexpr int kItems = kRows * (D / 8), kThreads = 64 * kCachedWaves, kEach = (kItems + kThreads - 1) / kThreads;
+    float qx[kEach][8];
+    auto load_q = [&](int s) {  // eight elements of a row per item: row tid / (D / 8), ..
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int i = tid + n * kThreads, r = i / (D / 8), l8 = i % (D / 8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) qx[n][e] = 0.f;
+            if (i < kItems && r < rows) load_run8<1>(a.q.data, row_at(a, s, row0 + r, kvh, group).q + 8 * l8, a.q.vec, qx[n]);
+        }
+    };
+    if (a.sequences == 1) load_q(0);  // ahead of the lengths: one round trip fewer
+    const bool faulted = *status != 0;
+    const Share<kTile * kCachedWaves> sh{a.kv_lens, (long)a.table_stride * a.l.page_tokens, a.sequences};
     const long all = total_units(sh, lane);
     const long active = workers < all ? workers : all;
     const long w = blockIdx.x;
+    // sequences without tokens have no units: their rows are zero
+    for (int s = (int)w; s < a.sequences; s += workers) {
+        if (sh.units(s)) continue;
+        const float zero[8] = {};
+        for (int i = tid; i < rows * (D / 8); i += kThreads)
+            store_run8<1>(a.out.data, row_at(a, s, row0 + i / (D / 8), kvh, group).out + 8 * (i % (D / 8)), a.out.vec, zero);
+    }
     if (w >= active) return;
-    long unit = w * all / active;
-    const long last = (w + 1) * all / active;
+    long unit = mul_div(w, all, active);
+    const long last = mul_div(w + 1, all, active);
     long first;
     int s = find_unit(sh, unit, lane, first);
-    const Parts parts = parts_of(ws, D, slots, blockIdx.y);
+    // the worker that holds unit u: the last w with w all / active <= u
+    auto worker_of = [&](long u) {
+        const long n = (u + 1) * active - 1;
+        return n <= 0xffffffffl && all <= 0xffffffffl ? (long)((uint32_t)n / (uint32_t)all) : n / all;
+    };
+    const Parts parts = parts_of(ws, D, rows, slots, blockIdx.y);
     _Float16 *const qhi = (_Float16 *)lds, *const qlo = qhi + kRows * D;
-    float *const stat = lds + kCachedWaves * kRows * D;  // (maximum, sum) of [wave][row]
+    float *const stat = lds + kCachedWaves * kRows * kPitch;  // (maximum, sum) of [wave][row]
     const float c = a.scale * kLog2e;
 
     while (unit < last && s < a.sequences) {  // one sequence's part at a time
@@ -256,22 +308,21 @@ __global__ __launch_bounds__(64 * kCachedWaves) void attention_cached_kernel(Cac
         }
         const int u0 = (int)(unit - first), u1 = (int)(last - first < units ? last - first : units);
         // queries: rotated, split in two fp16 parts
+        if (a.sequences != 1) load_q(s);
         __syncthreads();
 #pragma unroll
-        for (int i = tid; i < kRows * (D / 8); i += 64 * kCachedWaves) {
-            const int r = i / (D / 8), l8 = i % (D / 8);
-            const RowAt at = row_at(a, s, row0 + r, kvh, group);
-            float x[8] = {};
-            if (at.on) load_run8<1>(a.q.data, at.q + 8 * l8, a.q.vec, x);
-            h32_run8(x, lane);
+        for (int n = 0; n < kEach; ++n) {
+            const int i = tid + n * kThreads;
+            if (i >= kItems) break;
+            h32_run8(qx[n], lane);
             h8 hi, lo;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                hi[e] = (_Float16)x[e];
-                lo[e] = (_Float16)(x[e] - (float)hi[e]);
+                hi[e] = (_Float16)qx[n][e];
+                lo[e] = (_Float16)(qx[n][e] - (float)hi[e]);
             }
-            *(h8 *)(qhi + r * D + 8 * l8) = hi;
-            *(h8 *)(qlo + r * D + 8 * l8) = lo;
+            *(h8 *)(qhi + 8 * i) = hi;
+            *(h8 *)(qlo + 8 * i) = lo;
         }
         __syncthreads();
         h8 bh[C::NJ], bl[C::NJ];
@@ -446,39 +497,121 @@ __global__ __launch_bounds__(64 * kCachedWaves) void attention_cached_kernel(Cac
         const float part = __builtin_amdgcn_exp2f(top - whole);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float *row = lds + (size_t)(wave * kRows + m) * D + (4 * g + e) * C::NT;
+            float *row = lds + (wave * kRows + m) * kPitch + (4 * g + e) * C::NT;
 #pragma unroll
             for (int t = 0; t < C::NT; ++t) row[t] = o[t][e] * part;
         }
         __syncthreads();
-        const bool final = u0 == 0 && u1 == units;
-        const size_t slot = (size_t)(w + s);
+        // The whole sequence, or a part of it: then the worker that stores the last of the parts sums them, in
+        // the workers' order whichever it is.  A part's stores have reached device scope (vmcnt) before its
+        // arrival is counted; the count is left zero.
+        const long w0 = worker_of(first), w1 = worker_of(first + units - 1);
+        const bool whole_sequence = w0 == w1;
+        auto finish = [&](int r, int l8, float (&v)[8], float total) {
+            const bool sees = len > a.q_len - 1 - (row0 + r) / group;
+            const float inv = faulted ? __builtin_nanf("") : 1.0f / total;
 #pragma unroll
-        for (int i = tid; i < kRows * (D / 8); i += 64 * kCachedWaves) {
-            const int r = i / (D / 8), l8 = i % (D / 8);
+            for (int e = 0; e < 8; ++e) v[e] = sees ? v[e] * inv : 0.f;
+            h32_run8(v, lane);
+            if (r < rows)
+                store_run8<1>(a.out.data, row_at(a, s, row0 + r, kvh, group).out + 8 * l8, a.out.vec, v);
+        };
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int i = tid + n * kThreads, r = i / (D / 8), l8 = i % (D / 8);
+            if (r >= rows) break;
             float v[8] = {}, peak = kStart, total = 0.f;
 #pragma unroll
             for (int k = 0; k < kCachedWaves; ++k) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += lds[(size_t)(k * kRows + r) * D + 8 * l8 + e];
+                for (int e = 0; e < 8; ++e) v[e] += lds[(k * kRows + r) * kPitch + 8 * l8 + e];
                 peak = fmaxf(peak, stat[(k * kRows + r) * 2]);
             }
 #pragma unroll
             for (int k = 0; k < kCachedWaves; ++k)
                 total += stat[(k * kRows + r) * 2 + 1] * __builtin_amdgcn_exp2f(stat[(k * kRows + r) * 2] - peak);
-            if (final) {
-                const RowAt at = row_at(a, s, row0 + r, kvh, group);
-                const bool sees = len > a.q_len - 1 - (row0 + r) / group;
-                const float inv = sees ? 1.0f / total : 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = sees ? v[e] * inv : 0.f;
-                h32_run8(v, lane);
-                if (at.on) store_run8<1>(a.out.data, at.out + 8 * l8, a.out.vec, v);
+            if (whole_sequence || faulted) {
+                finish(r, l8, v, total);
             } else {
-                store_run8<0>(parts.sums, (slot * kRows + r) * D + 8 * l8, 1, v);
-                if (l8 == 0) {
-                    parts.stats[(slot * kRows + r) * 2] = peak;
-                    parts.stats[(slot * kRows + r) * 2 + 1] = total;
+                const size_t at = (size_t)(w + s) * rows + r;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) put_pair(parts.sums + at * (D / 2) + 4 * l8 + e / 2, v[e], v[e + 1]);
+                if (l8 == 0) put_pair(parts.stats + at, peak, total);
+            }
+        }
+        if (!whole_sequence && !faulted) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            uint32_t *count = counts + (size_t)blockIdx.y * a.sequences + s;
+            if (tid == 0)
+                arrived = (int)__hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (arrived == (int)(w1 - w0)) {
+                if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                // pairs of elements; thread groups take every split-th part, eight of them in flight
+                const int items = rows * (D / 2), lanes = items < kThreads ? items : kThreads, split = kThreads / lanes;
+                const int grp = tid / lanes;
+                for (int i0 = 0; i0 < items; i0 += lanes) {
+                    const int i = i0 + tid - grp * lanes, r = i / (D / 2);
+                    float v0 = 0.f, v1 = 0.f, peak = kStart, total = 0.f;
+                    if (i < items && grp < split) {
+                        for (long k = w0 + grp; k <= w1; k += 8 * split) {
+                            float x0[8], x1[8], px[8], tx[8];
+#pragma unroll
+                            for (int n = 0; n < 8; ++n) {
+                                const long kn = k + n * split < w1 ? k + n * split : w1;
+                                const size_t at = (size_t)(kn + s) * rows;
+                                take_pair(parts.stats + at + r, px[n], tx[n]);
+                                take_pair(parts.sums + at * (D / 2) + i, x0[n], x1[n]);
+                            }
+                            float now = peak;
+#pragma unroll
+                            for (int n = 0; n < 8; ++n) now = fmaxf(now, px[n]);
+                            const float f = __builtin_amdgcn_exp2f(peak - now);
+                            v0 *= f;
+                            v1 *= f;
+                            total *= f;
+                            peak = now;
+#pragma unroll
+                            for (int n = 0; n < 8; ++n) {
+                                const float g_ = __builtin_amdgcn_exp2f(px[n] - now);
+                                if (k + n * split <= w1) {
+                                    v0 = __builtin_fmaf(x0[n], g_, v0);
+                                    v1 = __builtin_fmaf(x1[n], g_, v1);
+                                    total = __builtin_fmaf(tx[n], g_, total);
+                                }
+                            }
+                        }
+                    }
+                    if (split > 1) {
+                        f4 *const mine = (f4 *)lds + tid;
+                        *mine = (f4){v0, v1, peak, total};
+                        __syncthreads();
+                        if (grp == 0) {
+                            for (int k = 1; k < split; ++k) {
+                                const f4 x = ((f4 *)lds)[k * lanes + tid];
+                                const float now = fmaxf(peak, x[2]);
+                                const float f0 = __builtin_amdgcn_exp2f(peak - now), f1 = __builtin_amdgcn_exp2f(x[2] - now);
+                                peak = now;
+                                v0 = v0 * f0 + x[0] * f1;
+                                v1 = v1 * f0 + x[1] * f1;
+                                total = total * f0 + x[3] * f1;
+                            }
+                        }
+                        __syncthreads();
+                    }
+                    if (i < items && grp == 0) {
+                        lds[2 * i] = v0;
+                        lds[2 * i + 1] = v1;
+                        if (i % (D / 2) == 0) stat[r] = total;
+                    }
+                }
+                __syncthreads();
+                for (int i = tid; i < rows * (D / 8); i += kThreads) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = lds[8 * i + e];
+                    finish(i / (D / 8), i % (D / 8), v, stat[i / (D / 8)]);
                 }
             }
         }
@@ -488,90 +621,50 @@ __global__ __launch_bounds__(64 * kCachedWaves) void attention_cached_kernel(Cac
     }
 }
 
-// Sums the parts of each sequence that more than one worker had, and writes the rows of sequences
-// that have no tokens.
-template <int D>
-__global__ __launch_bounds__(256) void attention_join_kernel(CachedArgs a, float *ws, int workers, size_t slots,
-                                                             int row_tiles) {
-    const int tid = threadIdx.x, lane = tid & 63, s = blockIdx.x;
-    const int kvh = blockIdx.y / row_tiles, row0 = (blockIdx.y - kvh * row_tiles) * kRows;
-    const int group = a.q.heads / a.l.kv_heads;
-    const Share sh{a.kv_lens, (long)a.table_stride * a.l.page_tokens, a.sequences};
-    const int len = sh.len(s), units = sh.units(s);
-    const long all = total_units(sh, lane);
-    const long active = workers < all ? workers : all;
-    long first = 0;
-    for (int s0 = 0; s0 < s; s0 += 64) first += wave_sum(s0 + lane < s ? sh.units(s0 + lane) : 0);
-    // worker w holds unit u when w = ((u + 1) active - 1) / all
-    long w0 = 0, w1 = -1;
-    if (units) {
-        w0 = ((first + 1) * active - 1) / all;
-        w1 = ((first + units) * active - 1) / all;
-        if (w0 == w1) return;
-    }
-    const Parts parts = parts_of(ws, D, slots, blockIdx.y);
-#pragma unroll
-    for (int i = tid; i < kRows * (D / 8); i += 256) {
-        const int r = i / (D / 8), l8 = i % (D / 8);
-        float peak = kStart;
-        for (long w = w0; w <= w1; ++w) peak = fmaxf(peak, parts.stats[((size_t)(w + s) * kRows + r) * 2]);
-        float v[8] = {}, total = 0.f;
-        for (long w = w0; w <= w1; ++w) {
-            const size_t at = (size_t)(w + s) * kRows + r;
-            const float f = __builtin_amdgcn_exp2f(parts.stats[at * 2] - peak);
-            total += parts.stats[at * 2 + 1] * f;
-            float x[8];
-            load_run8<0>(parts.sums, at * D + 8 * l8, 1, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(x[e], f, v[e]);
-        }
-        const bool sees = len > a.q_len - 1 - (row0 + r) / group;
-        const float inv = sees ? 1.0f / total : 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = sees ? v[e] * inv : 0.f;
-        h32_run8(v, lane);
-        const RowAt at = row_at(a, s, row0 + r, kvh, group);
-        if (at.on) store_run8<1>(a.out.data, at.out + 8 * l8, a.out.vec, v);
-    }
-}
-
 struct CachedPlan {
-    int row_tiles, workers;
+    int row_tiles, rows, workers;
     size_t slots;
 };
 CachedPlan cached_plan(size_t q_heads, size_t kv_heads, size_t sequences, size_t q_len) {
     CachedPlan p;
-    p.row_tiles = (int)((q_heads / kv_heads * q_len + kRows - 1) / kRows);
+    const size_t all = q_heads / kv_heads * q_len;
+    p.row_tiles = (int)((all + kRows - 1) / kRows);
+    p.rows = (int)(all < kRows ? all : kRows);
     const size_t tiles = kv_heads * p.row_tiles;
-    p.workers = (int)(tiles < kCachedTarget ? (kCachedTarget + tiles - 1) / tiles : 1);
+    p.workers = (int)(tiles < kCachedGroups ? (kCachedGroups + tiles - 1) / tiles : 1);
     p.slots = p.workers + sequences;
     return p;
 }
 
 template <int D>
-hipError_t launch_d(const CachedArgs &a, float *ws, hipStream_t stream) {
+hipError_t launch_d(const CachedArgs &a, void *workspace, hipStream_t stream) {
     const CachedPlan p = cached_plan(a.q.heads, a.l.kv_heads, a.sequences, a.q_len);
-    const dim3 grid(p.workers, a.l.kv_heads * p.row_tiles), join(a.sequences, a.l.kv_heads * p.row_tiles);
+    const dim3 grid(p.workers, a.l.kv_heads * p.row_tiles);
+    void *ws = (uint8_t *)workspace + kSharedPrefixBytes;
+    uint32_t *counts = (uint32_t *)workspace, *status = (uint32_t *)((uint8_t *)workspace + kStatusOffset);
     if (a.l.bits == 4)
-        attention_cached_kernel<D, 4><<<grid, 64 * kCachedWaves, 0, stream>>>(a, ws, p.workers, p.slots, p.row_tiles);
+        attention_cached_kernel<D, 4><<<grid, 64 * cached_waves(D), 0, stream>>>(a, ws, counts, status, p.workers, p.slots, p.row_tiles);
     else
-        attention_cached_kernel<D, 8><<<grid, 64 * kCachedWaves, 0, stream>>>(a, ws, p.workers, p.slots, p.row_tiles);
-    attention_join_kernel<D><<<join, 256, 0, stream>>>(a, ws, p.workers, p.slots, p.row_tiles);
+        attention_cached_kernel<D, 8><<<grid, 64 * cached_waves(D), 0, stream>>>(a, ws, counts, status, p.workers, p.slots, p.row_tiles);
     return hipGetLastError();
 }
 
 }  // namespace
 
+bool attention_cached_fits(size_t q_heads, size_t kv_heads, size_t sequences, size_t q_len) {
+    const size_t y = kv_heads * cached_plan(q_heads, kv_heads, sequences, q_len).row_tiles;
+    return y <= 65535 && y * sequences * sizeof(uint32_t) <= kGemvExchangeBytes;
+}
+
 size_t attention_cached_bytes(size_t q_heads, size_t kv_heads, size_t head_dim, size_t sequences, size_t q_len) {
     const CachedPlan p = cached_plan(q_heads, kv_heads, sequences, q_len);
-    return kSharedPrefixBytes + kv_heads * p.row_tiles * p.slots * kRows * (head_dim + 2) * sizeof(float);
+    return kSharedPrefixBytes + kv_heads * p.row_tiles * p.slots * p.rows * (head_dim + 2) * sizeof(float);
 }
 
 hipError_t launch_attention_cached(const CachedArgs &a, void *workspace, hipStream_t stream) {
-    float *ws = (float *)((uint8_t *)workspace + kSharedPrefixBytes);
-    if (a.l.head_dim == 64) return launch_d<64>(a, ws, stream);
-    if (a.l.head_dim == 128) return launch_d<128>(a, ws, stream);
-    return launch_d<256>(a, ws, stream);
+    if (a.l.head_dim == 64) return launch_d<64>(a, workspace, stream);
+    if (a.l.head_dim == 128) return launch_d<128>(a, workspace, stream);
+    return launch_d<256>(a, workspace, stream);
 }
 
 }  // namespace exl3k

@@ -521,17 +521,39 @@ def validate_records(records, bits, stream=None):
     return int(res.item())
 
 
-# ---- the attention block: rows of heads are [tokens, heads, head_dim] tensors, last dimension dense
-def _heads(t):
-    tokens_stride, head_stride, dense = t.stride()
-    assert dense == 1, "the elements of a head must be dense"
-    return HeadView(t.data_ptr(), t.shape[1], tokens_stride, head_stride)
+# ---- the attention block: rows of heads are [tokens, heads, head_dim] tensors, last dimension dense.
+# These calls go through exl3_torch.so (csrc/exl3_torch.cpp), which checks the tensors, allocates outputs
+# and enters libexl3_hip.so: at decode sizes the host time of a call is what counts.
+TORCH_PATH = HERE / "exl3_torch.so"
+_TORCH = None
 
 
-def _float_type(dtype):
-    import torch
-    assert dtype in (torch.float16, torch.float32), dtype
-    return F16 if dtype == torch.float16 else F32
+def _torch_module():
+    global _TORCH
+    if _TORCH is None:
+        import importlib.machinery
+        import importlib.util
+        import sys
+        import torch  # noqa: F401  (its libraries come first)
+        lib()
+        if not TORCH_PATH.exists():
+            raise ImportError(f"{TORCH_PATH} is not built (run __graft_entry__.build() or make -C "
+                              "xiaomi-hexagon-exl3_amd)")
+        name = "exl3_torch"
+        if name not in sys.modules:
+            loader = importlib.machinery.ExtensionFileLoader(name, str(TORCH_PATH))
+            spec = importlib.util.spec_from_file_location(name, str(TORCH_PATH), loader=loader)
+            mod = importlib.util.module_from_spec(spec)
+            loader.exec_module(mod)
+            sys.modules[name] = mod
+        _TORCH = sys.modules[name]
+    return _TORCH
+
+
+def _taken(result, what):
+    if type(result) is int:
+        raise Exl3Error(result, what)
+    return result
 
 
 def qk_norm_rope(q, k, positions=None, inv_freq=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
@@ -540,30 +562,9 @@ def qk_norm_rope(q, k, positions=None, inv_freq=None, q_weight=None, k_weight=No
     [tokens, heads, head_dim] and keys (or None) in one launch.  positions int32 [tokens], inv_freq fp32
     [rot_dim / 2] (None: no rotation); pairs are (p, p + rot_dim / 2), or (2p, 2p + 1) with interleaved.
     Returns (q_out, k_out), new dense tensors unless given (q_out = q: in place)."""
-    import torch
-    tokens, _, d = q.shape
-    if q_out is None:
-        q_out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
-    assert q_out.shape == q.shape
-    kv = ko = None
-    if k is not None:
-        if k_out is None:
-            k_out = torch.empty(k.shape, dtype=q_out.dtype, device=k.device)
-        assert k.shape[0] == tokens and k.shape[2] == d and k.dtype == q.dtype
-        assert k_out.shape == k.shape and k_out.dtype == q_out.dtype
-        kv, ko = ctypes.byref(_heads(k)), ctypes.byref(_heads(k_out))
-    rot = 0
-    if inv_freq is not None:
-        assert inv_freq.dtype == torch.float32 and inv_freq.is_contiguous()
-        assert positions.dtype == torch.int32 and positions.is_contiguous() and positions.numel() == tokens
-        rot = 2 * inv_freq.numel()
-    for w in (q_weight, k_weight):
-        assert w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() == d)
-    _check(lib().exl3_hip_qk_norm_rope(
-        ctypes.byref(_heads(q)), kv, _float_type(q.dtype), tokens, d, _ptr(q_weight), _ptr(k_weight), eps,
-        _ptr(positions), _ptr(inv_freq), rot, int(interleaved), rope_scale, ctypes.byref(_heads(q_out)), ko,
-        _float_type(q_out.dtype), _stream(stream)), "qk_norm_rope")
-    return q_out, k_out
+    return _taken((_TORCH or _torch_module()).qk_norm_rope(
+        q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, rope_scale, out_dtype, q_out, k_out, stream),
+        "qk_norm_rope")
 
 
 def kv_page_bytes(kv_heads, head_dim, bits=4, page_tokens=256):
@@ -580,43 +581,20 @@ def new_kv_cache(page_count, kv_heads, head_dim, bits=4, page_tokens=256, device
                        device=device)
 
 
-def _check_pages(pages, kv_heads, head_dim, bits, page_tokens):
-    import torch
-    assert pages.dtype == torch.uint8 and pages.dim() == 2 and pages.is_contiguous()
-    assert pages.shape[1] == lib().exl3_hip_kv_page_bytes(bits, kv_heads, head_dim, page_tokens), "page bytes"
-
-
 def kv_cache_write(pages, k, v, slots, bits=4, page_tokens=256, bad_slots=None, stream=None):
     """Quantises keys and values [tokens, kv_heads, head_dim] (fp16 or fp32) into their slots (int64
     [tokens], page * page_tokens + offset; negative: skipped) of the cache.  bad_slots: optional int32
     tensor of one element, set to 1 when a slot is beyond the cache."""
-    import torch
-    tokens, heads, d = k.shape
-    _check_pages(pages, heads, d, bits, page_tokens)
-    assert v.shape == k.shape and v.dtype == k.dtype
-    assert slots.dtype == torch.int64 and slots.is_contiguous() and slots.numel() == tokens
-    _check(lib().exl3_hip_kv_cache_write(_ptr(pages), pages.shape[0], bits, page_tokens, d, ctypes.byref(_heads(k)),
-                                         ctypes.byref(_heads(v)), _float_type(k.dtype), tokens, _ptr(slots),
-                                         _ptr(bad_slots), _stream(stream)), "kv_cache_write")
+    _check((_TORCH or _torch_module()).kv_cache_write(pages, k, v, slots, bits, page_tokens, bad_slots, stream),
+           "kv_cache_write")
 
 
 def kv_cache_read(pages, slots, kv_heads, head_dim, bits=4, page_tokens=256, out_dtype=None, k=None, v=None,
                   bad_slots=None, stream=None):
     """(k, v) [tokens, kv_heads, head_dim] of the slots (int64 [tokens]) as the cache holds them, fp16
     unless out_dtype says otherwise; NaN for a slot outside the cache."""
-    import torch
-    _check_pages(pages, kv_heads, head_dim, bits, page_tokens)
-    assert slots.dtype == torch.int64 and slots.is_contiguous()
-    shape = (slots.numel(), kv_heads, head_dim)
-    if k is None:
-        k = torch.empty(shape, dtype=out_dtype or torch.float16, device=pages.device)
-    if v is None:
-        v = torch.empty(shape, dtype=k.dtype, device=pages.device)
-    assert tuple(k.shape) == shape and v.shape == k.shape and v.dtype == k.dtype
-    _check(lib().exl3_hip_kv_cache_read(_ptr(pages), pages.shape[0], bits, page_tokens, head_dim, _ptr(slots),
-                                        slots.numel(), ctypes.byref(_heads(k)), ctypes.byref(_heads(v)),
-                                        _float_type(k.dtype), _ptr(bad_slots), _stream(stream)), "kv_cache_read")
-    return k, v
+    return _taken((_TORCH or _torch_module()).kv_cache_read(
+        pages, slots, kv_heads, head_dim, bits, page_tokens, out_dtype, k, v, bad_slots, stream), "kv_cache_read")
 
 
 def attention_cached_workspace_bytes(q_heads, kv_heads, head_dim, sequences, q_len=1):
@@ -628,40 +606,14 @@ def attention_cached(q, pages, page_table, kv_lens, kv_heads, bits=4, page_token
     """Attention of the last q_len tokens of each sequence, q fp16 [sequences * q_len, q_heads, head_dim], over
     the cache: page_table int32 [sequences, pages], kv_lens int32 [sequences] (with the q_len new tokens).
     scale: 1 / sqrt(head_dim) unless given."""
-    import torch
-    rows, _, d = q.shape
-    _check_pages(pages, kv_heads, d, bits, page_tokens)
-    assert page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.is_contiguous()
-    sequences, width = page_table.shape
-    assert kv_lens.dtype == torch.int32 and kv_lens.is_contiguous() and kv_lens.numel() == sequences
-    assert q.dtype == torch.float16 and rows == sequences * q_len
-    if out is None:
-        out = torch.empty(q.shape, dtype=torch.float16, device=q.device)
-    assert out.shape == q.shape and out.dtype == torch.float16
-    ws_ptr, ws_bytes = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel())
-    _check(lib().exl3_hip_attention_cached(
-        ctypes.byref(_heads(q)), ctypes.byref(_heads(out)), d, _ptr(pages), pages.shape[0], bits, page_tokens,
-        kv_heads, _ptr(page_table), width, _ptr(kv_lens), sequences, q_len, d ** -0.5 if scale is None else scale,
-        ws_ptr, ws_bytes, _stream(stream)), "attention_cached")
-    return out
+    return _taken((_TORCH or _torch_module()).attention_cached(
+        q, pages, page_table, kv_lens, kv_heads, bits, page_tokens, q_len, scale, out, workspace, stream),
+        "attention_cached")
 
 
 def attention_prompt(q, k, v, q_starts, kv_starts=None, causal=True, scale=None, out=None, stream=None):
     """Attention of packed sequences, all fp16: q [q_tokens, q_heads, head_dim], k and v [kv_tokens, kv_heads,
     head_dim]; q_starts and kv_starts (int32 [sequences + 1], None: q_starts) are the first rows of the
     sequences.  causal aligns each sequence's ends: keys ahead of its queries are a prefix."""
-    import torch
-    kv_starts = q_starts if kv_starts is None else kv_starts
-    for t in (q_starts, kv_starts):
-        assert t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous()
-    assert q_starts.numel() == kv_starts.numel() >= 1
-    assert q.dtype == k.dtype == v.dtype == torch.float16 and k.shape == v.shape and k.shape[2] == q.shape[2]
-    if out is None:
-        out = torch.empty(q.shape, dtype=torch.float16, device=q.device)
-    assert out.shape == q.shape and out.dtype == torch.float16
-    d = q.shape[2]
-    _check(lib().exl3_hip_attention_prompt(
-        ctypes.byref(_heads(q)), ctypes.byref(_heads(k)), ctypes.byref(_heads(v)), ctypes.byref(_heads(out)), d,
-        _ptr(q_starts), _ptr(kv_starts), q_starts.numel() - 1, q.shape[0], k.shape[0],
-        d ** -0.5 if scale is None else scale, int(causal), _stream(stream)), "attention_prompt")
-    return out
+    return _taken((_TORCH or _torch_module()).attention_prompt(q, k, v, q_starts, kv_starts, causal, scale, out,
+                                                               stream), "attention_prompt")
