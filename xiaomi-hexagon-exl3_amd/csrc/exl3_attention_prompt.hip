@@ -79,19 +79,30 @@ struct Prompt {
         return r * CH + (D == 64 ? c ^ (((r >> 1) & 1) << 2) : c ^ ((r & 3) << 2));
     }
 
-    // this thread's chunks of the tile at key n0 (keys beyond the last are the last)
-    static __device__ __forceinline__ void fetch(const Heads &m, const _Float16 *base, int n0, int nk, int tid,
+    // This thread's chunks of the tile at key n0; keys beyond the last are the last.  `near`: a tile's rows
+    // span less than 2^31 bytes and are 16-byte aligned, so a chunk is a 32-bit offset from the tile's first row.
+    static __device__ __forceinline__ void fetch(const Heads &m, const _Float16 *base, bool near, int n0, int nk, int tid,
                                                  h8 (&x)[PER]) {
+        const int r0 = tid / CH, c = tid % CH;
+        const char *tile = (const char *)(base + (size_t)n0 * m.token_stride);
+        if (near) {
+            const uint32_t stride = (uint32_t)m.token_stride * 2;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int at = tid + i * 64 * kPromptWaves, r = at / CH, c = at % CH;
-            const int n = n0 + r < nk ? n0 + r : nk - 1;
-            const _Float16 *p = base + (size_t)n * m.token_stride + 8 * c;
-            if (m.vec) {
-                x[i] = *(const h8 *)p;
-            } else {
+            for (int i = 0; i < PER; ++i) {
+                const int r = r0 + i * (64 * kPromptWaves / CH);
+                x[i] = *(const h8 *)(tile + ((uint32_t)min(r, nk - 1 - n0) * stride + 16 * c));
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < PER; ++i) {
+                const int r = r0 + i * (64 * kPromptWaves / CH);
+                const _Float16 *p = (const _Float16 *)tile + (size_t)min(r, nk - 1 - n0) * m.token_stride + 8 * c;
+                h8 t;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][e] = p[e];
+                for (int e = 0; e < 8; ++e) t[e] = p[e];
+#pragma unroll
+                for (int k = 0; k < PER; ++k)
+                    if (k == i) x[k] = t;
             }
         }
     }
@@ -162,9 +173,17 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
     for (int t = 0; t < P::NT; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
-    float top = kStart, sum = 0.f;
-    const float c = a.scale * kLog2e;
+    float top = kStart, sum = 0.f;  // top: the running maximum, as a score times c
+    // the largest score is that of the largest product: a negative scale goes into the queries' signs (and
+    // 0 * -infinity, the masked places of a zero scale, must stay -infinity)
+    if (a.scale < 0.f) {
+#pragma unroll
+        for (int s = 0; s < P::NS; ++s) q[s] = -q[s];
+    }
+    const float c = fmaxf(__builtin_fabsf(a.scale) * kLog2e, 1e-30f);
 
+    const bool k_near = a.k.vec && a.k.token_stride * (2 * KT) < ((size_t)1 << 31);
+    const bool v_near = a.v.vec && a.v.token_stride * (2 * KT) < ((size_t)1 << 31);
     h8 kx[P::PER], vx[P::PER];
     auto put = [&](int buf) {
 #pragma unroll
@@ -174,11 +193,21 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
             *(h8 *)(vs[buf] + 8 * P::v_at(r, ch)) = vx[i];
         }
     };
+    // Where the lane reads in a tile: the swizzles repeat every 16 rows, so rows further on are constant
+    // offsets.
+    int k_lane[P::NS], v_lane[P::NT];
+#pragma unroll
+    for (int s = 0; s < P::NS; ++s) k_lane[s] = 8 * P::k_at(m, 2 * s + h);
+#pragma unroll
+    for (int t = 0; t < P::NT; ++t) {
+        const int i = lane & 15;
+        v_lane[t] = 8 * P::v_at(4 * h + (i >> 2), 4 * t + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) + 4 * (i & 1);
+    }
     const int steps = (last + KT - 1) / KT;
     const int open = seen(sp.row0);  // tiles that end at or before this key have no masked place
     if (steps) {
-        P::fetch(a.k, kb, 0, sp.nk, tid, kx);
-        P::fetch(a.v, vb, 0, sp.nk, tid, vx);
+        P::fetch(a.k, kb, k_near, 0, sp.nk, tid, kx);
+        P::fetch(a.v, vb, v_near, 0, sp.nk, tid, vx);
     }
     for (int step = 0; step < steps; ++step) {
         const int n0 = step * KT, buf = step & 1;
@@ -193,8 +222,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
         if (n0 + KT > open) odd = __syncthreads_or(odd);
         else __syncthreads();
         if (step + 1 < steps) {
-            P::fetch(a.k, kb, n0 + KT, sp.nk, tid, kx);
-            P::fetch(a.v, vb, n0 + KT, sp.nk, tid, vx);
+            P::fetch(a.k, kb, k_near, n0 + KT, sp.nk, tid, kx);
+            P::fetch(a.v, vb, v_near, n0 + KT, sp.nk, tid, vx);
         }
         if (n0 >= wave_max_) continue;  // no row of this wave sees the tile
         f16v st[KT / 32];
@@ -204,21 +233,23 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
             for (int e = 0; e < 16; ++e) st[b][e] = 0.f;
 #pragma unroll
             for (int s = 0; s < P::NS; ++s) {
-                const h8 k = *(const h8 *)(ks[buf] + 8 * P::k_at(32 * b + m, 2 * s + h));
+                const h8 k = *(const h8 *)(ks[buf] + k_lane[s] + b * 32 * D);
                 st[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[s], st[b], 0, 0, 0);
             }
         }
-        float best = -INFINITY;
-        const bool edge = n0 + KT > wave_min;
+        if (n0 + KT > wave_min) {
+#pragma unroll
+            for (int b = 0; b < KT / 32; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    st[b][e] = n0 + 32 * b + 8 * (e >> 2) + 4 * h + (e & 3) < limit ? st[b][e] : -INFINITY;
+        }
+        float best = st[0][0];
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float x = st[b][e] * c;
-                if (edge && n0 + 32 * b + 8 * (e >> 2) + 4 * h + (e & 3) >= limit) x = -INFINITY;
-                st[b][e] = x;
-                best = fmaxf(best, x);
-            }
+            for (int e = 0; e < 16; ++e) best = fmaxf(best, st[b][e]);
+        best *= c;
         if (__ballot(best > top + kSlack)) {
             const float now = fmaxf(top, fmaxf(best, other_half(best)));
             const float keep = __builtin_amdgcn_exp2f(top - now);
@@ -229,27 +260,26 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[t][e] *= keep;
         }
+        // weights, rounded to fp16 for the product; the sum is that of the rounded ones
         h8 p[KT / 16];
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float v = __builtin_amdgcn_exp2f(st[b][e] - top);
-                sum += v;
-                p[2 * b + e / 8][e % 8] = (_Float16)v;
+            for (int e = 0; e < 16; e += 2) {
+                const h2 w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[b][e], c, -top)),
+                              (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[b][e + 1], c, -top))};
+                sum = __builtin_amdgcn_fdot2(w, (h2){(_Float16)1.f, (_Float16)1.f}, sum, false);
+                p[2 * b + e / 8][e % 8] = w[0];
+                p[2 * b + e / 8][e % 8 + 1] = w[1];
             }
 #pragma unroll
         for (int u = 0; u < KT / 16; ++u) {
 #pragma unroll
             for (int t = 0; t < P::NT; ++t) {
-                const int i = lane & 15, key = 16 * u + 4 * h + (i >> 2);
-                const int ch = 4 * t + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (lds_s4 *)(vs[buf] + 8 * P::v_at(key, ch) + 4 * (i & 1)));
-                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (lds_s4 *)(vs[buf] + 8 * P::v_at(key + 8, ch) + 4 * (i & 1)));
-                const h4 l4 = bitcast<h4>(lo), u4_ = bitcast<h4>(hi);
-                const h8 v = {l4[0], l4[1], l4[2], l4[3], u4_[0], u4_[1], u4_[2], u4_[3]};
+                const _Float16 *at = vs[buf] + v_lane[t] + u * 16 * D;
+                const h4 lo = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at));
+                const h4 hi = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + 8 * D)));
+                const h8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
                 o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u], o[t], 0, 0, 0);
             }
         }
