@@ -63,6 +63,9 @@ __device__ __forceinline__ Span find_tile(const PromptArgs &a, int t, int lane) 
     return x;
 }
 
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
 template <int D>
 struct Prompt {
     static constexpr int KT = D == 256 ? 32 : 64;  // keys of a tile
@@ -70,39 +73,42 @@ struct Prompt {
     static constexpr int NS = D / 16;              // MFMA steps over the elements
     static constexpr int NT = D / 32;              // O^T tiles
     static constexpr int PER = KT * CH / (64 * kPromptWaves);  // chunks of each matrix per thread
+    static constexpr int RS = 64 * kPromptWaves / CH;          // rows between a thread's chunks
 
-    // place of chunk c of row r in an LDS tile, in chunks
+    // Place of chunk c of row r in an LDS tile, in chunks: its own inverse, and the same for rows RS apart (one
+    // thread's rows).
     static __device__ __forceinline__ int k_at(int r, int c) {
-        return r * CH + (D == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15));
+        return r * CH + (D == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & (RS - 1) & 15));
     }
     static __device__ __forceinline__ int v_at(int r, int c) {
         return r * CH + (D == 64 ? c ^ (((r >> 1) & 1) << 2) : c ^ ((r & 3) << 2));
     }
 
-    // This thread's chunks of the tile at key n0; keys beyond the last are the last.  `near`: a tile's rows
-    // span less than 2^31 bytes and are 16-byte aligned, so a chunk is a 32-bit offset from the tile's first row.
-    static __device__ __forceinline__ void fetch(const Heads &m, const _Float16 *base, bool near, int n0, int nk, int tid,
-                                                 h8 (&x)[PER]) {
-        const int r0 = tid / CH, c = tid % CH;
+    // Brings the tile at key n0 (keys beyond the last are the last) into an LDS tile; complete after a
+    // wait for vmcnt and a barrier.  The loads write LDS directly, 16 bytes a lane in lane order, so the
+    // lane takes the chunk that belongs at its place.  `near`: a tile's rows span less than 2^31 bytes
+    // and are 16-byte aligned; else the chunks go through registers.
+    template <bool V>
+    static __device__ __forceinline__ void stage(const Heads &m, const _Float16 *base, bool near, int n0, int nk, int tid,
+                                                 _Float16 *lds) {
+        const int r0 = tid / CH, p = tid % CH;
+        const int c = (V ? v_at(r0, p) : k_at(r0, p)) - r0 * CH;
         const char *tile = (const char *)(base + (size_t)n0 * m.token_stride);
         if (near) {
             const uint32_t stride = (uint32_t)m.token_stride * 2;
+            _Float16 *const wave_lds = lds + __builtin_amdgcn_readfirstlane(tid >> 6) * 512;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int r = r0 + i * (64 * kPromptWaves / CH);
-                x[i] = *(const h8 *)(tile + ((uint32_t)min(r, nk - 1 - n0) * stride + 16 * c));
-            }
+            for (int i = 0; i < PER; ++i)
+                __builtin_amdgcn_global_load_lds(
+                    (global_void *)(tile + ((uint32_t)min(r0 + i * RS, nk - 1 - n0) * stride + 16 * c)),
+                    (lds_void *)(wave_lds + i * (512 * kPromptWaves)), 16, 0, 0);
         } else {
-#pragma unroll 1
             for (int i = 0; i < PER; ++i) {
-                const int r = r0 + i * (64 * kPromptWaves / CH);
-                const _Float16 *p = (const _Float16 *)tile + (size_t)min(r, nk - 1 - n0) * m.token_stride + 8 * c;
+                const _Float16 *q = (const _Float16 *)tile + (size_t)min(r0 + i * RS, nk - 1 - n0) * m.token_stride + 8 * c;
                 h8 t;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[e] = p[e];
-#pragma unroll
-                for (int k = 0; k < PER; ++k)
-                    if (k == i) x[k] = t;
+                for (int e = 0; e < 8; ++e) t[e] = q[e];
+                *(h8 *)(lds + 8 * (tid + i * 64 * kPromptWaves)) = t;
             }
         }
     }
@@ -146,7 +152,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
     const _Float16 *kb = (const _Float16 *)a.k.data + (size_t)sp.k0 * a.k.token_stride + kvh * a.k.head_stride;
     const _Float16 *vb = (const _Float16 *)a.v.data + (size_t)sp.k0 * a.v.token_stride + kvh * a.v.head_stride;
 
-    // keys that this lane's row, the wave's first row and the workgroup's last row see
+    // keys that this lane's row, the wave's last row and the workgroup's last row see
     const int row = sp.row0 + 32 * wave + m;
     const int shift = a.causal ? sp.nk - sp.nq + 1 : 0;
     auto seen = [&](int r) {
@@ -154,7 +160,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
         return n < 0 ? 0 : n;
     };
     const int limit = seen(row);
-    const int wave_min = seen(sp.row0 + 32 * wave), wave_max_ = seen(sp.row0 + 32 * wave + 31);
+    const int wave_max_ = seen(sp.row0 + 32 * wave + 31);
     const int last = seen(sp.row0 + kPromptRows - 1);
     const int q_row = row < sp.nq ? row : sp.nq - 1;
     const _Float16 *qp = (const _Float16 *)a.q.data + (size_t)(sp.q0 + q_row) * a.q.token_stride + head * a.q.head_stride;
@@ -184,15 +190,6 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
 
     const bool k_near = a.k.vec && a.k.token_stride * (2 * KT) < ((size_t)1 << 31);
     const bool v_near = a.v.vec && a.v.token_stride * (2 * KT) < ((size_t)1 << 31);
-    h8 kx[P::PER], vx[P::PER];
-    auto put = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < P::PER; ++i) {
-            const int at = tid + i * 64 * kPromptWaves, r = at / P::CH, ch = at % P::CH;
-            *(h8 *)(ks[buf] + 8 * P::k_at(r, ch)) = kx[i];
-            *(h8 *)(vs[buf] + 8 * P::v_at(r, ch)) = vx[i];
-        }
-    };
     // Where the lane reads in a tile: the swizzles repeat every 16 rows, so rows further on are constant
     // offsets.
     int k_lane[P::NS], v_lane[P::NT];
@@ -204,46 +201,23 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
         v_lane[t] = 8 * P::v_at(4 * h + (i >> 2), 4 * t + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) + 4 * (i & 1);
     }
     const int steps = (last + KT - 1) / KT;
-    const int open = seen(sp.row0);  // tiles that end at or before this key have no masked place
-    if (steps) {
-        P::fetch(a.k, kb, k_near, 0, sp.nk, tid, kx);
-        P::fetch(a.v, vb, v_near, 0, sp.nk, tid, vx);
-    }
-    for (int step = 0; step < steps; ++step) {
-        const int n0 = step * KT, buf = step & 1;
-        // a masked value must not reach a row: 0 * NaN.  In a tile with masked places non-finite values
-        // are taken out here and added below for the rows that see them.
-        bool odd = false;
-        if (n0 + KT > open) {
-#pragma unroll
-            for (int i = 0; i < P::PER; ++i) odd |= drop_non_finite(vx[i]);
-        }
-        put(buf);
-        if (n0 + KT > open) odd = __syncthreads_or(odd);
-        else __syncthreads();
-        if (step + 1 < steps) {
-            P::fetch(a.k, kb, k_near, n0 + KT, sp.nk, tid, kx);
-            P::fetch(a.v, vb, v_near, n0 + KT, sp.nk, tid, vx);
-        }
-        if (n0 >= wave_max_) continue;  // no row of this wave sees the tile
-        f16v st[KT / 32];
+    const int open = seen(sp.row0);
+    const int whole = open / KT < steps ? open / KT : steps;  // tiles without a masked place
+
+    f16v st[KT / 32], ahead[KT / 32];
+    h8 p[KT / 16];
+    auto scores = [&](const _Float16 *kt, f16v (&x)[KT / 32]) {
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) st[b][e] = 0.f;
+            for (int e = 0; e < 16; ++e) x[b][e] = 0.f;
 #pragma unroll
-            for (int s = 0; s < P::NS; ++s) {
-                const h8 k = *(const h8 *)(ks[buf] + k_lane[s] + b * 32 * D);
-                st[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[s], st[b], 0, 0, 0);
-            }
+            for (int s = 0; s < P::NS; ++s)
+                x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const h8 *)(kt + k_lane[s] + b * 32 * D), q[s], x[b], 0, 0, 0);
         }
-        if (n0 + KT > wave_min) {
-#pragma unroll
-            for (int b = 0; b < KT / 32; ++b)
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    st[b][e] = n0 + 32 * b + 8 * (e >> 2) + 4 * h + (e & 3) < limit ? st[b][e] : -INFINITY;
-        }
+    };
+    // the running maximum moves only when a score passes it by kSlack
+    auto raise = [&] {
         float best = st[0][0];
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b)
@@ -260,8 +234,9 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[t][e] *= keep;
         }
-        // weights, rounded to fp16 for the product; the sum is that of the rounded ones
-        h8 p[KT / 16];
+    };
+    // weights, rounded to fp16 for the product; the sum is that of the rounded ones
+    auto weigh = [&] {
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b)
 #pragma unroll
@@ -272,28 +247,82 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
                 p[2 * b + e / 8][e % 8] = w[0];
                 p[2 * b + e / 8][e % 8 + 1] = w[1];
             }
+    };
+    auto add_values = [&](const _Float16 *vt) {
 #pragma unroll
-        for (int u = 0; u < KT / 16; ++u) {
+        for (int u = 0; u < KT / 16; ++u)
 #pragma unroll
             for (int t = 0; t < P::NT; ++t) {
-                const _Float16 *at = vs[buf] + v_lane[t] + u * 16 * D;
+                const _Float16 *at = vt + v_lane[t] + u * 16 * D;
                 const h4 lo = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at));
                 const h4 hi = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + 8 * D)));
                 const h8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
                 o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u], o[t], 0, 0, 0);
             }
-        }
-        if (odd) {  // rare
-            for (int n = n0; n < n0 + KT && n < sp.nk; ++n) {
-                const _Float16 *vr = vb + (size_t)n * a.v.token_stride;
+    };
+    // Step i ends with the scores of tile i + 1, so their MFMAs and the exponentials of tile i share it.
+    // Its tiles (keys i + 1, values i) were asked for in step i - 1; it asks for keys i + 2 and values
+    // i + 1 in the buffers that step i - 1 was done with.
+    auto next = [&](int i) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (i + 2 < steps) P::template stage<false>(a.k, kb, k_near, (i + 2) * KT, sp.nk, tid, ks[i & 1]);
+        if (i + 1 < steps) P::template stage<true>(a.v, vb, v_near, (i + 1) * KT, sp.nk, tid, vs[(i + 1) & 1]);
+    };
+    if (steps) {
+        P::template stage<false>(a.k, kb, k_near, 0, sp.nk, tid, ks[0]);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (steps > 1) P::template stage<false>(a.k, kb, k_near, KT, sp.nk, tid, ks[1]);
+        P::template stage<true>(a.v, vb, v_near, 0, sp.nk, tid, vs[0]);
+        scores(ks[0], st);
+    }
+    for (int i = 0; i < whole; ++i) {
+        next(i);
+        raise();
+        scores(ks[(i + 1) & 1], ahead);  // after the last tile: of no use, and not used
+        weigh();
+        add_values(vs[i & 1]);
 #pragma unroll
-                for (int t = 0; t < P::NT; ++t)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float x = (float)vr[32 * t + 8 * (e >> 2) + 4 * h + (e & 3)];
-                        if (!__builtin_isfinite(x) && n < limit) o[t][e] += x;
-                    }
+        for (int b = 0; b < KT / 32; ++b) st[b] = ahead[b];
+    }
+    for (int i = whole; i < steps; ++i) {  // tiles with masked places
+        const int n0 = i * KT;
+        next(i);
+        // a masked value must not reach a row: 0 * NaN.  Non-finite values are taken out of the tile here
+        // and added below for the rows that see them.
+        bool odd = false;
+        for (int j = 0; j < P::PER; ++j) {
+            h8 *const at = (h8 *)(vs[i & 1]) + tid + j * 64 * kPromptWaves;
+            h8 v = *at;
+            if (drop_non_finite(v)) {
+                *at = v;
+                odd = true;
             }
+        }
+        odd = __syncthreads_or(odd);
+        if (n0 < wave_max_) {  // else no row of this wave sees the tile
+#pragma unroll
+            for (int b = 0; b < KT / 32; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    st[b][e] = n0 + 32 * b + 8 * (e >> 2) + 4 * h + (e & 3) < limit ? st[b][e] : -INFINITY;
+            raise();
+            weigh();
+            add_values(vs[i & 1]);
+            if (odd) {  // rare
+                for (int n = n0; n < n0 + KT && n < sp.nk; ++n) {
+                    const _Float16 *vr = vb + (size_t)n * a.v.token_stride;
+#pragma unroll
+                    for (int t = 0; t < P::NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float x = (float)vr[32 * t + 8 * (e >> 2) + 4 * h + (e & 3)];
+                            if (!__builtin_isfinite(x) && n < limit) o[t][e] += x;
+                        }
+                }
+            }
+            if (i + 1 < steps) scores(ks[(i + 1) & 1], st);
         }
     }
     sum += other_half(sum);
