@@ -480,7 +480,8 @@ size_t exl3_hip_attention_cached_workspace_bytes(size_t q_heads, size_t kv_heads
  * outside them is read or written, whatever the starts hold; a query row that no
  * sequence has is not written).  Scores, softmax statistics and sums in fp32, weights
  * rounded to fp16.  The same inputs give the same bits on every call.  EXL3_NO_SUPPORT
- * from 2^31 - 2^7 query rows times heads.  sequences = 0 or q_tokens = 0 is a no-op. */
+ * where (q_tokens / 128 + sequences) * q heads reaches 2^23.  sequences = 0 or q_tokens = 0
+ * is a no-op. */
 exl3_status exl3_hip_attention_prompt(const exl3_head_view *q, const exl3_head_view *k, const exl3_head_view *v,
                                       const exl3_head_view *out, size_t head_dim, const int32_t *q_starts,
                                       const int32_t *kv_starts, size_t sequences, size_t q_tokens, size_t kv_tokens,

@@ -58,13 +58,20 @@ PROMPTS = [  # query lengths, key lengths, hq, hk, d, causal
     ([129, 64], [257, 1], 5, 1, 256, False),
     ([300], [300], 2, 1, 256, True),
     ([513], [700], 2, 2, 128, True),
+    # a few rows over many keys, so that two groups of waves share them, and many empty places of a batch
+    ([130], [1000], 2, 2, 64, True),
+    ([140, 3], [1500, 900], 2, 1, 128, True),
+    ([33], [850], 1, 1, 256, False),
+    ([300, 70] + [0] * 270 + [513], [300, 75] + [3] + [0] * 269 + [600], 2, 1, 128, True),
+    ([257] + [0] * 300 + [40], [257] + [0] * 300 + [1], 1, 1, 64, True),
+    ([100, 400] + [0] * 300, [700, 33] + [0] * 300, 1, 1, 256, False),
 ]
 
 
-@pytest.mark.parametrize("case", PROMPTS, ids=str)
+@pytest.mark.parametrize("case", PROMPTS, ids=lambda c: f"{sum(c[0])}x{sum(c[1])}s{len(c[0])}h{c[2]}-{c[3]}d{c[4]}c{int(c[5])}")
 def test_prompt_matches_formula(amd, case):
     lq, lk, hq, hk, d, causal = case
-    print("  attention_prompt", case, flush=True)
+    print("  attention_prompt", [x for x in lq if x], [x for x in lk if x], case[2:], flush=True)
     qs, ks = starts(lq), starts(lk)
     q, k, v = rows(70, qs[-1], hq, d, sigma=2.0), rows(71, max(1, ks[-1]), hk, d), rows(72, max(1, ks[-1]), hk, d)
     want, bound, used = prompt_reference(q, k, v, qs, ks, causal, d ** -0.5)

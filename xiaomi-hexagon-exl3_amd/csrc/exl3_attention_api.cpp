@@ -12,7 +12,7 @@ constexpr size_t kMaxHeads = 1024;
 constexpr size_t kMaxGroup = 64;                 // q heads per kv head
 constexpr size_t kMaxTokens = (size_t)1 << 30;   // rows of a view: 32-bit row numbers in the kernels
 constexpr size_t kMaxSequences = 65536;
-constexpr size_t kMaxGridX = ((size_t)1 << 24) - 1;  // workgroups of 256: fewer than 2^32 work-items
+constexpr size_t kMaxGridX = ((size_t)1 << 23) - 1;  // workgroups of 512: fewer than 2^32 work-items
 constexpr size_t kMaxStride = (size_t)1 << 40;   // elements: row * stride stays within 64 bits
 
 exl3_status from_hip(hipError_t e) { return e == hipSuccess ? EXL3_OK : EXL3_HIP_ERROR; }

@@ -1,9 +1,10 @@
 // exl3_attention_prompt.hip -- attention of packed sequences over their own keys and values.
 //
-// A workgroup of four waves has 128 query rows of one head, 32 per wave, and walks its
-// sequence's keys in tiles of KT through two LDS buffers, with the running maximum and sum of
-// the softmax: 4 D flops per query and key on mfma_f32_32x32x16_f16, which bounds a long
-// prompt.  Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T: a lane's column is one
+// A group of four waves has 128 query rows of one head, 32 per wave, and walks its sequence's
+// keys in tiles of KT through two LDS buffers with the running maximum and sum of the softmax.
+// A workgroup has one such group, or two that take the even and the odd tiles and are joined
+// at the end. 4 D flops per query and key on mfma_f32_32x32x16_f16, which
+// bounds a long prompt.  Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T: a lane's column is one
 // query row throughout, so the row's statistics and factors are one register and one exchange
 // (lanes l and l ^ 32), and S^T leaves each lane with the weights that it needs as the B
 // operand of O^T: keys 8 b + 4 (l / 32) + i of each 32.  V's A operand for those keys is a column of
@@ -19,9 +20,15 @@ namespace {
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
+typedef __attribute__((address_space(3))) h8 lds_h8;
 
-constexpr int kPromptWaves = 4;
+constexpr int kPromptWaves = 4;  // of a group
 constexpr int kPromptRows = 32 * kPromptWaves;  // query rows of a workgroup
+// Two groups of waves per workgroup, which share its keys, where one would leave CUs idle and the walk is long:
+// one prompt of 2,000 tokens, 8 / 2 heads of 256 (136 workgroups): 60.9 against 73.4 us, of 128: 34.2 against
+// 37.7; but 300 tokens of 128: 12.7 against 11.6, and seven packed prompts, 16 / 4 heads of 64 (650
+// workgroups): 55.8 against 49.6.
+constexpr size_t kTwoGroups = 256, kTwoGroupsKeys = 512;  // at most workgroups, at least keys of a sequence on average
 constexpr float kStart = -1e30f;                // running maximum before the first key
 constexpr float kSlack = 8.f;                   // scores may pass the running maximum by 2^8
 constexpr float kLog2e = 1.4426950408889634f;
@@ -50,15 +57,16 @@ __device__ __forceinline__ Span find_tile(const PromptArgs &a, int t, int lane) 
         const unsigned long long hit = __ballot(t < before + end);
         if (hit) {
             const int l = __builtin_ctzll(hit), s = s0 + l;
+            const int lead = __builtin_amdgcn_readlane(end - n, l);  // the lane and so the span are the wave's
             x.q0 = clamp_to(a.q_starts[s], a.q_tokens);
             x.nq = rows_of(a, s);
-            x.row0 = (t - before - __shfl(end - n, l)) * kPromptRows;
+            x.row0 = (t - before - lead) * kPromptRows;
             x.k0 = clamp_to(a.kv_starts[s], a.kv_tokens);
             x.nk = clamp_to(a.kv_starts[s + 1], a.kv_tokens) - x.k0;
             if (x.nk < 0) x.nk = 0;
             return x;
         }
-        before += __shfl(end, 63);
+        before += __builtin_amdgcn_readlane(end, 63);
     }
     return x;
 }
@@ -86,15 +94,15 @@ struct Prompt {
 
     // Brings the tile at key n0 (keys beyond the last are the last) into an LDS tile; complete after a
     // wait for vmcnt and a barrier.  The loads write LDS directly, 16 bytes a lane in lane order, so the
-    // lane takes the chunk that belongs at its place.  `near`: a tile's rows span less than 2^31 bytes
+    // lane takes the chunk that belongs at its place.  NEAR: a tile's rows span less than 2^31 bytes
     // and are 16-byte aligned; else the chunks go through registers.
-    template <bool V>
-    static __device__ __forceinline__ void stage(const Heads &m, const _Float16 *base, bool near, int n0, int nk, int tid,
+    template <bool V, bool NEAR>
+    static __device__ __forceinline__ void stage(const Heads &m, const _Float16 *base, int n0, int nk, int tid,
                                                  _Float16 *lds) {
         const int r0 = tid / CH, p = tid % CH;
         const int c = (V ? v_at(r0, p) : k_at(r0, p)) - r0 * CH;
         const char *tile = (const char *)(base + (size_t)n0 * m.token_stride);
-        if (near) {
+        if constexpr (NEAR) {
             const uint32_t stride = (uint32_t)m.token_stride * 2;
             _Float16 *const wave_lds = lds + __builtin_amdgcn_readfirstlane(tid >> 6) * 512;
 #pragma unroll
@@ -111,6 +119,22 @@ struct Prompt {
                 *(h8 *)(lds + 8 * (tid + i * 64 * kPromptWaves)) = t;
             }
         }
+    }
+    // Chunk i of it where all its rows are there: the thread's offset `at` (offset_in) is the same for every
+    // tile, the rest is the scalar base.
+    template <bool V>
+    static __device__ __forceinline__ uint32_t offset_in(const Heads &m, int tid) {
+        const int r0 = tid / CH, p = tid % CH;
+        return (uint32_t)r0 * (uint32_t)(m.token_stride * 2) + 16 * ((V ? v_at(r0, p) : k_at(r0, p)) - r0 * CH);
+    }
+    static __device__ __forceinline__ void stage_chunk(const Heads &m, const _Float16 *base, int n0, int wave, int i,
+                                                       uint32_t at, _Float16 *lds) {
+        const char *rows = (const char *)(base + (size_t)(n0 + i * RS) * m.token_stride);
+        const uint32_t to = (uint32_t)(uintptr_t)(lds_void *)(lds + wave * 512 + i * (512 * kPromptWaves));
+        // The builtin's instruction (M0: the wave's place in LDS).  After the builtin the compiler has every LDS read
+        // wait for the load, since it cannot tell the slots apart.  It writes no register; the slot is read
+        // after the next step's wait and barrier.
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(at), "s"(rows) : "m0");
     }
 };
 
@@ -138,14 +162,19 @@ __device__ __forceinline__ bool drop_non_finite(h8 &v) {
     return found;
 }
 
-template <int D>
-__global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(PromptArgs a, int tiles) {
+template <int D, bool NEAR, int kGroups>
+__global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prompt_kernel(PromptArgs a, int tiles) {
     using P = Prompt<D>;
     constexpr int KT = P::KT;
-    __shared__ __align__(16) _Float16 ks[2][KT * D], vs[2][KT * D];
-    const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, h = lane >> 5;
+    __shared__ __align__(1024) _Float16 keys[kGroups][2][KT * D], values[kGroups][2][KT * D];
+    const int tid = threadIdx.x % (64 * kPromptWaves), lane = tid & 63, m = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int head = blockIdx.x % a.q.heads;
+    const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * kPromptWaves));
+    auto &ks = keys[group], &vs = values[group];
+    // Workgroup b runs on XCD b % 8, each with its own L2: where the heads divide by 8, an XCD takes
+    // neighbouring heads, which share keys and values (8,192 tokens, 32 / 8 heads of 128: PLACEHOLDER).
+    const int place = blockIdx.x % a.q.heads;
+    const int head = a.q.heads % 8 ? place : place % 8 * (a.q.heads / 8) + place / 8;
     const Span sp = find_tile(a, tiles - 1 - (int)(blockIdx.x / a.q.heads), lane);  // a causal sequence's longest first
     if (!sp.nq) return;
     const int kvh = head / (a.q.heads / a.k.heads);
@@ -188,41 +217,48 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
     }
     const float c = fmaxf(__builtin_fabsf(a.scale) * kLog2e, 1e-30f);
 
-    const bool k_near = a.k.vec && a.k.token_stride * (2 * KT) < ((size_t)1 << 31);
-    const bool v_near = a.v.vec && a.v.token_stride * (2 * KT) < ((size_t)1 << 31);
-    // Where the lane reads in a tile: the swizzles repeat every 16 rows, so rows further on are constant
-    // offsets.
-    int k_lane[P::NS], v_lane[P::NT];
-#pragma unroll
-    for (int s = 0; s < P::NS; ++s) k_lane[s] = 8 * P::k_at(m, 2 * s + h);
-#pragma unroll
-    for (int t = 0; t < P::NT; ++t) {
-        const int i = lane & 15;
-        v_lane[t] = 8 * P::v_at(4 * h + (i >> 2), 4 * t + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) + 4 * (i & 1);
-    }
+    // Where the lane reads in a tile, in bytes: a chunk index enters its swizzle as an exclusive or of whole
+    // bits, so chunk 2 s + h of a key is k_lane ^ 32 s and tile t of a value v_lane ^ 64 t; rows 16 on are
+    // constant offsets.
+    const int k_lane = 16 * P::k_at(m, h);
+    const int li = lane & 15;
+    const int v_lane = 16 * P::v_at(4 * h + (li >> 2), 2 * ((lane >> 4) & 1) + ((li & 3) >> 1)) + 8 * (li & 1);
     const int steps = (last + KT - 1) / KT;
     const int open = seen(sp.row0);
     const int whole = open / KT < steps ? open / KT : steps;  // tiles without a masked place
 
-    f16v st[KT / 32], ahead[KT / 32];
+    f16v st[KT / 32];  // a tile's scores
     h8 p[KT / 16];
-    auto scores = [&](const _Float16 *kt, f16v (&x)[KT / 32]) {
-#pragma unroll
-        for (int b = 0; b < KT / 32; ++b) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[b][e] = 0.f;
-#pragma unroll
-            for (int s = 0; s < P::NS; ++s)
-                x[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const h8 *)(kt + k_lane[s] + b * 32 * D), q[s], x[b], 0, 0, 0);
-        }
+    // operands from LDS: MFMA n of a tile's scores, MFMA n of its weighted values
+    auto key_frag = [&](int kt, int n) {
+        return *(const lds_h8 *)(uint32_t)((kt ^ (n % P::NS * 32)) + n / P::NS * 64 * D);
+    };
+    auto value_frag = [&](int vt, int n) {
+        const uint32_t at = (uint32_t)((vt ^ (n % P::NT * 64)) + n / P::NT * 32 * D);
+        const h4 lo = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at));
+        const h4 hi = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + 16 * D)));
+        return (h8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    const int k_base = (int)(uintptr_t)(lds_void *)ks[0] + k_lane, v_base = (int)(uintptr_t)(lds_void *)vs[0] + v_lane;
+    constexpr int kBuf = KT * D * 2;  // bytes of a buffer
+    auto score = [&](int n, h8 k) {
+        const f16v zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        st[n / P::NS] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[n % P::NS], n % P::NS ? st[n / P::NS] : zero, 0, 0, 0);
+    };
+    auto add_value = [&](int n, h8 v) {
+        o[n % P::NT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[n / P::NT], o[n % P::NT], 0, 0, 0);
+    };
+    // two weights, rounded to fp16 for the product; the sum is that of the rounded ones
+    auto weigh = [&](int j) {
+        const int b = j / 8, e = j % 8 * 2;
+        const h2 w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[b][e], c, -top)),
+                      (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[b][e + 1], c, -top))};
+        sum = __builtin_amdgcn_fdot2(w, (h2){(_Float16)1.f, (_Float16)1.f}, sum, false);
+        p[2 * b + e / 8][e % 8] = w[0];
+        p[2 * b + e / 8][e % 8 + 1] = w[1];
     };
     // the running maximum moves only when a score passes it by kSlack
-    auto raise = [&] {
-        float best = st[0][0];
-#pragma unroll
-        for (int b = 0; b < KT / 32; ++b)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) best = fmaxf(best, st[b][e]);
+    auto raise = [&](float best) {
         best *= c;
         if (__ballot(best > top + kSlack)) {
             const float now = fmaxf(top, fmaxf(best, other_half(best)));
@@ -235,81 +271,100 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
                 for (int e = 0; e < 16; ++e) o[t][e] *= keep;
         }
     };
-    // weights, rounded to fp16 for the product; the sum is that of the rounded ones
-    auto weigh = [&] {
+    auto largest = [&] {
+        float best = st[0][0];
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b)
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-                const h2 w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[b][e], c, -top)),
-                              (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[b][e + 1], c, -top))};
-                sum = __builtin_amdgcn_fdot2(w, (h2){(_Float16)1.f, (_Float16)1.f}, sum, false);
-                p[2 * b + e / 8][e % 8] = w[0];
-                p[2 * b + e / 8][e % 8 + 1] = w[1];
-            }
+            for (int e = 0; e < 16; ++e) best = fmaxf(best, st[b][e]);
+        return best;
     };
-    auto add_values = [&](const _Float16 *vt) {
-#pragma unroll
-        for (int u = 0; u < KT / 16; ++u)
-#pragma unroll
-            for (int t = 0; t < P::NT; ++t) {
-                const _Float16 *at = vt + v_lane[t] + u * 16 * D;
-                const h4 lo = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at));
-                const h4 hi = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + 8 * D)));
-                const h8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[u], o[t], 0, 0, 0);
-            }
-    };
-    // Step i ends with the scores of tile i + 1, so their MFMAs and the exponentials of tile i share it.
-    // Its tiles (keys i + 1, values i) were asked for in step i - 1; it asks for keys i + 2 and values
+    constexpr int kMfma = KT / 32 * P::NS, kPairs = KT / 4;  // MFMAs of each product, pairs of weights
+    static_assert(kMfma == KT / 16 * P::NT, "both products take as many MFMAs");
+    // Step i of a group is tile 2 i + group.  It ends with the scores of step i + 1.  Its tiles (keys of
+    // step i + 1, values of step i) were asked for in step i - 1; it asks for the keys of i + 2 and the values of
     // i + 1 in the buffers that step i - 1 was done with.
+    auto key_of = [&](int i) { return (i * kGroups + group) * KT; };  // a step's first key
+    const int end = steps * KT;
     auto next = [&](int i) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (i + 2 < steps) P::template stage<false>(a.k, kb, k_near, (i + 2) * KT, sp.nk, tid, ks[i & 1]);
-        if (i + 1 < steps) P::template stage<true>(a.v, vb, v_near, (i + 1) * KT, sp.nk, tid, vs[(i + 1) & 1]);
+        if (key_of(i + 2) < end) P::template stage<false, NEAR>(a.k, kb, key_of(i + 2), sp.nk, tid, ks[i & 1]);
+        if (key_of(i + 1) < end) P::template stage<true, NEAR>(a.v, vb, key_of(i + 1), sp.nk, tid, vs[(i + 1) & 1]);
     };
-    if (steps) {
-        P::template stage<false>(a.k, kb, k_near, 0, sp.nk, tid, ks[0]);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (steps > 1) P::template stage<false>(a.k, kb, k_near, KT, sp.nk, tid, ks[1]);
-        P::template stage<true>(a.v, vb, v_near, 0, sp.nk, tid, vs[0]);
-        scores(ks[0], st);
+    const int rounds = (steps + kGroups - 1) / kGroups;
+    if (key_of(0) < end) {
+        P::template stage<false, NEAR>(a.k, kb, key_of(0), sp.nk, tid, ks[0]);
+        P::template stage<true, NEAR>(a.v, vb, key_of(0), sp.nk, tid, vs[0]);
     }
-    for (int i = 0; i < whole; ++i) {
-        next(i);
-        raise();
-        scores(ks[(i + 1) & 1], ahead);  // after the last tile: of no use, and not used
-        weigh();
-        add_values(vs[i & 1]);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (key_of(1) < end) P::template stage<false, NEAR>(a.k, kb, key_of(1), sp.nk, tid, ks[1]);
 #pragma unroll
-        for (int b = 0; b < KT / 32; ++b) st[b] = ahead[b];
+    for (int n = 0; n < kMfma; ++n) score(n, key_frag(k_base, n));  // without a tile: not used
+    // Tiles without masked places, while the tiles to ask for have all their rows.
+    const uint32_t k_at = P::template offset_in<false>(a.k, tid), v_at = P::template offset_in<true>(a.v, tid);
+    const int plain = NEAR ? min(whole / kGroups, sp.nk / (kGroups * KT) - 2) : 0;
+    auto ask_chunk = [&](int i, int n) {  // of the keys of step i + 2 and the values of step i + 1, in turn
+        if (n % 2 == 0) P::stage_chunk(a.k, kb, key_of(i + 2), wave, n / 2, k_at, ks[i & 1]);
+        else P::stage_chunk(a.v, vb, key_of(i + 1), wave, n / 2, v_at, vs[(i + 1) & 1]);
+    };
+    // A tile's weights free its scores' registers for the next tile's, whose MFMAs and those of the values follow
+    // with the loads between them (asked for at once they hold the wave for 650 cycles: 32 KB at the 64 bytes a
+    // clock of a CU's address path); the exponentials run beside the other waves' MFMAs.  Two tiles of scores
+    // in flight, or an order fixed by hand, gain nothing more: 597 against 600 us at 8,192 tokens of 32 / 8
+    // heads of 128, which runs into the power limit (the MFMAs alone: 400 us).
+    int i = 0;
+    float best = largest();
+    for (; i < plain; ++i) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        raise(best);
+        int kt = k_base + ((i + 1) & 1) * kBuf, vt = v_base + (i & 1) * kBuf;
+        asm volatile("" : "+v"(kt), "+v"(vt));  // else every read's address is kept across the loop, and operands spilt
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) weigh(j);
+#pragma unroll
+        for (int n = 0; n < kMfma; ++n) {
+            score(n, key_frag(kt, n));
+            if (n % (kMfma / P::PER) == 0) ask_chunk(i, 2 * n / (kMfma / P::PER));
+        }
+#pragma unroll
+        for (int n = 0; n < kMfma; ++n) {
+            add_value(n, value_frag(vt, n));
+            if (n % (kMfma / P::PER) == 0) ask_chunk(i, 2 * n / (kMfma / P::PER) + 1);
+        }
+        best = largest();
     }
-    for (int i = whole; i < steps; ++i) {  // tiles with masked places
-        const int n0 = i * KT;
+    for (; i < rounds; ++i) {  // the others
+        const int n0 = key_of(i);
         next(i);
         // a masked value must not reach a row: 0 * NaN.  Non-finite values are taken out of the tile here
         // and added below for the rows that see them.
         bool odd = false;
-        for (int j = 0; j < P::PER; ++j) {
-            h8 *const at = (h8 *)(vs[i & 1]) + tid + j * 64 * kPromptWaves;
-            h8 v = *at;
-            if (drop_non_finite(v)) {
-                *at = v;
-                odd = true;
+        if (i >= whole / kGroups) {
+            for (int j = 0; j < P::PER; ++j) {
+                h8 *const at = (h8 *)(vs[i & 1]) + tid + j * 64 * kPromptWaves;
+                h8 v = *at;
+                if (drop_non_finite(v)) {
+                    *at = v;
+                    odd = true;
+                }
             }
+            odd = __syncthreads_or(odd);
         }
-        odd = __syncthreads_or(odd);
-        if (n0 < wave_max_) {  // else no row of this wave sees the tile
+        if (n0 < wave_max_) {  // else no row of this wave sees the tile, or there is none
 #pragma unroll
             for (int b = 0; b < KT / 32; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     st[b][e] = n0 + 32 * b + 8 * (e >> 2) + 4 * h + (e & 3) < limit ? st[b][e] : -INFINITY;
-            raise();
-            weigh();
-            add_values(vs[i & 1]);
+            raise(largest());
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) weigh(j);
+#pragma unroll
+            for (int n = 0; n < kMfma; ++n) add_value(n, value_frag(v_base + (i & 1) * kBuf, n));
             if (odd) {  // rare
                 for (int n = n0; n < n0 + KT && n < sp.nk; ++n) {
                     const _Float16 *vr = vb + (size_t)n * a.v.token_stride;
@@ -322,8 +377,40 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attention_prompt_kernel(
                         }
                 }
             }
-            if (i + 1 < steps) scores(ks[(i + 1) & 1], st);
+            if (key_of(i + 1) < end) {
+#pragma unroll
+                for (int n = 0; n < kMfma; ++n) score(n, key_frag(k_base + ((i + 1) & 1) * kBuf, n));
+            }
         }
+    }
+    if constexpr (kGroups == 2) {
+        // the odd tiles' part into the even ones', register by register of the same lane
+        __shared__ float stats[2][64 * kPromptWaves];
+        f4 *const parts = (f4 *)&keys[0][0][0];  // 16 NT floats a lane: half of the tiles' LDS
+        static_assert(sizeof(keys) + sizeof(values) >= 64 * kPromptWaves * 16 * P::NT * sizeof(float), "the tiles' LDS holds a group's sums");
+        __syncthreads();
+        if (group == 1) {
+            stats[0][tid] = top;
+            stats[1][tid] = sum;
+    #pragma unroll
+            for (int t = 0; t < P::NT; ++t)
+    #pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    parts[(4 * t + b) * (64 * kPromptWaves) + tid] = (f4){o[t][4 * b], o[t][4 * b + 1], o[t][4 * b + 2], o[t][4 * b + 3]};
+        }
+        __syncthreads();
+        if (group == 1) return;
+        const float other = stats[0][tid], peak = fmaxf(top, other);
+        const float mine = __builtin_amdgcn_exp2f(top - peak), theirs = __builtin_amdgcn_exp2f(other - peak);
+        sum = sum * mine + stats[1][tid] * theirs;
+    #pragma unroll
+        for (int t = 0; t < P::NT; ++t)
+    #pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const f4 x = parts[(4 * t + b) * (64 * kPromptWaves) + tid];
+    #pragma unroll
+                for (int e = 0; e < 4; ++e) o[t][4 * b + e] = o[t][4 * b + e] * mine + x[e] * theirs;
+            }
     }
     sum += other_half(sum);
     if (row >= sp.nq) return;
@@ -350,7 +437,18 @@ template <int D>
 hipError_t launch_d(const PromptArgs &a, hipStream_t stream) {
     // every sequence may end in a part tile
     const int tiles = a.q_tokens / kPromptRows + a.sequences;
-    attention_prompt_kernel<D><<<dim3((unsigned)tiles * a.q.heads), 64 * kPromptWaves, 0, stream>>>(a, tiles);
+    const dim3 grid((unsigned)tiles * a.q.heads);
+    constexpr size_t kSpan = (size_t)1 << 31;
+    const bool near = a.k.vec && a.v.vec && a.k.token_stride * (2 * Prompt<D>::KT) < kSpan &&
+                      a.v.token_stride * (2 * Prompt<D>::KT) < kSpan;
+    const int block = 64 * kPromptWaves;
+    if (grid.x <= kTwoGroups && (size_t)a.kv_tokens >= kTwoGroupsKeys * a.sequences) {
+        if (near) attention_prompt_kernel<D, true, 2><<<grid, 2 * block, 0, stream>>>(a, tiles);
+        else attention_prompt_kernel<D, false, 2><<<grid, 2 * block, 0, stream>>>(a, tiles);
+    } else {
+        if (near) attention_prompt_kernel<D, true, 1><<<grid, block, 0, stream>>>(a, tiles);
+        else attention_prompt_kernel<D, false, 1><<<grid, block, 0, stream>>>(a, tiles);
+    }
     return hipGetLastError();
 }
 
