@@ -48,12 +48,9 @@ struct Share {
     }
     __device__ __forceinline__ int units(int s) const { return s < sequences ? (len(s) + UNIT - 1) / UNIT : 0; }
 };
-__device__ __forceinline__ int wave_sum(int v) {
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
-}
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
-    for (int d = 1; d < 64; d <<= 1) {
+// over the first n lanes, n > 0 (the others hold zero)
+__device__ __forceinline__ int wave_scan(int v, int lane, int n) {  // inclusive
+    for (int d = 1; d < min(n, 64); d <<= 1) {
         const int o = __shfl_up(v, d);
         v += lane >= d ? o : 0;
     }
@@ -62,7 +59,10 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
 template <typename S>
 __device__ __forceinline__ long total_units(const S &sh, int lane) {
     long all = 0;
-    for (int s0 = 0; s0 < sh.sequences; s0 += 64) all += wave_sum(sh.units(s0 + lane));
+    for (int s0 = 0; s0 < sh.sequences; s0 += 64) {
+        const int n = sh.sequences - s0;
+        all += __builtin_amdgcn_readlane(wave_scan(sh.units(s0 + lane), lane, n), min(n, 64) - 1);
+    }
     return all;
 }
 // the sequence that holds unit u (u < the total), and its first unit
@@ -71,14 +71,14 @@ __device__ __forceinline__ int find_unit(const S &sh, long u, int lane, long &fi
     long before = 0;
     for (int s0 = 0;; s0 += 64) {
         const int n = sh.units(s0 + lane);
-        const int end = wave_scan(n, lane);
+        const int end = wave_scan(n, lane, sh.sequences - s0);
         const unsigned long long hit = __ballot(u < before + end);
         if (hit) {
             const int l = __builtin_ctzll(hit);
-            first = before + __shfl(end - n, l);
+            first = before + __builtin_amdgcn_readlane(end - n, l);
             return s0 + l;
         }
-        before += __shfl(end, 63);
+        before += __builtin_amdgcn_readlane(end, 63);
     }
 }
 
@@ -307,37 +307,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             continue;
         }
         const int u0 = (int)(unit - first), u1 = (int)(last - first < units ? last - first : units);
-        // queries: rotated, split in two fp16 parts
-        if (a.sequences != 1) load_q(s);
-        __syncthreads();
-#pragma unroll
-        for (int n = 0; n < kEach; ++n) {
-            const int i = tid + n * kThreads;
-            if (i >= kItems) break;
-            h32_run8(qx[n], lane);
-            h8 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                hi[e] = (_Float16)qx[n][e];
-                lo[e] = (_Float16)(qx[n][e] - (float)hi[e]);
-            }
-            *(h8 *)(qhi + 8 * i) = hi;
-            *(h8 *)(qlo + 8 * i) = lo;
-        }
-        __syncthreads();
-        h8 bh[C::NJ], bl[C::NJ];
-#pragma unroll
-        for (int j = 0; j < C::NJ; ++j) {
-            bh[j] = C::q_order(*(const h8 *)(qhi + m * D + g * (D / 4) + 8 * j));
-            bl[j] = C::q_order(*(const h8 *)(qlo + m * D + g * (D / 4) + 8 * j));
-        }
-        // keys that this lane's row sees
-        const int limit = len - (a.q_len - 1 - (row0 + m) / group);
-
-        f4 o[C::NT];
-#pragma unroll
-        for (int t = 0; t < C::NT; ++t) o[t] = (f4){0.f, 0.f, 0.f, 0.f};
-        float top = kStart, sum = 0.f;
+        // the first tile is on its way while the queries are prepared
         const int tile_end = (int)((long)u1 * kCachedWaves < (len + kTile - 1) / kTile ? u1 * kCachedWaves
                                                                                       : (len + kTile - 1) / kTile);
         const int32_t *table = a.page_table + (size_t)s * a.table_stride;
@@ -382,6 +352,37 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             look_up(piece0);
             fetch(tile_first, piece0, nxt, bad_nxt);
         }
+        // queries: rotated, split in two fp16 parts
+        if (a.sequences != 1) load_q(s);
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int i = tid + n * kThreads;
+            if (i >= kItems) break;
+            h32_run8(qx[n], lane);
+            h8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                hi[e] = (_Float16)qx[n][e];
+                lo[e] = (_Float16)(qx[n][e] - (float)hi[e]);
+            }
+            *(h8 *)(qhi + 8 * i) = hi;
+            *(h8 *)(qlo + 8 * i) = lo;
+        }
+        __syncthreads();
+        h8 bh[C::NJ], bl[C::NJ];
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j) {
+            bh[j] = C::q_order(*(const h8 *)(qhi + m * D + g * (D / 4) + 8 * j));
+            bl[j] = C::q_order(*(const h8 *)(qlo + m * D + g * (D / 4) + 8 * j));
+        }
+        // keys that this lane's row sees
+        const int limit = len - (a.q_len - 1 - (row0 + m) / group);
+
+        f4 o[C::NT];
+#pragma unroll
+        for (int t = 0; t < C::NT; ++t) o[t] = (f4){0.f, 0.f, 0.f, 0.f};
+        float top = kStart, sum = 0.f;
         for (int tile = tile_first; tile < tile_end; tile += kCachedWaves) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -548,17 +549,17 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             __syncthreads();
             if (arrived == (int)(w1 - w0)) {
                 if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                // pairs of elements; thread groups take every split-th part, eight of them in flight
+                // pairs of elements; thread groups take every split-th part, 16 of them in flight
                 const int items = rows * (D / 2), lanes = items < kThreads ? items : kThreads, split = kThreads / lanes;
                 const int grp = tid / lanes;
                 for (int i0 = 0; i0 < items; i0 += lanes) {
                     const int i = i0 + tid - grp * lanes, r = i / (D / 2);
                     float v0 = 0.f, v1 = 0.f, peak = kStart, total = 0.f;
                     if (i < items && grp < split) {
-                        for (long k = w0 + grp; k <= w1; k += 8 * split) {
-                            float x0[8], x1[8], px[8], tx[8];
+                        for (long k = w0 + grp; k <= w1; k += 16 * split) {
+                            float x0[16], x1[16], px[16], tx[16];
 #pragma unroll
-                            for (int n = 0; n < 8; ++n) {
+                            for (int n = 0; n < 16; ++n) {
                                 const long kn = k + n * split < w1 ? k + n * split : w1;
                                 const size_t at = (size_t)(kn + s) * rows;
                                 take_pair(parts.stats + at + r, px[n], tx[n]);
@@ -566,14 +567,14 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
                             }
                             float now = peak;
 #pragma unroll
-                            for (int n = 0; n < 8; ++n) now = fmaxf(now, px[n]);
+                            for (int n = 0; n < 16; ++n) now = fmaxf(now, px[n]);
                             const float f = __builtin_amdgcn_exp2f(peak - now);
                             v0 *= f;
                             v1 *= f;
                             total *= f;
                             peak = now;
 #pragma unroll
-                            for (int n = 0; n < 8; ++n) {
+                            for (int n = 0; n < 16; ++n) {
                                 const float g_ = __builtin_amdgcn_exp2f(px[n] - now);
                                 if (k + n * split <= w1) {
                                     v0 = __builtin_fmaf(x0[n], g_, v0);

@@ -39,34 +39,30 @@ struct Span {
     int q0, nq, k0, nk, row0;  // row0: the tile's first row in the sequence; nq = 0: no such tile
 };
 __device__ __forceinline__ int clamp_to(int v, int top) { return v < 0 ? 0 : (v > top ? top : v); }
-__device__ __forceinline__ int rows_of(const PromptArgs &a, int s) {
-    if (s >= a.sequences) return 0;
-    const int b = clamp_to(a.q_starts[s], a.q_tokens), e = clamp_to(a.q_starts[s + 1], a.q_tokens);
-    return e > b ? e - b : 0;
-}
 __device__ __forceinline__ Span find_tile(const PromptArgs &a, int t, int lane) {
     Span x{};
     int before = 0;
     for (int s0 = 0; s0 < a.sequences; s0 += 64) {
-        const int n = (rows_of(a, s0 + lane) + kPromptRows - 1) / kPromptRows;
+        const int s = s0 + lane < a.sequences ? s0 + lane : a.sequences - 1, left = a.sequences - s0;
+        const int q0 = clamp_to(a.q_starts[s], a.q_tokens), q1 = clamp_to(a.q_starts[s + 1], a.q_tokens);
+        const int k0 = clamp_to(a.kv_starts[s], a.kv_tokens), k1 = clamp_to(a.kv_starts[s + 1], a.kv_tokens);
+        const int n = lane < left && q1 > q0 ? (q1 - q0 + kPromptRows - 1) / kPromptRows : 0;
         int end = n;
-        for (int d = 1; d < 64; d <<= 1) {
+        for (int d = 1; d < min(left, 64); d <<= 1) {
             const int o = __shfl_up(end, d);
             end += lane >= d ? o : 0;
         }
         const unsigned long long hit = __ballot(t < before + end);
         if (hit) {
-            const int l = __builtin_ctzll(hit), s = s0 + l;
-            const int lead = __builtin_amdgcn_readlane(end - n, l);  // the lane and so the span are the wave's
-            x.q0 = clamp_to(a.q_starts[s], a.q_tokens);
-            x.nq = rows_of(a, s);
-            x.row0 = (t - before - lead) * kPromptRows;
-            x.k0 = clamp_to(a.kv_starts[s], a.kv_tokens);
-            x.nk = clamp_to(a.kv_starts[s + 1], a.kv_tokens) - x.k0;
-            if (x.nk < 0) x.nk = 0;
+            const int l = __builtin_ctzll(hit);  // the lane and so the span are the wave's
+            x.q0 = __builtin_amdgcn_readlane(q0, l);
+            x.nq = __builtin_amdgcn_readlane(q1, l) - x.q0;
+            x.row0 = (t - before - __builtin_amdgcn_readlane(end - n, l)) * kPromptRows;
+            x.k0 = __builtin_amdgcn_readlane(k0, l);
+            x.nk = max(0, __builtin_amdgcn_readlane(k1, l) - x.k0);
             return x;
         }
-        before += __builtin_amdgcn_readlane(end, 63);
+        before += __builtin_amdgcn_readlane(end, min(left, 64) - 1);
     }
     return x;
 }
@@ -337,6 +333,8 @@ __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prom
         }
         best = largest();
     }
+    __shared__ int odd_tile[2];  // whether the step's values held a non-finite one
+    if (threadIdx.x < 2) odd_tile[threadIdx.x] = 0;
     for (; i < rounds; ++i) {  // the others
         const int n0 = key_of(i);
         next(i);
@@ -352,7 +350,10 @@ __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prom
                     odd = true;
                 }
             }
-            odd = __syncthreads_or(odd);
+            if (__ballot(odd) && lane == 0) odd_tile[i & 1] = 1;
+            __syncthreads();
+            odd = odd_tile[i & 1];
+            if (threadIdx.x == 0) odd_tile[(i + 1) & 1] = 0;
         }
         if (n0 < wave_max_) {  // else no row of this wave sees the tile, or there is none
 #pragma unroll

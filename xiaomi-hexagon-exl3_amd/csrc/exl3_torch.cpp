@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -59,7 +60,7 @@ at::Tensor output(PyObject *o, at::IntArrayRef shape, at::ScalarType type, const
         need(t.sizes() == shape, "out has another shape");
         return t;
     }
-    return at::empty(shape, like.options().dtype(type));
+    return at::detail::empty_cuda(shape, type, like.device(), std::nullopt);  // at::empty without its dispatch
 }
 at::ScalarType dtype_or(PyObject *o, at::ScalarType otherwise) {
     if (!given(o)) return otherwise;
