@@ -30,13 +30,19 @@ constexpr int kRows = 16;                          // query rows of a workgroup
 // dimension 256), so that a part to be joined covers as many tokens as can be.
 constexpr int cached_waves(int d) { return d == 256 ? 4 : 8; }
 constexpr int kCachedGroups = 256;                 // workgroups: one per CU
+// Units of a sequence up to which each has a workgroup (1,000 tokens, 4 rows of 256: 13.4 us against 14.5
+// shared out; with 576 workgroups, most of them without tokens, 17.0 against 13.6).
+constexpr int kDirectUnits = 8;
 constexpr float kStart = -1e30f;                   // running maximum before the first key
 constexpr float kSlack = 8.f;                      // scores may pass the running maximum by 2^8
 constexpr float kLog2e = 1.4426950408889634f;
 
-// The tokens of all sequences as one row of units (a tile for every wave), which the workers of a
-// kv head share evenly: worker w of n has units [w U / n, (w + 1) U / n).
-// A worker's part of sequence s is partial w + s (one of them grows at each step).
+// The work in units of a tile for every wave.  Either (few units: `direct`) a workgroup for each unit of
+// each sequence that the page table has room for, which knows its place without the lengths, so that
+// lengths, page table and queries come in one round trip, not three; a unit's part of sequence s is partial
+// s * direct + unit.  Or the tokens of all sequences are one row of units, which the workers of a kv head
+// share evenly: worker w of n has units [w U / n, (w + 1) U / n), and its part of sequence s is partial
+// w + s (one of them grows at each step).
 template <int UNIT>
 struct Share {
     const int32_t *lens;
@@ -56,14 +62,26 @@ __device__ __forceinline__ int wave_scan(int v, int lane, int n) {  // inclusive
     }
     return v;
 }
+// all sequences' units, and those of the longest
 template <typename S>
-__device__ __forceinline__ long total_units(const S &sh, int lane) {
+__device__ __forceinline__ long total_units(const S &sh, int lane, int &longest) {
     long all = 0;
+    longest = 0;
     for (int s0 = 0; s0 < sh.sequences; s0 += 64) {
-        const int n = sh.sequences - s0;
-        all += __builtin_amdgcn_readlane(wave_scan(sh.units(s0 + lane), lane, n), min(n, 64) - 1);
+        const int n = min(sh.sequences - s0, 64);
+        int units = sh.units(s0 + lane);
+        all += __builtin_amdgcn_readlane(wave_scan(units, lane, n), n - 1);
+        for (int d = 1; d < n; d <<= 1) units = max(units, __shfl_xor(units, d));
+        longest = max(longest, __builtin_amdgcn_readfirstlane(units));
     }
     return all;
+}
+// Units of a worker: t units take t a, and the last worker of a sequence of u units then joins u / t
+// parts of `size` elements, b size each, one round trip for eight; the sum is least at t = sqrt(u size b / a).
+// b / a = 1 / 8192 is measured: 16,000 tokens, 4 rows of 256 (125 units): t = 1, 2, 4, 8 take 50.9, 33.9, 27.7,
+// 30.1 us; 4,000 tokens: 21.9, 19.1, 20.3, 26.7; 16,000 tokens, 4 rows of 64 (63 units): 13.3, 13.0, 14.8, 19.2.
+__device__ __forceinline__ int units_each(int longest, int size) {
+    return max(1, (int)(__builtin_sqrtf((float)longest * (float)size * (1.f / 8192.f)) + 0.4f));
 }
 // the sequence that holds unit u (u < the total), and its first unit
 template <typename S>
@@ -250,7 +268,7 @@ __device__ __forceinline__ RowAt row_at(const CachedArgs &a, int s, int r, int k
 template <int D, int BITS>
 __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(CachedArgs a, void *ws,
                                                                              uint32_t *counts, const uint32_t *status,
-                                                                             int workers, size_t slots, int row_tiles) {
+                                                                             int workers, size_t slots, int row_tiles, int direct) {
     using C = Cached<D, BITS>;
     constexpr int kCachedWaves = cached_waves(D);
     constexpr int kPitch = D + 4;  // floats of a row of sums in LDS: rows in different banks
@@ -272,24 +290,50 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             if (i < kItems && r < rows) load_run8<1>(a.q.data, row_at(a, s, row0 + r, kvh, group).q + 8 * l8, a.q.vec, qx[n]);
         }
     };
-    if (a.sequences == 1) load_q(0);  // ahead of the lengths: one round trip fewer
-    const bool faulted = *status != 0;
-    const Share<kTile * kCachedWaves> sh{a.kv_lens, (long)a.table_stride * a.l.page_tokens, a.sequences};
-    const long all = total_units(sh, lane);
-    const long active = workers < all ? workers : all;
+    constexpr int kUnit = kTile * kCachedWaves;
+    const Share<kUnit> sh{a.kv_lens, (long)a.table_stride * a.l.page_tokens, a.sequences};
+    // Lane i's 16-token piece: piece i of the next 64 of this wave, whose tiles are tile0, tile0 + waves, ..
+    const int32_t *table = nullptr;
+    int page = 0, in_page = 0, id = 0;
+    auto look_up = [&](int s, int tile0) {  // asks for its page; table places beyond the last are the last
+        table = a.page_table + (size_t)s * a.table_stride;
+        const int piece = (tile0 + (lane >> 1) * kCachedWaves) * 2 + (lane & 1), per = a.l.page_tokens / 16;
+        page = piece / per;
+        in_page = (piece - page * per) * 16;
+        id = table[min(page, (int)a.table_stride - 1)];
+    };
+    int s = 0;
+    long unit, last, first = 0, all = 0, active = 0;
     const long w = blockIdx.x;
-    // sequences without tokens have no units: their rows are zero
-    for (int s = (int)w; s < a.sequences; s += workers) {
-        if (sh.units(s)) continue;
+    if (direct) {
+        s = blockIdx.x / (unsigned)direct;
+        unit = blockIdx.x - (unsigned)(s * direct);
+        last = unit + 1;
+        load_q(s);
+        look_up(s, (int)unit * kCachedWaves + wave);
+    }
+    const bool faulted = *status != 0;
+    auto zero_rows = [&](int s) {  // a sequence without tokens has no units: its rows are zero
         const float zero[8] = {};
         for (int i = tid; i < rows * (D / 8); i += kThreads)
             store_run8<1>(a.out.data, row_at(a, s, row0 + i / (D / 8), kvh, group).out + 8 * (i % (D / 8)), a.out.vec, zero);
+    };
+    if (direct) {
+        const int units = sh.units(s);
+        if (unit == 0 && !units) zero_rows(s);
+        if (unit >= units) return;
+    } else {
+        int longest;
+        all = total_units(sh, lane, longest);
+        const int each = units_each(longest, rows * D);
+        active = min((long)workers, (all + each - 1) / each);
+        for (int z = (int)w; z < a.sequences; z += workers)
+            if (!sh.units(z)) zero_rows(z);
+        if (w >= active) return;
+        unit = mul_div(w, all, active);
+        last = mul_div(w + 1, all, active);
+        s = find_unit(sh, unit, lane, first);
     }
-    if (w >= active) return;
-    long unit = mul_div(w, all, active);
-    const long last = mul_div(w + 1, all, active);
-    long first;
-    int s = find_unit(sh, unit, lane, first);
     // the worker that holds unit u: the last w with w all / active <= u
     auto worker_of = [&](long u) {
         const long n = (u + 1) * active - 1;
@@ -310,50 +354,40 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
         // the first tile is on its way while the queries are prepared
         const int tile_end = (int)((long)u1 * kCachedWaves < (len + kTile - 1) / kTile ? u1 * kCachedWaves
                                                                                       : (len + kTile - 1) / kTile);
-        const int32_t *table = a.page_table + (size_t)s * a.table_stride;
         const int halves = (len + 15) / 16;  // 16-token pieces that hold tokens
 
-        // lane i holds where the 16-token piece i of the next 64 is: byte offset of its head region, place in
-        // the page, and whether its table entry is outside the cache
+        // where lane i's piece is: byte offset of its head region, place in the page, and whether its table entry
+        // is outside the cache
         uint32_t at_lo = 0, at_hi = 0, place = 0;
         typename C::Half cur[2], nxt[2];
         bool bad_cur[2] = {false, false}, bad_nxt[2] = {false, false};
-        int piece0 = -64;
-        auto fetch = [&](int tile, int piece_base, typename C::Half (&h)[2], bool (&bad)[2]) {
+        int tile0 = u0 * kCachedWaves + wave;
+        auto places = [&] {
+            const bool on = (tile0 + (lane >> 1) * kCachedWaves) * 2 + (lane & 1) < halves;
+            const bool in = id >= 0 && (size_t)id < a.page_count;
+            const uint64_t off = (on && in ? (uint64_t)id * a.l.page_bytes : 0) + (uint64_t)kvh * a.l.region;
+            at_lo = (uint32_t)off;
+            at_hi = (uint32_t)(off >> 32);
+            place = on ? (in ? in_page : 0x80000000u) : 0;  // none: the first piece of the first page, masked below
+        };
+        auto fetch = [&](int tile, typename C::Half (&h)[2], bool (&bad)[2]) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int at = (tile - piece_base) / kCachedWaves * 2 + i;
+                const int at = (tile - tile0) / kCachedWaves * 2 + i;
                 const uint32_t lo = __builtin_amdgcn_readlane(at_lo, at), hi = __builtin_amdgcn_readlane(at_hi, at);
                 const uint32_t pl = __builtin_amdgcn_readlane(place, at);
                 bad[i] = pl >> 31;
                 C::load(a.pages + (((uint64_t)hi << 32) | lo), (int)(pl & 0x7fffffffu), a.l, m, g, h[i]);
             }
         };
-        // this wave's tiles are tile0, tile0 + 4, ..; the table is looked up for 32 of them at once
-        auto look_up = [&](int tile0) {
-            const int tile = tile0 + (lane >> 1) * kCachedWaves, piece = tile * 2 + (lane & 1);
-            uint64_t off = 0;
-            uint32_t pl = 0;
-            if (piece < halves) {
-                const int tok = piece * 16, page = tok / a.l.page_tokens;
-                const int id = table[page];
-                pl = tok - page * a.l.page_tokens;
-                if (id >= 0 && (size_t)id < a.page_count) off = (uint64_t)id * a.l.page_bytes;
-                else pl |= 0x80000000u;
-            }
-            off += (uint64_t)kvh * a.l.region;
-            at_lo = (uint32_t)off;
-            at_hi = (uint32_t)(off >> 32);
-            place = pl;
-        };
-        const int tile_first = u0 * kCachedWaves + wave;
+        const int tile_first = tile0;
         if (tile_first < tile_end) {
-            piece0 = tile_first;
-            look_up(piece0);
-            fetch(tile_first, piece0, nxt, bad_nxt);
+            if (!direct) look_up(s, tile0);
+            places();
+            fetch(tile_first, nxt, bad_nxt);
         }
         // queries: rotated, split in two fp16 parts
-        if (a.sequences != 1) load_q(s);
+        if (!direct) load_q(s);
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < kEach; ++n) {
@@ -391,11 +425,12 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             }
             const int ahead = tile + kCachedWaves;
             if (ahead < tile_end) {
-                if (ahead - piece0 >= 32 * kCachedWaves) {
-                    piece0 = ahead;
-                    look_up(piece0);
+                if (ahead - tile0 >= 32 * kCachedWaves) {
+                    tile0 = ahead;
+                    look_up(s, tile0);
+                    places();
                 }
-                fetch(ahead, piece0, nxt, bad_nxt);
+                fetch(ahead, nxt, bad_nxt);
             }
             const int n0 = tile * kTile;
             const bool edge = n0 + kTile > len - (a.q_len - 1);  // some row does not see all of the tile
@@ -506,8 +541,10 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
         // The whole sequence, or a part of it: then the worker that stores the last of the parts sums them, in
         // the workers' order whichever it is.  A part's stores have reached device scope (vmcnt) before its
         // arrival is counted; the count is left zero.
-        const long w0 = worker_of(first), w1 = worker_of(first + units - 1);
+        const long w0 = direct ? 0 : worker_of(first), w1 = direct ? units - 1 : worker_of(first + units - 1);
         const bool whole_sequence = w0 == w1;
+        const size_t part0 = direct ? (size_t)s * direct : (size_t)s;  // partial of worker 0
+        const long me = direct ? unit : w;
         auto finish = [&](int r, int l8, float (&v)[8], float total) {
             const bool sees = len > a.q_len - 1 - (row0 + r) / group;
             const float inv = faulted ? __builtin_nanf("") : 1.0f / total;
@@ -534,7 +571,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             if (whole_sequence || faulted) {
                 finish(r, l8, v, total);
             } else {
-                const size_t at = (size_t)(w + s) * rows + r;
+                const size_t at = (part0 + me) * rows + r;
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) put_pair(parts.sums + at * (D / 2) + 4 * l8 + e / 2, v[e], v[e + 1]);
                 if (l8 == 0) put_pair(parts.stats + at, peak, total);
@@ -549,62 +586,68 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             __syncthreads();
             if (arrived == (int)(w1 - w0)) {
                 if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                // pairs of elements; thread groups take every split-th part, 16 of them in flight
-                const int items = rows * (D / 2), lanes = items < kThreads ? items : kThreads, split = kThreads / lanes;
+                // four elements each; thread groups take every split-th part, eight of them in flight
+                const int items = rows * (D / 4), lanes = items < kThreads ? items : kThreads, split = kThreads / lanes;
                 const int grp = tid / lanes;
                 for (int i0 = 0; i0 < items; i0 += lanes) {
-                    const int i = i0 + tid - grp * lanes, r = i / (D / 2);
-                    float v0 = 0.f, v1 = 0.f, peak = kStart, total = 0.f;
+                    const int i = i0 + tid - grp * lanes, r = i / (D / 4);
+                    f4 v = {0.f, 0.f, 0.f, 0.f};
+                    float peak = kStart, total = 0.f;
                     if (i < items && grp < split) {
-                        for (long k = w0 + grp; k <= w1; k += 16 * split) {
-                            float x0[16], x1[16], px[16], tx[16];
+                        for (long k = w0 + grp; k <= w1; k += 8 * split) {
+                            f4 x[8];
+                            float px[8], tx[8];
 #pragma unroll
-                            for (int n = 0; n < 16; ++n) {
-                                const long kn = k + n * split < w1 ? k + n * split : w1;
-                                const size_t at = (size_t)(kn + s) * rows;
-                                take_pair(parts.stats + at + r, px[n], tx[n]);
-                                take_pair(parts.sums + at * (D / 2) + i, x0[n], x1[n]);
+                            for (int n = 0; n < 8; ++n) {
+                                x[n] = (f4){0.f, 0.f, 0.f, 0.f};
+                                px[n] = kStart;
+                                tx[n] = 0.f;
+                                if (k + n * split <= w1) {
+                                    const size_t at = (part0 + k + n * split) * rows;
+                                    float e[4];
+                                    take_pair(parts.stats + at + r, px[n], tx[n]);
+                                    take_pair(parts.sums + at * (D / 2) + 2 * i, e[0], e[1]);
+                                    take_pair(parts.sums + at * (D / 2) + 2 * i + 1, e[2], e[3]);
+                                    x[n] = (f4){e[0], e[1], e[2], e[3]};
+                                }
                             }
                             float now = peak;
 #pragma unroll
-                            for (int n = 0; n < 16; ++n) now = fmaxf(now, px[n]);
+                            for (int n = 0; n < 8; ++n) now = fmaxf(now, px[n]);
                             const float f = __builtin_amdgcn_exp2f(peak - now);
-                            v0 *= f;
-                            v1 *= f;
+                            v *= f;
                             total *= f;
                             peak = now;
 #pragma unroll
-                            for (int n = 0; n < 16; ++n) {
-                                const float g_ = __builtin_amdgcn_exp2f(px[n] - now);
-                                if (k + n * split <= w1) {
-                                    v0 = __builtin_fmaf(x0[n], g_, v0);
-                                    v1 = __builtin_fmaf(x1[n], g_, v1);
-                                    total = __builtin_fmaf(tx[n], g_, total);
-                                }
+                            for (int n = 0; n < 8; ++n) {
+                                const float f1 = __builtin_amdgcn_exp2f(px[n] - now);
+                                v += x[n] * f1;
+                                total += tx[n] * f1;
                             }
                         }
                     }
                     if (split > 1) {
-                        f4 *const mine = (f4 *)lds + tid;
-                        *mine = (f4){v0, v1, peak, total};
+                        f4 *const sums = (f4 *)lds;
+                        float *const stats = lds + 4 * kThreads;
+                        sums[tid] = v;
+                        stats[2 * tid] = peak;
+                        stats[2 * tid + 1] = total;
                         __syncthreads();
                         if (grp == 0) {
                             for (int k = 1; k < split; ++k) {
-                                const f4 x = ((f4 *)lds)[k * lanes + tid];
-                                const float now = fmaxf(peak, x[2]);
-                                const float f0 = __builtin_amdgcn_exp2f(peak - now), f1 = __builtin_amdgcn_exp2f(x[2] - now);
+                                const int at = k * lanes + tid;
+                                const float now = fmaxf(peak, stats[2 * at]);
+                                const float f0 = __builtin_amdgcn_exp2f(peak - now), f1 = __builtin_amdgcn_exp2f(stats[2 * at] - now);
                                 peak = now;
-                                v0 = v0 * f0 + x[0] * f1;
-                                v1 = v1 * f0 + x[1] * f1;
-                                total = total * f0 + x[3] * f1;
+                                v = v * f0 + sums[at] * f1;
+                                total = total * f0 + stats[2 * at + 1] * f1;
                             }
                         }
                         __syncthreads();
                     }
                     if (i < items && grp == 0) {
-                        lds[2 * i] = v0;
-                        lds[2 * i + 1] = v1;
-                        if (i % (D / 2) == 0) stat[r] = total;
+                        ((f4 *)lds)[i] = v;
+                        if (i % (D / 4) == 0) stat[r] = total;
                     }
                 }
                 __syncthreads();
@@ -640,13 +683,18 @@ CachedPlan cached_plan(size_t q_heads, size_t kv_heads, size_t sequences, size_t
 template <int D>
 hipError_t launch_d(const CachedArgs &a, void *workspace, hipStream_t stream) {
     const CachedPlan p = cached_plan(a.q.heads, a.l.kv_heads, a.sequences, a.q_len);
-    const dim3 grid(p.workers, a.l.kv_heads * p.row_tiles);
+    const size_t tiles = (size_t)a.l.kv_heads * p.row_tiles, unit = (size_t)kTile * cached_waves(D);
+    const size_t units = (a.table_stride * a.l.page_tokens + unit - 1) / unit;
+    const int direct = units <= (size_t)kDirectUnits && units * a.sequences <= (size_t)p.workers ? (int)units : 0;
+    const dim3 grid(direct ? direct * a.sequences : p.workers, (unsigned)tiles);
     void *ws = (uint8_t *)workspace + kSharedPrefixBytes;
     uint32_t *counts = (uint32_t *)workspace, *status = (uint32_t *)((uint8_t *)workspace + kStatusOffset);
     if (a.l.bits == 4)
-        attention_cached_kernel<D, 4><<<grid, 64 * cached_waves(D), 0, stream>>>(a, ws, counts, status, p.workers, p.slots, p.row_tiles);
+        attention_cached_kernel<D, 4><<<grid, 64 * cached_waves(D), 0, stream>>>(a, ws, counts, status, p.workers, p.slots,
+                                                                                 p.row_tiles, direct);
     else
-        attention_cached_kernel<D, 8><<<grid, 64 * cached_waves(D), 0, stream>>>(a, ws, counts, status, p.workers, p.slots, p.row_tiles);
+        attention_cached_kernel<D, 8><<<grid, 64 * cached_waves(D), 0, stream>>>(a, ws, counts, status, p.workers, p.slots,
+                                                                                 p.row_tiles, direct);
     return hipGetLastError();
 }
 
