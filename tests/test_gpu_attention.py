@@ -252,6 +252,47 @@ def test_cached_long(amd, bits):
     assert np.all(np.abs(got - want) <= bound)
 
 
+@pytest.mark.parametrize("sigma,scale", [(30.0, None), (0.01, None), (1.0, -0.2), (1.0, 0.0), (8.0, 1.0)])
+def test_cached_score_ranges(amd, sigma, scale):
+    """scores from almost equal to hundreds apart, a negative scale and a zero one"""
+    lens, hq, hk, d, bits, p = [300, 45], 4, 2, 128, 4, 16
+    pages, table, kept = make_cache(amd, lens, hk, d, bits, p)
+    q = rows(170, 2 * 3, hq, d, sigma=sigma)
+    want, bound = cached_reference(q, kept, 3, hk, d ** -0.5 if scale is None else scale)
+    got = run_cached(amd, q, pages, table, lens, hk, bits, p, 3, scale=scale).astype(np.float64)
+    assert np.all(np.abs(got - want) <= bound)
+
+
+@pytest.mark.parametrize("bits,d", [(4, 64), (4, 128), (4, 256), (8, 128)])
+def test_cached_non_finite_tokens(amd, bits, d):
+    """a new token whose keys or values are not finite reaches the rows that see it, and only those"""
+    lens, hq, hk, p, q_len = [70, 129], 4, 2, 16, 4
+    pages, table, kept = make_cache(amd, lens, hk, d, bits, p)
+    import torch
+    q = rows(180, 2 * q_len, hq, d)
+    clean = run_cached(amd, q, pages, table, lens, hk, bits, p, q_len)
+    for which in ("k", "v"):
+        for back in (0, 1, 3):  # tokens from the end of sequence 1: token j of q_len sees it when j >= q_len - 1 - back
+            dirty = pages.clone()
+            at = lens[1] - 1 - back
+            slot = int(table[1, at // p]) * p + at % p
+            k, v = amd.kv_cache_read(pages, torch.tensor([slot], device="cuda"), hk, d, bits=bits, page_tokens=p)
+            (k if which == "k" else v)[0, 1, 5] = float("nan")
+            amd.kv_cache_write(dirty, k, v, torch.tensor([slot], device="cuda"), bits=bits, page_tokens=p)
+            got = run_cached(amd, q, dirty, table, lens, hk, bits, p, q_len)
+            per = hq // hk
+            assert np.array_equal(got[:q_len], clean[:q_len])
+            rest = got[q_len:]
+            sees = np.arange(q_len) >= q_len - 1 - back
+            bad = np.isnan(rest[:, per:])  # the q heads of kv head 1
+            if which == "k":
+                assert bad[sees].all()
+            else:
+                assert bad[sees][:, :, :32].all() and not bad[sees][:, :, 32:].any()
+            assert not np.isnan(rest[~sees]).any() and not np.isnan(rest[:, :per]).any()
+            assert np.array_equal(rest[~sees][:, per:], clean[q_len:][~sees][:, per:])
+
+
 def test_cached_workspaces_streams_and_repeats(amd):
     """the caller's workspace (which mul_mat may share), the internal one, another stream: the same bits"""
     import torch

@@ -122,19 +122,25 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[N]) {
     }
 }
 
-// Two 4-bit codes in the low halves' bits 0..3, or 4..7, as fp16 values -8 .. 7: or-ing them into
-// 1024 (spacing 1) or 1024 at spacing 16 gives 1024 + c and 1024 + 16 c exactly.
-__device__ __forceinline__ h2 low_codes(uint32_t w) {
-    const h2 t = bitcast<h2>((w & 0x000f000fu) | 0x64006400u);
-    return t + (h2){(_Float16)-1032.f, (_Float16)-1032.f};
+// The masks and the 1024 (0x6400) that codes are or-ed into, in registers: a v_and_or_b32 takes no literals, so
+// with constants each is a v_and and a v_or.
+struct Masks {
+    uint32_t low, high, base;  // scalar, scalar, vector
+    __device__ __forceinline__ Masks() : low(0x000f000fu), high(0x00f000f0u), base(0x64006400u) {
+        asm volatile("" : "+s"(low), "+s"(high), "+v"(base));
+    }
+};
+// Two 4-bit codes in the halves' bits 0..3, or 4..7, as fp16 values -8 .. 7: in 1024 (spacing 1) they give
+// 1024 + c and 1024 + 16 c exactly.
+__device__ __forceinline__ h2 low_codes(uint32_t w, const Masks &k) {
+    return bitcast<h2>((w & k.low) | k.base) + (h2){(_Float16)-1032.f, (_Float16)-1032.f};
 }
-__device__ __forceinline__ h2 high_codes(uint32_t w) {
-    const h2 t = bitcast<h2>((w & 0x00f000f0u) | 0x64006400u);
-    return __builtin_elementwise_fma(t, (h2){(_Float16)0.0625f, (_Float16)0.0625f},
+__device__ __forceinline__ h2 high_codes(uint32_t w, const Masks &k) {
+    return __builtin_elementwise_fma(bitcast<h2>((w & k.high) | k.base), (h2){(_Float16)0.0625f, (_Float16)0.0625f},
                                      (h2){(_Float16)-72.f, (_Float16)-72.f});
 }
-__device__ __forceinline__ h2 byte_codes(uint32_t w) {  // 8 bits: -128 .. 127
-    return bitcast<h2>(w | 0x64006400u) + (h2){(_Float16)-1152.f, (_Float16)-1152.f};
+__device__ __forceinline__ h2 byte_codes(uint32_t w, const Masks &k) {  // 8 bits: -128 .. 127
+    return bitcast<h2>(w | k.base) + (h2){(_Float16)-1152.f, (_Float16)-1152.f};
 }
 
 template <int D, int BITS>
@@ -150,33 +156,42 @@ struct Cached {
         u2 vs;
     };
 
-    // base: the head's region of the page; off: the first token's place in it
-    static __device__ __forceinline__ void load(const uint8_t *base, int off, const KvLayout &l, int m, int g, Half &h) {
-        load_words<NW>(base + (size_t)(off + m) * RUN + g * (RUN / 4), h.k);
-        load_words<NW>(base + l.v_off + (size_t)((off >> 2) + g) * (4 * RUN) + m * (RUN / 4), h.v);
-        const uint8_t *ks = base + l.ks_off + (size_t)(off + m) * (2 * G);
-        if constexpr (G == 8) h.ks = *(const uint32_t *)(ks + 4 * g);
-        else h.ks = *(const uint16_t *)(ks + 2 * (G == 4 ? g : g >> 1));
-        h.vs = *(const u2 *)(base + l.vs_off + (size_t)((off >> 2) + g) * (8 * G) + 8 * (m * G / 16));
+    // A lane's places in 16 tokens, the same for all of them: the rest of an address is scalar.
+    struct Lane {
+        uint32_t k, v, ks, vs;
+    };
+    static __device__ __forceinline__ Lane lane_of(int m, int g) {
+        return {(uint32_t)(m * RUN + g * (RUN / 4)), (uint32_t)(g * (4 * RUN) + m * (RUN / 4)),
+                (uint32_t)(m * (2 * G) + (G == 8 ? 4 * g : 2 * (G == 4 ? g : g >> 1))),
+                (uint32_t)(g * (8 * G) + 8 * (m * G / 16))};
+    }
+    // base: the head's region of the page; off: the first token's place in it (a multiple of 16), both scalar
+    static __device__ __forceinline__ void load(const uint8_t *base, uint32_t off, const KvLayout &l, const Lane &at, Half &h) {
+        load_words<NW>(base + off * (uint32_t)RUN + at.k, h.k);
+        load_words<NW>(base + l.v_off + off * (uint32_t)RUN + at.v, h.v);
+        const uint8_t *ks = base + l.ks_off + off * (uint32_t)(2 * G) + at.ks;
+        if constexpr (G == 8) h.ks = *(const uint32_t *)ks;
+        else h.ks = *(const uint16_t *)ks;
+        h.vs = *(const u2 *)(base + l.vs_off + off * (uint32_t)(2 * G) + at.vs);
     }
 
     // Fragment j of a lane's key: elements 8 j .. 8 j + 7 of its quarter row, in the order that
     // q_order undoes.
-    static __device__ __forceinline__ h8 key(const Half &h, int j) {
+    static __device__ __forceinline__ h8 key(const Half &h, int j, const Masks &c) {
         const uint32_t sw = G == 8 ? (j < 4 ? h.ks & 0xffffu : h.ks >> 16) : h.ks;
         const _Float16 s = bitcast<_Float16>((uint16_t)sw);
         const h2 s2 = {s, s};
         h2 p[4];
         if constexpr (BITS == 4) {
             const uint32_t w = h.k[j], w8 = w >> 8;
-            p[0] = low_codes(w);
-            p[1] = high_codes(w);
-            p[2] = low_codes(w8);
-            p[3] = high_codes(w8);
+            p[0] = low_codes(w, c);
+            p[1] = high_codes(w, c);
+            p[2] = low_codes(w8, c);
+            p[3] = high_codes(w8, c);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                p[i] = byte_codes(__builtin_amdgcn_perm(0u, h.k[2 * j + i / 2], i & 1 ? 0x0c030c02u : 0x0c010c00u));
+                p[i] = byte_codes(__builtin_amdgcn_perm(0u, h.k[2 * j + i / 2], i & 1 ? 0x0c030c02u : 0x0c010c00u), c);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[i] = p[i] * s2;
@@ -189,12 +204,12 @@ struct Cached {
     }
 
     // element t of the lane's slice for its four tokens (as two pairs)
-    static __device__ __forceinline__ void value(const Half &h, int t, h2 &a, h2 &b) {
+    static __device__ __forceinline__ void value(const Half &h, int t, h2 &a, h2 &b, const Masks &c) {
         const h2 s01 = bitcast<h2>(h.vs.x), s23 = bitcast<h2>(h.vs.y);
         if constexpr (D == 64 && BITS == 4) {  // 2-byte slices: a word holds two tokens
             const uint32_t x = t < 2 ? h.v[0] : h.v[0] >> 8, y = t < 2 ? h.v[1] : h.v[1] >> 8;
-            a = (t & 1) ? high_codes(x) : low_codes(x);
-            b = (t & 1) ? high_codes(y) : low_codes(y);
+            a = (t & 1) ? high_codes(x, c) : low_codes(x, c);
+            b = (t & 1) ? high_codes(y, c) : low_codes(y, c);
         } else {
             constexpr int PW = NW / 4;  // words of a token's slice
             const int byte = BITS == 4 ? (t / 2) % 4 : t % 4, word = BITS == 4 ? t / 8 : t / 4;
@@ -202,11 +217,11 @@ struct Cached {
             const uint32_t x = __builtin_amdgcn_perm(h.v[PW + word], h.v[word], sel);
             const uint32_t y = __builtin_amdgcn_perm(h.v[3 * PW + word], h.v[2 * PW + word], sel);
             if constexpr (BITS == 4) {
-                a = (t & 1) ? high_codes(x) : low_codes(x);
-                b = (t & 1) ? high_codes(y) : low_codes(y);
+                a = (t & 1) ? high_codes(x, c) : low_codes(x, c);
+                b = (t & 1) ? high_codes(y, c) : low_codes(y, c);
             } else {
-                a = byte_codes(x);
-                b = byte_codes(y);
+                a = byte_codes(x, c);
+                b = byte_codes(y, c);
             }
         }
         a = a * s01;
@@ -342,7 +357,11 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
     const Parts parts = parts_of(ws, D, rows, slots, blockIdx.y);
     _Float16 *const qhi = (_Float16 *)lds, *const qlo = qhi + kRows * D;
     float *const stat = lds + kCachedWaves * kRows * kPitch;  // (maximum, sum) of [wave][row]
-    const float c = a.scale * kLog2e;
+    // the largest score is that of the largest product: a negative scale goes into the queries' signs (and 0 *
+    // -infinity, the masked places of a zero scale, must stay -infinity)
+    const float c = fmaxf(__builtin_fabsf(a.scale) * kLog2e, 1e-30f), sign = a.scale < 0.f ? -1.f : 1.f;
+    const Masks masks;
+    const typename C::Lane at_lane = C::lane_of(m, g);
 
     while (unit < last && s < a.sequences) {  // one sequence's part at a time
         const int len = sh.len(s), units = sh.units(s);
@@ -377,7 +396,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
                 const uint32_t lo = __builtin_amdgcn_readlane(at_lo, at), hi = __builtin_amdgcn_readlane(at_hi, at);
                 const uint32_t pl = __builtin_amdgcn_readlane(place, at);
                 bad[i] = pl >> 31;
-                C::load(a.pages + (((uint64_t)hi << 32) | lo), (int)(pl & 0x7fffffffu), a.l, m, g, h[i]);
+                C::load(a.pages + (((uint64_t)hi << 32) | lo), pl & 0x7fffffffu, a.l, at_lane, h[i]);
             }
         };
         const int tile_first = tile0;
@@ -397,6 +416,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             h8 hi, lo;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
+                qx[n][e] *= sign;
                 hi[e] = (_Float16)qx[n][e];
                 lo[e] = (_Float16)(qx[n][e] - (float)hi[e]);
             }
@@ -459,14 +479,14 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
                 st[i] = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < C::NJ; ++j) {
-                    const h8 k = C::key(cur[i], j);
+                    const h8 k = C::key(cur[i], j, masks);
                     st[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, bl[j], st[i], 0, 0, 0);
                     st[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, bh[j], st[i], 0, 0, 0);
                 }
             }
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = st[e >> 2][e & 3] * c;
+            for (int e = 0; e < 8; ++e) x[e] = st[e >> 2][e & 3];
             if (edge) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -475,6 +495,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             float best = x[0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) best = fmaxf(best, x[e]);
+            best *= c;
             if (__ballot(best > top + kSlack)) {
                 const float now = fmaxf(top, over_groups_max(best));
                 const float keep = __builtin_amdgcn_exp2f(top - now);
@@ -488,15 +509,15 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             h8 p;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float v = __builtin_amdgcn_exp2f(x[e] - top);
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c, -top));
                 sum += v;
                 p[e] = (_Float16)v;
             }
 #pragma unroll
             for (int t = 0; t < C::NT; ++t) {
                 h2 v[4];
-                C::value(cur[0], t, v[0], v[1]);
-                C::value(cur[1], t, v[2], v[3]);
+                C::value(cur[0], t, v[0], v[1], masks);
+                C::value(cur[1], t, v[2], v[3], masks);
                 const h8 vt = {v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
                 o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, p, o[t], 0, 0, 0);
             }
