@@ -479,13 +479,20 @@ size_t exl3_hip_attention_cached_workspace_bytes(size_t q_heads, size_t kv_heads
  * multiple of kv heads.  q_tokens and kv_tokens are the rows of the views (no row
  * outside them is read or written, whatever the starts hold; a query row that no
  * sequence has is not written).  Scores, softmax statistics and sums in fp32, weights
- * rounded to fp16.  The same inputs give the same bits on every call.  EXL3_NO_SUPPORT
- * where (q_tokens / 128 + sequences) * q heads reaches 2^23.  sequences = 0 or q_tokens = 0
+ * rounded to fp16.  The same inputs give the same bits on every call.
+ *   workspace   device, 256-byte aligned, >= exl3_hip_attention_prompt_workspace_bytes() where that
+ *               is not 0 (few query rows over many keys: parts of the walk are joined there); it may
+ *               be one that other calls use too.  NULL: the internal one of this stream
+ * EXL3_NO_SUPPORT where (q_tokens / 128 + sequences) * q heads reaches 2^23.  sequences = 0 or q_tokens = 0
  * is a no-op. */
 exl3_status exl3_hip_attention_prompt(const exl3_head_view *q, const exl3_head_view *k, const exl3_head_view *v,
                                       const exl3_head_view *out, size_t head_dim, const int32_t *q_starts,
                                       const int32_t *kv_starts, size_t sequences, size_t q_tokens, size_t kv_tokens,
-                                      float scale, int causal, hipStream_t stream);
+                                      float scale, int causal, void *workspace, size_t workspace_bytes,
+                                      hipStream_t stream);
+/* 0 where exl3_hip_attention_prompt takes no workspace (and for arguments that it refuses) */
+size_t exl3_hip_attention_prompt_workspace_bytes(size_t q_heads, size_t head_dim, size_t sequences, size_t q_tokens,
+                                                 size_t kv_tokens);
 
 /* *result (device int) = 1 when every su/sv value of every record is finite,
  * 0 otherwise; EXL3_INVAL_PARAMS when nbytes is not a whole number of records. */

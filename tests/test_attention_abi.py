@@ -113,11 +113,11 @@ def test_cached_refusals(L):
 
 
 def call_prompt(L, q=None, k=None, v=None, out=None, **kw):
-    a = dict(d=128, qs=P, ks=P, seqs=1, nq=3, nk=3)
+    a = dict(d=128, qs=P, ks=P, seqs=1, nq=3, nk=3, ws=None, wb=0)
     a.update(kw)
     return L.exl3_hip_attention_prompt(ctypes.byref(q or view()), ctypes.byref(k or view(heads=1)),
                                        ctypes.byref(v or view(heads=1)), ctypes.byref(out or view(Q)), a["d"], a["qs"],
-                                       a["ks"], a["seqs"], a["nq"], a["nk"], 0.1, 1, None)
+                                       a["ks"], a["seqs"], a["nq"], a["nk"], 0.1, 1, a["ws"], a["wb"], None)
 
 
 def test_prompt_refusals(L):
@@ -131,3 +131,15 @@ def test_prompt_refusals(L):
     assert call_prompt(L, out=view(Q, heads=1)) == INVAL
     assert call_prompt(L, out=view(Q, token=200)) == INVAL
     assert call_prompt(L, q=view(P + 1)) == INVAL
+
+
+def test_prompt_workspace(L):
+    size = L.exl3_hip_attention_prompt_workspace_bytes
+    need = size(2, 128, 1, 3, 4000)
+    assert need > 0
+    assert call_prompt(L, nk=4000, ws=P, wb=need - 1) == 3
+    assert call_prompt(L, nk=4000, ws=P + 1, wb=need) == INVAL
+    # none: short walks, workgroups enough, refused arguments
+    for none in ((2, 128, 1, 3, 300), (32, 128, 1, 8192, 8192), (2, 128, 0, 3, 4000), (2, 128, 1, 0, 4000),
+                 (2, 96, 1, 3, 4000), (0, 128, 1, 3, 4000)):
+        assert size(*none) == 0, none

@@ -80,6 +80,66 @@ def test_prompt_matches_formula(amd, case):
     assert np.all(np.abs(got - want) <= bound), float((np.abs(got - want) / np.maximum(bound, 1e-30)).max())
 
 
+LONG = [  # a few rows over many keys: parts of a walk go to several workgroups
+    ([1], [2000], 2, 1, 64, True),
+    ([20], [1281], 4, 1, 128, True),
+    ([130], [3001], 2, 2, 128, True),
+    ([3], [1100], 8, 2, 256, True),
+    ([257, 1], [2100, 1600], 1, 1, 256, False),
+    ([1000], [1000], 3, 1, 64, True),
+    ([700], [1025], 2, 1, 256, True),
+    ([0, 5, 40], [2500, 2500, 90], 2, 2, 128, True),
+    ([50, 200], [5000, 0], 2, 1, 64, False),
+    ([1300, 9], [900, 2400], 1, 1, 128, True),  # the first rows see nothing
+]
+
+
+@pytest.mark.parametrize("case", LONG, ids=lambda c: f"{sum(c[0])}x{sum(c[1])}s{len(c[0])}h{c[2]}-{c[3]}d{c[4]}c{int(c[5])}")
+def test_prompt_in_parts(amd, case):
+    """against the formula; with a workspace of its own and again the bits are the same"""
+    lq, lk, hq, hk, d, causal = case
+    print("  attention_prompt in parts", case, flush=True)
+    qs, ks = starts(lq), starts(lk)
+    nbytes = amd.attention_prompt_workspace_bytes(hq, d, len(lq), qs[-1], ks[-1])
+    assert nbytes > 0
+    q, k, v = rows(75, qs[-1], hq, d, sigma=2.0), rows(76, ks[-1], hk, d), rows(77, ks[-1], hk, d)
+    want, bound, _ = prompt_reference(q, k, v, qs, ks, causal, d ** -0.5)
+    got = run_prompt(amd, q, k, v, qs, ks, causal)
+    assert np.isfinite(got).all()
+    assert np.all(np.abs(got.astype(np.float64) - want) <= bound)
+    ws = amd.new_workspace(128, 128, 1, nbytes=nbytes)
+    ws[-4096:] = 0xff  # what it held does not matter
+    assert np.array_equal(got, run_prompt(amd, q, k, v, qs, ks, causal, workspace=ws))
+    assert np.array_equal(got, run_prompt(amd, q, k, v, qs, ks, causal))
+    with pytest.raises(amd.Exl3Error):
+        run_prompt(amd, q, k, v, qs, ks, causal, workspace=ws[:nbytes - 256])
+
+
+def test_prompt_in_parts_ranges(amd):
+    """scores that rise or fall with the keys, so that parts differ by hundreds, and a NaN that only the last rows see"""
+    n, pre, d = 70, 1900, 64
+    qs, ks = [0, n], [0, n + pre]
+    ramp = (np.arange(n + pre) * 0.01).astype(np.float16)
+    v = rows(78, n + pre, 1, d)
+    for k_of in (ramp, ramp[::-1]):
+        q, k = np.ones((n, 1, d), np.float16), np.zeros((n + pre, 1, d), np.float16)
+        k[:, 0, :] = k_of[:, None]
+        want, bound, _ = prompt_reference(q, k, v, qs, ks, True, 1.0)
+        got = run_prompt(amd, q, k, v, qs, ks, True, 1.0).astype(np.float64)
+        assert np.all(np.abs(got - want) <= bound)
+    clean = run_prompt(amd, q, k, v, qs, ks, True)
+    for bad, column in ((np.nan, 5), (np.inf, 60)):
+        v2, k2 = v.copy(), k.copy()
+        v2[-20, 0, column] = bad  # seen by the last 20 rows
+        got = run_prompt(amd, q, k2, v2, qs, ks, True)
+        assert np.array_equal(got[:-20], clean[:-20]) and not np.isfinite(got[-20:, 0, column]).any()
+        others = np.arange(d) != column
+        assert np.array_equal(got[-20:, 0, others], clean[-20:, 0, others])
+        k2[-20, 0, column] = np.nan
+        got = run_prompt(amd, q, k2, v, qs, ks, True)
+        assert np.array_equal(got[:-20], clean[:-20]) and np.isnan(got[-20:]).all()
+
+
 @pytest.mark.parametrize("sigma,scale", [(30.0, None), (0.01, None), (1.0, -0.2), (1.0, 0.0), (8.0, 1.0)])
 def test_prompt_score_ranges(amd, sigma, scale):
     """scores from almost equal to hundreds apart, a negative scale and a zero one"""

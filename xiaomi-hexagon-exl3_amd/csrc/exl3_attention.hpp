@@ -83,6 +83,8 @@ struct PromptArgs {
     int head_dim, sequences, q_tokens, kv_tokens, causal;
     float scale;
 };
-hipError_t launch_attention_prompt(const PromptArgs &a, hipStream_t stream);
+// 0: the call takes no workspace
+size_t attention_prompt_bytes(size_t q_heads, int head_dim, int sequences, int q_tokens, int kv_tokens);
+hipError_t launch_attention_prompt(const PromptArgs &a, void *workspace, hipStream_t stream);
 
 }  // namespace exl3k

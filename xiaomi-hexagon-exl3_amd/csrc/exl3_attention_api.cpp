@@ -172,10 +172,19 @@ exl3_status exl3_hip_attention_cached(const exl3_head_view *q, const exl3_head_v
     return from_hip(exl3k::launch_attention_cached(a, workspace, stream));
 }
 
+size_t exl3_hip_attention_prompt_workspace_bytes(size_t q_heads, size_t head_dim, size_t sequences, size_t q_tokens,
+                                                 size_t kv_tokens) {
+    if (!attention_dim(head_dim) || q_heads < 1 || q_heads > kMaxHeads || sequences > kMaxSequences ||
+        q_tokens > kMaxTokens || kv_tokens > kMaxTokens || !sequences || !q_tokens)
+        return 0;
+    return exl3k::attention_prompt_bytes(q_heads, (int)head_dim, (int)sequences, (int)q_tokens, (int)kv_tokens);
+}
+
 exl3_status exl3_hip_attention_prompt(const exl3_head_view *q, const exl3_head_view *k, const exl3_head_view *v,
                                       const exl3_head_view *out, size_t head_dim, const int32_t *q_starts,
                                       const int32_t *kv_starts, size_t sequences, size_t q_tokens, size_t kv_tokens,
-                                      float scale, int causal, hipStream_t stream) {
+                                      float scale, int causal, void *workspace, size_t workspace_bytes,
+                                      hipStream_t stream) {
     if (!attention_dim(head_dim) || sequences > kMaxSequences || q_tokens > kMaxTokens || kv_tokens > kMaxTokens)
         return EXL3_INVAL_PARAMS;
     if (!sequences || !q_tokens) return EXL3_OK;
@@ -198,7 +207,12 @@ exl3_status exl3_hip_attention_prompt(const exl3_head_view *q, const exl3_head_v
     a.kv_tokens = (int)kv_tokens;
     a.causal = causal != 0;
     a.scale = scale;
-    return from_hip(exl3k::launch_attention_prompt(a, stream));
+    const size_t need = exl3k::attention_prompt_bytes(q->heads, a.head_dim, a.sequences, a.q_tokens, a.kv_tokens);
+    if (need) {
+        const exl3_status st = exl3k::take_workspace(need, stream, &workspace, &workspace_bytes);
+        if (st != EXL3_OK) return st;
+    }
+    return from_hip(exl3k::launch_attention_prompt(a, need ? workspace : nullptr, stream));
 }
 
 }  // extern "C"

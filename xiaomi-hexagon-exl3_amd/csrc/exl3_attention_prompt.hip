@@ -3,7 +3,8 @@
 // A group of four waves has 128 query rows of one head, 32 per wave, and walks its sequence's
 // keys in tiles of KT through two LDS buffers with the running maximum and sum of the softmax.
 // A workgroup has one such group, or two that take the even and the odd tiles and are joined
-// at the end. 4 D flops per query and key on mfma_f32_32x32x16_f16, which
+// at the end; few rows over many keys are walked in parts by several workgroups, which a second kernel joins.
+// 4 D flops per query and key on mfma_f32_32x32x16_f16, which
 // bounds a long prompt.  Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T: a lane's column is one
 // query row throughout, so the row's statistics and factors are one register and one exchange
 // (lanes l and l ^ 32), and S^T leaves each lane with the weights that it needs as the B
@@ -158,8 +159,36 @@ __device__ __forceinline__ bool drop_non_finite(h8 &v) {
     return found;
 }
 
-template <int D, bool NEAR, int kGroups>
-__global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prompt_kernel(PromptArgs a, int tiles) {
+// Four elements of a row, 32 t + 8 b + 4 h on, where h is the lane's half and j = 4 t + b.
+__device__ __forceinline__ void store_out(const PromptArgs &a, const Span &sp, int head, int row, int j, int h, const h4 &x) {
+    _Float16 *at = (_Float16 *)a.out.data + (size_t)(sp.q0 + row) * a.out.token_stride + head * a.out.head_stride + 8 * j + 4 * h;
+    if (a.out.vec) {
+        *(h4 *)at = x;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) at[e] = x[e];
+    }
+}
+// Workgroup b runs on XCD b % 8, each with its own L2: where the heads divide by 8, an XCD takes
+// neighbouring heads, which share keys and values (8,192 tokens, 32 / 8 heads of 128: 575 against 580 us).
+__device__ __forceinline__ int head_of(const PromptArgs &a, unsigned block) {
+    const int place = block % a.q.heads;
+    return a.q.heads % 8 ? place : place % 8 * (a.q.heads / 8) + place / 8;
+}
+// keys that row r of the sequence sees
+__device__ __forceinline__ int seen_by(const PromptArgs &a, const Span &sp, int r) {
+    const int n = a.causal ? (r < sp.nq ? r : sp.nq - 1) + sp.nk - sp.nq + 1 : sp.nk;
+    return n < 0 ? 0 : n;
+}
+// tiles of a part of a walk of `all` tiles
+__device__ __forceinline__ int part_tiles(int all, int parts) { return (all + parts - 1) / parts; }
+// floats of a part: f4 [D / 8][thread] sums, then (maximum, sum) [thread]
+template <int D>
+constexpr size_t kPartFloats = 64 * kPromptWaves * (D / 2 + 2);
+
+// SPLIT: workgroup (b, i) walks part i of the keys and leaves its sums in `ws` for attention_prompt_join_kernel.
+template <int D, bool NEAR, int kGroups, bool SPLIT>
+__global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prompt_kernel(PromptArgs a, int tiles, float *ws) {
     using P = Prompt<D>;
     constexpr int KT = P::KT;
     __shared__ __align__(1024) _Float16 keys[kGroups][2][KT * D], values[kGroups][2][KT * D];
@@ -167,10 +196,7 @@ __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prom
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * kPromptWaves));
     auto &ks = keys[group], &vs = values[group];
-    // Workgroup b runs on XCD b % 8, each with its own L2: where the heads divide by 8, an XCD takes
-    // neighbouring heads, which share keys and values (8,192 tokens, 32 / 8 heads of 128: PLACEHOLDER).
-    const int place = blockIdx.x % a.q.heads;
-    const int head = a.q.heads % 8 ? place : place % 8 * (a.q.heads / 8) + place / 8;
+    const int head = head_of(a, blockIdx.x);
     const Span sp = find_tile(a, tiles - 1 - (int)(blockIdx.x / a.q.heads), lane);  // a causal sequence's longest first
     if (!sp.nq) return;
     const int kvh = head / (a.q.heads / a.k.heads);
@@ -179,14 +205,18 @@ __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prom
 
     // keys that this lane's row, the wave's last row and the workgroup's last row see
     const int row = sp.row0 + 32 * wave + m;
-    const int shift = a.causal ? sp.nk - sp.nq + 1 : 0;
-    auto seen = [&](int r) {
-        const int n = a.causal ? (r < sp.nq ? r : sp.nq - 1) + shift : sp.nk;
-        return n < 0 ? 0 : n;
-    };
-    const int limit = seen(row);
-    const int wave_max_ = seen(sp.row0 + 32 * wave + 31);
-    const int last = seen(sp.row0 + kPromptRows - 1);
+    const int limit = seen_by(a, sp, row);
+    const int last = seen_by(a, sp, sp.row0 + kPromptRows - 1);
+    const int all = (last + KT - 1) / KT;  // tiles of the walk; this workgroup's are lo .. lo + steps - 1
+    int lo = 0, steps = all;
+    if constexpr (SPLIT) {
+        const int per = part_tiles(all, gridDim.y);
+        lo = min((int)blockIdx.y * per, all);
+        steps = min(per, all - lo);
+        if (!steps) return;
+    }
+    const int end = (lo + steps) * KT;
+    const int wave_end = min(seen_by(a, sp, sp.row0 + 32 * wave + 31), end);
     const int q_row = row < sp.nq ? row : sp.nq - 1;
     const _Float16 *qp = (const _Float16 *)a.q.data + (size_t)(sp.q0 + q_row) * a.q.token_stride + head * a.q.head_stride;
     h8 q[P::NS];
@@ -219,9 +249,8 @@ __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prom
     const int k_lane = 16 * P::k_at(m, h);
     const int li = lane & 15;
     const int v_lane = 16 * P::v_at(4 * h + (li >> 2), 2 * ((lane >> 4) & 1) + ((li & 3) >> 1)) + 8 * (li & 1);
-    const int steps = (last + KT - 1) / KT;
-    const int open = seen(sp.row0);
-    const int whole = open / KT < steps ? open / KT : steps;  // tiles without a masked place
+    // tiles of this workgroup without a masked place
+    const int whole = max(0, min(seen_by(a, sp, sp.row0) / KT - lo, steps));
 
     f16v st[KT / 32];  // a tile's scores
     h8 p[KT / 16];
@@ -277,11 +306,10 @@ __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prom
     };
     constexpr int kMfma = KT / 32 * P::NS, kPairs = KT / 4;  // MFMAs of each product, pairs of weights
     static_assert(kMfma == KT / 16 * P::NT, "both products take as many MFMAs");
-    // Step i of a group is tile 2 i + group.  It ends with the scores of step i + 1.  Its tiles (keys of
+    // Step i of a group is tile lo + 2 i + group.  It ends with the scores of step i + 1.  Its tiles (keys of
     // step i + 1, values of step i) were asked for in step i - 1; it asks for the keys of i + 2 and the values of
     // i + 1 in the buffers that step i - 1 was done with.
-    auto key_of = [&](int i) { return (i * kGroups + group) * KT; };  // a step's first key
-    const int end = steps * KT;
+    auto key_of = [&](int i) { return (lo + i * kGroups + group) * KT; };  // a step's first key
     auto next = [&](int i) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -300,7 +328,8 @@ __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prom
     for (int n = 0; n < kMfma; ++n) score(n, key_frag(k_base, n));  // without a tile: not used
     // Tiles without masked places, while the tiles to ask for have all their rows.
     const uint32_t k_at = P::template offset_in<false>(a.k, tid), v_at = P::template offset_in<true>(a.v, tid);
-    const int plain = NEAR ? min(whole / kGroups, sp.nk / (kGroups * KT) - 2) : 0;
+    // At least one step is left to the loop after: its wait ends the loads under way.
+    const int plain = NEAR ? min(min(whole / kGroups, rounds - 1), (sp.nk / KT - lo) / kGroups - 2) : 0;
     auto ask_chunk = [&](int i, int n) {  // of the keys of step i + 2 and the values of step i + 1, in turn
         if (n % 2 == 0) P::stage_chunk(a.k, kb, key_of(i + 2), wave, n / 2, k_at, ks[i & 1]);
         else P::stage_chunk(a.v, vb, key_of(i + 1), wave, n / 2, v_at, vs[(i + 1) & 1]);
@@ -342,7 +371,7 @@ __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prom
         // and added below for the rows that see them.
         bool odd = false;
         if (i >= whole / kGroups) {
-            for (int j = 0; j < P::PER; ++j) {
+            for (int j = 0; j < P::PER && n0 < end; ++j) {
                 h8 *const at = (h8 *)(vs[i & 1]) + tid + j * 64 * kPromptWaves;
                 h8 v = *at;
                 if (drop_non_finite(v)) {
@@ -355,7 +384,7 @@ __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prom
             odd = odd_tile[i & 1];
             if (threadIdx.x == 0) odd_tile[(i + 1) & 1] = 0;
         }
-        if (n0 < wave_max_) {  // else no row of this wave sees the tile, or there is none
+        if (n0 < wave_end) {  // else no row of this wave sees the tile, or there is none
 #pragma unroll
             for (int b = 0; b < KT / 32; ++b)
 #pragma unroll
@@ -404,6 +433,7 @@ __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prom
         const float other = stats[0][tid], peak = fmaxf(top, other);
         const float mine = __builtin_amdgcn_exp2f(top - peak), theirs = __builtin_amdgcn_exp2f(other - peak);
         sum = sum * mine + stats[1][tid] * theirs;
+        top = peak;
     #pragma unroll
         for (int t = 0; t < P::NT; ++t)
     #pragma unroll
@@ -415,50 +445,119 @@ __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prom
     }
     sum += other_half(sum);
     if (row >= sp.nq) return;
+    if constexpr (SPLIT) {
+        f4 *const part = (f4 *)(ws + ((size_t)blockIdx.x * gridDim.y + blockIdx.y) * kPartFloats<D>);
+#pragma unroll
+        for (int j = 0; j < 4 * P::NT; ++j)
+            part[j * (64 * kPromptWaves) + tid] = (f4){o[j / 4][j % 4 * 4], o[j / 4][j % 4 * 4 + 1], o[j / 4][j % 4 * 4 + 2], o[j / 4][j % 4 * 4 + 3]};
+        ((float2 *)(part + 4 * P::NT * (64 * kPromptWaves)))[tid] = float2{top, sum};
+        return;
+    }
     const float inv = limit > 0 ? 1.0f / sum : 0.f;
-    _Float16 *out = (_Float16 *)a.out.data + (size_t)(sp.q0 + row) * a.out.token_stride + head * a.out.head_stride;
 #pragma unroll
-    for (int t = 0; t < P::NT; ++t)
+    for (int j = 0; j < 4 * P::NT; ++j) {
+        h4 x;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            h4 x;
+        for (int e = 0; e < 4; ++e) x[e] = (_Float16)(limit > 0 ? o[j / 4][j % 4 * 4 + e] * inv : 0.f);
+        store_out(a, sp, head, row, j, h, x);
+    }
+}
+
+// The parts of each row together, in their order: thread tid of workgroup (b, i) has the elements that lane tid of
+// workgroups (b, part) had in their sums 4 i .. 4 i + 3.
+template <int D>
+__global__ __launch_bounds__(64 * kPromptWaves) void attention_prompt_join_kernel(PromptArgs a, int tiles, const float *ws,
+                                                                               int parts) {
+    constexpr int kThreads = 64 * kPromptWaves;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const Span sp = find_tile(a, tiles - 1 - (int)(blockIdx.x / a.q.heads), lane);
+    const int row = sp.row0 + 32 * (tid >> 6) + (lane & 31);
+    if (row >= sp.nq) return;
+    const int all = (seen_by(a, sp, sp.row0 + kPromptRows - 1) + Prompt<D>::KT - 1) / Prompt<D>::KT;
+    const int some = all ? (all + part_tiles(all, parts) - 1) / part_tiles(all, parts) : 0;  // parts with tiles
+    const bool sees = seen_by(a, sp, row) > 0;
+    const f4 *part = (const f4 *)(ws + (size_t)blockIdx.x * parts * kPartFloats<D>);
+    constexpr size_t kStep = kPartFloats<D> / 4;
+    auto stats = [&](int i) { return ((const float2 *)(part + i * kStep + D / 8 * kThreads))[tid]; };
+    float peak = kStart, total = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < some; ++i) peak = fmaxf(peak, stats(i).x);
+    f4 v[4] = {};
+    const f4 *mine = part + blockIdx.y * 4 * kThreads + tid;
+#pragma unroll 4
+    for (int i = 0; i < some; ++i) {
+        const float2 st = stats(i);
+        const float w = __builtin_amdgcn_exp2f(st.x - peak);
+        total += st.y * w;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = (_Float16)(limit > 0 ? o[t][4 * b + e] * inv : 0.f);
-            _Float16 *at = out + 32 * t + 8 * b + 4 * h;
-            if (a.out.vec) {
-                *(h4 *)at = x;
-            } else {
+        for (int j = 0; j < 4; ++j) v[j] += mine[i * kStep + j * kThreads] * w;
+    }
+    const float inv = 1.0f / total;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) at[e] = x[e];
-            }
-        }
+    for (int j = 0; j < 4; ++j) {
+        h4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = (_Float16)(sees ? v[j][e] * inv : 0.f);
+        store_out(a, sp, head_of(a, blockIdx.x), row, blockIdx.y * 4 + j, lane >> 5, x);
+    }
+}
+
+int prompt_tiles(int q_tokens, int sequences) { return q_tokens / kPromptRows + sequences; }  // each may end in a part tile
+
+// Parts of a walk.  Where the workgroups leave CUs idle, parts of the keys go to them, one workgroup a CU, and a
+// second kernel joins the parts.  A round of two tiles takes 1.3 us, the join 4 us and 0.3 us a part more, so
+// r rounds are best cut in about 2 sqrt(r), and the cut has to save 5 of them: 16 tokens after 8,192 others,
+// 32 / 8 heads of 128: 26.8 against 95.8 us (8 parts), 8 / 2 heads of 256: 29.6 against 188.6 (16); 1,000 tokens,
+// 4 / 1 heads of 128: 15.7 against 19.8 (5); but four prompts of 300 after 256 others: 16.1 against 15.1 (4).
+// More workgroups than CUs: 2,000 tokens, 4 / 1 heads of 128: 28.6 us at 6 parts, 20.4 at 4.
+constexpr size_t kSplitGroups = 256, kSplitGain = 5;
+int prompt_parts(size_t q_heads, int head_dim, int sequences, int q_tokens, int kv_tokens) {
+    const size_t groups = (size_t)prompt_tiles(q_tokens, sequences) * q_heads, idle = kSplitGroups / groups;
+    const size_t round = 2 * (head_dim == 256 ? Prompt<256>::KT : head_dim == 128 ? Prompt<128>::KT : Prompt<64>::KT);
+    const size_t rounds = (size_t)kv_tokens / sequences / round;
+    size_t parts = 1;
+    while (parts < idle && parts * parts < 4 * rounds) ++parts;
+    return rounds * (parts - 1) >= kSplitGain * parts ? (int)parts : 1;
+}
+
+template <int D, bool NEAR>
+void launch_near(const PromptArgs &a, float *workspace, hipStream_t stream) {
+    const int tiles = prompt_tiles(a.q_tokens, a.sequences), block = 64 * kPromptWaves;
+    const unsigned groups = (unsigned)tiles * a.q.heads;
+    const int parts = prompt_parts(a.q.heads, D, a.sequences, a.q_tokens, a.kv_tokens);
+    if (parts > 1) {
+        attention_prompt_kernel<D, NEAR, 2, true><<<dim3(groups, parts), 2 * block, 0, stream>>>(a, tiles, workspace);
+        attention_prompt_join_kernel<D><<<dim3(groups, D / 32), block, 0, stream>>>(a, tiles, workspace, parts);
+    } else if (groups <= kTwoGroups && (size_t)a.kv_tokens >= kTwoGroupsKeys * a.sequences) {
+        attention_prompt_kernel<D, NEAR, 2, false><<<groups, 2 * block, 0, stream>>>(a, tiles, nullptr);
+    } else {
+        attention_prompt_kernel<D, NEAR, 1, false><<<groups, block, 0, stream>>>(a, tiles, nullptr);
+    }
 }
 
 template <int D>
-hipError_t launch_d(const PromptArgs &a, hipStream_t stream) {
-    // every sequence may end in a part tile
-    const int tiles = a.q_tokens / kPromptRows + a.sequences;
-    const dim3 grid((unsigned)tiles * a.q.heads);
-    constexpr size_t kSpan = (size_t)1 << 31;
-    const bool near = a.k.vec && a.v.vec && a.k.token_stride * (2 * Prompt<D>::KT) < kSpan &&
-                      a.v.token_stride * (2 * Prompt<D>::KT) < kSpan;
-    const int block = 64 * kPromptWaves;
-    if (grid.x <= kTwoGroups && (size_t)a.kv_tokens >= kTwoGroupsKeys * a.sequences) {
-        if (near) attention_prompt_kernel<D, true, 2><<<grid, 2 * block, 0, stream>>>(a, tiles);
-        else attention_prompt_kernel<D, false, 2><<<grid, 2 * block, 0, stream>>>(a, tiles);
-    } else {
-        if (near) attention_prompt_kernel<D, true, 1><<<grid, block, 0, stream>>>(a, tiles);
-        else attention_prompt_kernel<D, false, 1><<<grid, block, 0, stream>>>(a, tiles);
-    }
+hipError_t launch_d(const PromptArgs &a, void *workspace, hipStream_t stream) {
+    constexpr size_t kNear = (size_t)1 << 31;
+    const bool near = a.k.vec && a.v.vec && a.k.token_stride * (2 * Prompt<D>::KT) < kNear &&
+                      a.v.token_stride * (2 * Prompt<D>::KT) < kNear;
+    float *const ws = workspace ? (float *)((uint8_t *)workspace + kSharedPrefixBytes) : nullptr;
+    if (near) launch_near<D, true>(a, ws, stream);
+    else launch_near<D, false>(a, ws, stream);
     return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_attention_prompt(const PromptArgs &a, hipStream_t stream) {
-    if (a.head_dim == 64) return launch_d<64>(a, stream);
-    if (a.head_dim == 128) return launch_d<128>(a, stream);
-    return launch_d<256>(a, stream);
+size_t attention_prompt_bytes(size_t q_heads, int head_dim, int sequences, int q_tokens, int kv_tokens) {
+    const size_t parts = prompt_parts(q_heads, head_dim, sequences, q_tokens, kv_tokens);
+    if (parts < 2) return 0;
+    return kSharedPrefixBytes + prompt_tiles(q_tokens, sequences) * q_heads * parts * 64 * kPromptWaves * (head_dim / 2 + 2) * sizeof(float);
+}
+
+hipError_t launch_attention_prompt(const PromptArgs &a, void *workspace, hipStream_t stream) {
+    if (a.head_dim == 64) return launch_d<64>(a, workspace, stream);
+    if (a.head_dim == 128) return launch_d<128>(a, workspace, stream);
+    return launch_d<256>(a, workspace, stream);
 }
 
 }  // namespace exl3k

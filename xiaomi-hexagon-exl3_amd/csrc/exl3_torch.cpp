@@ -182,6 +182,14 @@ PyObject *kv_cache_read(PyObject *const *a) {
 
 float scale_of(PyObject *o, int64_t head_dim) { return given(o) ? real_of(o) : 1.0f / std::sqrt((float)head_dim); }
 
+void *workspace(PyObject *o, size_t *bytes) {  // None: the library's own
+    *bytes = 0;
+    if (!given(o)) return nullptr;
+    const at::Tensor &t = tensor(o, "workspace is a tensor");
+    *bytes = t.nbytes();
+    return t.data_ptr();
+}
+
 // (q, pages, page_table, kv_lens, kv_heads, bits, page_tokens, q_len, scale, out, workspace, stream)
 PyObject *attention_cached(PyObject *const *a) {
     const at::Tensor &q = tensor(a[0], "q is a tensor");
@@ -197,20 +205,15 @@ PyObject *attention_cached(PyObject *const *a) {
     const at::Tensor out = output(a[9], q.sizes(), at::kHalf, q);
     const exl3_head_view ov = heads(out);
     need(out.scalar_type() == at::kHalf, "out: float16");
-    void *ws = nullptr;
-    size_t ws_bytes = 0;
-    if (given(a[10])) {
-        const at::Tensor &t = tensor(a[10], "workspace is a tensor");
-        ws = t.data_ptr();
-        ws_bytes = t.nbytes();
-    }
+    size_t ws_bytes;
+    void *const ws = workspace(a[10], &ws_bytes);
     return one(exl3_hip_attention_cached(&qv, &ov, d, p.data, p.count, p.bits, p.tokens, h,
                                          (const int32_t *)table.data_ptr(), (size_t)table.size(1), (const int32_t *)lens,
                                          n, q_len, scale_of(a[8], (int64_t)d), ws, ws_bytes, stream_of(a[11])),
                out);
 }
 
-// (q, k, v, q_starts, kv_starts, causal, scale, out, stream)
+// (q, k, v, q_starts, kv_starts, causal, scale, out, workspace, stream)
 PyObject *attention_prompt(PyObject *const *a) {
     const at::Tensor &q = tensor(a[0], "q is a tensor"), &k = tensor(a[1], "k is a tensor"),
                      &v = tensor(a[2], "v is a tensor");
@@ -227,9 +230,11 @@ PyObject *attention_prompt(PyObject *const *a) {
     const at::Tensor out = output(a[7], q.sizes(), at::kHalf, q);
     const exl3_head_view ov = heads(out);
     need(out.scalar_type() == at::kHalf, "out: float16");
+    size_t ws_bytes;
+    void *const ws = workspace(a[8], &ws_bytes);
     return one(exl3_hip_attention_prompt(&qv, &kv, &vv, &ov, (size_t)q.size(2), (const int32_t *)qs,
                                          (const int32_t *)kst, (size_t)starts - 1, (size_t)q.size(0),
-                                         (size_t)k.size(0), scale_of(a[6], q.size(2)), causal, stream_of(a[8])),
+                                         (size_t)k.size(0), scale_of(a[6], q.size(2)), causal, ws, ws_bytes, stream_of(a[9])),
                out);
 }
 
@@ -254,7 +259,7 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
     { #name, (PyCFunction)(void (*)(void))entry<name, n>, METH_FASTCALL, nullptr }
 PyMethodDef methods[] = {EXL3_ENTRY(qk_norm_rope, 13),     EXL3_ENTRY(kv_cache_write, 8),
                          EXL3_ENTRY(kv_cache_read, 11),    EXL3_ENTRY(attention_cached, 12),
-                         EXL3_ENTRY(attention_prompt, 9),  {nullptr, nullptr, 0, nullptr}};
+                         EXL3_ENTRY(attention_prompt, 10),  {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "exl3_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

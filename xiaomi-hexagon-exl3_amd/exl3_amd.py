@@ -30,6 +30,7 @@ EXPORTS = [
     "exl3_hip_mul_mat_group_workspace_bytes", "exl3_hip_workspace_status", "exl3_hip_test_exchange_fault",
     "exl3_hip_qk_norm_rope", "exl3_hip_kv_page_bytes", "exl3_hip_kv_cache_write", "exl3_hip_kv_cache_read",
     "exl3_hip_attention_cached", "exl3_hip_attention_cached_workspace_bytes", "exl3_hip_attention_prompt",
+    "exl3_hip_attention_prompt_workspace_bytes",
 ]
 
 # ggml op predicates (exl3_hip_supports_op)
@@ -180,7 +181,9 @@ def load(path=LIB_PATH):
     L.exl3_hip_attention_cached_workspace_bytes.restype = sz
     L.exl3_hip_attention_cached_workspace_bytes.argtypes = [sz, sz, sz, sz, sz]
     L.exl3_hip_attention_prompt.restype = i
-    L.exl3_hip_attention_prompt.argtypes = [hv, hv, hv, hv, sz, vp, vp, sz, sz, sz, f, i, st]
+    L.exl3_hip_attention_prompt.argtypes = [hv, hv, hv, hv, sz, vp, vp, sz, sz, sz, f, i, vp, sz, st]
+    L.exl3_hip_attention_prompt_workspace_bytes.restype = sz
+    L.exl3_hip_attention_prompt_workspace_bytes.argtypes = [sz, sz, sz, sz, sz]
     return L
 
 
@@ -611,9 +614,14 @@ def attention_cached(q, pages, page_table, kv_lens, kv_heads, bits=4, page_token
         "attention_cached")
 
 
-def attention_prompt(q, k, v, q_starts, kv_starts=None, causal=True, scale=None, out=None, stream=None):
+def attention_prompt_workspace_bytes(q_heads, head_dim, sequences, q_tokens, kv_tokens):
+    """0: such a call takes no workspace"""
+    return lib().exl3_hip_attention_prompt_workspace_bytes(q_heads, head_dim, sequences, q_tokens, kv_tokens)
+
+
+def attention_prompt(q, k, v, q_starts, kv_starts=None, causal=True, scale=None, out=None, workspace=None, stream=None):
     """Attention of packed sequences, all fp16: q [q_tokens, q_heads, head_dim], k and v [kv_tokens, kv_heads,
     head_dim]; q_starts and kv_starts (int32 [sequences + 1], None: q_starts) are the first rows of the
     sequences.  causal aligns each sequence's ends: keys ahead of its queries are a prefix."""
     return _taken((_TORCH or _torch_module()).attention_prompt(q, k, v, q_starts, kv_starts, causal, scale, out,
-                                                               stream), "attention_prompt")
+                                                               workspace, stream), "attention_prompt")
