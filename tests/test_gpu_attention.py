@@ -301,6 +301,19 @@ def test_cached_matches_formula(amd, case):
     assert np.all(np.abs(got - want) <= bound), float((np.abs(got - want) / np.maximum(bound, 1e-30)).max())
 
 
+@pytest.mark.parametrize("q_len,hq,hk,d,bits", [(7, 16, 2, 128, 8), (3, 24, 3, 64, 4), (5, 7, 1, 256, 4), (17, 2, 1, 128, 4)])
+def test_cached_last_row_tile_is_smaller(amd, q_len, hq, hk, d, bits):
+    """rows that are no multiple of 16, over sequences that several workgroups share"""
+    lens, p = [4100, 900, 0, 2600, 17], 64
+    print("  attention_cached", q_len, hq, hk, d, bits, flush=True)
+    pages, table, kept = make_cache(amd, lens, hk, d, bits, p)
+    q = rows(140, len(lens) * q_len, hq, d, sigma=2.0)
+    want, bound = cached_reference(q, kept, q_len, hk, d ** -0.5)
+    for _ in range(2):
+        got = run_cached(amd, q, pages, table, lens, hk, bits, p, q_len).astype(np.float64)
+        assert np.all(np.abs(got - want) <= bound)
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_cached_long(amd, bits):
     """one long sequence beside short ones; the table is wider than any of them"""

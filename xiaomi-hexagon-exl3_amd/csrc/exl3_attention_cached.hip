@@ -243,7 +243,7 @@ __device__ __forceinline__ float over_groups_sum(float v) {
 }
 
 // Partials of one (kv head, row tile): sums [slot][rows][D], then (maximum, sum) [slot][rows], rows the
-// real rows of a tile.  They cross XCDs, each with its own L2, so they are stored and loaded as
+// real rows of the tile; every tile has room for those of the first.  They cross XCDs, each with its own L2, so they are stored and loaded as
 // relaxed agent-scope atomics (coherent at device scope, no cache maintenance; a release fence writes
 // back a whole L2).
 struct Parts {
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
         const long n = (u + 1) * active - 1;
         return n <= 0xffffffffl && all <= 0xffffffffl ? (long)((uint32_t)n / (uint32_t)all) : n / all;
     };
-    const Parts parts = parts_of(ws, D, rows, slots, blockIdx.y);
+    const Parts parts = parts_of(ws, D, min(kRows, a.q_len * group), slots, blockIdx.y);
     _Float16 *const qhi = (_Float16 *)lds, *const qlo = qhi + kRows * D;
     float *const stat = lds + kCachedWaves * kRows * kPitch;  // (maximum, sum) of [wave][row]
     // the largest score is that of the largest product: a negative scale goes into the queries' signs (and 0 *
