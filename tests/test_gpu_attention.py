@@ -314,6 +314,28 @@ def test_cached_last_row_tile_is_smaller(amd, q_len, hq, hk, d, bits):
         assert np.all(np.abs(got - want) <= bound)
 
 
+@pytest.mark.parametrize("q_len,hq,hk,d,bits", [(1, 4, 1, 256, 4), (3, 8, 1, 256, 8), (8, 8, 2, 128, 4), (9, 16, 1, 64, 8)])
+def test_cached_joined_apart(amd, q_len, hq, hk, d, bits):
+    """sequences long enough that a second kernel joins their parts, beside short and empty ones; a NaN token"""
+    import torch
+    lens, p = [9000, 0, 300, 5001, 1], 64
+    print("  attention_cached", q_len, hq, hk, d, bits, flush=True)
+    pages, table, kept = make_cache(amd, lens, hk, d, bits, p)
+    q = rows(150, len(lens) * q_len, hq, d, sigma=2.0)
+    want, bound = cached_reference(q, kept, q_len, hk, d ** -0.5)
+    got = run_cached(amd, q, pages, table, lens, hk, bits, p, q_len)
+    assert np.all(np.abs(got.astype(np.float64) - want) <= bound)
+    assert np.array_equal(got, run_cached(amd, q, pages, table, lens, hk, bits, p, q_len))
+    slot = torch.tensor([int(table[3, 40]) * p + 7], device="cuda")
+    k, v = amd.kv_cache_read(pages, slot, hk, d, bits=bits, page_tokens=p)
+    k[:] = float("nan")
+    amd.kv_cache_write(pages, k, v, slot, bits=bits, page_tokens=p)
+    bad = run_cached(amd, q, pages, table, lens, hk, bits, p, q_len)
+    assert np.isnan(bad[3 * q_len:4 * q_len]).all()
+    others = np.r_[0:3 * q_len, 4 * q_len:5 * q_len]
+    assert np.array_equal(bad[others], got[others])
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_cached_long(amd, bits):
     """one long sequence beside short ones; the table is wider than any of them"""

@@ -3,7 +3,8 @@
 // One pass over the cached tokens: 16 query rows (the q heads of one kv head times the new
 // tokens) meet every key, with the running maximum and sum of the softmax.  Bound by the
 // cache's bytes: a token of one kv head is D * bits / 4 + D / 8 bytes and 2 * 16 * 2 D
-// multiply-adds on the matrix cores.
+// multiply-adds on the matrix cores.  Workgroups share a long sequence; the last of them to end joins their parts, or
+// a second kernel does.
 //
 // A wave takes 32 tokens at a time and computes S^T = K Q^T and O^T = V^T P^T with
 // mfma_f32_16x16x32_f16.  The layout of the page makes each operand one or two wide loads and a
@@ -280,10 +281,30 @@ __device__ __forceinline__ RowAt row_at(const CachedArgs &a, int s, int r, int k
     return x;
 }
 
+// the worker that has unit u (< all) of `active` workers: 32-bit arithmetic where it holds
+__device__ __forceinline__ long worker_of(long u, long active, long all) {
+    const long n = (u + 1) * active - 1;
+    return n <= 0xffffffffl && all <= 0xffffffffl ? (long)((uint32_t)n / (uint32_t)all) : n / all;
+}
+
+// Elements 8 l8 .. 8 l8 + 7 of row r of a kv head (the four lanes of a rotation group together): the sums over
+// the softmax's total, rotated back.  store: whether there is such a row.
+__device__ __forceinline__ void finish_row(const CachedArgs &a, int s, int len, int r, int kvh, int group, int l8, int lane,
+                                           bool faulted, bool store, float (&v)[8], float total) {
+    const bool sees = len > a.q_len - 1 - r / group;
+    const float inv = faulted ? __builtin_nanf("") : 1.0f / total;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = sees ? v[e] * inv : 0.f;
+    h32_run8(v, lane);
+    if (store) store_run8<1>(a.out.data, row_at(a, s, r, kvh, group).out + 8 * l8, a.out.vec, v);
+}
+
+// apart: the parts of a sequence that workers share are left for attention_cached_join_kernel.
 template <int D, int BITS>
 __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(CachedArgs a, void *ws,
                                                                              uint32_t *counts, const uint32_t *status,
-                                                                             int workers, size_t slots, int row_tiles, int direct) {
+                                                                             int workers, size_t slots, int row_tiles, int direct,
+                                                                             int apart) {
     using C = Cached<D, BITS>;
     constexpr int kCachedWaves = cached_waves(D);
     constexpr int kPitch = D + 4;  // floats of a row of sums in LDS: rows in different banks
@@ -340,7 +361,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
     } else {
         int longest;
         all = total_units(sh, lane, longest);
-        const int each = units_each(longest, rows * D);
+        const int each = apart ? 1 : units_each(longest, rows * D);
         active = min((long)workers, (all + each - 1) / each);
         for (int z = (int)w; z < a.sequences; z += workers)
             if (!sh.units(z)) zero_rows(z);
@@ -350,10 +371,6 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
         s = find_unit(sh, unit, lane, first);
     }
     // the worker that holds unit u: the last w with w all / active <= u
-    auto worker_of = [&](long u) {
-        const long n = (u + 1) * active - 1;
-        return n <= 0xffffffffl && all <= 0xffffffffl ? (long)((uint32_t)n / (uint32_t)all) : n / all;
-    };
     const Parts parts = parts_of(ws, D, min(kRows, a.q_len * group), slots, blockIdx.y);
     _Float16 *const qhi = (_Float16 *)lds, *const qlo = qhi + kRows * D;
     float *const stat = lds + kCachedWaves * kRows * kPitch;  // (maximum, sum) of [wave][row]
@@ -562,18 +579,13 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
         // The whole sequence, or a part of it: then the worker that stores the last of the parts sums them, in
         // the workers' order whichever it is.  A part's stores have reached device scope (vmcnt) before its
         // arrival is counted; the count is left zero.
-        const long w0 = direct ? 0 : worker_of(first), w1 = direct ? units - 1 : worker_of(first + units - 1);
+        const long w0 = direct ? 0 : worker_of(first, active, all),
+                   w1 = direct ? units - 1 : worker_of(first + units - 1, active, all);
         const bool whole_sequence = w0 == w1;
         const size_t part0 = direct ? (size_t)s * direct : (size_t)s;  // partial of worker 0
         const long me = direct ? unit : w;
         auto finish = [&](int r, int l8, float (&v)[8], float total) {
-            const bool sees = len > a.q_len - 1 - (row0 + r) / group;
-            const float inv = faulted ? __builtin_nanf("") : 1.0f / total;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = sees ? v[e] * inv : 0.f;
-            h32_run8(v, lane);
-            if (r < rows)
-                store_run8<1>(a.out.data, row_at(a, s, row0 + r, kvh, group).out + 8 * l8, a.out.vec, v);
+            finish_row(a, s, len, row0 + r, kvh, group, l8, lane, faulted, r < rows, v, total);
         };
 #pragma unroll
         for (int n = 0; n < kEach; ++n) {
@@ -598,7 +610,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
                 if (l8 == 0) put_pair(parts.stats + at, peak, total);
             }
         }
-        if (!whole_sequence && !faulted) {
+        if (!whole_sequence && !faulted && !apart) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
             uint32_t *count = counts + (size_t)blockIdx.y * a.sequences + s;
@@ -686,6 +698,70 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
     }
 }
 
+// One row of a sequence that workers share: workgroup (sequence, row tile, row).  The parts' weights first, then their
+// sums, four elements a thread, every split-th part by a group of D / 4 threads.
+constexpr int kJoinThreads = 512;
+template <int D>
+__global__ __launch_bounds__(kJoinThreads) void attention_cached_join_kernel(CachedArgs a, void *ws, const uint32_t *status,
+                                                                            int workers, size_t slots, int row_tiles) {
+    constexpr int kItems = D / 4, kSplit = kJoinThreads / kItems;
+    __shared__ float weight[kCachedGroups], sums[kSplit][D + 4], tops[kJoinThreads / 64], totals[kJoinThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, s = blockIdx.x, r = blockIdx.z;
+    const int kvh = blockIdx.y / row_tiles, row0 = (blockIdx.y - kvh * row_tiles) * kRows;
+    const int group = a.q.heads / a.l.kv_heads, rows = min(kRows, a.q_len * group - row0);
+    if (r >= rows || *status) return;  // a faulted workspace: the rows are NaN already
+    const Share<kTile * cached_waves(D)> sh{a.kv_lens, (long)a.table_stride * a.l.page_tokens, a.sequences};
+    long all = 0, first = 0;
+    for (int s0 = 0; s0 < a.sequences; s0 += 64) {
+        const int n = sh.units(s0 + lane), end = wave_scan(n, lane, 64);
+        if (s >= s0 && s < s0 + 64) first = all + __builtin_amdgcn_readlane(end - n, s - s0);
+        all += __builtin_amdgcn_readlane(end, 63);
+    }
+    const int len = sh.len(s), units = sh.units(s);
+    if (!units) return;
+    const long active = min((long)workers, all);
+    const long w0 = worker_of(first, active, all);
+    const int count = (int)(worker_of(first + units - 1, active, all) - w0) + 1;  // at most kCachedGroups
+    if (count == 1) return;  // its worker has stored it
+    const Parts parts = parts_of(ws, D, min(kRows, a.q_len * group), slots, blockIdx.y);
+    const size_t part0 = (size_t)(s + w0);
+    const float2 st = tid < count ? ((const float2 *)parts.stats)[(part0 + tid) * rows + r] : float2{kStart, 0.f};
+    auto over_wave = [](float v, auto f) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) v = f(v, __shfl_xor(v, d));
+        return v;
+    };
+    const float top = over_wave(st.x, [](float x, float y) { return fmaxf(x, y); });
+    if (lane == 0) tops[tid >> 6] = top;
+    __syncthreads();
+    float peak = kStart;
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 64; ++i) peak = fmaxf(peak, tops[i]);
+    const float w = __builtin_amdgcn_exp2f(st.x - peak);
+    if (tid < count) weight[tid] = w;
+    const float part_total = over_wave(st.y * w, [](float x, float y) { return x + y; });
+    if (lane == 0) totals[tid >> 6] = part_total;
+    __syncthreads();
+    float total = 0.f;
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 64; ++i) total += totals[i];
+    const int item = tid % kItems, grp = tid / kItems;
+    const f4 *x = (const f4 *)parts.sums + (part0 * rows + r) * kItems + item;
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int k = grp; k < count; k += kSplit) v += x[(size_t)k * rows * kItems] * weight[k];
+    *(f4 *)&sums[grp][4 * item] = v;
+    __syncthreads();
+    if (tid < 64) {  // whole waves: the rotation exchanges between lanes
+        const int l8 = lane % (D / 8);
+        float y[8] = {};
+        for (int k = 0; k < min(kSplit, count); ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] += sums[k][8 * l8 + e];
+        finish_row(a, s, len, row0 + r, kvh, group, l8, lane, false, lane < D / 8, y, total);
+    }
+}
+
 struct CachedPlan {
     int row_tiles, rows, workers;
     size_t slots;
@@ -701,6 +777,18 @@ CachedPlan cached_plan(size_t q_heads, size_t kv_heads, size_t sequences, size_t
     return p;
 }
 
+// Whether a second kernel joins the parts of long sequences.  In the first one a single workgroup joins a sequence's,
+// so it makes few and long ones (units_each); a kernel of its own costs 4 us and takes as many as there are
+// workers.  It pays from about `units` * rows * d^2 = 2^22 (one of a wider head has more to join, and fewer tokens in a
+// unit): 16,000 tokens, 4 rows of 256: 18.5 against 26.8 us; 30,723, 5 rows of 256 at 8 bits: 21.4 against 45.9; 16,000, 16
+// rows of 128: 16.6 against 19.4; 32,768, 4 rows of 64: 14.1 against 13.1; and not where each sequence has a few
+// workers only: 16 of up to 32,768 tokens, 4 rows of 128, 2 workers each: 48.7 against 46.9.  `units` are those
+// that the page table has room for: 500 tokens in a table for 32,768, 4 rows of 256: 15.2 against 13.5.
+constexpr size_t kApart = (size_t)1 << 22, kApartWorkers = 4;
+bool join_apart(size_t units, const CachedPlan &p, size_t d, size_t sequences) {
+    return units * p.rows * d * d >= kApart && p.workers >= kApartWorkers * sequences;
+}
+
 template <int D>
 hipError_t launch_d(const CachedArgs &a, void *workspace, hipStream_t stream) {
     const CachedPlan p = cached_plan(a.q.heads, a.l.kv_heads, a.sequences, a.q_len);
@@ -710,12 +798,12 @@ hipError_t launch_d(const CachedArgs &a, void *workspace, hipStream_t stream) {
     const dim3 grid(direct ? direct * a.sequences : p.workers, (unsigned)tiles);
     void *ws = (uint8_t *)workspace + kSharedPrefixBytes;
     uint32_t *counts = (uint32_t *)workspace, *status = (uint32_t *)((uint8_t *)workspace + kStatusOffset);
-    if (a.l.bits == 4)
-        attention_cached_kernel<D, 4><<<grid, 64 * cached_waves(D), 0, stream>>>(a, ws, counts, status, p.workers, p.slots,
-                                                                                 p.row_tiles, direct);
-    else
-        attention_cached_kernel<D, 8><<<grid, 64 * cached_waves(D), 0, stream>>>(a, ws, counts, status, p.workers, p.slots,
-                                                                                 p.row_tiles, direct);
+    const bool apart = !direct && join_apart(units, p, D, a.sequences);
+    const auto kernel = a.l.bits == 4 ? attention_cached_kernel<D, 4> : attention_cached_kernel<D, 8>;
+    kernel<<<grid, 64 * cached_waves(D), 0, stream>>>(a, ws, counts, status, p.workers, p.slots, p.row_tiles, direct, apart);
+    if (apart)
+        attention_cached_join_kernel<D><<<dim3(a.sequences, (unsigned)tiles, p.rows), kJoinThreads, 0, stream>>>(
+            a, ws, status, p.workers, p.slots, p.row_tiles);
     return hipGetLastError();
 }
 
