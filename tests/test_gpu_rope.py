@@ -59,6 +59,18 @@ def test_matches_formula(amd, case):
         check(y, want, size, yt)
 
 
+@pytest.mark.parametrize("size", [1e-17, 1e-10, 1e15])
+def test_norm_of_small_and_large_rows(amd, size):
+    """without an eps, rows whose squares are near the ends of binary32"""
+    import torch
+    x = (synth.normal(15, 7 * 3 * 128, 1.0).reshape(7, 3, 128) * size).astype(np.float32)
+    w = (1 + synth.normal(16, 128, 0.3)).astype(np.float32)
+    y, _ = amd.qk_norm_rope(torch.from_numpy(x).cuda(), None, q_weight=torch.from_numpy(w).cuda(), eps=0.0,
+                            out_dtype=torch.float32)
+    want, mass = ref.norm_rope(x, w, 0.0, None, None, False, 1.0)
+    check(y, want, mass, "f32")
+
+
 @pytest.mark.parametrize("pairs", [False, True])
 def test_views_in_place_and_unaligned(amd, pairs):
     """slices of a fused buffer, at an offset that is not 16-byte aligned, head-major outputs, and in place"""

@@ -3,7 +3,7 @@
 // y = x / sqrt(mean(x^2) + eps) * weight, then each pair (a, b) turned by position * frequency.  Bound by
 // the rows' bytes, each read and written once: D / 8 lanes hold a row, its pairs meet by lane exchange or
 // within a lane, and the sines are worked out in the kernel (a table would be read as often as the rows).
-// 8,192 tokens, 32 / 8 heads of 128 in fp16: 32 us in a kernel trace (5.2 TB/s), 44 us a call in a loop of calls; one
+// 8,192 tokens, 32 / 8 heads of 128 in fp16: 30 us in a kernel trace (5.6 TB/s), 44 us a call in a loop of calls; one
 // token: 3.1 us, a launch and two dependent round trips.
 #include "exl3_head_rows.hpp"
 
@@ -58,6 +58,7 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs a, 
     const bool on = 8 * l < a.head_dim;  // the others only take part in the exchanges
     const int half = a.rot_dim / 2;
     const size_t units = a.tokens * slices;
+    const float inv_dim = 1.0f / (float)a.head_dim;
     for (size_t unit = (size_t)blockIdx.x * (kRopeThreads / VL) + threadIdx.x / VL; unit < units;
          unit += (size_t)gridDim.x * (kRopeThreads / VL)) {  // whole lane groups
         const size_t token = unit / slices;
@@ -91,7 +92,10 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs a, 
                 float sum = 0.f;
     #pragma unroll
                 for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(v[e], v[e], sum);
-                const float r = 1.0f / __builtin_sqrtf(row_sum<VL>(sum) / (float)a.head_dim + a.eps);
+                // v_rsq_f32 is good to 1 ulp, of normal numbers
+                const float mean = __builtin_fmaf(row_sum<VL>(sum), inv_dim, a.eps);
+                const bool tiny = mean < 0x1p-100f;
+                const float r = __builtin_amdgcn_rsqf(tiny ? mean * 0x1p64f : mean) * (tiny ? 0x1p32f : 1.f);
                 if (on) {
                     float wt[8];
                     load_run8<0>(w, 8 * l, 0, wt);
@@ -105,8 +109,8 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs a, 
     #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float x = v[2 * e], y = v[2 * e + 1];
-                            v[2 * e] = x * cs[e] - y * sn[e];
-                            v[2 * e + 1] = y * cs[e] + x * sn[e];
+                            v[2 * e] = __builtin_fmaf(x, cs[e], -(y * sn[e]));
+                            v[2 * e + 1] = __builtin_fmaf(y, cs[e], x * sn[e]);
                         }
                     }
                 } else {
@@ -115,7 +119,7 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs a, 
                     for (int e = 0; e < 8; ++e) o[e] = __shfl(v[e], partner & 63);
                     if (turned) {
     #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = v[e] * cs[e] - o[e] * sn[e];
+                        for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(v[e], cs[e], -(o[e] * sn[e]));
                     }
                 }
             }
