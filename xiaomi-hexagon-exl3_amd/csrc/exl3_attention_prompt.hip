@@ -12,9 +12,9 @@
 // the tile, read with ds_read_b64_tr_b16: within 16 lanes it hands lane i the i-th of 16 elements of
 // four rows.  16-byte chunks of a row are swizzled so that the rows of one read lie in
 // different banks.
-// One causal prompt of 8,192 tokens, 32 / 8 heads of 128: 535 us, 1,030 TFLOP/s, at the 1.63 GHz that
+// One causal prompt of 8,192 tokens, 32 / 8 heads of 128: 532 us, 1,034 TFLOP/s, at the 1.63 GHz that
 // the chip's power leaves (a large fp16 product: 1,150 to 1,390); seven packed prompts of up to 2,111 tokens, some after
-// 500 others, 16 / 4 heads of 64: 47 us, 505 TFLOP/s, bound by the exponentials (two MFMAs of 32 cycles for 16 of them
+// 500 others, 16 / 4 heads of 64: 46 us, 518 TFLOP/s, bound by the exponentials (two MFMAs of 32 cycles for 16 of them
 // a lane) and the longest sequence's last tiles; 37 tokens, 8 / 2 heads of 256: 9.6 us.
 #include "exl3_head_rows.hpp"
 
@@ -73,7 +73,6 @@ __device__ __forceinline__ Span find_tile(const PromptArgs &a, int t, int lane) 
 }
 
 typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void global_void;
 
 template <int D>
 struct Prompt {
@@ -93,6 +92,14 @@ struct Prompt {
         return r * CH + (D == 64 ? c ^ (((r >> 1) & 1) << 2) : c ^ ((r & 3) << 2));
     }
 
+    // 16 bytes a lane into LDS, in lane order from `to`.  After the builtin of this instruction the compiler has
+    // every LDS read wait for the load, since it cannot tell the buffers apart (a prompt of 320 tokens,
+    // 12 / 3 heads of 256: 21.5 against 20.6 us).  It writes no register; the place is read after a later step's wait and barrier.
+    static __device__ __forceinline__ void load_chunk(const char *base, uint32_t at, _Float16 *to) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"((uint32_t)(uintptr_t)(lds_void *)to),
+                     "v"(at), "s"(base)
+                     : "m0");
+    }
     // Brings the tile at key n0 (keys beyond the last are the last) into an LDS tile; complete after a
     // wait for vmcnt and a barrier.  The loads write LDS directly, 16 bytes a lane in lane order, so the
     // lane takes the chunk that belongs at its place.  NEAR: a tile's rows span less than 2^31 bytes
@@ -108,9 +115,7 @@ struct Prompt {
             _Float16 *const wave_lds = lds + __builtin_amdgcn_readfirstlane(tid >> 6) * 512;
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                __builtin_amdgcn_global_load_lds(
-                    (global_void *)(tile + ((uint32_t)min(r0 + i * RS, nk - 1 - n0) * stride + 16 * c)),
-                    (lds_void *)(wave_lds + i * (512 * kPromptWaves)), 16, 0, 0);
+                load_chunk(tile, (uint32_t)min(r0 + i * RS, nk - 1 - n0) * stride + 16 * c, wave_lds + i * (512 * kPromptWaves));
         } else {
             for (int i = 0; i < PER; ++i) {
                 const _Float16 *q = (const _Float16 *)tile + (size_t)min(r0 + i * RS, nk - 1 - n0) * m.token_stride + 8 * c;
@@ -131,11 +136,7 @@ struct Prompt {
     static __device__ __forceinline__ void stage_chunk(const Heads &m, const _Float16 *base, int n0, int wave, int i,
                                                        uint32_t at, _Float16 *lds) {
         const char *rows = (const char *)(base + (size_t)(n0 + i * RS) * m.token_stride);
-        const uint32_t to = (uint32_t)(uintptr_t)(lds_void *)(lds + wave * 512 + i * (512 * kPromptWaves));
-        // The builtin's instruction (M0: the wave's place in LDS).  After the builtin the compiler has every LDS read
-        // wait for the load, since it cannot tell the slots apart.  It writes no register; the slot is read
-        // after the next step's wait and barrier.
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(at), "s"(rows) : "m0");
+        load_chunk(rows, at, lds + wave * 512 + i * (512 * kPromptWaves));
     }
 };
 
