@@ -18,7 +18,8 @@
 //      m D / 16 + t of the head.
 // Every value scale * code is an fp16 number, so dequantising adds no rounding.  The queries are
 // rotated by H32 like the cached rows and kept as an fp16 pair (high and low part: two
-// MFMAs, which the VALU work hides); the result is rotated back at the end.
+// MFMAs, which the VALU work hides; a row that the rotation could take beyond fp16's range is kept as an eighth, with
+// eight times its factor in the exponent); the result is rotated back at the end.
 // 16 sequences of 32,768 tokens, 32 / 8 heads of 128 at 4 bits (604 MB): 120 us, 5.0 TB/s, the rate of a large
 // copy, with the VALU at work 64 % of the time; 1,000 tokens, 8 / 2 heads of 256: 13.1 us, a launch and four
 // dependent round trips.
@@ -40,6 +41,9 @@ constexpr int kDirectUnits = 8;
 constexpr float kStart = -1e30f;                   // running maximum before the first key
 constexpr float kSlack = 8.f;                      // scores may pass the running maximum by 2^8
 constexpr float kLog2e = 1.4426950408889634f;
+// H32 makes an element at most sqrt(32) times a row's largest: up to this fp16 value the rotated row is within
+// 65,504.  A row beyond it is kept as an eighth (46,319 at most), the other rows as they are.
+constexpr float kFullQuery = 11576.f;
 
 // The work in units of a tile for every wave.  Either (few units: `direct`) a workgroup for each unit of
 // each sequence that the page table has room for, which knows its place without the lengths, so that
@@ -376,6 +380,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
     // the worker that holds unit u: the last w with w all / active <= u
     const Parts parts = parts_of(ws, D, min(kRows, a.q_len * group), slots, blockIdx.y);
     _Float16 *const qhi = (_Float16 *)lds, *const qlo = qhi + kRows * D;
+    float *const q_unit = (float *)(qlo + kRows * D);         // of each row: 1, or 8 where an eighth is kept
     float *const stat = lds + kCachedWaves * kRows * kPitch;  // (maximum, sum) of [wave][row]
     // the largest score is that of the largest product: a negative scale goes into the queries' signs (and 0 *
     // -infinity, the masked places of a zero scale, must stay -infinity)
@@ -431,12 +436,19 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
 #pragma unroll
         for (int n = 0; n < kEach; ++n) {
             const int i = tid + n * kThreads;
-            if (i >= kItems) break;
+            if (i >= kItems) break;  // whole waves
+            float large = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) large = fmaxf(large, __builtin_fabsf(qx[n][e]));
+            const unsigned long long row_lanes = ((1ull << (D / 8)) - 1) << (lane & ~(D / 8 - 1));
+            const bool eighth = __ballot(large > kFullQuery) & row_lanes;
+            if (i % (D / 8) == 0) q_unit[i / (D / 8)] = eighth ? 8.f : 1.f;
+            const float part = eighth ? sign * 0.125f : sign;
             h32_run8(qx[n], lane);
             h8 hi, lo;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                qx[n][e] *= sign;
+                qx[n][e] *= part;
                 hi[e] = (_Float16)qx[n][e];
                 lo[e] = (_Float16)(qx[n][e] - (float)hi[e]);
             }
@@ -450,6 +462,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             bh[j] = C::q_order(*(const h8 *)(qhi + m * D + g * (D / 4) + 8 * j));
             bl[j] = C::q_order(*(const h8 *)(qlo + m * D + g * (D / 4) + 8 * j));
         }
+        const float cq = c * q_unit[m];
         // keys that this lane's row sees
         const int limit = len - (a.q_len - 1 - (row0 + m) / group);
 
@@ -515,7 +528,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             float best = x[0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) best = fmaxf(best, x[e]);
-            best *= c;
+            best *= cq;
             if (__ballot(best > top + kSlack)) {
                 const float now = fmaxf(top, over_groups_max(best));
                 const float keep = __builtin_amdgcn_exp2f(top - now);
@@ -529,7 +542,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             h8 p;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], c, -top));
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], cq, -top));
                 sum += v;
                 p[e] = (_Float16)v;
             }
