@@ -413,9 +413,11 @@ exl3_status exl3_hip_qk_norm_rope(const exl3_head_view *q, const exl3_head_view 
  * Walsh-Hadamard matrix H32 (which spreads a large channel over the group), ext is its
  * element of largest magnitude (the negative one of two equal), scale = fp16(-ext /
  * 2^(bits-1)) with its magnitude rounded up to 12 - bits significant bits (a zero is +0), and code =
- * clamp(rint(y / scale), -2^(bits-1), 2^(bits-1) - 1): every scale * code is an fp16
- * number, so attention reads the cache without a further rounding.  A group with a
- * non-finite element, or beyond fp16's range, reads back as NaN.
+ * clamp(rint(y / scale), -2^(bits-1), 2^(bits-1) - 1): every scale * code has at most 11
+ * significant bits, so attention reads the cache without a further rounding (a product
+ * above 65,504, which H32 can make of an fp16 row, included).  A group with a non-finite
+ * element, or whose scale is beyond fp16's range (an extreme of half a million at 4 bits,
+ * 7.8 million at 8), reads back as NaN.
  * A page is, for each kv head, four runs:
  *   keys    [P][head_dim * bits / 8]          code + 2^(bits-1); 4 bits: the even element low
  *   values  [P/4][16][4][head_dim * bits / 128]  blocks of 4 tokens: 16 slices of a row, each
@@ -457,7 +459,8 @@ exl3_status exl3_hip_kv_cache_read(const void *pages, size_t page_count, unsigne
  *               that exl3_hip_mul_mat uses too.  NULL: the internal one of this stream
  * head_dim 64, 128 or 256; q heads a multiple of kv_heads, up to 64 of them per kv head;
  * q_len 1..65536.  Scores, softmax statistics and sums in fp32; q as an fp16 pair (high
- * and low part), weights rounded to fp16.  The same inputs give the same bits on every
+ * and low part; an eighth of a row with elements above 11,576, so every finite row is
+ * held), weights rounded to fp16.  The same inputs give the same bits on every
  * call.  A workspace whose exchange gave up (exl3_hip_workspace_status) gives NaN rows until
  * it is initialised again.  EXL3_NO_SUPPORT where kv_heads * ceil(group * q_len / 16) is
  * above 65,535, or times the sequences above 2^22.  sequences = 0 is a no-op. */

@@ -16,7 +16,8 @@
 //   V: a lane's block of four tokens holds those four keys for its slice of D / 16 elements;
 //      the A operand of O^T tile t is element t of the slice: row m of the tile is element
 //      m D / 16 + t of the head.
-// Every value scale * code is an fp16 number, so dequantising adds no rounding.  The queries are
+// Every value scale * code has at most 11 significant bits, so dequantising adds no rounding; groups that
+// pass fp16's range (one extreme above 65,504 after the rotation) are multiplied apart, at 2^-8.  The queries are
 // rotated by H32 like the cached rows and kept as an fp16 pair (high and low part: two
 // MFMAs, which the VALU work hides; a row that the rotation could take beyond fp16's range is kept as an eighth, with
 // eight times its factor in the exponent); the result is rotated back at the end.
@@ -209,6 +210,31 @@ struct Cached {
     static __device__ __forceinline__ h8 q_order(h8 v) {
         if constexpr (BITS == 4) return (h8){v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};
         else return v;
+    }
+
+    // Scales whose product with the lowest code, -2^(BITS - 1), is beyond fp16 (one step more than 65,504), or that are
+    // not finite: their groups are taken apart from the others, at 2^-8 of their size, which is exact for them.
+    static constexpr uint32_t kLargeScale = BITS == 4 ? 0x7000u : 0x6000u;  // 8,192, 512
+    static __device__ __forceinline__ bool any_large(const Half (&h)[2]) {
+        constexpr uint32_t magnitude = 0x7fff7fffu;
+        typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+        us2 most = bitcast<us2>(h[0].ks & magnitude);
+        for (const uint32_t w : {h[0].vs.x, h[0].vs.y, h[1].ks, h[1].vs.x, h[1].vs.y})
+            most = __builtin_elementwise_max(most, bitcast<us2>(w & magnitude));
+        return __ballot((bitcast<uint32_t>(most) + (0x8000u - kLargeScale) * 0x10001u) & 0x80008000u) != 0;
+    }
+    static __device__ __forceinline__ uint32_t large_mask(uint32_t w) {
+        return ((((w & 0x7fff7fffu) + (0x8000u - kLargeScale) * 0x10001u) >> 15) & 0x10001u) * 0xffffu;
+    }
+    // the large ones of two scales, times 2^-8, and the others
+    static __device__ __forceinline__ uint32_t large_only(uint32_t w) {
+        return bitcast<uint32_t>(bitcast<h2>(w & large_mask(w)) * (h2){(_Float16)0x1p-8f, (_Float16)0x1p-8f});
+    }
+    static __device__ __forceinline__ uint32_t without_large(uint32_t w) { return w & ~large_mask(w); }
+    // keeps the compiler from holding the numbers made of these words for their next use
+    static __device__ __forceinline__ void forget(uint32_t (&w)[NW]) {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) asm volatile("" : "+v"(w[i]));
     }
 
     // element t of the lane's slice for its four tokens (as two pairs)
@@ -508,15 +534,29 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             }
             f4 st[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                st[i] = (f4){0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 2; ++i) st[i] = (f4){0.f, 0.f, 0.f, 0.f};
+            auto add_scores = [&](const typename C::Half &h, f4 &to) {
 #pragma unroll
                 for (int j = 0; j < C::NJ; ++j) {
-                    const h8 k = C::key(cur[i], j, masks);
-                    st[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, bl[j], st[i], 0, 0, 0);
-                    st[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, bh[j], st[i], 0, 0, 0);
+                    const h8 k = C::key(h, j, masks);
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, bl[j], to, 0, 0, 0);
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, bh[j], to, 0, 0, 0);
+                }
+            };
+            const bool large = C::any_large(cur);  // rare
+            if (__builtin_expect(large, false)) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t scales = cur[i].ks;
+                    cur[i].ks = C::large_only(scales);
+                    add_scores(cur[i], st[i]);
+                    st[i] *= 256.f;
+                    cur[i].ks = C::without_large(scales);
+                    C::forget(cur[i].k);
                 }
             }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) add_scores(cur[i], st[i]);
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = st[e >> 2][e & 3];
@@ -546,14 +586,27 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
                 sum += v;
                 p[e] = (_Float16)v;
             }
-#pragma unroll
-            for (int t = 0; t < C::NT; ++t) {
+            auto weighted = [&](const typename C::Half (&h)[2], int t, f4 to) {
                 h2 v[4];
-                C::value(cur[0], t, v[0], v[1], masks);
-                C::value(cur[1], t, v[2], v[3], masks);
+                C::value(h[0], t, v[0], v[1], masks);
+                C::value(h[1], t, v[2], v[3], masks);
                 const h8 vt = {v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, p, o[t], 0, 0, 0);
+                return __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, p, to, 0, 0, 0);
+            };
+            if (__builtin_expect(large, false)) {
+                const u2 scales[2] = {cur[0].vs, cur[1].vs};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) cur[i].vs = (u2){C::large_only(scales[i].x), C::large_only(scales[i].y)};
+#pragma unroll
+                for (int t = 0; t < C::NT; ++t) o[t] = weighted(cur, t, o[t] * 0x1p-8f) * 256.f;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    cur[i].vs = (u2){C::without_large(scales[i].x), C::without_large(scales[i].y)};
+                    C::forget(cur[i].v);
+                }
             }
+#pragma unroll
+            for (int t = 0; t < C::NT; ++t) o[t] = weighted(cur, t, o[t]);
             if (edge && __ballot(lost)) {  // rare: NaN for the rows that see such a token, in its group's elements
                 for (int n = n0; n < n0 + kTile && n < len; ++n) {
                     const int page = n / a.l.page_tokens, id = table[page];
