@@ -458,7 +458,7 @@ exl3_status exl3_hip_kv_cache_read(const void *pages, size_t page_count, unsigne
  *               zero-filled before first use (exl3_hip_workspace_init); it may be one
  *               that exl3_hip_mul_mat uses too.  NULL: the internal one of this stream
  * head_dim 64, 128 or 256; q heads a multiple of kv_heads, up to 64 of them per kv head;
- * q_len 1..65536.  Scores, softmax statistics and sums in fp32; q as an fp16 pair (high
+ * q_len 1..65536; scale finite.  Scores, softmax statistics and sums in fp32; q as an fp16 pair (high
  * and low part; an eighth of a row with elements above 11,576, so every finite row is
  * held), weights rounded to fp16.  The same inputs give the same bits on every
  * call.  A workspace whose exchange gave up (exl3_hip_workspace_status) gives NaN rows until
@@ -479,7 +479,7 @@ size_t exl3_hip_attention_cached_workspace_bytes(size_t q_heads, size_t kv_heads
  * sees the first nk - (nq - 1 - i) of its nk keys (the sequences' ends aligned: keys
  * ahead of the queries are a prefix), else all; a row that sees none is zero.  q, k, v
  * and out are F16, out disjoint from the inputs; head_dim 64, 128 or 256; q heads a
- * multiple of kv heads.  q_tokens and kv_tokens are the rows of the views (no row
+ * multiple of kv heads; scale finite.  q_tokens and kv_tokens are the rows of the views (no row
  * outside them is read or written, whatever the starts hold; a query row that no
  * sequence has is not written).  Scores, softmax statistics and sums in fp32, weights
  * rounded to fp16.  The same inputs give the same bits on every call.

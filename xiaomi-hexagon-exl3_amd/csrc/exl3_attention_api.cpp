@@ -2,6 +2,8 @@
 // argument checks, views and dispatch to its gfx950 kernels.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
+
 #include "exl3_attention.hpp"
 #include "exl3_hip.h"
 #include "exl3_launch.hpp"
@@ -157,6 +159,7 @@ exl3_status exl3_hip_attention_cached(const exl3_head_view *q, const exl3_head_v
         return EXL3_INVAL_PARAMS;
     if (!pages || !aligned(pages, 16) || !page_table || !aligned(page_table, 4) || !kv_lens || !aligned(kv_lens, 4))
         return EXL3_INVAL_PARAMS;
+    if (!std::isfinite(scale)) return EXL3_INVAL_PARAMS;  // the kernels bound it from below, which a NaN would pass
     if (!exl3k::attention_cached_fits(q->heads, kv_heads, sequences, q_len)) return EXL3_NO_SUPPORT;
     const exl3_status st = exl3k::take_workspace(need, stream, &workspace, &workspace_bytes);
     if (st != EXL3_OK) return st;
@@ -198,6 +201,7 @@ exl3_status exl3_hip_attention_prompt(const exl3_head_view *q, const exl3_head_v
         a.out.data == a.k.data || a.out.data == a.v.data)
         return EXL3_INVAL_PARAMS;
     if (!q_starts || !kv_starts || !aligned(q_starts, 4) || !aligned(kv_starts, 4)) return EXL3_INVAL_PARAMS;
+    if (!std::isfinite(scale)) return EXL3_INVAL_PARAMS;
     if ((q_tokens / 128 + sequences) * q->heads > kMaxGridX) return EXL3_NO_SUPPORT;
     a.q_starts = q_starts;
     a.kv_starts = kv_starts;
