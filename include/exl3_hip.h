@@ -377,7 +377,8 @@ exl3_status exl3_hip_iface_matmul(unsigned bits, unsigned codebook, size_t k, si
 
 /* Rows of heads: element i of head h of token t is at data[t * token_stride + h *
  * head_stride + i] (strides in elements, the head's elements dense), so a slice of a
- * fused q/k/v buffer is a view.  Outputs: no two heads overlap. */
+ * fused q/k/v buffer is a view.  Outputs: no two heads overlap.  A stride is at most 2^40
+ * elements, and tokens and heads each span at most 2^48. */
 typedef struct exl3_head_view {
     void *data;          /* device */
     size_t heads;

@@ -1,4 +1,5 @@
-"""Arguments of the attention block's entry points that have to be refused on the host: scales that are not finite."""
+"""Arguments of the attention block's entry points that have to be refused on the host: scales that are not finite, views
+beyond any address space."""
 import ctypes
 
 import pytest
@@ -24,3 +25,22 @@ def test_scale_is_finite(L, scale):
     assert L.exl3_hip_attention_cached(view(), view(Q), 128, P, 4, 4, 16, 1, P, 9, P, 2, 1, scale, None, 0, None) == INVAL
     assert L.exl3_hip_attention_prompt(view(), view(heads=1), view(heads=1), view(Q), 128, P, P, 1, 3, 3, scale, 1, None,
                                        0, None) == INVAL
+
+
+WRAPS = (2, 1 << 35, 1 << 36, (1 << 29) + 1)  # heads, token stride, head stride, tokens: (tokens - 1) * stride is 2^64
+
+
+def test_views_whose_offsets_wrap(L):
+    """the overlap test's products wrap in 64 bits: token 2 of head 0 is token 0 of head 1, and passed as disjoint"""
+    heads, token, head, tokens = WRAPS
+    out = view(Q, heads, token, head)
+    one = view(heads=heads)
+    assert L.exl3_hip_qk_norm_rope(one, None, 1, tokens, 128, None, None, 0.0, None, None, 0, 0, 1.0, out, None, 1,
+                                   None) == INVAL
+    assert L.exl3_hip_kv_cache_read(P, 4, 4, 16, 128, P, tokens, out, out, 1, None, None) == INVAL
+    assert L.exl3_hip_attention_prompt(one, view(heads=1), view(heads=1), out, 128, P, P, 1, tokens, 3, 0.1, 1, None, 0,
+                                       None) == INVAL
+    # and rows that are only read, from 2^48 elements on
+    for x, n in ((view(P, 2, 1 << 40, 128), 1 << 9), (view(P, 300, 256, 1 << 40), 1)):
+        assert L.exl3_hip_qk_norm_rope(x, None, 1, n, 128, None, None, 0.0, None, None, 0, 0, 1.0,
+                                       view(Q, 2 if n > 1 else 300), None, 1, None) == INVAL

@@ -15,7 +15,9 @@ constexpr size_t kMaxGroup = 64;                 // q heads per kv head
 constexpr size_t kMaxTokens = (size_t)1 << 30;   // rows of a view: 32-bit row numbers in the kernels
 constexpr size_t kMaxSequences = 65536;
 constexpr size_t kMaxGridX = ((size_t)1 << 23) - 1;  // workgroups of 512: fewer than 2^32 work-items
-constexpr size_t kMaxStride = (size_t)1 << 40;   // elements: row * stride stays within 64 bits
+constexpr size_t kMaxStride = (size_t)1 << 40;   // elements
+constexpr size_t kMaxSpan = (size_t)1 << 48;     // elements from a view's first token (head) to its last: sums of the two
+                                                 // and their bytes stay far below 2^64
 
 exl3_status from_hip(hipError_t e) { return e == hipSuccess ? EXL3_OK : EXL3_HIP_ERROR; }
 bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
@@ -28,6 +30,9 @@ bool attention_dim(size_t d) { return d == 64 || d == 128 || d == 256; }
 bool head_view(const exl3_head_view *v, size_t tokens, size_t head_dim, exl3_dtype t, bool written, exl3k::Heads *out) {
     if (!v || (tokens && !v->data) || !aligned(v->data, dtype_size(t))) return false;
     if (v->heads < 1 || v->heads > kMaxHeads || v->token_stride > kMaxStride || v->head_stride > kMaxStride)
+        return false;
+    if ((tokens > 1 && v->token_stride > kMaxSpan / (tokens - 1)) ||
+        (v->heads > 1 && v->head_stride > kMaxSpan / (v->heads - 1)))
         return false;
     if (written) {
         const bool by_token = (v->heads == 1 || v->head_stride >= head_dim) &&
