@@ -44,3 +44,12 @@ def test_views_whose_offsets_wrap(L):
     for x, n in ((view(P, 2, 1 << 40, 128), 1 << 9), (view(P, 300, 256, 1 << 40), 1)):
         assert L.exl3_hip_qk_norm_rope(x, None, 1, n, 128, None, None, 0.0, None, None, 0, 0, 1.0,
                                        view(Q, 2 if n > 1 else 300), None, 1, None) == INVAL
+
+
+def test_partials_are_aligned(L):
+    """the partials of every (kv head, row tile) are read 16 bytes at a time: their sizes are whole 256 bytes, for odd rows,
+    tiles and partial counts too"""
+    prefix = (16 << 20) + 256  # the exchange and the status block
+    for hq, hk, d, seqs, q_len, tiles in ((10, 2, 128, 1, 1, 2), (3, 1, 64, 7, 1, 1), (9, 3, 256, 5, 3, 3), (7, 1, 64, 2, 5, 3)):
+        need = L.exl3_hip_attention_cached_workspace_bytes(hq, hk, d, seqs, q_len)
+        assert need > prefix and (need - prefix) % (256 * tiles) == 0, (hq, hk, d, seqs, q_len)

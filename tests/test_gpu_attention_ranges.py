@@ -71,3 +71,14 @@ def test_cached_groups_whose_products_pass_fp16(amd, case):
         got = run_cached(amd, q, pages, table, lens, hk, bits, p, q_len, scale=scale)
         assert np.isfinite(got).all()
         assert np.all(np.abs(got.astype(np.float64) - want) <= bound)
+
+
+@pytest.mark.parametrize("d,n", [(64, 53000), (128, 14000), (256, 6000)])
+def test_joined_apart_with_odd_rows(amd, d, n):
+    """five rows of each of two kv heads over one long sequence, whose parts a second kernel joins"""
+    print("  attention_cached", d, n, flush=True)
+    pages, table, kept = make_cache(amd, [n], 2, d, 4, 64)
+    q = rows(220, 1, 10, d, sigma=2.0)
+    want, bound = cached_reference(q, kept, 1, 2, d ** -0.5)
+    got = run_cached(amd, q, pages, table, [n], 2, 4, 64, 1)
+    assert np.all(np.abs(got.astype(np.float64) - want) <= bound)

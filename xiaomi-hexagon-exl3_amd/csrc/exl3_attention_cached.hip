@@ -277,15 +277,18 @@ __device__ __forceinline__ float over_groups_sum(float v) {
 }
 
 // Partials of one (kv head, row tile): sums [slot][rows][D], then (maximum, sum) [slot][rows], rows the
-// real rows of the tile; every tile has room for those of the first.  They cross XCDs, each with its own
+// real rows of the tile; every tile has room for those of the first, in whole 256 bytes (the join reads 16 at a time).  They cross XCDs, each with its own
 // L2, so they are stored and loaded as relaxed agent-scope atomics (coherent at device scope, no cache maintenance; a release fence writes
 // back a whole L2).
 struct Parts {
     unsigned long long *sums, *stats;  // pairs of binary32
 };
+__host__ __device__ constexpr size_t part_words(size_t d, size_t rows, size_t slots) {
+    return (slots * rows * (d / 2 + 1) + 31) / 32 * 32;
+}
 __device__ __forceinline__ Parts parts_of(void *ws, int d, int rows, size_t slots, size_t y) {
     Parts p;
-    p.sums = (unsigned long long *)ws + y * slots * (size_t)(rows * (d / 2 + 1));
+    p.sums = (unsigned long long *)ws + y * part_words(d, rows, slots);
     p.stats = p.sums + slots * (size_t)(rows * (d / 2));
     return p;
 }
@@ -314,7 +317,7 @@ __device__ __forceinline__ RowAt row_at(const CachedArgs &a, int s, int r, int k
     return x;
 }
 
-// the worker that has unit u (< all) of `active` workers: 32-bit arithmetic where it holds
+// the worker that has unit u (< all) of `active` workers, the last w with w all / active <= u: 32-bit arithmetic where it holds
 __device__ __forceinline__ long worker_of(long u, long active, long all) {
     const long n = (u + 1) * active - 1;
     return n <= 0xffffffffl && all <= 0xffffffffl ? (long)((uint32_t)n / (uint32_t)all) : n / all;
@@ -403,7 +406,6 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
         last = mul_div(w + 1, all, active);
         s = find_unit(sh, unit, lane, first);
     }
-    // the worker that holds unit u: the last w with w all / active <= u
     const Parts parts = parts_of(ws, D, min(kRows, a.q_len * group), slots, blockIdx.y);
     _Float16 *const qhi = (_Float16 *)lds, *const qlo = qhi + kRows * D;
     float *const q_unit = (float *)(qlo + kRows * D);         // of each row: 1, or 8 where an eighth is kept
@@ -885,7 +887,7 @@ bool attention_cached_fits(size_t q_heads, size_t kv_heads, size_t sequences, si
 
 size_t attention_cached_bytes(size_t q_heads, size_t kv_heads, size_t head_dim, size_t sequences, size_t q_len) {
     const CachedPlan p = cached_plan(q_heads, kv_heads, sequences, q_len);
-    return kSharedPrefixBytes + kv_heads * p.row_tiles * p.slots * p.rows * (head_dim + 2) * sizeof(float);
+    return kSharedPrefixBytes + kv_heads * p.row_tiles * part_words(head_dim, p.rows, p.slots) * sizeof(unsigned long long);
 }
 
 hipError_t launch_attention_cached(const CachedArgs &a, void *workspace, hipStream_t stream) {
