@@ -138,7 +138,9 @@ int exl3_hip_supports_op(exl3_op op, const exl3_tensor_info *dst, const exl3_ten
  * before its first use (exl3_hip_workspace_init).  One workspace serves any
  * sequence of calls when it holds at least exl3_hip_mul_mat_workspace_bytes(k,
  * n, rows) of every one of them; calls that share one must not run concurrently
- * (order them on one stream).  A GEMV call whose split-K partials would not fit
+ * (order them on one stream; a call may be several launches, so threads that share one
+ * make their calls one at a time.  The internal workspace, NULL, is held by a call until
+ * its launches are enqueued).  A GEMV call whose split-K partials would not fit
  * the 16 MiB runs the GEMM path instead (k * n above about 134 M weights at 32
  * rows). */
 size_t exl3_hip_mul_mat_workspace_bytes(size_t k, size_t n, size_t rows);

@@ -7,7 +7,6 @@
 
 #include <hip/hip_runtime.h>
 
-#include <map>
 #include <mutex>
 #include <algorithm>
 #include <utility>
@@ -15,6 +14,7 @@
 
 #include "exl3_attention.hpp"
 #include "exl3_launch.hpp"
+#include "exl3_workspace.hpp"
 
 namespace {
 
@@ -33,18 +33,23 @@ bool valid_matrix(size_t k, size_t n, size_t multiple) {
 }
 
 // Internal workspaces, one per (device, stream), grown on demand, zero-filled
-// when created and kept until process exit.  A workspace that is outgrown is retired, never freed: a call on another thread
-// may still be enqueuing kernels that use it.  Growth allocates, so it is
+// when created and kept until process exit.  A call holds its workspace until its launches are
+// enqueued (exl3_workspace.hpp).  A workspace that is outgrown is retired, never freed: kernels
+// that use it may still be running.  Growth allocates, so it is
 // refused while the stream is being captured into a HIP graph: a caller that
 // captures passes its own workspace, or makes one uncaptured call of the
 // largest shape first.
-struct InternalWs {
-    void *ptr = nullptr;
-    size_t bytes = 0;
-};
-std::mutex g_ws_mutex;
-std::map<std::pair<int, hipStream_t>, InternalWs> g_ws;
+typedef exl3k::WorkspaceTable<std::pair<int, hipStream_t>> InternalWorkspaces;
+InternalWorkspaces g_ws;
+std::mutex g_retired_mutex;
 std::vector<void *> g_ws_retired;
+
+// the workspace of the current device and this stream, held by the lease; null without a device
+InternalWorkspaces::Slot *internal_slot(hipStream_t stream, exl3k::WorkspaceLease *lease) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return nullptr;
+    return &g_ws.take(std::make_pair(dev, stream), lease);
+}
 
 // Calls f with the largest row count of each GEMM plan up to `rows` rows (a plan depends
 // on the tile height and the number of m-tiles; r_hi >= r, so every pass moves on).
@@ -60,11 +65,11 @@ void for_gemm_plans(size_t rows, F f) {
 }
 
 // `want` bytes if the workspace may grow, else the `need` it must have; *bytes: what it has.
-exl3_status internal_workspace(size_t need, size_t want, hipStream_t stream, void **out, size_t *bytes) {
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess) return EXL3_HIP_ERROR;
-    std::lock_guard<std::mutex> lock(g_ws_mutex);
-    InternalWs &ws = g_ws[std::make_pair(dev, stream)];
+exl3_status internal_workspace(size_t need, size_t want, hipStream_t stream, exl3k::WorkspaceLease *lease, void **out,
+                               size_t *bytes) {
+    InternalWorkspaces::Slot *const slot = internal_slot(stream, lease);
+    if (!slot) return EXL3_HIP_ERROR;
+    InternalWorkspaces::Slot &ws = *slot;
     if (ws.bytes < want) {
         hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
         if (hipStreamIsCapturing(stream, &capture) != hipSuccess) return EXL3_HIP_ERROR;
@@ -86,7 +91,10 @@ exl3_status internal_workspace(size_t need, size_t want, hipStream_t stream, voi
                     (void)hipFree(p);
                     return EXL3_HIP_ERROR;
                 }
-                if (ws.ptr) g_ws_retired.push_back(ws.ptr);
+                if (ws.ptr) {
+                    std::lock_guard<std::mutex> lock(g_retired_mutex);
+                    g_ws_retired.push_back(ws.ptr);
+                }
                 ws.ptr = p;
                 ws.bytes = grown;
             }
@@ -101,13 +109,15 @@ exl3_status internal_workspace(size_t need, size_t want, hipStream_t stream, voi
 // want() bytes where it may grow (a group's one GEMM launch takes more than its calls
 // one by one; the bits are the same either way).
 template <typename F>
-exl3_status call_workspace(size_t need, F want, hipStream_t stream, void **workspace, size_t *bytes) {
-    if (!*workspace) return internal_workspace(need, want(), stream, workspace, bytes);
+exl3_status call_workspace(size_t need, F want, hipStream_t stream, exl3k::WorkspaceLease *lease, void **workspace,
+                           size_t *bytes) {
+    if (!*workspace) return internal_workspace(need, want(), stream, lease, workspace, bytes);
     if (!aligned(*workspace, 256)) return EXL3_INVAL_PARAMS;
     return *bytes < need ? EXL3_WORKSPACE_TOO_SMALL : EXL3_OK;
 }
-exl3_status call_workspace(size_t need, hipStream_t stream, void **workspace, size_t *bytes) {
-    return call_workspace(need, [=] { return need; }, stream, workspace, bytes);
+exl3_status call_workspace(size_t need, hipStream_t stream, exl3k::WorkspaceLease *lease, void **workspace,
+                           size_t *bytes) {
+    return call_workspace(need, [=] { return need; }, stream, lease, workspace, bytes);
 }
 
 // Largest plan over every row count 1..rows and both paths a row count can take
@@ -162,8 +172,8 @@ size_t group_need(size_t k, const size_t *n, size_t count, size_t rows, bool fus
 }  // namespace
 
 namespace exl3k {
-exl3_status take_workspace(size_t need, hipStream_t stream, void **workspace, size_t *bytes) {
-    return call_workspace(need, stream, workspace, bytes);
+exl3_status take_workspace(size_t need, hipStream_t stream, WorkspaceLease *lease, void **workspace, size_t *bytes) {
+    return call_workspace(need, stream, lease, workspace, bytes);
 }
 }  // namespace exl3k
 
@@ -282,12 +292,10 @@ size_t exl3_hip_mul_mat_workspace_bytes(size_t k, size_t n, size_t rows) { retur
 
 exl3_status exl3_hip_workspace_init(void *workspace, size_t workspace_bytes, hipStream_t stream) {
     if (!workspace) {  // the internal workspace of (current device, stream), if there is one
-        int dev = 0;
-        if (hipGetDevice(&dev) != hipSuccess) return EXL3_HIP_ERROR;
-        std::lock_guard<std::mutex> lock(g_ws_mutex);
-        const auto it = g_ws.find(std::make_pair(dev, stream));
-        if (it == g_ws.end() || !it->second.ptr) return EXL3_OK;
-        return from_hip(exl3k::launch_zero(it->second.ptr, it->second.bytes, stream));
+        exl3k::WorkspaceLease lease;
+        const InternalWorkspaces::Slot *const ws = internal_slot(stream, &lease);
+        if (!ws) return EXL3_HIP_ERROR;
+        return ws->ptr ? from_hip(exl3k::launch_zero(ws->ptr, ws->bytes, stream)) : EXL3_OK;
     }
     if (!aligned(workspace, 256)) return EXL3_INVAL_PARAMS;
     return from_hip(exl3k::launch_zero(workspace, workspace_bytes, stream));
@@ -299,12 +307,11 @@ exl3_status exl3_hip_workspace_status(const void *workspace, size_t workspace_by
     *faulted = 0;
     const uint8_t *ws = (const uint8_t *)workspace;
     if (!ws) {
-        int dev = 0;
-        if (hipGetDevice(&dev) != hipSuccess) return EXL3_HIP_ERROR;
-        std::lock_guard<std::mutex> lock(g_ws_mutex);
-        const auto it = g_ws.find(std::make_pair(dev, stream));
-        if (it == g_ws.end() || !it->second.ptr) return EXL3_OK;  // never used: nothing can have failed
-        ws = (const uint8_t *)it->second.ptr;
+        exl3k::WorkspaceLease lease;
+        const InternalWorkspaces::Slot *const slot = internal_slot(stream, &lease);
+        if (!slot) return EXL3_HIP_ERROR;
+        if (!slot->ptr) return EXL3_OK;  // never used: nothing can have failed
+        ws = (const uint8_t *)slot->ptr;
     } else if (!aligned(ws, 256) || workspace_bytes < exl3k::kSharedPrefixBytes) {
         return EXL3_INVAL_PARAMS;
     }
@@ -329,7 +336,8 @@ static exl3_status mul_mat_impl(const void *records, unsigned bits, unsigned cod
     if (!records || !x || !y || !aligned(records, 16)) return EXL3_INVAL_PARAMS;
     if (!aligned(x, dtype_size(xt)) || !aligned(y, dtype_size(yt))) return EXL3_INVAL_PARAMS;
     if (x_row_stride < k || y_row_stride < n) return EXL3_INVAL_PARAMS;
-    const exl3_status st = call_workspace(mul_mat_need(k, n, rows), stream, &workspace, &workspace_bytes);
+    exl3k::WorkspaceLease lease;
+    const exl3_status st = call_workspace(mul_mat_need(k, n, rows), stream, &lease, &workspace, &workspace_bytes);
     if (st != EXL3_OK) return st;
     exl3k::GemvTargets tg{};
     tg.records[0] = (const uint8_t *)records;
@@ -389,9 +397,10 @@ exl3_status exl3_hip_mul_mat_group(const exl3_matrix_desc *mats, size_t count, u
     // enqueued, for whichever of the two paths below the call takes
     size_t ns[exl3k::kGemvMaxTargets];
     for (size_t i = 0; i < count; ++i) ns[i] = mats[i].n;
+    exl3k::WorkspaceLease lease;
     const exl3_status st = call_workspace(group_need(k, ns, count, rows, false),
-                                          [&] { return group_need(k, ns, count, rows, true); }, stream, &workspace,
-                                          &workspace_bytes);
+                                          [&] { return group_need(k, ns, count, rows, true); }, stream, &lease,
+                                          &workspace, &workspace_bytes);
     if (st != EXL3_OK) return st;
     if (count == 1)
         return exl3_hip_mul_mat(mats[0].records, bits, codebook, k, mats[0].n, x, xt, rows, x_row_stride, mats[0].y,
@@ -447,7 +456,8 @@ exl3_status exl3_hip_mul_mat_nd(const void *records, unsigned bits, unsigned cod
     if (!exl3_hip_supports_mul_mat(bits, codebook, k, n, rows, xt, yt) || !records || !x || !y)
         return EXL3_INVAL_PARAMS;
     // every call below needs at most this
-    const exl3_status wst = call_workspace(mul_mat_need(k, n, rows), stream, &workspace, &workspace_bytes);
+    exl3k::WorkspaceLease lease;
+    const exl3_status wst = call_workspace(mul_mat_need(k, n, rows), stream, &lease, &workspace, &workspace_bytes);
     if (wst != EXL3_OK) return wst;
     // Row dimensions 1, 2, 3 in order join one run while both views step through
     // them with one row stride (a run's stride at least a row, as exl3_hip_mul_mat
@@ -638,8 +648,9 @@ exl3_status exl3_hip_iface_matmul(unsigned bits, unsigned codebook, size_t k, si
     if (!packed || !suh || !svh || !x || !y) return EXL3_INVAL_PARAMS;
     if (!aligned(packed, 16) || !aligned(suh, 16) || !aligned(svh, 16) || !aligned(x, 4) || !aligned(y, 4))
         return EXL3_INVAL_PARAMS;
-    exl3_status st = call_workspace(exl3_hip_iface_matmul_workspace_bytes(bits, k, n, batch), stream, &workspace,
-                                    &workspace_bytes);
+    exl3k::WorkspaceLease lease;
+    exl3_status st = call_workspace(exl3_hip_iface_matmul_workspace_bytes(bits, k, n, batch), stream, &lease,
+                                    &workspace, &workspace_bytes);
     if (st != EXL3_OK) return st;
     // the GEMV reads the tiles as they are (2048 x 6144, 5 bits, batch 8: 15.0 -> 10.3 us per
     // call against packing records first); the GEMM, which reads each weight once per row

@@ -9,12 +9,13 @@
 #include <stdint.h>
 
 #include "exl3_hip.h"
+#include "exl3_workspace.hpp"
 
 namespace exl3k {
 
 // The caller's workspace checked, or the internal one of this device and stream
-// (exl3_api.cpp).
-exl3_status take_workspace(size_t need, hipStream_t stream, void **workspace, size_t *bytes);
+// (exl3_api.cpp), which the lease holds until the call's launches are enqueued.
+exl3_status take_workspace(size_t need, hipStream_t stream, WorkspaceLease *lease, void **workspace, size_t *bytes);
 
 // A view of heads inside a kernel (exl3_head_view).
 struct Heads {

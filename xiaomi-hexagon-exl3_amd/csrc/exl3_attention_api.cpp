@@ -166,7 +166,8 @@ exl3_status exl3_hip_attention_cached(const exl3_head_view *q, const exl3_head_v
         return EXL3_INVAL_PARAMS;
     if (!std::isfinite(scale)) return EXL3_INVAL_PARAMS;  // the kernels bound it from below, which a NaN would pass
     if (!exl3k::attention_cached_fits(q->heads, kv_heads, sequences, q_len)) return EXL3_NO_SUPPORT;
-    const exl3_status st = exl3k::take_workspace(need, stream, &workspace, &workspace_bytes);
+    exl3k::WorkspaceLease lease;
+    const exl3_status st = exl3k::take_workspace(need, stream, &lease, &workspace, &workspace_bytes);
     if (st != EXL3_OK) return st;
     a.pages = (const uint8_t *)pages;
     a.page_count = page_count;
@@ -217,8 +218,9 @@ exl3_status exl3_hip_attention_prompt(const exl3_head_view *q, const exl3_head_v
     a.causal = causal != 0;
     a.scale = scale;
     const size_t need = exl3k::attention_prompt_bytes(q->heads, a.head_dim, a.sequences, a.q_tokens, a.kv_tokens);
+    exl3k::WorkspaceLease lease;
     if (need) {
-        const exl3_status st = exl3k::take_workspace(need, stream, &workspace, &workspace_bytes);
+        const exl3_status st = exl3k::take_workspace(need, stream, &lease, &workspace, &workspace_bytes);
         if (st != EXL3_OK) return st;
     }
     return from_hip(exl3k::launch_attention_prompt(a, need ? workspace : nullptr, stream));
