@@ -196,11 +196,11 @@ template <int D, bool NEAR, int kGroups, bool SPLIT>
 __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prompt_kernel(PromptArgs a, int tiles, float *ws) {
     using P = Prompt<D>;
     constexpr int KT = P::KT;
-    __shared__ __align__(1024) _Float16 keys[kGroups][2][KT * D], values[kGroups][2][KT * D];
+    __shared__ __align__(1024) _Float16 tile_lds[2][kGroups][2][KT * D];  // keys, values; of each group two buffers
     const int tid = threadIdx.x % (64 * kPromptWaves), lane = tid & 63, m = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * kPromptWaves));
-    auto &ks = keys[group], &vs = values[group];
+    auto &ks = tile_lds[0][group], &vs = tile_lds[1][group];
     const int head = head_of(a, blockIdx.x);
     const Span sp = find_tile(a, tiles - 1 - (int)(blockIdx.x / a.q.heads), lane);  // a causal sequence's longest first
     if (!sp.nq) return;
@@ -421,8 +421,8 @@ __global__ __launch_bounds__(64 * kPromptWaves * kGroups, 2) void attention_prom
     if constexpr (kGroups == 2) {
         // the odd tiles' part into the even ones', register by register of the same lane
         __shared__ float stats[2][64 * kPromptWaves];
-        f4 *const parts = (f4 *)&keys[0][0][0];  // 16 NT floats a lane: half of the tiles' LDS
-        static_assert(sizeof(keys) + sizeof(values) >= 64 * kPromptWaves * 16 * P::NT * sizeof(float), "the tiles' LDS holds a group's sums");
+        f4 *const parts = (f4 *)tile_lds;  // 16 NT floats a lane: half of the tiles' LDS, at head dimension 256 all of it
+        static_assert(sizeof(tile_lds) >= 64 * kPromptWaves * 16 * P::NT * sizeof(float), "the tiles' LDS holds a group's sums");
         __syncthreads();
         if (group == 1) {
             stats[0][tid] = top;
