@@ -94,11 +94,14 @@ struct Prompt {
 
     // 16 bytes a lane into LDS, in lane order from `to`.  After the builtin of this instruction the compiler has
     // every LDS read wait for the load, since it cannot tell the buffers apart (a prompt of 320 tokens,
-    // 12 / 3 heads of 256: 21.5 against 20.6 us).  It writes no register; the place is read after a later step's wait and barrier.
+    // 12 / 3 heads of 256: 21.5 against 20.6 us).  The load writes no register, takes its address and m0 when it is
+    // issued, and m0 is given back: the compiler does not know that it was used.  What it writes in LDS is read
+    // after a later step's wait and barrier, and no read between belongs to the buffer that it fills.
     static __device__ __forceinline__ void load_chunk(const char *base, uint32_t at, _Float16 *to) {
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"((uint32_t)(uintptr_t)(lds_void *)to),
-                     "v"(at), "s"(base)
-                     : "m0");
+        uint32_t m0_was;
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                     : "=&s"(m0_was)
+                     : "s"((uint32_t)(uintptr_t)(lds_void *)to), "v"(at), "s"(base));
     }
     // Brings the tile at key n0 (keys beyond the last are the last) into an LDS tile; complete after a
     // wait for vmcnt and a barrier.  The loads write LDS directly, 16 bytes a lane in lane order, so the
