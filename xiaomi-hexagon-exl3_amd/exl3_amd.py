@@ -526,7 +526,8 @@ def validate_records(records, bits, stream=None):
 
 # ---- the attention block: rows of heads are [tokens, heads, head_dim] tensors, last dimension dense.
 # These calls go through exl3_torch.so (csrc/exl3_torch.cpp), which checks the tensors, allocates outputs
-# and enters libexl3_hip.so: at decode sizes the host time of a call is what counts.
+# and enters libexl3_hip.so: at decode sizes the host time of a call is what counts.  With stream given, new
+# outputs belong to that stream's memory pool, as tensors made under torch.cuda.stream(stream) do.
 TORCH_PATH = HERE / "exl3_torch.so"
 _TORCH = None
 
