@@ -59,3 +59,12 @@ def test_tensors_of_the_host_and_of_two_devices_are_refused(amd):
     if torch.cuda.device_count() > 1:
         with pytest.raises(AssertionError, match="different devices"):
             amd.attention_prompt(x, x, x, starts.to("cuda:1"))
+
+
+def test_bits_are_not_cut_to_32_bits(amd):
+    import torch
+    x = torch.zeros(1, HK, D, dtype=torch.float16, device="cuda")
+    pages, slots = amd.new_kv_cache(1, HK, D, 4, P), torch.zeros(1, dtype=torch.int64, device="cuda")
+    for bits in (0, 5, (1 << 32) + 4):
+        with pytest.raises((AssertionError, amd.Exl3Error)):
+            amd.kv_cache_write(pages, x, x, slots, bits=bits, page_tokens=P)

@@ -185,7 +185,9 @@ struct Pages {
 Pages pages_of(Call &c, PyObject *o, PyObject *bits, PyObject *page_tokens, size_t kv_heads, size_t head_dim) {
     const at::Tensor &t = c.tensor(o, "pages is a tensor");
     need(t.scalar_type() == at::kByte && t.dim() == 2 && t.is_contiguous(), "pages: dense uint8 [pages, page bytes]");
-    Pages p{t.data_ptr(), (size_t)t.size(0), count_of(page_tokens), (unsigned)count_of(bits)};
+    const size_t b = count_of(bits);
+    need(b == 4 || b == 8, "bits: 4 or 8");
+    Pages p{t.data_ptr(), (size_t)t.size(0), count_of(page_tokens), (unsigned)b};
     need((size_t)t.size(1) == exl3_hip_kv_page_bytes(p.bits, kv_heads, head_dim, p.tokens), "page bytes");
     return p;
 }
