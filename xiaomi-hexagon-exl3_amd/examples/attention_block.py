@@ -56,16 +56,23 @@ class AttentionBlock:
         return self.amd.pack_records(packed, su, sv, self.bits, k, n)
 
     # ---- sequences and their pages
-    def _extend(self, seq, tokens):
-        """pages for `tokens` more tokens of a sequence; the slots of those tokens"""
-        p, start = self.cache["page_tokens"], self.length.get(seq, 0)
-        own = self.owned.setdefault(seq, [])
-        while len(own) * p < start + tokens:
-            if not self.free:
-                raise RuntimeError("the cache has no free page")
-            own.append(self.free.pop())
-        self.length[seq] = start + tokens
-        return [own[t // p] * p + t % p for t in range(start, start + tokens)]
+    def _extend(self, seqs, tokens):
+        """pages for tokens[i] more tokens of each sequence; the slots of those tokens.  All of them or, by an exception,
+        none."""
+        p = self.cache["page_tokens"]
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence is named twice")
+        start = [self.length.get(s, 0) for s in seqs]
+        more = [max(0, -(-(at + n) // p) - len(self.owned.get(s, ()))) for s, at, n in zip(seqs, start, tokens)]
+        if sum(more) > len(self.free):
+            raise RuntimeError("the cache has no free page")
+        slots = []
+        for s, at, n, pages in zip(seqs, start, tokens, more):
+            own = self.owned.setdefault(s, [])
+            own += [self.free.pop() for _ in range(pages)]
+            self.length[s] = at + n
+            slots += [own[t // p] * p + t % p for t in range(at, at + n)]
+        return slots
 
     def release(self, seq):
         self.free += reversed(self.owned.pop(seq, []))
@@ -92,12 +99,12 @@ class AttentionBlock:
         """x [sum of lengths, hidden]: the tokens of new sequences, one after the other.  Attention runs over keys
         and values as computed; the cache receives them for the steps that follow.  The layers take up to 65,536
         tokens in a call.  -> [tokens, hidden]"""
-        slots, positions, starts = [], [], [0]
-        for s, n in zip(seqs, lengths):
+        for s in seqs:
             if s in self.length:
                 raise ValueError(f"sequence {s} has been started")
+        slots, positions, starts = self._extend(seqs, lengths), [], [0]
+        for n in lengths:
             positions += range(n)
-            slots += self._extend(s, n)
             starts.append(starts[-1] + n)
         positions, starts = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in (positions, starts))
         q, k, v = self._qkv(x, positions)
@@ -106,9 +113,7 @@ class AttentionBlock:
 
     def plan(self, seqs, tokens=1):
         """the next `tokens` tokens of each sequence: (positions, slots, page table, lengths) on the GPU"""
-        slots = []
-        for s in seqs:
-            slots += self._extend(s, tokens)
+        slots = self._extend(seqs, [tokens] * len(seqs))
         lens = [self.length[s] for s in seqs]
         wide = max(len(self.owned[s]) for s in seqs)
         table = [self.owned[s] + [-1] * (wide - len(self.owned[s])) for s in seqs]
