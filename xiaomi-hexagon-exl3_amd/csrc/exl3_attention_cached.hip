@@ -16,8 +16,7 @@
 //   V: a lane's block of four tokens holds those four keys for its slice of D / 16 elements;
 //      the A operand of O^T tile t is element t of the slice: row m of the tile is element
 //      m D / 16 + t of the head.
-// Every value scale * code has at most 11 significant bits, so dequantising adds no rounding; groups that
-// pass fp16's range (one extreme above 65,504 after the rotation) are multiplied apart, at 2^-8.  The queries are
+// Dequantising adds no rounding and leaves no value out of fp16's range (Masks).  The queries are
 // rotated by H32 like the cached rows and kept as an fp16 pair (high and low part: two
 // MFMAs, which the VALU work hides; a row that the rotation could take beyond fp16's range is kept as an eighth, with
 // eight times its factor in the exponent); the result is rotated back at the end.
@@ -131,25 +130,30 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[N]) {
     }
 }
 
-// The masks and the 1024 (0x6400) that codes are or-ed into, in registers: a v_and_or_b32 takes no literals, so
-// with constants each is a v_and and a v_or.
+// Codes become fp16 numbers code / 2^(BITS - 1), -1 to just below 1, by or-ing them into the last bits of a number
+// whose spacing is that (128 at 4 bits, 8 at 8) and taking it off again.  Times a scale of 12 - BITS significant bits
+// that is exact to the last subnormal (whole multiples of 2^-24) and within fp16's range for every finite scale
+// (65,280 at most), where code * scale is not: 32 equal elements of 12,000 rotate to 67,882.  The power of two is in the
+// exponent's factor and in the last division.
+// The masks and that number are in registers: a v_and_or_b32 takes no literals, so with constants each is a
+// v_and and a v_or.
+template <int BITS>
 struct Masks {
     uint32_t low, high, base;  // scalar, scalar, vector
-    __device__ __forceinline__ Masks() : low(0x000f000fu), high(0x00f000f0u), base(0x64006400u) {
+    __device__ __forceinline__ Masks() : low(0x000f000fu), high(0x00f000f0u), base(BITS == 4 ? 0x58005800u : 0x48004800u) {
         asm volatile("" : "+s"(low), "+s"(high), "+v"(base));
     }
 };
-// Two 4-bit codes in the halves' bits 0..3, or 4..7, as fp16 values -8 .. 7: in 1024 (spacing 1) they give
-// 1024 + c and 1024 + 16 c exactly.
-__device__ __forceinline__ h2 low_codes(uint32_t w, const Masks &k) {
-    return bitcast<h2>((w & k.low) | k.base) + (h2){(_Float16)-1032.f, (_Float16)-1032.f};
+// two 4-bit codes in the halves' bits 0..3, or 4..7: 128 + c / 8 and 128 + 2 c
+__device__ __forceinline__ h2 low_codes(uint32_t w, const Masks<4> &k) {
+    return bitcast<h2>((w & k.low) | k.base) + (h2){(_Float16)-129.f, (_Float16)-129.f};
 }
-__device__ __forceinline__ h2 high_codes(uint32_t w, const Masks &k) {
+__device__ __forceinline__ h2 high_codes(uint32_t w, const Masks<4> &k) {
     return __builtin_elementwise_fma(bitcast<h2>((w & k.high) | k.base), (h2){(_Float16)0.0625f, (_Float16)0.0625f},
-                                     (h2){(_Float16)-72.f, (_Float16)-72.f});
+                                     (h2){(_Float16)-9.f, (_Float16)-9.f});
 }
-__device__ __forceinline__ h2 byte_codes(uint32_t w, const Masks &k) {  // 8 bits: -128 .. 127
-    return bitcast<h2>(w | k.base) + (h2){(_Float16)-1152.f, (_Float16)-1152.f};
+__device__ __forceinline__ h2 byte_codes(uint32_t w, const Masks<8> &k) {  // 8 bits: 8 + c / 128
+    return bitcast<h2>(w | k.base) + (h2){(_Float16)-9.f, (_Float16)-9.f};
 }
 
 template <int D, int BITS>
@@ -186,7 +190,7 @@ struct Cached {
 
     // Fragment j of a lane's key: elements 8 j .. 8 j + 7 of its quarter row, in the order that
     // q_order undoes.
-    static __device__ __forceinline__ h8 key(const Half &h, int j, const Masks &c) {
+    static __device__ __forceinline__ h8 key(const Half &h, int j, const Masks<BITS> &c) {
         const uint32_t sw = G == 8 ? (j < 4 ? h.ks & 0xffffu : h.ks >> 16) : h.ks;
         const _Float16 s = bitcast<_Float16>((uint16_t)sw);
         const h2 s2 = {s, s};
@@ -212,33 +216,8 @@ struct Cached {
         else return v;
     }
 
-    // Scales whose product with the lowest code, -2^(BITS - 1), is beyond fp16 (one step more than 65,504), or that are
-    // not finite: their groups are taken apart from the others, at 2^-8 of their size, which is exact for them.
-    static constexpr uint32_t kLargeScale = BITS == 4 ? 0x7000u : 0x6000u;  // 8,192, 512
-    static __device__ __forceinline__ bool any_large(const Half (&h)[2]) {
-        constexpr uint32_t magnitude = 0x7fff7fffu;
-        typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-        us2 most = bitcast<us2>(h[0].ks & magnitude);
-        for (const uint32_t w : {h[0].vs.x, h[0].vs.y, h[1].ks, h[1].vs.x, h[1].vs.y})
-            most = __builtin_elementwise_max(most, bitcast<us2>(w & magnitude));
-        return __ballot((bitcast<uint32_t>(most) + (0x8000u - kLargeScale) * 0x10001u) & 0x80008000u) != 0;
-    }
-    static __device__ __forceinline__ uint32_t large_mask(uint32_t w) {
-        return ((((w & 0x7fff7fffu) + (0x8000u - kLargeScale) * 0x10001u) >> 15) & 0x10001u) * 0xffffu;
-    }
-    // the large ones of two scales, times 2^-8, and the others
-    static __device__ __forceinline__ uint32_t large_only(uint32_t w) {
-        return bitcast<uint32_t>(bitcast<h2>(w & large_mask(w)) * (h2){(_Float16)0x1p-8f, (_Float16)0x1p-8f});
-    }
-    static __device__ __forceinline__ uint32_t without_large(uint32_t w) { return w & ~large_mask(w); }
-    // keeps the compiler from holding the numbers made of these words for their next use
-    static __device__ __forceinline__ void forget(uint32_t (&w)[NW]) {
-#pragma unroll
-        for (int i = 0; i < NW; ++i) asm volatile("" : "+v"(w[i]));
-    }
-
     // element t of the lane's slice for its four tokens (as two pairs)
-    static __device__ __forceinline__ void value(const Half &h, int t, h2 &a, h2 &b, const Masks &c) {
+    static __device__ __forceinline__ void value(const Half &h, int t, h2 &a, h2 &b, const Masks<BITS> &c) {
         const h2 s01 = bitcast<h2>(h.vs.x), s23 = bitcast<h2>(h.vs.y);
         if constexpr (D == 64 && BITS == 4) {  // 2-byte slices: a word holds two tokens
             const uint32_t x = t < 2 ? h.v[0] : h.v[0] >> 8, y = t < 2 ? h.v[1] : h.v[1] >> 8;
@@ -328,7 +307,7 @@ __device__ __forceinline__ long worker_of(long u, long active, long all) {
 __device__ __forceinline__ void finish_row(const CachedArgs &a, int s, int len, int r, int kvh, int group, int l8, int lane,
                                            bool faulted, bool store, float (&v)[8], float total) {
     const bool sees = len > a.q_len - 1 - r / group;
-    const float inv = faulted ? __builtin_nanf("") : 1.0f / total;
+    const float inv = faulted ? __builtin_nanf("") : (float)(1 << (a.l.bits - 1)) / total;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = sees ? v[e] * inv : 0.f;
     h32_run8(v, lane);
@@ -413,7 +392,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
     // the largest score is that of the largest product: a negative scale goes into the queries' signs (and 0 *
     // -infinity, the masked places of a zero scale, must stay -infinity)
     const float c = fmaxf(__builtin_fabsf(a.scale) * kLog2e, 1e-30f), sign = a.scale < 0.f ? -1.f : 1.f;
-    const Masks masks;
+    const Masks<BITS> masks;
     const typename C::Lane at_lane = C::lane_of(m, g);
 
     while (unit < last && s < a.sequences) {  // one sequence's part at a time
@@ -490,7 +469,7 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             bh[j] = C::q_order(*(const h8 *)(qhi + m * D + g * (D / 4) + 8 * j));
             bl[j] = C::q_order(*(const h8 *)(qlo + m * D + g * (D / 4) + 8 * j));
         }
-        const float cq = c * q_unit[m];
+        const float cq = c * q_unit[m] * (1 << (BITS - 1));
         // keys that this lane's row sees
         const int limit = len - (a.q_len - 1 - (row0 + m) / group);
 
@@ -536,29 +515,15 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
             }
             f4 st[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) st[i] = (f4){0.f, 0.f, 0.f, 0.f};
-            auto add_scores = [&](const typename C::Half &h, f4 &to) {
+            for (int i = 0; i < 2; ++i) {
+                st[i] = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < C::NJ; ++j) {
-                    const h8 k = C::key(h, j, masks);
-                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, bl[j], to, 0, 0, 0);
-                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, bh[j], to, 0, 0, 0);
-                }
-            };
-            const bool large = C::any_large(cur);  // rare
-            if (__builtin_expect(large, false)) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t scales = cur[i].ks;
-                    cur[i].ks = C::large_only(scales);
-                    add_scores(cur[i], st[i]);
-                    st[i] *= 256.f;
-                    cur[i].ks = C::without_large(scales);
-                    C::forget(cur[i].k);
+                    const h8 k = C::key(cur[i], j, masks);
+                    st[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, bl[j], st[i], 0, 0, 0);
+                    st[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, bh[j], st[i], 0, 0, 0);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) add_scores(cur[i], st[i]);
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = st[e >> 2][e & 3];
@@ -588,27 +553,14 @@ __global__ __launch_bounds__(64 * cached_waves(D)) void attention_cached_kernel(
                 sum += v;
                 p[e] = (_Float16)v;
             }
-            auto weighted = [&](const typename C::Half (&h)[2], int t, f4 to) {
+#pragma unroll
+            for (int t = 0; t < C::NT; ++t) {
                 h2 v[4];
-                C::value(h[0], t, v[0], v[1], masks);
-                C::value(h[1], t, v[2], v[3], masks);
+                C::value(cur[0], t, v[0], v[1], masks);
+                C::value(cur[1], t, v[2], v[3], masks);
                 const h8 vt = {v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
-                return __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, p, to, 0, 0, 0);
-            };
-            if (__builtin_expect(large, false)) {
-                const u2 scales[2] = {cur[0].vs, cur[1].vs};
-#pragma unroll
-                for (int i = 0; i < 2; ++i) cur[i].vs = (u2){C::large_only(scales[i].x), C::large_only(scales[i].y)};
-#pragma unroll
-                for (int t = 0; t < C::NT; ++t) o[t] = weighted(cur, t, o[t] * 0x1p-8f) * 256.f;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    cur[i].vs = (u2){C::without_large(scales[i].x), C::without_large(scales[i].y)};
-                    C::forget(cur[i].v);
-                }
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, p, o[t], 0, 0, 0);
             }
-#pragma unroll
-            for (int t = 0; t < C::NT; ++t) o[t] = weighted(cur, t, o[t]);
             if (edge && __ballot(lost)) {  // rare: NaN for the rows that see such a token, in its group's elements
                 for (int n = n0; n < n0 + kTile && n < len; ++n) {
                     const int page = n / a.l.page_tokens, id = table[page];
