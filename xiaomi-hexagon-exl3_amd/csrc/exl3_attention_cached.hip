@@ -20,9 +20,9 @@
 // rotated by H32 like the cached rows and kept as an fp16 pair (high and low part: two
 // MFMAs, which the VALU work hides; a row that the rotation could take beyond fp16's range is kept as an eighth, with
 // eight times its factor in the exponent); the result is rotated back at the end.
-// 16 sequences of 32,768 tokens, 32 / 8 heads of 128 at 4 bits (604 MB): 120 us, 5.0 TB/s, the rate of a large
-// copy, with the VALU at work 64 % of the time; 1,000 tokens, 8 / 2 heads of 256: 13.1 us, a launch and four
-// dependent round trips.
+// 16 sequences of 32,768 tokens, 32 / 8 heads of 128 at 4 bits (604 MB): 117 to 122 us, 5.0 to 5.2 TB/s, the rate of a
+// large copy, with the VALU at work 62 % of the time; of 20,000 at 8 bits: 124 us, 5.6 TB/s; 1,000 tokens, 8 / 2
+// heads of 256: 13.2 us, a launch and four dependent round trips.
 #include "exl3_head_rows.hpp"
 
 namespace exl3k {

@@ -12,10 +12,11 @@
 // the tile, read with ds_read_b64_tr_b16: within 16 lanes it hands lane i the i-th of 16 elements of
 // four rows.  16-byte chunks of a row are swizzled so that the rows of one read lie in
 // different banks.
-// One causal prompt of 8,192 tokens, 32 / 8 heads of 128: 532 us, 1,034 TFLOP/s, at the 1.63 GHz that
-// the chip's power leaves (a large fp16 product: 1,150 to 1,390); seven packed prompts of up to 2,111 tokens, some after
-// 500 others, 16 / 4 heads of 64: 46 us, 518 TFLOP/s, bound by the exponentials (two MFMAs of 32 cycles for 16 of them
-// a lane) and the longest sequence's last tiles; 37 tokens, 8 / 2 heads of 256: 9.6 us.
+// One causal prompt of 8,192 tokens, 32 / 8 heads of 128: 532 to 547 us, 1,005 to 1,034 TFLOP/s, at the 1.63 to 1.69 GHz
+// that the chip's power leaves (a large fp16 product: 1,150 to 1,390); seven packed prompts of up to 2,111 tokens, some
+// after 500 others, 16 / 4 heads of 64: 47 us, 507 TFLOP/s, bound by waves that are not there (1.2 resident a SIMD on
+// average where three fit): the longest sequence has 272 of the 650 workgroups, of up to 41 tiles each, and comes
+// last; 37 tokens, 8 / 2 heads of 256: 9.6 us.
 #include "exl3_head_rows.hpp"
 
 namespace exl3k {
@@ -30,9 +31,9 @@ typedef __attribute__((address_space(3))) h8 lds_h8;
 constexpr int kPromptWaves = 4;  // of a group
 constexpr int kPromptRows = 32 * kPromptWaves;  // query rows of a workgroup
 // Two groups of waves per workgroup, which share its keys, where one would leave CUs idle and the walk is long:
-// one prompt of 2,000 tokens, 8 / 2 heads of 256 (136 workgroups): 60.9 against 73.4 us, of 128: 34.2 against
-// 37.7; but 300 tokens of 128: 12.7 against 11.6, and seven packed prompts, 16 / 4 heads of 64 (650
-// workgroups): 55.8 against 49.6.
+// one prompt of 3,000 tokens, 8 / 2 heads of 256 (192 workgroups): 80 against 107 us, of 128: 40.9 against
+// 49.0; but 300 tokens, 64 / 8 heads of 128 (192 workgroups): 12.5 against 11.5, and seven packed prompts, 16 / 4 heads
+// of 64 (650 workgroups): 48.2 against 46.9.
 constexpr size_t kTwoGroups = 256, kTwoGroupsKeys = 512;  // at most workgroups, at least keys of a sequence on average
 constexpr float kStart = -1e30f;                // running maximum before the first key
 constexpr float kSlack = 8.f;                   // scores may pass the running maximum by 2^8
@@ -515,8 +516,8 @@ int prompt_tiles(int q_tokens, int sequences) { return q_tokens / kPromptRows + 
 // Parts of a walk.  Where the workgroups leave CUs idle, parts of the keys go to them, one workgroup a CU, and a
 // second kernel joins the parts.  A round of two tiles takes 1.3 us, the join 4 us and 0.3 us a part more, so
 // r rounds are best cut in about 2 sqrt(r), and the cut has to save 5 of them: 16 tokens after 8,192 others,
-// 32 / 8 heads of 128: 26.8 against 95.8 us (8 parts), 8 / 2 heads of 256: 29.6 against 188.6 (16); 1,000 tokens,
-// 4 / 1 heads of 128: 15.7 against 19.8 (5); but four prompts of 300 after 256 others: 16.1 against 15.1 (4).
+// 32 / 8 heads of 128: 26.9 against 94.9 us (8 parts), 8 / 2 heads of 256: 30.2 against 194.7 (16); 1,000 tokens,
+// 4 / 1 heads of 128: 16.0 against 20.4 (5); 2,000 tokens, 8 / 2 heads of 256: 49.0 against 58.9 (2); but four prompts of 300 after 256 others: 16.1 against 15.1 (4).
 // More workgroups than CUs: 2,000 tokens, 4 / 1 heads of 128: 28.6 us at 6 parts, 20.4 at 4.
 constexpr size_t kSplitGroups = 256, kSplitGain = 5;
 int prompt_parts(size_t q_heads, int head_dim, int sequences, int q_tokens, int kv_tokens) {

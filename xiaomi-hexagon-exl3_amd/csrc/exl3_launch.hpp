@@ -26,11 +26,13 @@ constexpr int kGemvSingleMaxRows = 14;
 constexpr int kGemvSinglePrepBlocks = 64;
 constexpr int kGemvWaves = 8;     // waves per GEMV workgroup (a multiple of 4)
 
-// Every plan starts with the same region, which only the GEMV's split-K hand-off
-// touches: the exchange, kGemvExchangeBytes of 32-bit words carrying split
-// partials.  It is zero before a workspace's first use, every GEMV call leaves
-// it zero again (the workgroup that sums a column group's partials clears what
-// it consumed) and no other kernel writes it.  One workspace therefore serves
+// Every plan starts with the same region, the exchange, kGemvExchangeBytes of 32-bit
+// words.  It is zero before a workspace's first use.  Two kernels write it, and each call
+// of theirs leaves it zero again: the GEMV's split-K hand-off, which keeps split
+// partials there (the workgroup that sums a column group's partials clears what
+// it consumed), and attention over the cache, which counts there the parts of a (row tile,
+// sequence) that have arrived (the workgroup that finds the last one clears the
+// count).  One workspace therefore serves
 // calls of any shape and row count in turn, when it is as large as each needs.
 // A GEMV whose partials would not fit the exchange runs as a GEMM instead.  The
 // GEMM splits k only while it has fewer than kGemmSplitTiles output tiles; a

@@ -3,8 +3,9 @@
 // y = x / sqrt(mean(x^2) + eps) * weight, then each pair (a, b) turned by position * frequency.  Bound by
 // the rows' bytes, each read and written once: D / 8 lanes hold a row, its pairs meet by lane exchange or
 // within a lane, and the sines are worked out in the kernel (a table would be read as often as the rows).
-// 8,192 tokens, 32 / 8 heads of 128 in fp16: 30 us in a kernel trace (5.6 TB/s), 44 us a call in a loop of calls; one
-// token: 3.1 us, a launch and two dependent round trips.
+// 8,192 tokens, 32 / 8 heads of 128 in fp16 (168 MB): 44 us a call over buffers in turn (3.8 TB/s), 35 us over
+// the same ones, which the 256 MB cache holds (30 us in a kernel trace); one token: 3.1 us, a launch and two dependent
+// round trips.
 #include "exl3_head_rows.hpp"
 
 namespace exl3k {

@@ -1,8 +1,8 @@
 // exl3_torch.cpp -- the attention block's C-ABI for torch tensors, as a CPython module.
 //
 // Through ctypes, with views, checks and allocations in Python, the host time of a call is several
-// times its kernel's at decode sizes: one token's qk_norm_rope took 16.8 us a call, here 5.3; a cache
-// write and read of eight tokens 24.3, here 9.0.  The module
+// times its kernel's at decode sizes: one token's qk_norm_rope took 16.8 us a call, here 5.2; a cache
+// write and read of eight tokens 24.3, here 9.2.  The module
 // holds no state and no kernels: every function ends in one exl3_hip_* call.  A refused
 // argument raises AssertionError; a status other than EXL3_OK is returned as an int.
 #include <torch/csrc/Dtype.h>
