@@ -500,6 +500,87 @@ exl3_status exl3_hip_attention_prompt(const exl3_head_view *q, const exl3_head_v
 size_t exl3_hip_attention_prompt_workspace_bytes(size_t q_heads, size_t head_dim, size_t sequences, size_t q_tokens,
                                                  size_t kv_tokens);
 
+/* ---- the linear-attention block and the norms between blocks --------------
+ * Beside the attention block: the operators of a hybrid model's linear-attention layer between
+ * its projections and its output layer, and the norm ahead of a layer.  The reference leaves
+ * these to llama.cpp's graph too.  In the order of a layer:
+ *   exl3_hip_rms_norm    the block's input: residual addition and norm
+ *   exl3_hip_short_conv  the projected rows through a causal depthwise convolution
+ *   exl3_hip_delta_rule  the gated delta rule over the sequences
+ *   exl3_hip_rms_norm    each head's norm, gated
+ * Rows are packed sequences: sequence s has the rows starts[s] .. starts[s + 1] - 1 (device
+ * int32[sequences + 1], ascending from 0); with starts NULL each has tokens / sequences rows
+ * (a whole number).  No row outside the views is read or written, whatever the starts hold; a
+ * row that no sequence has is not written.
+ * A sequence goes on from a state that an earlier call left.  States lie in a pool of `slots`
+ * of them: sequence s starts from state slots_in[s] (from zeros where that is negative or
+ * slots_in is NULL) and leaves its state in slots_out[s] (nowhere where that is negative or
+ * slots_out is NULL); both device int32[sequences].  A slot_in beyond the pool counts as a state
+ * of NaN, a slot_out beyond the pool is not written.  A slot that a sequence leaves its state in is
+ * no other sequence's in the call, in or out; it may be its own slot_in.  A sequence without rows leaves
+ * the state that it starts from. */
+
+/* Root-mean-square norm of rows of heads:
+ *   h = x + residual                                   (residual NULL: h = x)
+ *   out = h / sqrt(mean(h^2) + eps) * weight * silu(gate)   (weight NULL: 1; gate NULL: no factor)
+ *   residual_out = h                                   (NULL: not kept; needs a residual)
+ * with silu(z) = z / (1 + exp(-z)).  Computed in fp32 from h as summed, each output rounded once.
+ *   x, gate    xt rows; all views have x's heads, each head `width` elements, 1 .. 65536
+ *   residual, residual_out   rt rows
+ *   weight     device fp32[width] or NULL, shared by the heads
+ *   out        yt rows.  out may be x's view (xt = yt) and residual_out residual's; otherwise
+ *              outputs are disjoint from the inputs and from each other
+ * tokens = 0 is a no-op. */
+exl3_status exl3_hip_rms_norm(const exl3_head_view *x, const exl3_head_view *gate, exl3_dtype xt,
+                              const exl3_head_view *residual, const exl3_head_view *residual_out, exl3_dtype rt,
+                              size_t tokens, size_t width, const float *weight, float eps, const exl3_head_view *out,
+                              exl3_dtype yt, hipStream_t stream);
+
+/* Causal depthwise convolution of packed sequences:
+ *   y[t][c] = act(bias[c] + sum_j weight[c][j] x[t - (width - 1) + j][c]),  j < width
+ * where rows ahead of a sequence's first come from its state, and act is silu or the identity.
+ * The state it leaves is its last width - 1 rows (those of the old state counted where it is
+ * shorter), in xt: [slots][width - 1][channels], the oldest first.  Sums in fp32, rounded once.
+ *   x, y       rows of `channels` elements, row strides in elements (at least channels), disjoint
+ *   channels   1 .. 2^20; width 2 .. 4
+ *   weight     device fp32[channels][width]; bias device fp32[channels] or NULL
+ *   states     device, 16-byte aligned, or NULL with both slot lists NULL
+ * EXL3_NO_SUPPORT where (tokens / 32 + sequences) * ceil(channels / 256) reaches 2^23.
+ * sequences = 0 is a no-op. */
+exl3_status exl3_hip_short_conv(const void *x, exl3_dtype xt, size_t x_row_stride, size_t tokens, size_t channels,
+                                const float *weight, size_t width, const float *bias, int silu, const int32_t *starts,
+                                size_t sequences, void *states, size_t slots, const int32_t *slots_in,
+                                const int32_t *slots_out, void *y, exl3_dtype yt, size_t y_row_stride,
+                                hipStream_t stream);
+
+/* The gated delta rule of packed sequences.  Value head h has a state S, fp32 [key_dim][value_dim],
+ * and reads key head h / (v heads / k heads); for each row in turn
+ *   S <- exp(g) S,   u = beta (v - S^T k),   S <- S + k u^T,   out = scale S^T q
+ * with q and k divided by sqrt(sum(x^2) + qk_eps) first (qk_eps negative: as they are), and
+ *   g = -exp(a_log) softplus(g_in + dt_bias),  beta = 1 / (1 + exp(-beta_in))
+ * where a_log is given, else g_in (a log decay, at most 0 in earnest; -inf empties the state) and beta_in.
+ *   q, k       F16, the same heads; v, out F16, v heads a multiple of k heads; out disjoint from all
+ *   key_dim    64 or 128; value_dim a multiple of 16 up to 256
+ *   g, beta    device fp32, row t of v heads at t * gate_stride (at least v heads) elements
+ *   a_log, dt_bias   device fp32[v heads], both or neither
+ *   states     device fp32 [slots][v heads][key_dim][value_dim], 16-byte aligned, or NULL with both
+ *              slot lists NULL
+ *   scale      finite
+ *   workspace  device, 256-byte aligned, >= exl3_hip_delta_rule_workspace_bytes() where that is
+ *              not 0; it may be one that other calls use too.  NULL: the internal one of this stream
+ * States and sums in fp32; products of the prompt kernel as fp16 pairs (high and low part, 22
+ * bits).  The same inputs give the same bits on every call.  EXL3_NO_SUPPORT where (tokens / 64 +
+ * sequences) * v heads * ceil(value_dim / 16) reaches 2^23.  sequences = 0 is a no-op. */
+exl3_status exl3_hip_delta_rule(const exl3_head_view *q, const exl3_head_view *k, const exl3_head_view *v,
+                                const float *g, const float *beta, size_t gate_stride, const float *a_log,
+                                const float *dt_bias, const exl3_head_view *out, size_t key_dim, size_t value_dim,
+                                const int32_t *starts, size_t sequences, size_t tokens, float *states, size_t slots,
+                                const int32_t *slots_in, const int32_t *slots_out, float scale, float qk_eps,
+                                void *workspace, size_t workspace_bytes, hipStream_t stream);
+/* 0 where exl3_hip_delta_rule takes no workspace (and for arguments that it refuses) */
+size_t exl3_hip_delta_rule_workspace_bytes(size_t v_heads, size_t key_dim, size_t value_dim, size_t sequences,
+                                           size_t tokens);
+
 /* *result (device int) = 1 when every su/sv value of every record is finite,
  * 0 otherwise; EXL3_INVAL_PARAMS when nbytes is not a whole number of records. */
 exl3_status exl3_hip_validate_records(const void *records, size_t nbytes, unsigned bits, int *result,

@@ -1,0 +1,55 @@
+// exl3_linear_attention.hpp -- internal interface between the C-ABI of the linear-attention block
+// (exl3_linear_attention_api.cpp) and its gfx950 kernels (exl3_rms_norm.hip, exl3_short_conv.hip,
+// exl3_delta_{step,prompt}.hip).  Launchers assume validated arguments; they only enqueue work
+// and return hipGetLastError().
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "exl3_attention.hpp"
+
+namespace exl3k {
+
+struct NormArgs {
+    Heads x, gate, res, res_out, out;  // data null where left out
+    const float *weight;
+    size_t tokens;
+    int width, x_f16, res_f16, y_f16;
+    int vec;  // every run of eight elements of each view is 16-byte aligned, and width whole runs
+    float eps;
+};
+hipError_t launch_rms_norm(const NormArgs &a, hipStream_t stream);
+
+// Packed sequences and the states that they start from and leave.
+struct Sequences {
+    const int32_t *starts;  // null: `tokens / sequences` rows each
+    const int32_t *slots_in, *slots_out;
+    int sequences, tokens;
+    int slots;
+};
+
+struct ConvArgs {
+    Sequences s;
+    const void *x;
+    void *y, *states;
+    const float *weight, *bias;
+    size_t x_stride, y_stride;
+    int channels, width, silu;
+    int vec;  // eight channels at a time: whole runs of eight, 16-byte aligned
+};
+hipError_t launch_short_conv(const ConvArgs &a, int x_f16, int y_f16, hipStream_t stream);
+
+struct DeltaArgs {
+    Sequences s;
+    Heads q, k, v, out;
+    const float *g, *beta, *a_log, *dt_bias;
+    size_t gate_stride;
+    float *states;
+    int key_dim, value_dim;
+    float scale, eps;  // eps < 0: q and k as they are
+};
+hipError_t launch_delta_step(const DeltaArgs &a, hipStream_t stream);
+
+}  // namespace exl3k

@@ -1,0 +1,138 @@
+// exl3_short_conv.hip -- causal depthwise convolution of packed sequences, with their states.
+//
+// Bound by the rows' bytes.  A thread takes C channels of a tile of rows of one sequence and keeps the last
+// W - 1 rows in registers.  The rows ahead of a sequence's first come from its state, and only the
+// threads of its first tile read that state: they also write the one that it leaves, so a slot may be both.
+#include "exl3_activation.hpp"
+#include "exl3_head_rows.hpp"
+#include "exl3_packed_rows.hpp"
+
+namespace exl3k {
+
+namespace {
+
+constexpr int kConvThreads = 256;
+
+template <int F16, int C>
+__device__ __forceinline__ void load_channels(const void *p, size_t at, float (&v)[C]) {
+    if constexpr (C == 8) load_run8<F16>(p, at, 1, v);
+    else v[0] = F16 ? (float)((const _Float16 *)p)[at] : ((const float *)p)[at];
+}
+template <int F16, int C>
+__device__ __forceinline__ void store_channels(void *p, size_t at, const float (&v)[C]) {
+    if constexpr (C == 8) store_run8<F16>(p, at, 1, v);
+    else if constexpr (F16) ((_Float16 *)p)[at] = (_Float16)v[0];
+    else ((float *)p)[at] = v[0];
+}
+
+// blockIdx.x = tile * channel blocks + channel block; `per` rows a tile, at least W - 1
+template <int W, int C, int XF16, int YF16>
+__global__ __launch_bounds__(kConvThreads) void short_conv_kernel(ConvArgs a, int per, unsigned channel_blocks) {
+    const unsigned tile = blockIdx.x / channel_blocks;
+    const int c = (int)((blockIdx.x - tile * channel_blocks) * kConvThreads + threadIdx.x) * C;
+    const Tile t = find_tile(a.s, (int)tile, per, threadIdx.x & 63);
+    if (t.s < 0 || c >= a.channels) return;
+    float w[C][W], bias[C];
+    if constexpr (C == 8) {
+        float flat[8 * W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) load_run8<0>(a.weight, (size_t)c * W + 8 * i, 1, *(float(*)[8]) & flat[8 * i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int j = 0; j < W; ++j) w[e][j] = flat[e * W + j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[0][j] = a.weight[(size_t)c * W + j];
+    }
+#pragma unroll
+    for (int e = 0; e < C; ++e) bias[e] = a.bias ? a.bias[c + e] : 0.f;
+
+    float last[W - 1][C];  // the rows ahead of the next one, the oldest first
+    const size_t first = t.rows.first;
+    if (t.row0 == 0) {
+        const int in = slot_in(a.s, t.s), out = slot_out(a.s, t.s);
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) {
+#pragma unroll
+            for (int e = 0; e < C; ++e) last[j][e] = in == kBadState ? __builtin_nanf("") : 0.f;
+            if (in >= 0) load_channels<XF16, C>(a.states, ((size_t)in * (W - 1) + j) * a.channels + c, last[j]);
+        }
+        if (out >= 0) {
+#pragma unroll
+            for (int j = 0; j < W - 1; ++j) {
+                const int row = t.rows.count - (W - 1) + j;
+                float v[C];
+                if (row >= 0) {
+                    load_channels<XF16, C>(a.x, (first + row) * a.x_stride + c, v);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < C; ++e) {
+                        v[e] = 0.f;
+#pragma unroll
+                        for (int i = 0; i < W - 1; ++i) v[e] = i == W - 1 + row ? last[i][e] : v[e];
+                    }
+                }
+                store_channels<XF16, C>(a.states, ((size_t)out * (W - 1) + j) * a.channels + c, v);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j)
+            load_channels<XF16, C>(a.x, (first + t.row0 - (W - 1) + j) * a.x_stride + c, last[j]);
+    }
+
+    constexpr int U = 4;  // rows whose loads are on the way at once
+    const int end = min(t.row0 + per, t.rows.count);
+    for (int row = t.row0; row < end; row += U) {
+        float x[U][C];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            load_channels<XF16, C>(a.x, (first + min(row + u, end - 1)) * a.x_stride + c, x[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float y[C];
+#pragma unroll
+            for (int e = 0; e < C; ++e) {
+                y[e] = bias[e];
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) y[e] = __builtin_fmaf(w[e][j], last[j][e], y[e]);
+                y[e] = __builtin_fmaf(w[e][W - 1], x[u][e], y[e]);
+                if (a.silu) y[e] = silu_f32(y[e]);
+#pragma unroll
+                for (int j = 0; j + 1 < W - 1; ++j) last[j][e] = last[j + 1][e];
+                last[W - 2][e] = x[u][e];
+            }
+            if (row + u < end) store_channels<YF16, C>(a.y, (first + row + u) * a.y_stride + c, y);
+        }
+    }
+}
+
+template <int W, int C, int XF16, int YF16>
+hipError_t launch_tiles(const ConvArgs &a, hipStream_t stream) {
+    const unsigned channel_blocks = (a.channels + kConvThreads * C - 1) / (kConvThreads * C);
+    int per = 32;
+    while (per > 4 && tile_count(a.s, per) * channel_blocks < 2048) per /= 2;
+    const size_t blocks = tile_count(a.s, per) * channel_blocks;
+    short_conv_kernel<W, C, XF16, YF16><<<dim3((unsigned)blocks), dim3(kConvThreads), 0, stream>>>(a, per, channel_blocks);
+    return hipGetLastError();
+}
+template <int W, int C>
+hipError_t launch_types(const ConvArgs &a, int x_f16, int y_f16, hipStream_t stream) {
+    if (x_f16) return y_f16 ? launch_tiles<W, C, 1, 1>(a, stream) : launch_tiles<W, C, 1, 0>(a, stream);
+    return y_f16 ? launch_tiles<W, C, 0, 1>(a, stream) : launch_tiles<W, C, 0, 0>(a, stream);
+}
+template <int W>
+hipError_t launch_width(const ConvArgs &a, int x_f16, int y_f16, hipStream_t stream) {
+    return a.vec ? launch_types<W, 8>(a, x_f16, y_f16, stream) : launch_types<W, 1>(a, x_f16, y_f16, stream);
+}
+
+}  // namespace
+
+hipError_t launch_short_conv(const ConvArgs &a, int x_f16, int y_f16, hipStream_t stream) {
+    if (a.width == 2) return launch_width<2>(a, x_f16, y_f16, stream);
+    if (a.width == 3) return launch_width<3>(a, x_f16, y_f16, stream);
+    return launch_width<4>(a, x_f16, y_f16, stream);
+}
+
+}  // namespace exl3k

@@ -1,4 +1,4 @@
-// exl3_torch.cpp -- the attention block's C-ABI for torch tensors, as a CPython module.
+// exl3_torch.cpp -- the C-ABI of the attention and linear-attention blocks for torch tensors, as a CPython module.
 //
 // Through ctypes, with views, checks and allocations in Python, the host time of a call is several
 // times its kernel's at decode sizes: one token's qk_norm_rope took 16.8 us a call, here 5.2; a cache
@@ -14,6 +14,7 @@
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <stdexcept>
@@ -104,7 +105,7 @@ struct Call {
 // rows of heads [tokens, heads, head_dim], F16 or F32, a head's elements dense
 exl3_head_view heads(const at::Tensor &t) {
     need(t.dim() == 3, "rows of heads are [tokens, heads, head_dim]");
-    need(t.size(2) <= 1 || t.stride(2) == 1, "the elements of a head must be dense");
+    need(t.size(2) <= 1 || t.stride(2) == 1 || !t.numel(), "the elements of a head must be dense");
     need(t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat, "heads are float16 or float32");
     return {t.data_ptr(), (size_t)t.size(1), (size_t)t.stride(0), (size_t)t.stride(1)};
 }
@@ -280,6 +281,143 @@ PyObject *attention_prompt(PyObject *const *a) {
                out);
 }
 
+// rows [tokens, heads, width], or [tokens, width] as one head each
+exl3_head_view rows_or_heads(const at::Tensor &t) {
+    if (t.dim() == 3) return heads(t);
+    need(t.dim() == 2, "rows are [tokens, width] or [tokens, heads, width]");
+    need(t.size(1) <= 1 || t.stride(1) == 1 || !t.numel(), "the elements of a row must be dense");
+    need(t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat, "rows are float16 or float32");
+    return {t.data_ptr(), 1, (size_t)t.stride(0), 0};
+}
+
+// (x, weight, residual, gate, eps, out_dtype, out, residual_out, stream)
+PyObject *rms_norm(PyObject *const *a) {
+    Call c;
+    const at::Tensor &x = c.tensor(a[0], "x is a tensor");
+    c.on(a[8]);
+    const exl3_head_view xv = rows_or_heads(x);
+    const int64_t width = x.size(x.dim() - 1);
+    const void *w = c.dense(a[1], at::kFloat, width, "weight: dense float32, one per element of a row", true);
+    exl3_head_view rv{}, zv{}, rov{};
+    at::Tensor kept;
+    const bool res = given(a[2]), gated = given(a[3]);
+    exl3_dtype rt = EXL3_F32;
+    need(res || !given(a[7]), "residual_out without a residual");
+    if (res) {
+        const at::Tensor &r = c.tensor(a[2], "residual is a tensor");
+        need(same_shape(x, r), "x and residual differ in shape");
+        rv = rows_or_heads(r);
+        rt = type_of(r);
+        kept = c.output(a[7], r.sizes(), r.scalar_type());
+        need(kept.scalar_type() == r.scalar_type(), "residual and residual_out differ in type");
+        rov = rows_or_heads(kept);
+    }
+    if (gated) {
+        const at::Tensor &z = c.tensor(a[3], "gate is a tensor");
+        need(same_shape(x, z) && z.scalar_type() == x.scalar_type(), "x and gate differ in shape or type");
+        zv = rows_or_heads(z);
+    }
+    const at::Tensor out = c.output(a[6], x.sizes(), dtype_or(a[5], x.scalar_type()));
+    const exl3_head_view ov = rows_or_heads(out);
+    const exl3_status st = exl3_hip_rms_norm(&xv, gated ? &zv : nullptr, type_of(x), res ? &rv : nullptr,
+                                             res ? &rov : nullptr, rt, (size_t)x.size(0), (size_t)width,
+                                             (const float *)w, real_of(a[4]), &ov, type_of(out), c.stream);
+    if (st == EXL3_OK && res) return two(st, out, &kept);
+    return one(st, out);
+}
+
+// starts int32 [sequences + 1], or None and the sequences' number; the pool's slots of the sequences
+struct Packed {
+    const int32_t *starts, *in, *out;
+    size_t sequences, slots;
+    void *states;
+};
+Packed packed(Call &c, PyObject *starts, PyObject *sequences, PyObject *states, PyObject *in, PyObject *out,
+              at::ScalarType type, at::IntArrayRef shape) {
+    Packed p{};
+    if (given(starts)) {
+        p.starts = (const int32_t *)c.dense(starts, at::kInt, -1, "starts: dense int32");
+        const int64_t n = THPVariable_Unpack(starts).numel();
+        need(n >= 1, "starts: sequences + 1 elements");
+        p.sequences = (size_t)n - 1;
+    } else {
+        p.sequences = count_of(sequences);
+    }
+    if (given(states)) {
+        const at::Tensor &t = c.tensor(states, "states is a tensor");
+        need(t.scalar_type() == type && t.is_contiguous() && t.dim() == (int64_t)shape.size() + 1 &&
+                 t.sizes().slice(1) == shape,
+             "states: dense, of the operator's state shape and type");
+        p.slots = (size_t)t.size(0);
+        p.states = t.data_ptr();
+    }
+    p.in = (const int32_t *)c.dense(in, at::kInt, (int64_t)p.sequences, "slots_in: dense int32, one per sequence", true);
+    p.out = (const int32_t *)c.dense(out, at::kInt, (int64_t)p.sequences, "slots_out: dense int32, one per sequence", true);
+    return p;
+}
+// the row stride of a matrix whose rows are dense; one of a single row may have any
+size_t row_stride(const at::Tensor &t) {
+    return (size_t)(t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1)));
+}
+
+// (x, weight, bias, silu, starts, sequences, states, slots_in, slots_out, out_dtype, out, stream)
+PyObject *short_conv(PyObject *const *a) {
+    Call c;
+    const at::Tensor &x = c.tensor(a[0], "x is a tensor");
+    c.on(a[11]);
+    need(x.dim() == 2, "x: [tokens, channels]");
+    rows_or_heads(x);
+    const int64_t n = x.size(0), ch = x.size(1);
+    const at::Tensor &w = c.tensor(a[1], "weight is a tensor");
+    need(w.scalar_type() == at::kFloat && w.is_contiguous() && w.dim() == 2 && w.size(0) == ch,
+         "weight: dense float32 [channels, width]");
+    const int64_t state[2] = {w.size(1) - 1, ch};
+    const Packed p = packed(c, a[4], a[5], a[6], a[7], a[8], x.scalar_type(), state);
+    const void *bias = c.dense(a[2], at::kFloat, ch, "bias: dense float32, one per channel", true);
+    const int act = PyObject_IsTrue(a[3]);
+    if (act < 0) throw python_error();
+    const at::Tensor out = c.output(a[10], x.sizes(), dtype_or(a[9], x.scalar_type()));
+    rows_or_heads(out);
+    return one(exl3_hip_short_conv(x.data_ptr(), type_of(x), row_stride(x), (size_t)n, (size_t)ch,
+                                   (const float *)w.data_ptr(), (size_t)w.size(1), (const float *)bias, act, p.starts,
+                                   p.sequences, p.states, p.slots, p.in, p.out, out.data_ptr(), type_of(out),
+                                   row_stride(out), c.stream),
+               out);
+}
+
+// (q, k, v, g, beta, a_log, dt_bias, starts, sequences, states, slots_in, slots_out, scale, qk_eps, out, workspace,
+//  stream)
+PyObject *delta_rule(PyObject *const *a) {
+    Call c;
+    const at::Tensor &q = c.tensor(a[0], "q is a tensor"), &k = c.tensor(a[1], "k is a tensor"),
+                     &v = c.tensor(a[2], "v is a tensor");
+    c.on(a[16]);
+    const exl3_head_view qv = heads(q), kv = heads(k), vv = heads(v);
+    need(q.scalar_type() == at::kHalf && k.scalar_type() == at::kHalf && v.scalar_type() == at::kHalf,
+         "q, k and v are float16");
+    need(same_shape(q, k) && v.size(0) == q.size(0), "q, k and v differ in shape");
+    const int64_t n = q.size(0), h = v.size(1), dk = q.size(2), dv = v.size(2);
+    const at::Tensor &g = c.tensor(a[3], "g is a tensor"), &beta = c.tensor(a[4], "beta is a tensor");
+    need(g.scalar_type() == at::kFloat && beta.scalar_type() == at::kFloat && g.dim() == 2 && g.size(0) == n &&
+             g.size(1) == h && same_shape(g, beta) && (h == 1 || !n || (g.stride(1) == 1 && beta.stride(1) == 1)) &&
+             row_stride(g) == row_stride(beta),
+         "g and beta: float32 [tokens, v heads] with the same row stride, dense rows");
+    const void *al = c.dense(a[5], at::kFloat, h, "a_log: dense float32 [v heads]", true);
+    const void *dt = c.dense(a[6], at::kFloat, h, "dt_bias: dense float32 [v heads]", true);
+    const int64_t state[3] = {h, dk, dv};
+    const Packed p = packed(c, a[7], a[8], a[9], a[10], a[11], at::kFloat, state);
+    const at::Tensor out = c.output(a[14], v.sizes(), at::kHalf);
+    const exl3_head_view ov = heads(out);
+    need(out.scalar_type() == at::kHalf, "out: float16");
+    size_t ws_bytes;
+    void *const ws = c.workspace(a[15], &ws_bytes);
+    return one(exl3_hip_delta_rule(&qv, &kv, &vv, (const float *)g.data_ptr(), (const float *)beta.data_ptr(),
+                                   row_stride(g), (const float *)al, (const float *)dt, &ov, (size_t)dk, (size_t)dv,
+                                   p.starts, p.sequences, (size_t)n, (float *)p.states, p.slots, p.in, p.out,
+                                   scale_of(a[12], dk), given(a[13]) ? real_of(a[13]) : -1.f, ws, ws_bytes, c.stream),
+               out);
+}
+
 // a METH_FASTCALL entry of N positional arguments around F
 template <PyObject *(*F)(PyObject *const *), Py_ssize_t N>
 PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
@@ -301,7 +439,9 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
     { #name, (PyCFunction)(void (*)(void))entry<name, n>, METH_FASTCALL, nullptr }
 PyMethodDef methods[] = {EXL3_ENTRY(qk_norm_rope, 13),     EXL3_ENTRY(kv_cache_write, 8),
                          EXL3_ENTRY(kv_cache_read, 11),    EXL3_ENTRY(attention_cached, 12),
-                         EXL3_ENTRY(attention_prompt, 10),  {nullptr, nullptr, 0, nullptr}};
+                         EXL3_ENTRY(attention_prompt, 10), EXL3_ENTRY(rms_norm, 9),
+                         EXL3_ENTRY(short_conv, 12),       EXL3_ENTRY(delta_rule, 17),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "exl3_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -30,7 +30,8 @@ EXPORTS = [
     "exl3_hip_mul_mat_group_workspace_bytes", "exl3_hip_workspace_status", "exl3_hip_test_exchange_fault",
     "exl3_hip_qk_norm_rope", "exl3_hip_kv_page_bytes", "exl3_hip_kv_cache_write", "exl3_hip_kv_cache_read",
     "exl3_hip_attention_cached", "exl3_hip_attention_cached_workspace_bytes", "exl3_hip_attention_prompt",
-    "exl3_hip_attention_prompt_workspace_bytes",
+    "exl3_hip_attention_prompt_workspace_bytes", "exl3_hip_rms_norm", "exl3_hip_short_conv", "exl3_hip_delta_rule",
+    "exl3_hip_delta_rule_workspace_bytes",
 ]
 
 # ggml op predicates (exl3_hip_supports_op)
@@ -184,6 +185,15 @@ def load(path=LIB_PATH):
     L.exl3_hip_attention_prompt.argtypes = [hv, hv, hv, hv, sz, vp, vp, sz, sz, sz, f, i, vp, sz, st]
     L.exl3_hip_attention_prompt_workspace_bytes.restype = sz
     L.exl3_hip_attention_prompt_workspace_bytes.argtypes = [sz, sz, sz, sz, sz]
+    L.exl3_hip_rms_norm.restype = i
+    L.exl3_hip_rms_norm.argtypes = [hv, hv, i, hv, hv, i, sz, sz, vp, f, hv, i, st]
+    L.exl3_hip_short_conv.restype = i
+    L.exl3_hip_short_conv.argtypes = [vp, i, sz, sz, sz, vp, sz, vp, i, vp, sz, vp, sz, vp, vp, vp, i, sz, st]
+    L.exl3_hip_delta_rule.restype = i
+    L.exl3_hip_delta_rule.argtypes = [hv, hv, hv, vp, vp, sz, vp, vp, hv, sz, sz, vp, sz, sz, vp, sz, vp, vp, f, f, vp,
+                                      sz, st]
+    L.exl3_hip_delta_rule_workspace_bytes.restype = sz
+    L.exl3_hip_delta_rule_workspace_bytes.argtypes = [sz, sz, sz, sz, sz]
     return L
 
 
@@ -626,3 +636,54 @@ def attention_prompt(q, k, v, q_starts, kv_starts=None, causal=True, scale=None,
     sequences.  causal aligns each sequence's ends: keys ahead of its queries are a prefix."""
     return _taken((_TORCH or _torch_module()).attention_prompt(q, k, v, q_starts, kv_starts, causal, scale, out,
                                                                workspace, stream), "attention_prompt")
+
+
+# ---- the linear-attention block and the norms between blocks, on the same tensors.  Packed sequences: `starts` int32
+# [sequences + 1] holds their first rows; None: `sequences` of them with as many rows each.  States are kept in a pool,
+# one slot a sequence: slots_in (int32 [sequences], negative or None: from zeros) are read, slots_out (negative or
+# None: not kept) written; both may be the same.
+def rms_norm(x, weight=None, residual=None, gate=None, eps=1e-6, out_dtype=None, out=None, residual_out=None,
+             stream=None):
+    """RMS norm of rows x [tokens, width] or [tokens, heads, width] (fp16 or fp32), times weight (fp32 [width]):
+    of x + residual where a residual is given, which returns (out, residual_out), the sum in the residual's
+    type (residual_out = residual: in place); times silu(gate), of x's shape and type, where a gate is given."""
+    return _taken((_TORCH or _torch_module()).rms_norm(x, weight, residual, gate, eps, out_dtype, out, residual_out,
+                                                       stream), "rms_norm")
+
+
+def new_conv_states(slots, channels, width=4, dtype=None, device="cuda"):
+    """[slots, width - 1, channels] of x's type (fp16 unless dtype says otherwise), zeros"""
+    import torch
+    return torch.zeros((slots, width - 1, channels), dtype=dtype or torch.float16, device=device)
+
+
+def short_conv(x, weight, bias=None, silu=True, starts=None, sequences=1, states=None, slots_in=None, slots_out=None,
+               out_dtype=None, out=None, stream=None):
+    """Causal depthwise convolution of packed rows x [tokens, channels] with weight fp32 [channels, width], width 2 to
+    4 (the last tap is the row's own), and bias fp32 [channels], then silu.  states: [slots, width - 1,
+    channels] of x's type, the last rows of each sequence."""
+    return _taken((_TORCH or _torch_module()).short_conv(x, weight, bias, silu, starts, sequences, states, slots_in,
+                                                         slots_out, out_dtype, out, stream), "short_conv")
+
+
+def new_delta_states(slots, v_heads, key_dim, value_dim, device="cuda"):
+    """fp32 [slots, v_heads, key_dim, value_dim], zeros"""
+    import torch
+    return torch.zeros((slots, v_heads, key_dim, value_dim), dtype=torch.float32, device=device)
+
+
+def delta_rule_workspace_bytes(v_heads, key_dim, value_dim, sequences, tokens):
+    """0: such a call takes no workspace"""
+    return lib().exl3_hip_delta_rule_workspace_bytes(v_heads, key_dim, value_dim, sequences, tokens)
+
+
+def delta_rule(q, k, v, g, beta, a_log=None, dt_bias=None, starts=None, sequences=1, states=None, slots_in=None,
+               slots_out=None, scale=None, qk_eps=None, out=None, workspace=None, stream=None):
+    """The gated delta rule over packed rows, all fp16: q and k [tokens, k_heads, key_dim], v [tokens, v_heads,
+    value_dim] -> [tokens, v_heads, value_dim].  g (log decay) and beta fp32 [tokens, v_heads]; with a_log and
+    dt_bias (fp32 [v_heads]) they are -exp(a_log) softplus(g + dt_bias) and sigmoid(beta).  qk_eps: q and k are
+    divided by sqrt(sum of squares + qk_eps) (None: as they are); scale: 1 / sqrt(key_dim) unless given.
+    states: fp32 [slots, v_heads, key_dim, value_dim]."""
+    return _taken((_TORCH or _torch_module()).delta_rule(
+        q, k, v, g, beta, a_log, dt_bias, starts, sequences, states, slots_in, slots_out, scale, qk_eps, out, workspace,
+        stream), "delta_rule")
