@@ -55,13 +55,29 @@ def short_conv(x, weight, bias, silu, lens, states, slots_in, slots_out):
     return y, after, err
 
 
+def _norm(k, g, beta):
+    """largest row sum of (1 + A)^-1, A_ij = beta_i exp(g_j+1 + .. + g_i) k_i . k_j (j < i)"""
+    n = len(g)
+    a = np.zeros((n, n))
+    for i in range(n):
+        fall = np.exp(np.cumsum(g[i:0:-1])[::-1])  # of rows 0 .. i - 1
+        a[i, :i] = beta[i] * fall * (k[:i] @ k[i])
+    return np.abs(np.linalg.inv(np.eye(n) + a)).sum(1).max() if np.all(np.isfinite(a)) else 1.0
+
+
 def delta_rule(q, k, v, g, beta, lens, scale, states=None, slots_in=None, slots_out=None, a_log=None, dt_bias=None,
-               qk_eps=None, unit=40 * E32):
+               qk_eps=None, unit=40 * E32, chunk=None):
     """(out, states afterwards, bounds on both ahead of out's rounding).  A column of S is off by e, |e| its
     2-norm.  Where 0 <= beta |k|^2 <= 2, the map e -> exp(g) (I - beta k k^T) e does not lengthen it, so a row adds
     only what it rounds itself: `unit` times the column's and the row's size.  unit: for the row-by-row
     kernel a dot product is a chain of 16 fused multiply-adds and 3 sums, then 8 roundings of factors (gates,
-    lengths, u) and the fma of the update: 28 E32, and 2 |g| + 4 E32 for the decay."""
+    lengths, u) and the fma of the update: 28 E32, and 2 |g| + 4 E32 for the decay.  In chunks (of `chunk` rows) u is
+    T (beta (v - K S)): each of the four products that lead to S and out has operands of 22 bits (4 E32, and
+    4 E32 for the product of their low parts, left out) and sums of at most 128 in binary32, whose errors are
+    independent (16 E32): 4 * 24 E32, and T takes an error of its rows to at most ||T|| (largest row sum) times it.
+    Their pairs end at 2^-40 of a power of two at most 4 times the bound on a column of U, ||T|| (max |beta v| + max (beta e^G
+    |k|_1) max |S|): R's and U's (or W's) steps, over 64 keys of length 1, are 128 times that whatever is left of the
+    chunk's states at its end."""
     n, h, dv = v.shape
     dk, group = q.shape[2], h // q.shape[1]
     q, k = (np.repeat(t, group, 1) for t in (q, k))
@@ -77,7 +93,15 @@ def delta_rule(q, k, v, g, beta, lens, scale, states=None, slots_in=None, slots_
         i = -1 if slots_in is None else int(slots_in[s])
         S = np.zeros((h, dk, dv)) if i < 0 else states[i].copy() if i < len(states) else np.full((h, dk, dv), np.nan)
         e = np.zeros((h, dv))
+        first, growth = at, np.ones((h, 1))
         for t in range(at, at + count):
+            if chunk and (t - first) % chunk == 0:
+                growth = np.array([[_norm(k[t:min(t + chunk, at + count), i], g[t:min(t + chunk, at + count), i],
+                                          beta[t:min(t + chunk, at + count), i])] for i in range(h)])
+                rows = slice(t, min(t + chunk, at + count))
+                b = np.abs(beta[rows])[:, :, None]
+                l1 = (b * np.exp(np.cumsum(g[rows], 0))[:, :, None] * np.abs(k[rows]).sum(-1, keepdims=True)).max(0)
+                floor = 128 * 2.0 ** -38 * growth * ((b * np.abs(v[rows])).max(0) + l1 * np.abs(S).max(1))
             d = np.exp(g[t])[:, None, None]
             S = S * d
             u = beta[t][:, None] * (v[t] - np.einsum("hkv,hk->hv", S, k[t]))
@@ -85,9 +109,11 @@ def delta_rule(q, k, v, g, beta, lens, scale, states=None, slots_in=None, slots_
             S = S + k[t][:, :, None] * u[:, None, :]
             size = size + np.sqrt(np.sum(S * S, 1))
             gd = np.minimum(np.abs(np.where(np.isfinite(g[t]), g[t], 0)), 100)[:, None]
-            e = d[:, :, 0] * e + (unit + 2 * gd * E32) * size * np.maximum(1.0, np.linalg.norm(k[t], axis=-1))[:, None]
+            e = d[:, :, 0] * e + (growth * unit * (2.4 if chunk else 1) + 2 * gd * E32) * size * np.maximum(1.0, np.linalg.norm(k[t], axis=-1))[:, None]
             out[t] = scale * np.einsum("hkv,hk->hv", S, q[t])
-            bound[t] = abs(scale) * np.linalg.norm(q[t], axis=-1)[:, None] * (e + unit * size)
+            if chunk and ((t - first) % chunk == chunk - 1 or t == at + count - 1):
+                e = e + floor
+            bound[t] = abs(scale) * np.linalg.norm(q[t], axis=-1)[:, None] * (e + growth * unit * (2.4 if chunk else 1) * size)
         o = -1 if slots_out is None else int(slots_out[s])
         if 0 <= o < (0 if states is None else len(states)):
             after[o], off[o] = S, e

@@ -57,7 +57,7 @@ def call(amd, d, lens, states=None, sin=None, sout=None, norm=True, packed=True,
     want, after, bound, off = ref.delta_rule(
         f["q"], f["k"], f["v"], f["g"], f["beta"], lens, float(np.float32(scale)),
         None if states is None else states.astype(np.float64), sin, sout, f["a_log"], f["dt_bias"],
-        None if eps is None else float(np.float32(eps)))
+        None if eps is None else float(np.float32(eps)), chunk=64 if n >= 16 * len(lens) else None)
     assert bool((out[n:] == 9).all())
     got = out[:n].cpu().numpy().astype(np.float64)
     assert np.array_equal(np.isnan(got), np.isnan(want))

@@ -51,5 +51,10 @@ struct DeltaArgs {
     float scale, eps;  // eps < 0: q and k as they are
 };
 hipError_t launch_delta_step(const DeltaArgs &a, hipStream_t stream);
+// rows a sequence from which on the chunks take over
+constexpr size_t kDeltaPromptRows = 16;
+// 0: the call goes row by row and takes no workspace
+size_t delta_prompt_bytes(size_t heads, size_t sequences, size_t tokens);
+hipError_t launch_delta_prompt(const DeltaArgs &a, void *workspace, hipStream_t stream);
 
 }  // namespace exl3k

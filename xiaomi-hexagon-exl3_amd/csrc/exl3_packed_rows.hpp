@@ -32,20 +32,23 @@ __device__ __forceinline__ Tile find_tile(const Sequences &p, int t, int per, in
         const int n = p.tokens / p.sequences, tiles = n > per ? (n + per - 1) / per : 1, s = t / tiles;
         return {s < p.sequences ? s : -1, (t - s * tiles) * per, {s * n, n}};
     }
-    int before = 0;
+    unsigned before = 0;
     for (int s0 = 0; s0 < p.sequences; s0 += 64) {
         const int left = p.sequences - s0;
         const Rows r = rows_of(p, s0 + (lane < left ? lane : left - 1));
-        int end = lane >= left ? 0 : r.count > per ? (r.count + per - 1) / per : 1;
-        const int own = end;
+        const unsigned own = lane >= left ? 0 : r.count > per ? (r.count + per - 1) / per : 1;
+        unsigned end = own;
         for (int d = 1; d < min(left, 64); d <<= 1) {
-            const int o = __shfl_up(end, d);
+            const unsigned o = __shfl_up(end, d);
             end += lane >= d ? o : 0;
         }
-        const unsigned long long hit = __ballot(lane < left && t < before + end);
+        const unsigned long long hit = __ballot(lane < left && (unsigned)t < before + end);
         if (hit) {
             const int l = __builtin_ctzll(hit);
-            return {s0 + l, (t - before - __builtin_amdgcn_readlane(end - own, l)) * per,
+            const unsigned nth = t - before - __builtin_amdgcn_readlane(end - own, l);
+            // starts that overlap may count more tiles than 32 bits hold
+            if (nth >= (unsigned)__builtin_amdgcn_readlane(own, l)) break;
+            return {s0 + l, (int)nth * per,
                     {__builtin_amdgcn_readlane(r.first, l), __builtin_amdgcn_readlane(r.count, l)}};
         }
         before += __builtin_amdgcn_readlane(end, min(left, 64) - 1);
