@@ -36,7 +36,7 @@ constexpr int kFrag = 1024, kFrags = 6;
 constexpr int kRowFactors = 2 * kFrags * 2 * kFrag;  // byte offsets
 constexpr int kScalars = kRowFactors + 4 * kChunk * 4;
 constexpr int kChunkBytes = kScalars + 256;
-enum { kDecay, kUFit, kUBack, kPBack, kWFit, kWBack, kRState, kRValue };  // scalars
+enum { kRState, kRValue, kUFit, kUBack, kDecay, kWBack, kPBack };  // scalars
 // fragment of row tile t (16 rows) and columns 32 s .. 32 s + 31: s <= t / 2
 __device__ __forceinline__ int frag_of(int t, int s) { return (t < 2 ? t : 2 * t - 2) + s; }
 // the chunk's row that row m of row tile t stands for
@@ -54,12 +54,32 @@ __device__ __forceinline__ Fit fit_of(float bound) {
     return {__int_as_float((127 - e) << 23), __int_as_float((127 + e) << 23)};
 }
 
-// A number's parts.  x is kept opaque: fused into the conversion, the product that made it is rounded once for hi and
-// twice for the hi that lo is the rest of, and now and then they are a step apart.
-__device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) {
-    asm("" : "+v"(x));
-    hi = (_Float16)x;
-    lo = (_Float16)(x - (float)hi);
+// Two numbers' parts, packed.  In assembly for v_fma_mix_f32 (x - (float)hi in one instruction), and so that hi
+// is one value: the compiler fuses the product that made x into one conversion and not into the other, and now
+// and then the two are a step apart.
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    float a, b;
+    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(hi) : "v"(x), "v"(y));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(a) : "v"(hi), "v"(x));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(b) : "v"(hi), "v"(y));
+    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(lo) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void split4(f4 x, h4 &hi, h4 &lo) {
+    u2 a, b;
+    uint32_t h, l;
+    split2(x[0], x[1], h, l);
+    a.x = h, b.x = l;
+    split2(x[2], x[3], h, l);
+    a.y = h, b.y = l;
+    hi = bitcast<h4>(a);
+    lo = bitcast<h4>(b);
+}
+__device__ __forceinline__ void split8(f4 x, f4 y, h8 &hi, h8 &lo) {
+    h4 a, b, c, d;
+    split4(x, a, b);
+    split4(y, c, d);
+    hi = (h8){a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
+    lo = (h8){b[0], b[1], b[2], b[3], d[0], d[1], d[2], d[3]};
 }
 
 // maximum over lanes l ^ 16, l ^ 32
@@ -84,6 +104,9 @@ __device__ __forceinline__ h8 load_h8(const _Float16 *p, int vec) {
     return t;
 }
 
+// Loads stay in their order across this, ahead of the loop as in it: a wait for one is a wait for all that were
+// issued before it.
+__device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 // The LDS that waves share is complete; loads from memory stay on their way.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -279,13 +302,10 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
             const float *const from = (which ? Pm : T) + row_of(wave, m) * kRowFloats + 32 * s + 8 * q;
             const float to = which ? pf.to : tf.to;
             h8 hi, lo;
+            split8(*(const f4 *)from * to, *(const f4 *)(from + 4) * to, hi, lo);
+            if (!which) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                _Float16 x, y;
-                split(from[j] * to, x, y);
-                hi[j] = x;
-                lo[j] = y;
-                if (!which) t_sum += __builtin_fabsf(from[j]);
+                for (int j = 0; j < 8; ++j) t_sum += __builtin_fabsf(from[j]);
             }
             h8 *const at = (h8 *)(block + ((which * kFrags + frag_of(wave, s)) * 2) * kFrag) + lane;
             at[0] = hi;
@@ -298,15 +318,15 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
     if (wave == 0) {  // lane = row
         const float r = kr_lds[lane], e = decay_of((float)G);
         const float until = decay_of((float)(G_end - G)) * r;
+        int e_w = __builtin_amdgcn_frexp_expf(wave_max(__builtin_fabsf(until)));
+        e_w = e_w < -110 ? -110 : e_w;
         float *const f = (float *)(block + kRowFactors);
         f[lane] = e * r;
         f[kChunk + lane] = e * qr_lds[lane];
         f[2 * kChunk + lane] = gt.beta;
-        f[3 * kChunk + lane] = until;
-        const float until_most = wave_max(__builtin_fabsf(until)), beta_most = wave_max(__builtin_fabsf(gt.beta));
+        f[3 * kChunk + lane] = __builtin_amdgcn_ldexpf(until, -e_w);
+        const float beta_most = wave_max(__builtin_fabsf(gt.beta));
         if (lane == 0) {
-            const int e_w = __builtin_amdgcn_frexp_expf(until_most);
-            const int k = e_w < -110 ? -110 : e_w;
             float *const s = (float *)(block + kScalars);
             s[kDecay] = decay_of((float)G_end);
             // |U| <= (largest row sum of T) |R|: another power of two keeps U where R was
@@ -315,8 +335,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
             s[kUFit] = __builtin_amdgcn_ldexpf(tf.back, -e_u);
             s[kUBack] = __builtin_amdgcn_ldexpf(1.f, e_u);
             s[kPBack] = pf.back;
-            s[kWFit] = __builtin_amdgcn_ldexpf(1.f, -k);
-            s[kWBack] = __builtin_amdgcn_ldexpf(1.f, k);
+            s[kWBack] = __builtin_amdgcn_ldexpf(1.f, e_w);
             s[kRState] = fmaxf(fmaxf(l1_lds[0], l1_lds[1]), fmaxf(l1_lds[2], l1_lds[3]));
             s[kRValue] = beta_most;
         }
@@ -340,276 +359,380 @@ __device__ __forceinline__ size_t tiles_before(const Sequences &p, int s, int la
     return sum;
 }
 
-// A workgroup of KD / 32 waves has columns 16 slice .. of one head's state; wave w its rows 32 w .. 32 w + 31, as
-// two tiles, and TT of the chunk's four row tiles.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ size_t uniform(size_t v) {
+    return (uint32_t)uniform((int)(uint32_t)v) | (size_t)(uint32_t)uniform((int)(uint32_t)(v >> 32)) << 32;
+}
+
+// A workgroup has columns 16 slice .. of one head's state, and two kinds of waves, KD / 32 of each.  State wave w has
+// rows 32 w .. 32 w + 31 of the state, as two tiles, and TT of the chunk's four row tiles of R and U: what the next chunk
+// waits for.  Output wave w has Q S, P U and the rows of out of the same row tiles, a step behind, and brings K, V and the
+// rows' factors into LDS, a chunk ahead.  VEC: 16 bytes of a row are one load.
+//
+// LDS, by the barrier (1 to 3 of a chunk) that its writes are ahead of and the one that its reads are ahead of:
+// s, back: 1, 3;  v: 3 (of the chunk before), 2;  k, factor, scalar: 3 (of the chunk before), 1 of the next, and two of
+// each;  r, u_back: 2, 3;  w: 3, 1 of the next;  u: 3, 2 of the next.  A buffer is written again only past the barrier that
+// its reads are ahead of.  o is a wave's own.
 template <int KD>
-__global__ __launch_bounds__(2 * KD) void delta_scan_kernel(DeltaArgs a, const char *chunks, size_t tiles, int units,
-                                                            int slices) {
-    constexpr int NW = KD / 32, TT = 4 / NW;
-    __shared__ h8 s_lds[NW][2][64];          // the state's operand: 32 rows, high and low
-    __shared__ h8 r_lds[2][2][64];           // R's, 32 rows each
-    __shared__ h8 u_lds[2][2][64], w_lds[2][2][64];
-    __shared__ __attribute__((aligned(16))) _Float16 k_lds[NW][kChunk][32];  // 32 elements of each key
-    __shared__ float back_lds[NW][16], v_lds[NW][16];
+struct ScanLds {
+    static constexpr int NW = KD / 32;
+    h8 s[NW][2][64];                  // the state's operand: 32 rows, high and low
+    h8 r[2][2][64];                   // R's, 32 rows each
+    h8 u[2][2][64], w[2][2][64];
+    // 32 elements of each key, 16-byte runs c at c ^ (row / 8 % 4); another 64 bytes put the four runs of an element
+    // group into other banks than the next group's
+    _Float16 k[2][NW][kChunk * 32 + 32];
+    _Float16 v[kChunk][16], o[kChunk][16];
+    f4 factor[2][4][kChunk / 4];      // of the chunk's rows
+    float scalar[2][8];
+    float back[NW][16], u_back[16], v_top[NW];
+};
 
-    // the slices of a head on one XCD, whose L2 then holds what they share
-    const int id = blockIdx.x, at_xcd = id >> 3;
-    const int unit = at_xcd / slices * 8 + (id & 7), slice = at_xcd % slices;
-    if (unit >= units) return;
-    const int heads = a.v.heads, s = unit / heads, head = unit - s * heads;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+struct ScanPlace {
+    Rows rows;
+    const char *block0;  // the first chunk's part of the workspace, a chunk's distance from it to the next
+    size_t step;
+    int n_chunks, head, kh, slice, slot_in, slot_out;
+};
+
+// A chunk's rows as a buffer: what is beyond the sequence's last row reads as zero and is not written.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer chunk_rows(const Heads &h, const ScanPlace &p, int c, int head, int at, int width) {
+    const size_t stride = h.token_stride;
+    char *const base = (char *)((_Float16 *)h.data + (p.rows.first + (size_t)c * kChunk) * stride + head * h.head_stride + at);
+    const uint32_t left = min(p.rows.count - c * kChunk, kChunk);
+    return __builtin_amdgcn_make_buffer_rsrc(base, 0, ((left - 1) * (uint32_t)stride + width) * 2, 0x00020000);
+}
+template <bool VEC>
+__device__ __forceinline__ h8 load_run(Buffer b, uint32_t at) {
+    if constexpr (VEC) {
+        return bitcast<h8>(__builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0));
+    } else {
+        h8 t;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = bitcast<_Float16>(__builtin_amdgcn_raw_buffer_load_b16(b, at + 2 * e, 0, 0));
+        return t;
+    }
+}
+
+// T's or P's fragments of a wave's row tiles: G of them each
+template <int TT, int G>
+__device__ __forceinline__ void load_matrix(const ScanPlace &p, int c, int which, int wave, int lane, h8 (&to)[TT][G][2]) {
+    const h8 *const f = (const h8 *)(p.block0 + c * p.step + which * kFrags * 2 * kFrag) + lane;
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            to[tt][g][0] = f[frag_of(wave * TT + tt, g) * 128];
+            to[tt][g][1] = f[frag_of(wave * TT + tt, g) * 128 + 64];
+        }
+}
+// A row tile of T or P times R or U
+template <int G>
+__device__ __forceinline__ f4 lower_product(const h8 (&m)[G][2], const h8 (&b)[2][2][64], int lane) {
+    f4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        const h8 b_hi = b[g][0][lane], b_lo = b[g][1][lane];
+        x = mfma16(m[g][0], b_hi, x);
+        y = mfma16(m[g][0], b_lo, y);
+        y = mfma16(m[g][1], b_hi, y);
+    }
+    return x + y;
+}
+template <typename L>
+__device__ __forceinline__ void put_quarter(L &lds, int t, int lane, f4 x) {
+    h4 hi, lo;
+    split4(x, hi, lo);
+    *((h4 *)&lds[t >> 1][0][lane] + (t & 1)) = hi;
+    *((h4 *)&lds[t >> 1][1][lane] + (t & 1)) = lo;
+}
+// K S or Q S of a row tile
+template <int NW>
+__device__ __forceinline__ f4 state_product(const h8 (&rows)[NW], const h8 (&hi)[NW], const h8 (&lo)[NW], const float (&back)[NW]) {
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+    f4 x[NW], y;
+#pragma unroll
+    for (int g = 0; g < NW; ++g) x[g] = mfma16(rows[g], hi[g], zero);
+#pragma unroll
+    for (int g = 0; g < NW; ++g) x[g] = mfma16(rows[g], lo[g], x[g]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        y[i] = x[0][i] * back[0];
+#pragma unroll
+        for (int g = 1; g < NW; ++g) y[i] = __builtin_fmaf(x[g][i], back[g], y[i]);
+    }
+    return y;
+}
+
+// UPPER: the wave's row tiles are those of rows 32 .. 63, with two fragments of T or P each
+template <int KD, bool UPPER>
+__device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &p, ScanLds<KD> &lds, int wave, int lane) {
+    constexpr int NW = KD / 32, TT = 4 / NW, G = UPPER ? 2 : 1;
     const int m = lane & 15, q = lane >> 4;
-    const int kh = head / (heads / a.k.heads);
-    const Rows rows = rows_of(a.s, s);
-    const int in = slot_in(a.s, s), out = slot_out(a.s, s);
-    const size_t state_size = (size_t)heads * KD * a.value_dim;
-    const size_t state_at = ((size_t)head * KD + 32 * wave + 8 * q) * a.value_dim + 16 * slice + m;
-
-    float S[2][4];
-    const float start = in == kBadState ? __builtin_nanf("") : 0.f;
+    const size_t state_size = (size_t)a.v.heads * KD * a.value_dim;
+    const size_t state_at = ((size_t)p.head * KD + 32 * wave + 8 * q) * a.value_dim + 16 * p.slice + m;
+    f4 S[2];
+    const float start = p.slot_in == kBadState ? __builtin_nanf("") : 0.f;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            S[t][i] = in >= 0 ? a.states[in * state_size + state_at + (size_t)(4 * t + i) * a.value_dim] : start;
+            S[t][i] = p.slot_in >= 0 ? a.states[p.slot_in * state_size + state_at + (size_t)(4 * t + i) * a.value_dim] : start;
+    asm volatile("" : "+v"(S[0]), "+v"(S[1]));  // waited for here: in the loop it would be a wait for all loads
 
-    const size_t tile0 = tiles_before(a.s, s, lane);
-    // starts that overlap have more chunks than the workspace holds: those are left out
-    const int n_chunks = (int)min((size_t)(rows.count + kChunk - 1) / kChunk, tiles - min(tiles, tile0));
-    const char *const block0 = chunks + (tile0 * heads + head) * kChunkBytes;
-    const size_t step = (size_t)heads * kChunkBytes;
-
-    h8 kf[TT][NW], qf[TT][NW], tf[TT][2][2], pf[TT][2][2];
-    f4 fk[TT], fq[TT], fb[TT], fu[TT];
-    float v[TT][4];
-    auto load_kq = [&](int c) {
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            // a row beyond the last is the last: its factors are 0
-            const size_t row = (size_t)rows.first + min(c * kChunk + row_of(wave * TT + tt, m), rows.count - 1);
-            const _Float16 *const kp = (const _Float16 *)a.k.data + row * a.k.token_stride + kh * a.k.head_stride + 8 * q;
-            const _Float16 *const qp = (const _Float16 *)a.q.data + row * a.q.token_stride + kh * a.q.head_stride + 8 * q;
-#pragma unroll
-            for (int g = 0; g < NW; ++g) {
-                kf[tt][g] = load_h8(kp + 32 * g, a.k.vec);
-                qf[tt][g] = load_h8(qp + 32 * g, a.q.vec);
-            }
-        }
-    };
-    auto load_v = [&](int c) {
-        const float *const f = (const float *)(block0 + c * step + kRowFactors);
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            const int r0 = row_of(wave * TT + tt, 4 * q);
-            fk[tt] = *(const f4 *)(f + r0);
-            fb[tt] = *(const f4 *)(f + 2 * kChunk + r0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const size_t row = (size_t)rows.first + min(c * kChunk + r0 + i, rows.count - 1);
-                v[tt][i] = (float)((const _Float16 *)a.v.data)[row * a.v.token_stride + head * a.v.head_stride + 16 * slice + m];
-            }
-        }
-    };
-    auto load_matrix = [&](int c, int which, h8 (&to)[TT][2][2]) {
-        const h8 *const p = (const h8 *)(block0 + c * step + which * kFrags * 2 * kFrag) + lane;
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            const int t = wave * TT + tt;
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                if (g > t >> 1) continue;
-                to[tt][g][0] = p[frag_of(t, g) * 128];
-                to[tt][g][1] = p[frag_of(t, g) * 128 + 64];
-            }
-        }
-    };
-    auto load_u = [&](int c, int which, f4 (&to)[TT]) {
-        const float *const f = (const float *)(block0 + c * step + kRowFactors) + which * kChunk;
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) to[tt] = *(const f4 *)(f + row_of(wave * TT + tt, 4 * q));
-    };
-    if (n_chunks) {
-        load_kq(0);
-        load_v(0);
-        load_matrix(0, 0, tf);
-        load_u(0, 3, fu);
-        load_matrix(0, 1, pf);
-        load_u(0, 1, fq);
-    }
+    h8 tf[TT][G][2];
+    if (p.n_chunks) load_matrix<TT, G>(p, 0, 0, wave, lane, tf);
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < n_chunks; ++c) {
-        const int next = min(c + 1, n_chunks - 1);
-        const float *const scalar = (const float *)(block0 + c * step + kScalars);
-        const float decay = scalar[kDecay], u_fit = scalar[kUFit], u_more = scalar[kUBack], p_back = scalar[kPBack];
-        const float w_fit = scalar[kWFit], w_back = scalar[kWBack], r_state = scalar[kRState], r_value = scalar[kRValue];
+    if (p.n_chunks) lds_barrier();
+    for (int c = 0; c < p.n_chunks; ++c) {
+        const int next = min(c + 1, p.n_chunks - 1), buf = c & 1;
+        h8 kf[TT][NW];
+        f4 fk[TT], fb[TT], fu[TT];
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+            const int t = wave * TT + tt, r4 = row_of(t, 4 * q) / 4;
+#pragma unroll
+            for (int g = 0; g < NW; ++g) kf[tt][g] = *(const h8 *)&lds.k[buf][g][row_of(t, m) * 32 + 8 * (q ^ (m >> 2))];
+            fk[tt] = lds.factor[buf][0][r4];
+            fb[tt] = lds.factor[buf][2][r4];
+            fu[tt] = lds.factor[buf][3][r4];
+        }
+        const f4 sc = *(const f4 *)&lds.scalar[buf][0];
+        const float decay = lds.scalar[buf][kDecay], w_back = lds.scalar[buf][kWBack];
 
         // the state as an operand, each wave's rows by their own power of two a column
-        float top = 0.f, v_top = 0.f;
+        float top = 0.f;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fabsf(S[t][i]));
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v_top = fmaxf(v_top, __builtin_fabsf(v[tt][i]));
-        top = max_quarters(top);
-        v_top = max_quarters(v_top);
-        const Fit sf = fit_of(top);
+        const Fit sf = fit_of(max_quarters(top));
         h8 hi, lo;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            _Float16 x, y;
-            split(S[j / 4][j % 4] * sf.to, x, y);
-            hi[j] = x;
-            lo[j] = y;
-        }
-        s_lds[wave][0][lane] = hi;
-        s_lds[wave][1][lane] = lo;
-        if (q == 0) {
-            back_lds[wave][m] = sf.back;
-            v_lds[wave][m] = v_top;
-        }
-        lds_barrier();
-
-        // K S and Q S; the keys go to LDS for the update
-        f4 ks[TT], qs[TT];
-        float s_back = 0.f, v_most = 0.f;
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) ks[tt] = qs[tt] = zero;
-#pragma unroll
-        for (int g = 0; g < NW; ++g) {
-            const h8 b_hi = s_lds[g][0][lane], b_lo = s_lds[g][1][lane];
-            const float back = back_lds[g][m];
-            s_back = fmaxf(s_back, back);
-            v_most = fmaxf(v_most, v_lds[g][m]);
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt) {
-                const f4 x = mfma16(kf[tt][g], b_lo, mfma16(kf[tt][g], b_hi, zero));
-                const f4 y = mfma16(qf[tt][g], b_lo, mfma16(qf[tt][g], b_hi, zero));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    ks[tt][i] = __builtin_fmaf(x[i], back, ks[tt][i]);
-                    qs[tt][i] = __builtin_fmaf(y[i], back, qs[tt][i]);
-                }
-            }
-        }
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-            for (int g = 0; g < NW; ++g)
-                *(h8 *)&k_lds[g][row_of(wave * TT + tt, m)][8 * (q ^ (m >> 2))] = kf[tt][g];
-        load_kq(next);
+        split8(S[0] * sf.to, S[1] * sf.to, hi, lo);
+        lds.s[wave][0][lane] = hi;
+        lds.s[wave][1][lane] = lo;
+        lds.back[wave][m] = sf.back;  // the same from four lanes
+        lds_barrier();  // 1
 
         // R = beta (V - e^G K S), |R| <= r_value |V| + r_state |S|
-        const Fit rf = fit_of(__builtin_fmaf(r_value, v_most, r_state * (s_back * 32768.f)));
+        h8 s_hi[NW], s_lo[NW];
+        float back[NW], s_back = 0.f, v_top = 0.f;
+#pragma unroll
+        for (int g = 0; g < NW; ++g) {
+            s_hi[g] = lds.s[g][0][lane];
+            s_lo[g] = lds.s[g][1][lane];
+        }
+#pragma unroll
+        for (int g = 0; g < NW; ++g) {
+            back[g] = lds.back[g][m];
+            s_back = fmaxf(s_back, back[g]);
+            v_top = fmaxf(v_top, lds.v_top[g]);
+        }
+        const Fit rf = fit_of(__builtin_fmaf(sc[kRValue], v_top, sc[kRState] * (s_back * 32768.f)));
+        const float u_back = rf.back * sc[kUBack];
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
-            h4 r_hi, r_lo;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float r = fb[tt][i] * (v[tt][i] - fk[tt][i] * ks[tt][i]);
-                _Float16 x, y;
-                split(r * rf.to, x, y);
-                r_hi[i] = x;
-                r_lo[i] = y;
-            }
             const int t = wave * TT + tt;
-            *((h4 *)&r_lds[t >> 1][0][lane] + (t & 1)) = r_hi;
-            *((h4 *)&r_lds[t >> 1][1][lane] + (t & 1)) = r_lo;
+            // 16 lanes read four rows of V: lane m gets column m of them
+            const h4 v = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s4 *)&lds.v[row_of(t, 4 * q) + (m >> 2)][4 * (m & 3)]));
+            const f4 ks = state_product<NW>(kf[tt], s_hi, s_lo, back);
+            f4 r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = fb[tt][i] * rf.to * __builtin_fmaf(-fk[tt][i], ks[i], (float)v[i]);
+            put_quarter(lds.r, t, lane, r);
         }
-        load_v(next);
-        lds_barrier();
+        if (wave == 0) lds.u_back[m] = u_back;
+        lds_barrier();  // 2
 
-        // U = T R
-        const float u_back = rf.back * u_more;
+        // U = T R, and W = e^(G_64 - G) U for the state
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
-            const int t = wave * TT + tt;
-            f4 x = zero, y = zero;
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                if (g > t >> 1) continue;
-                const h8 b_hi = r_lds[g][0][lane], b_lo = r_lds[g][1][lane];
-                x = mfma16(tf[tt][g][0], b_hi, x);
-                y = mfma16(tf[tt][g][0], b_lo, y);
-                y = mfma16(tf[tt][g][1], b_hi, y);
-            }
-            h4 u_hi, u_lo, w_hi, w_lo;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float u = (x[i] + y[i]) * u_fit;
-                _Float16 e, f;
-                split(u * (fu[tt][i] * w_fit), e, f);
-                w_hi[i] = e;
-                w_lo[i] = f;
-                split(u, e, f);
-                u_hi[i] = e;
-                u_lo[i] = f;
-            }
-            *((h4 *)&w_lds[t >> 1][0][lane] + (t & 1)) = w_hi;
-            *((h4 *)&w_lds[t >> 1][1][lane] + (t & 1)) = w_lo;
-            *((h4 *)&u_lds[t >> 1][0][lane] + (t & 1)) = u_hi;
-            *((h4 *)&u_lds[t >> 1][1][lane] + (t & 1)) = u_lo;
+            const f4 u = lower_product<G>(tf[tt], lds.r, lane) * sc[kUFit];
+            put_quarter(lds.w, wave * TT + tt, lane, u * fu[tt]);
+            put_quarter(lds.u, wave * TT + tt, lane, u);
         }
-        load_matrix(next, 0, tf);
-        load_u(next, 3, fu);
-        lds_barrier();
+        in_order();
+        load_matrix<TT, G>(p, next, 0, wave, lane, tf);
+        lds_barrier();  // 3
 
         // S <- e^G_64 S + K^T W
         f4 acc[2] = {zero, zero};
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-            const h8 b_hi = w_lds[g][0][lane], b_lo = w_lds[g][1][lane];
+            const h8 b_hi = lds.w[g][0][lane], b_lo = lds.w[g][1][lane];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                // 16 lanes read four keys' elements 8 c + 4 t .. + 3 (c < 4): lane m gets column m of them
-                const _Float16 *const at = &k_lds[wave][32 * g + 8 * q + (m >> 2)][8 * ((m & 3) ^ q) + 4 * t];
-                const h4 k0 = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at));
-                const h4 k1 = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + 4 * 32)));
-                const h8 kt = {k0[0], k0[1], k0[2], k0[3], k1[0], k1[1], k1[2], k1[3]};
+                // elements 8 c + 4 t .. + 3 (c < 4) of four keys, alike
+                const _Float16 *const at = &lds.k[buf][wave][(32 * g + 8 * q + (m >> 2)) * 32 + 8 * ((m & 3) ^ q) + 4 * t];
+                const h4 x = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at));
+                const h4 y = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + 4 * 32)));
+                const h8 kt = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
                 acc[t] = mfma16(kt, b_lo, mfma16(kt, b_hi, acc[t]));
             }
         }
-        const float back = u_back * w_back;
+        const float s_more = u_back * w_back;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) S[t][i] = __builtin_fmaf(acc[t][i], back, decay * S[t][i]);
-
-        // out = e^G Q S + P U
-        const float o_back = u_back * p_back;
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            const int t = wave * TT + tt;
-            f4 x = zero, y = zero;
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                if (g > t >> 1) continue;
-                const h8 b_hi = u_lds[g][0][lane], b_lo = u_lds[g][1][lane];
-                x = mfma16(pf[tt][g][0], b_hi, x);
-                y = mfma16(pf[tt][g][0], b_lo, y);
-                y = mfma16(pf[tt][g][1], b_hi, y);
-            }
-            const int r0 = c * kChunk + row_of(t, 4 * q);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float o = __builtin_fmaf(x[i] + y[i], o_back, fq[tt][i] * qs[tt][i]);
-                if (r0 + i < rows.count)
-                    ((_Float16 *)a.out.data)[((size_t)rows.first + r0 + i) * a.out.token_stride +
-                                             head * a.out.head_stride + 16 * slice + m] = (_Float16)o;
-            }
-        }
-        load_matrix(next, 1, pf);
-        load_u(next, 1, fq);
+            for (int i = 0; i < 4; ++i) S[t][i] = __builtin_fmaf(acc[t][i], s_more, decay * S[t][i]);
     }
-    if (out >= 0) {
+    if (p.slot_out >= 0) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                a.states[out * state_size + state_at + (size_t)(4 * t + i) * a.value_dim] = S[t][i];
+                a.states[p.slot_out * state_size + state_at + (size_t)(4 * t + i) * a.value_dim] = S[t][i];
     }
+}
+
+template <int KD, bool VEC, bool UPPER>
+__device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace &p, ScanLds<KD> &lds, int wave, int lane) {
+    constexpr int NW = KD / 32, TT = 4 / NW, G = UPPER ? 2 : 1;
+    if (!p.n_chunks) return;
+    const int m = lane & 15, q = lane >> 4;
+    uint32_t q_at[TT], k_at[4];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt)
+        q_at[tt] = (uint32_t)row_of(wave * TT + tt, m) * (uint32_t)(2 * a.q.token_stride) + 16 * q;
+    // keys: KD / 8 lanes a row, 64 / NW rows a wave in four loads
+    constexpr int L = KD / 8;
+    const int k_row = wave * (64 / NW) + lane / L, k_run = lane % L;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) k_at[j] = (uint32_t)(k_row + j * (64 / L)) * (uint32_t)(2 * a.k.token_stride) + 16 * k_run;
+    // values: two lanes a row of 16 columns, 32 rows in each of the first two waves
+    const int v_row = 32 * wave + (lane >> 1);
+    const uint32_t v_at = (uint32_t)v_row * (uint32_t)(2 * a.v.token_stride) + 16 * (lane & 1);
+
+    h8 qf[TT][NW], pf[TT][G][2], kr[4], vr;
+    f4 qs[TT], factors;
+    float scalar, o_back;
+    auto load_q = [&](int c) {
+        const Buffer b = chunk_rows(a.q, p, c, p.kh, 0, KD);
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+            for (int g = 0; g < NW; ++g) qf[tt][g] = load_run<VEC>(b, q_at[tt] + 64 * g);
+        in_order();
+    };
+    auto load_next = [&](int c) {  // what goes to LDS
+        const Buffer b = chunk_rows(a.k, p, c, p.kh, 0, KD);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kr[j] = load_run<VEC>(b, k_at[j]);
+        if (wave < 2) vr = load_run<VEC>(chunk_rows(a.v, p, c, p.head, 16 * p.slice, 16), v_at);
+        if (wave == 0) {
+            const char *const f = p.block0 + c * p.step + kRowFactors;
+            factors = ((const f4 *)f)[lane];
+            scalar = ((const float *)(f + 4 * kChunk * 4))[lane & 7];
+        }
+        in_order();
+    };
+    auto put_next = [&](int buf) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int row = k_row + j * (64 / L);
+            *(h8 *)&lds.k[buf][k_run >> 2][row * 32 + 8 * ((k_run ^ (row >> 3)) & 3)] = kr[j];
+        }
+        if (wave < 2) {  // V's rows and the largest of them
+            *(h8 *)&lds.v[v_row][8 * (lane & 1)] = vr;
+            float top = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf((float)vr[e]));
+            lds.v_top[wave] = wave_max(top);
+        }
+        if (wave == 0) {
+            (&lds.factor[buf][0][0])[lane] = factors;
+            lds.scalar[buf][lane & 7] = scalar;
+        }
+    };
+    auto put_out = [&](int c) {  // e^G Q S + P U
+        const Buffer b = chunk_rows(a.out, p, c, p.head, 16 * p.slice, 16);
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+            const int t = wave * TT + tt;
+            const f4 x = lower_product<G>(pf[tt], lds.u, lane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                lds.o[16 * t + 4 * q + i][m] = (_Float16)__builtin_fmaf(x[i], o_back, qs[tt][i]);
+            // 16 rows, two lanes each
+            const uint32_t at = (uint32_t)row_of(t, (lane >> 1) & 15) * (uint32_t)(2 * a.out.token_stride) + 16 * (lane & 1);
+            const h8 o = *(const h8 *)&lds.o[16 * t + ((lane >> 1) & 15)][8 * (lane & 1)];
+            if (lane < 32) {
+                if constexpr (VEC) {
+                    __builtin_amdgcn_raw_buffer_store_b128(bitcast<u4>(o), b, at, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        __builtin_amdgcn_raw_buffer_store_b16(bitcast<uint16_t>((_Float16)o[e]), b, at + 2 * e, 0, 0);
+                }
+            }
+        }
+        in_order();
+    };
+    if (NW > 2 && wave >= 2) lds.v_top[wave] = 0.f;
+    load_next(0);
+    load_q(0);
+    put_next(0);
+    in_order();
+    load_next(min(1, p.n_chunks - 1));
+    lds_barrier();
+    for (int c = 0; c < p.n_chunks; ++c) {
+        const int next = min(c + 1, p.n_chunks - 1), after = min(c + 2, p.n_chunks - 1), buf = c & 1;
+        lds_barrier();  // 1
+        if (c) put_out(c - 1);
+        load_matrix<TT, G>(p, c, 1, wave, lane, pf);
+        lds_barrier();  // 2
+        h8 s_hi[NW], s_lo[NW];
+        float back[NW];
+#pragma unroll
+        for (int g = 0; g < NW; ++g) {
+            s_hi[g] = lds.s[g][0][lane];
+            s_lo[g] = lds.s[g][1][lane];
+            back[g] = lds.back[g][m];
+        }
+        o_back = lds.u_back[m] * lds.scalar[buf][kPBack];
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+            qs[tt] = state_product<NW>(qf[tt], s_hi, s_lo, back) * lds.factor[buf][1][row_of(wave * TT + tt, 4 * q) / 4];
+        in_order();
+        load_q(next);
+        put_next(buf ^ 1);
+        in_order();
+        load_next(after);
+        lds_barrier();  // 3
+    }
+    put_out(p.n_chunks - 1);
+}
+
+template <int KD, bool VEC>
+__global__ __launch_bounds__(4 * KD) void delta_scan_kernel(DeltaArgs a, const char *chunks, size_t tiles, int units,
+                                                            int slices) {
+    constexpr int NW = KD / 32;
+    __shared__ __attribute__((aligned(16))) ScanLds<KD> lds;
+    // the slices of a head on one XCD, whose L2 then holds what they share
+    const int id = blockIdx.x, at_xcd = id >> 3;
+    const int unit = at_xcd / slices * 8 + (id & 7);
+    if (unit >= units) return;
+    const int heads = a.v.heads, s = unit / heads;
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+    ScanPlace p;
+    p.slice = at_xcd % slices;
+    p.head = unit - s * heads;
+    p.kh = p.head / (heads / a.k.heads);
+    const Rows rows = rows_of(a.s, s);
+    p.rows = {uniform(rows.first), uniform(rows.count)};
+    p.slot_in = uniform(slot_in(a.s, s));
+    p.slot_out = uniform(slot_out(a.s, s));
+    const size_t tile0 = uniform(tiles_before(a.s, s, lane));
+    // starts that overlap have more chunks than the workspace holds: those are left out
+    p.n_chunks = (int)min((size_t)(p.rows.count + kChunk - 1) / kChunk, tiles - min(tiles, tile0));
+    p.block0 = chunks + (tile0 * heads + p.head) * kChunkBytes;
+    p.step = (size_t)heads * kChunkBytes;
+    if (wave < NW / 2) state_wave<KD, false>(a, p, lds, wave, lane);
+    else if (wave < NW) state_wave<KD, true>(a, p, lds, wave, lane);
+    else if (wave < NW + NW / 2) output_wave<KD, VEC, false>(a, p, lds, wave - NW, lane);
+    else output_wave<KD, VEC, true>(a, p, lds, wave - NW, lane);
 }
 
 template <int KD>
@@ -617,12 +740,21 @@ hipError_t launch_kd(const DeltaArgs &a, char *chunks, hipStream_t stream) {
     const size_t tiles = tile_count(a.s, kChunk);
     delta_prepare_kernel<KD><<<dim3((unsigned)(tiles * a.v.heads)), dim3(256), 0, stream>>>(a, chunks);
     const int units = a.s.sequences * a.v.heads, slices = a.value_dim / 16;
-    const unsigned blocks = (unsigned)((units + 7) / 8 * 8 * slices);
-    delta_scan_kernel<KD><<<dim3(blocks), dim3(2 * KD), 0, stream>>>(a, chunks, tiles, units, slices);
+    const dim3 blocks((unsigned)((units + 7) / 8 * 8 * slices));
+    if (a.q.vec && a.k.vec && a.v.vec && a.out.vec)
+        delta_scan_kernel<KD, true><<<blocks, dim3(4 * KD), 0, stream>>>(a, chunks, tiles, units, slices);
+    else
+        delta_scan_kernel<KD, false><<<blocks, dim3(4 * KD), 0, stream>>>(a, chunks, tiles, units, slices);
     return hipGetLastError();
 }
 
 }  // namespace
+
+bool delta_prompt_serves(const DeltaArgs &a) {
+    const size_t most = (size_t)1 << 24;
+    return a.q.token_stride <= most && a.k.token_stride <= most && a.v.token_stride <= most &&
+           a.out.token_stride <= most;
+}
 
 size_t delta_prompt_bytes(size_t heads, size_t sequences, size_t tokens) {
     if (tokens < kDeltaPromptRows * sequences) return 0;

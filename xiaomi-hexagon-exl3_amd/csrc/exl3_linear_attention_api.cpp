@@ -154,7 +154,7 @@ exl3_status exl3_hip_delta_rule(const exl3_head_view *q, const exl3_head_view *k
     a.scale = scale;
     a.eps = qk_eps;
     const size_t need = delta_prompt_bytes(v->heads, sequences, tokens);
-    if (!need) return from_hip(launch_delta_step(a, stream));
+    if (!need || !delta_prompt_serves(a)) return from_hip(launch_delta_step(a, stream));
     WorkspaceLease lease;
     const exl3_status st = take_workspace(need, stream, &lease, &workspace, &workspace_bytes);
     if (st != EXL3_OK) return st;
