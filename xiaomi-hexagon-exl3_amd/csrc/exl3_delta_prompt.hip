@@ -37,9 +37,13 @@ constexpr int kRowFactors = 2 * kFrags * 2 * kFrag;  // byte offsets
 constexpr int kScalars = kRowFactors + 4 * kChunk * 4;
 constexpr int kChunkBytes = kScalars + 256;
 enum { kRState, kRValue, kUFit, kUBack, kDecay, kWBack, kPBack };  // scalars
+// What a chunk and key head have there: the keys as rows (fragment 4 g + t: elements 32 g .., row tile t) and as
+// columns (fragment 4 g + 2 k + t: element tile t of 32 g .., rows 32 k ..), the queries as rows (fragment t KD / 32 + g).
+constexpr int kKeyFrags = 4;  // a 32 elements, of each
+__host__ __device__ constexpr size_t key_bytes(int key_dim) { return (size_t)3 * (key_dim / 32) * kKeyFrags * kFrag; }
 // fragment of row tile t (16 rows) and columns 32 s .. 32 s + 31: s <= t / 2
 __device__ __forceinline__ int frag_of(int t, int s) { return (t < 2 ? t : 2 * t - 2) + s; }
-// the chunk's row that row m of row tile t stands for
+// The chunk's row that row m of row tile t of K, R, U and T stands for (those of Q, P and out are in their order)
 __device__ __forceinline__ int row_of(int t, int m) { return 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3); }
 
 __device__ __forceinline__ f4 mfma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -82,12 +86,22 @@ __device__ __forceinline__ void split8(f4 x, f4 y, h8 &hi, h8 &lo) {
     lo = (h8){b[0], b[1], b[2], b[3], d[0], d[1], d[2], d[3]};
 }
 
-// maximum over lanes l ^ 16, l ^ 32
+// maximum over lanes l ^ 16, l ^ 32 of numbers that are not negative (as such their bits are in their order)
 __device__ __forceinline__ float max_quarters(float v) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
-    v = fmaxf(__int_as_float(a[0]), __int_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
-    return fmaxf(__int_as_float(b[0]), __int_as_float(b[1]));
+    const uint32_t w = max((uint32_t)a[0], (uint32_t)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return __uint_as_float(max((uint32_t)b[0], (uint32_t)b[1]));
+}
+__device__ __forceinline__ h2 larger(h2 a, h2 b) { return __builtin_elementwise_max(a, b); }
+// over the wave, without LDS
+__device__ __forceinline__ float max_lanes(float v) {
+    uint32_t w = __float_as_uint(v);
+    w = max(w, __float_as_uint(dpp_xor<1>(__uint_as_float(w))));
+    w = max(w, __float_as_uint(dpp_xor<2>(__uint_as_float(w))));
+    w = max(w, __float_as_uint(dpp_xor<4>(__uint_as_float(w))));
+    w = max(w, __float_as_uint(dpp_xor<8>(__uint_as_float(w))));
+    return max_quarters(__uint_as_float(w));
 }
 __device__ __forceinline__ float sum_quarters(float v) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
@@ -104,9 +118,17 @@ __device__ __forceinline__ h8 load_h8(const _Float16 *p, int vec) {
     return t;
 }
 
+// Where 16-byte run c of row r of rows of KD elements in LDS is: 16 rows' runs c lie in all banks, as do a row's runs.
+template <int KD>
+__device__ __forceinline__ int query_at(int r, int c) {
+    return KD == 128 ? r * 128 + 8 * (c ^ (r & 15)) : r * 64 + 8 * (c ^ ((r >> 1) & 7));
+}
+
 // Loads stay in their order across this, ahead of the loop as in it: a wait for one is a wait for all that were
 // issued before it.
 __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
+// What was read from LDS is there: reads that wait for the registers of the products ahead of them come a round trip later.
+__device__ __forceinline__ void lds_here() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 // The LDS that waves share is complete; loads from memory stay on their way.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -122,8 +144,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
     __shared__ double sum_lds[kChunk];
     __shared__ float kr_lds[kChunk], qr_lds[kChunk], most_lds[4], l1_lds[4], sum_T_lds[4];
     float *const A = lds, *const Pm = lds + kMatrix, *const T = lds + 2 * kMatrix;
-    h8 *const kf_lds = (h8 *)T;  // the keys' fragments, until T takes their place
-    static_assert(4 * NK * kFrag <= kMatrix * 4, "the keys fit");
+    static_assert(kChunk * KD * 2 <= kMatrix * 4, "the keys fit");
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int heads = a.v.heads, tile = blockIdx.x / heads, head = blockIdx.x - tile * heads;
@@ -135,18 +156,23 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
     const size_t first = (size_t)t.rows.first + t.row0;
     const int kh = head / (heads / a.k.heads);
 
-    // rows beyond the last: zero keys, decay 1, beta 0
+    // Rows are loaded whole, KD / 8 lanes each, and get into the operands' order through LDS (see output_wave): the
+    // keys where T will be, the queries where the wave's own rows of A will be.  Rows beyond the last: zeros, decay 1,
+    // beta 0.
+    constexpr int L = KD / 8;
     const int row = 16 * wave + m;
-    h8 kf[NK], qf[NK];
+    _Float16 *const k_lds = (_Float16 *)T, *const q_lds = (_Float16 *)(A + 16 * wave * kRowFloats);
 #pragma unroll
-    for (int s = 0; s < NK; ++s) {
-        kf[s] = qf[s] = (h8){};
-        if (row < count) {
-            kf[s] = load_h8((const _Float16 *)a.k.data + (first + row) * a.k.token_stride + kh * a.k.head_stride +
-                                32 * s + 8 * q, a.k.vec);
-            qf[s] = load_h8((const _Float16 *)a.q.data + (first + row) * a.q.token_stride + kh * a.q.head_stride +
-                                32 * s + 8 * q, a.q.vec);
+    for (int j = 0; j < 16 * L / 64; ++j) {
+        const int r = 64 / L * j + lane / L, c = lane % L;
+        h8 x{}, y{};
+        if (16 * wave + r < count) {
+            const size_t at = first + 16 * wave + r;
+            x = load_h8((const _Float16 *)a.k.data + at * a.k.token_stride + kh * a.k.head_stride + 8 * c, a.k.vec);
+            y = load_h8((const _Float16 *)a.q.data + at * a.q.token_stride + kh * a.q.head_stride + 8 * c, a.q.vec);
         }
+        *(h8 *)(k_lds + query_at<KD>(16 * wave + r, c)) = x;
+        *(h8 *)(q_lds + query_at<KD>(r, c)) = y;
     }
     Gates gt{0.f, 0.f};
     if (lane < count) gt = gates_of(a, first + lane, head);
@@ -157,9 +183,11 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
         G += lane >= d ? o : 0.0;
     }
     float kk = 0.f, qq = 0.f, k1 = 0.f;
+    h8 kf[NK], qf[NK];
 #pragma unroll
     for (int s = 0; s < NK; ++s) {
-        kf_lds[(wave * NK + s) * 64 + lane] = kf[s];
+        kf[s] = *(const h8 *)(k_lds + query_at<KD>(row, 4 * s + q));
+        qf[s] = *(const h8 *)(q_lds + query_at<KD>(m, 4 * s + q));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float x = (float)kf[s][j], y = (float)qf[s][j];
@@ -184,7 +212,22 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
     }
     __syncthreads();
 
-    char *const block = chunks + ((size_t)tile * heads + head) * kChunkBytes;
+    if (head == kh * (heads / a.k.heads)) {  // one value head of the key head's
+        char *const keys = chunks + gridDim.x * (size_t)kChunkBytes + ((size_t)kh * (gridDim.x / heads) + tile) * key_bytes(KD);
+        h8 *const rows = (h8 *)keys + lane, *const columns = rows + NK * kKeyFrags * 64, *const queries = columns + NK * kKeyFrags * 64;
+#pragma unroll
+        for (int s = 0; s < NK; ++s) {
+            rows[(s * 4 + wave) * 64] = *(const h8 *)(k_lds + query_at<KD>(row_of(wave, m), 4 * s + q));
+            queries[(wave * NK + s) * 64] = qf[s];
+            // 16 lanes read elements 32 s + 8 c + 4 t .. + 3 (c < 4) of four rows: lane m gets column m of them
+            const int k = wave >> 1, t = wave & 1, r = 32 * k + 8 * q + (m >> 2), c = 4 * s + (m & 3);
+            const h4 x = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(k_lds + query_at<KD>(r, c) + 4 * t)));
+            const h4 y = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(k_lds + query_at<KD>(r + 4, c) + 4 * t)));
+            columns[(s * 4 + wave) * 64] = (h8){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        }
+    }
+    // a head's chunks next to each other: the walk over them stays in few pages
+    char *const block = chunks + ((size_t)head * (gridDim.x / heads) + tile) * kChunkBytes;
     f4 kk_acc[4], qk_acc[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -192,7 +235,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
         if (j <= wave) {
 #pragma unroll
             for (int s = 0; s < NK; ++s) {
-                const h8 b = kf_lds[(j * NK + s) * 64 + lane];
+                const h8 b = *(const h8 *)(k_lds + query_at<KD>(16 * j + m, 4 * s + q));
                 kk_acc[j] = mfma16(kf[s], b, kk_acc[j]);
                 qk_acc[j] = mfma16(qf[s], b, qk_acc[j]);
             }
@@ -211,6 +254,12 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int c = 16 * j + m;
+        if (j > (wave | 1)) continue;  // above the diagonal's fragments
+        if (j > wave) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) Pm[(16 * wave + 4 * q + r) * kRowFloats + c] = 0.f;
+            continue;
+        }
         const double Gc = sum_lds[c];
         const float kc = kr_lds[c];
 #pragma unroll
@@ -227,12 +276,12 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
             p_most = fmaxf(p_most, __builtin_fabsf(pv));
         }
     }
-    p_most = wave_max(p_most);
+    p_most = max_lanes(p_most);
     if (lane == 0) most_lds[wave] = p_most;
     // row factors and scalars, by the wave that has the rows' k1: each wave its 16, wave 0 all
     const float beta_row = __shfl(gt.beta, row);
     const float since = decay_of((float)__shfl(G, row)) * rk;
-    const float l1 = wave_max(__builtin_fabsf(beta_row * since) * k1);
+    const float l1 = max_lanes(__builtin_fabsf(beta_row * since) * k1);
     if (lane == 0) l1_lds[wave] = l1;
     const double G_end = __shfl(G, 63);
     __syncthreads();
@@ -286,7 +335,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
         for (int r = 0; r < 4; ++r)
             T[(16 * bi + 4 * q + r) * kRowFloats + 16 * wave + m] = wave + i < 4 ? T_col[i][r] : 0.f;
     }
-    t_most = wave_max(t_most);
+    t_most = max_lanes(t_most);
     if (lane == 0) most_lds[wave] = t_most;
     __syncthreads();
     const float t_top = fmaxf(fmaxf(most_lds[0], most_lds[1]), fmaxf(most_lds[2], most_lds[3]));
@@ -299,7 +348,8 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
         if (s > wave >> 1) break;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
-            const float *const from = (which ? Pm : T) + row_of(wave, m) * kRowFloats + 32 * s + 8 * q;
+            const float *const from =
+                (which ? Pm + row * kRowFloats : T + row_of(wave, m) * kRowFloats) + 32 * s + 8 * q;
             const float to = which ? pf.to : tf.to;
             h8 hi, lo;
             split8(*(const f4 *)from * to, *(const f4 *)(from + 4) * to, hi, lo);
@@ -312,20 +362,20 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
             at[64] = lo;
         }
     }
-    t_sum = wave_max(sum_quarters(t_sum));
+    t_sum = max_lanes(sum_quarters(t_sum));
     if (lane == 0) sum_T_lds[wave] = t_sum;
     __syncthreads();
     if (wave == 0) {  // lane = row
         const float r = kr_lds[lane], e = decay_of((float)G);
         const float until = decay_of((float)(G_end - G)) * r;
-        int e_w = __builtin_amdgcn_frexp_expf(wave_max(__builtin_fabsf(until)));
+        int e_w = __builtin_amdgcn_frexp_expf(max_lanes(__builtin_fabsf(until)));
         e_w = e_w < -110 ? -110 : e_w;
         float *const f = (float *)(block + kRowFactors);
         f[lane] = e * r;
         f[kChunk + lane] = e * qr_lds[lane];
         f[2 * kChunk + lane] = gt.beta;
         f[3 * kChunk + lane] = __builtin_amdgcn_ldexpf(until, -e_w);
-        const float beta_most = wave_max(__builtin_fabsf(gt.beta));
+        const float beta_most = max_lanes(__builtin_fabsf(gt.beta));
         if (lane == 0) {
             float *const s = (float *)(block + kScalars);
             s[kDecay] = decay_of((float)G_end);
@@ -338,6 +388,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
             s[kWBack] = __builtin_amdgcn_ldexpf(1.f, e_w);
             s[kRState] = fmaxf(fmaxf(l1_lds[0], l1_lds[1]), fmaxf(l1_lds[2], l1_lds[3]));
             s[kRValue] = beta_most;
+            s[7] = 0.f;  // loaded along
         }
     }
 }
@@ -366,43 +417,50 @@ __device__ __forceinline__ size_t uniform(size_t v) {
 
 // A workgroup has columns 16 slice .. of one head's state, and two kinds of waves, KD / 32 of each.  State wave w has
 // rows 32 w .. 32 w + 31 of the state, as two tiles, and TT of the chunk's four row tiles of R and U: what the next chunk
-// waits for.  Output wave w has Q S, P U and the rows of out of the same row tiles, a step behind, and brings K, V and the
-// rows' factors into LDS, a chunk ahead.  VEC: 16 bytes of a row are one load.
+// waits for.  Output wave w has Q S, P U and out of TT row tiles, and the first two bring V into LDS.  Everything else is
+// read as operands, straight from the workspace.  VEC: 16 bytes of a row of v and out are one access.
 //
 // LDS, by the barrier (1 to 3 of a chunk) that its writes are ahead of and the one that its reads are ahead of:
-// s, back: 1, 3;  v: 3 (of the chunk before), 2;  k, factor, scalar: 3 (of the chunk before), 1 of the next, and two of
-// each;  r, u_back: 2, 3;  w: 3, 1 of the next;  u: 3, 2 of the next.  A buffer is written again only past the barrier that
-// its reads are ahead of.  o is a wave's own.
+// s, back, ks: 1, 2;  v: 3 of the chunk before, 2;  v_top: 1, 2;  r, u_back: 2, 3;  u, w: 3, 1 of the next.  A buffer is
+// written again only past the barrier that its reads are ahead of.  o is a wave's own.
 template <int KD>
 struct ScanLds {
     static constexpr int NW = KD / 32;
     h8 s[NW][2][64];                  // the state's operand: 32 rows, high and low
+    f4 ks[NW][4][64];                 // K S of those rows alone, the chunk's row tiles
     h8 r[2][2][64];                   // R's, 32 rows each
     h8 u[2][2][64], w[2][2][64];
-    // 32 elements of each key, 16-byte runs c at c ^ (row / 8 % 4); another 64 bytes put the four runs of an element
-    // group into other banks than the next group's
-    _Float16 k[2][NW][kChunk * 32 + 32];
     _Float16 v[kChunk][16], o[kChunk][16];
-    f4 factor[2][4][kChunk / 4];      // of the chunk's rows
-    float scalar[2][8];
-    float back[NW][16], u_back[16], v_top[NW];
+    float back[NW][16], u_back[16], v_top[2];
 };
 
 struct ScanPlace {
     Rows rows;
-    const char *block0;  // the first chunk's part of the workspace, a chunk's distance from it to the next
-    size_t step;
-    int n_chunks, head, kh, slice, slot_in, slot_out;
+    const char *block, *keys;  // the first chunk's parts of the workspace
+    int n_chunks, head, slice, slot_in, slot_out;
 };
 
-// A chunk's rows as a buffer: what is beyond the sequence's last row reads as zero and is not written.
+// A sequence's rows, a chunk of them at a time, as a buffer: what is beyond the last row reads as zero and is not written.
 typedef __amdgpu_buffer_rsrc_t Buffer;
-__device__ __forceinline__ Buffer chunk_rows(const Heads &h, const ScanPlace &p, int c, int head, int at, int width) {
-    const size_t stride = h.token_stride;
-    char *const base = (char *)((_Float16 *)h.data + (p.rows.first + (size_t)c * kChunk) * stride + head * h.head_stride + at);
-    const uint32_t left = min(p.rows.count - c * kChunk, kChunk);
-    return __builtin_amdgcn_make_buffer_rsrc(base, 0, ((left - 1) * (uint32_t)stride + width) * 2, 0x00020000);
-}
+struct ChunkRows {
+    char *base;      // the chunk's first row
+    uint32_t row;    // bytes from a row to the next
+    int left, width; // rows of the sequence from the chunk's on, bytes of a row that are used
+    __device__ __forceinline__ ChunkRows(const Heads &h, const ScanPlace &p, int head, int at, int elements) {
+        base = (char *)((_Float16 *)h.data + p.rows.first * h.token_stride + head * h.head_stride + at);
+        row = (uint32_t)(2 * h.token_stride);
+        left = p.rows.count;
+        width = 2 * elements;
+    }
+    __device__ __forceinline__ Buffer buffer() const {
+        const int n = min(left, kChunk);
+        return __builtin_amdgcn_make_buffer_rsrc(base, 0, n > 0 ? (n - 1) * row + width : 0, 0x00020000);
+    }
+    __device__ __forceinline__ void step() {
+        base += (size_t)row * kChunk;
+        left -= kChunk;
+    }
+};
 template <bool VEC>
 __device__ __forceinline__ h8 load_run(Buffer b, uint32_t at) {
     if constexpr (VEC) {
@@ -415,10 +473,18 @@ __device__ __forceinline__ h8 load_run(Buffer b, uint32_t at) {
     }
 }
 
+// A part of the workspace that is read chunk by chunk; behind the last chunk it is the last one's again.
+struct Part {
+    const char *at;
+    size_t distance;
+    int left;
+    __device__ __forceinline__ Part(const char *first, size_t step, int n) : at(first), distance(step), left(n) {}
+    __device__ __forceinline__ void step() { at += --left > 0 ? distance : 0; }
+};
 // T's or P's fragments of a wave's row tiles: G of them each
 template <int TT, int G>
-__device__ __forceinline__ void load_matrix(const ScanPlace &p, int c, int which, int wave, int lane, h8 (&to)[TT][G][2]) {
-    const h8 *const f = (const h8 *)(p.block0 + c * p.step + which * kFrags * 2 * kFrag) + lane;
+__device__ __forceinline__ void load_matrix(const char *from, int wave, int lane, h8 (&to)[TT][G][2]) {
+    const h8 *const f = (const h8 *)from + lane;
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
@@ -427,18 +493,23 @@ __device__ __forceinline__ void load_matrix(const ScanPlace &p, int c, int which
             to[tt][g][1] = f[frag_of(wave * TT + tt, g) * 128 + 64];
         }
 }
-// A row tile of T or P times R or U
+// A row tile of T or P times R or U (b's first 32 rows, or all 64)
 template <int G>
-__device__ __forceinline__ f4 lower_product(const h8 (&m)[G][2], const h8 (&b)[2][2][64], int lane) {
-    f4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+__device__ __forceinline__ void read_pairs(const h8 (&b)[2][2][64], int lane, h8 (&to)[G][2]) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) to[g][0] = b[g][0][lane], to[g][1] = b[g][1][lane];
+}
+template <int G>
+__device__ __forceinline__ f4 lower_product(const h8 (&m)[G][2], const h8 (&b)[G][2]) {
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+    f4 x = zero, y = zero, z = zero;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-        const h8 b_hi = b[g][0][lane], b_lo = b[g][1][lane];
-        x = mfma16(m[g][0], b_hi, x);
-        y = mfma16(m[g][0], b_lo, y);
-        y = mfma16(m[g][1], b_hi, y);
+        x = mfma16(m[g][0], b[g][0], x);
+        y = mfma16(m[g][0], b[g][1], y);
+        z = mfma16(m[g][1], b[g][0], z);
     }
-    return x + y;
+    return x + (y + z);
 }
 template <typename L>
 __device__ __forceinline__ void put_quarter(L &lds, int t, int lane, f4 x) {
@@ -481,26 +552,55 @@ __device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &
             S[t][i] = p.slot_in >= 0 ? a.states[p.slot_in * state_size + state_at + (size_t)(4 * t + i) * a.value_dim] : start;
     asm volatile("" : "+v"(S[0]), "+v"(S[1]));  // waited for here: in the loop it would be a wait for all loads
 
-    h8 tf[TT][G][2];
-    if (p.n_chunks) load_matrix<TT, G>(p, 0, 0, wave, lane, tf);
-    const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    if (p.n_chunks) lds_barrier();
-    for (int c = 0; c < p.n_chunks; ++c) {
-        const int next = min(c + 1, p.n_chunks - 1), buf = c & 1;
-        h8 kf[TT][NW];
-        f4 fk[TT], fb[TT], fu[TT];
+    // the keys' 32 elements of the wave, as rows of the chunk's tiles and as columns
+    h8 kf[4], kt[2][2], tf[TT][G][2];
+    f4 fk[TT], fb[TT], fu[TT];
+    float sc[8], next_sc[8];  // through registers of the lanes: a scalar load would be waited for with LDS
+    Part rows(p.keys + wave * 4 * kFrag, key_bytes(KD), p.n_chunks), factors(p.block + kRowFactors, kChunkBytes, p.n_chunks),
+        t_part(p.block, kChunkBytes, p.n_chunks), columns(p.keys + (NW + wave) * 4 * kFrag, key_bytes(KD), p.n_chunks);
+    auto load_rows = [&]() {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) kf[t] = ((const h8 *)rows.at)[64 * t + lane];
+        rows.step();
+        in_order();
+    };
+    auto load_factors = [&]() {
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
-            const int t = wave * TT + tt, r4 = row_of(t, 4 * q) / 4;
-#pragma unroll
-            for (int g = 0; g < NW; ++g) kf[tt][g] = *(const h8 *)&lds.k[buf][g][row_of(t, m) * 32 + 8 * (q ^ (m >> 2))];
-            fk[tt] = lds.factor[buf][0][r4];
-            fb[tt] = lds.factor[buf][2][r4];
-            fu[tt] = lds.factor[buf][3][r4];
+            const int r4 = row_of(wave * TT + tt, 4 * q) / 4;
+            fk[tt] = ((const f4 *)factors.at)[r4];
+            fb[tt] = ((const f4 *)factors.at)[2 * kChunk / 4 + r4];
+            fu[tt] = ((const f4 *)factors.at)[3 * kChunk / 4 + r4];
         }
-        const f4 sc = *(const f4 *)&lds.scalar[buf][0];
-        const float decay = lds.scalar[buf][kDecay], w_back = lds.scalar[buf][kWBack];
-
+        const f4 x = ((const f4 *)(factors.at + kScalars - kRowFactors))[0], y = ((const f4 *)(factors.at + kScalars - kRowFactors))[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) next_sc[i] = x[i], next_sc[4 + i] = y[i];
+        factors.step();
+        in_order();
+    };
+    auto load_t = [&]() {
+        load_matrix<TT, G>(t_part.at, wave, lane, tf);
+        t_part.step();
+        in_order();
+    };
+    auto load_columns = [&]() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kt[i >> 1][i & 1] = ((const h8 *)columns.at)[64 * i + lane];
+        columns.step();
+        in_order();
+    };
+    if (p.n_chunks) {
+        in_order();
+        load_rows();
+        load_factors();
+        load_t();
+        load_columns();
+        lds_barrier();
+    }
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < p.n_chunks; ++c) {
+#pragma unroll
+        for (int i = 0; i < 7; ++i) sc[i] = next_sc[i];
         // the state as an operand, each wave's rows by their own power of two a column
         float top = 0.f;
 #pragma unroll
@@ -510,73 +610,84 @@ __device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &
         const Fit sf = fit_of(max_quarters(top));
         h8 hi, lo;
         split8(S[0] * sf.to, S[1] * sf.to, hi, lo);
+        f4 x[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] = mfma16(kf[t], hi, zero);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] = mfma16(kf[t], lo, x[t]);
         lds.s[wave][0][lane] = hi;
         lds.s[wave][1][lane] = lo;
-        lds.back[wave][m] = sf.back;  // the same from four lanes
+        if (q == 0) lds.back[wave][m] = sf.back;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) lds.ks[wave][t][lane] = x[t] * sf.back;
         lds_barrier();  // 1
 
         // R = beta (V - e^G K S), |R| <= r_value |V| + r_state |S|
-        h8 s_hi[NW], s_lo[NW];
-        float back[NW], s_back = 0.f, v_top = 0.f;
+        f4 ks[TT][NW];
 #pragma unroll
-        for (int g = 0; g < NW; ++g) {
-            s_hi[g] = lds.s[g][0][lane];
-            s_lo[g] = lds.s[g][1][lane];
-        }
+        for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-        for (int g = 0; g < NW; ++g) {
-            back[g] = lds.back[g][m];
-            s_back = fmaxf(s_back, back[g]);
-            v_top = fmaxf(v_top, lds.v_top[g]);
-        }
-        const Fit rf = fit_of(__builtin_fmaf(sc[kRValue], v_top, sc[kRState] * (s_back * 32768.f)));
+            for (int g = 0; g < NW; ++g) ks[tt][g] = lds.ks[g][wave * TT + tt][lane];
+        in_order();  // loads are issued while LDS answers
+        load_rows();
+        float s_back = 0.f;
+#pragma unroll
+        for (int g = 0; g < NW; ++g) s_back = fmaxf(s_back, lds.back[g][m]);
+        const Fit rf = fit_of(__builtin_fmaf(sc[kRState] * 32768.f, s_back, sc[kRValue] * fmaxf(lds.v_top[0], lds.v_top[1])));
         const float u_back = rf.back * sc[kUBack];
+        f4 w_fit[TT];
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
             const int t = wave * TT + tt;
             // 16 lanes read four rows of V: lane m gets column m of them
             const h4 v = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (lds_s4 *)&lds.v[row_of(t, 4 * q) + (m >> 2)][4 * (m & 3)]));
-            const f4 ks = state_product<NW>(kf[tt], s_hi, s_lo, back);
-            f4 r;
+            f4 y = ks[tt][0], r;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = fb[tt][i] * rf.to * __builtin_fmaf(-fk[tt][i], ks[i], (float)v[i]);
+            for (int g = 1; g < NW; ++g) y += ks[tt][g];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = fb[tt][i] * rf.to * __builtin_fmaf(-fk[tt][i], y[i], (float)v[i]);
             put_quarter(lds.r, t, lane, r);
+            w_fit[tt] = fu[tt];
         }
-        if (wave == 0) lds.u_back[m] = u_back;
+        if (wave == 0 && q == 0) lds.u_back[m] = u_back;
         lds_barrier();  // 2
 
         // U = T R, and W = e^(G_64 - G) U for the state
+        h8 r[G][2];
+        read_pairs<G>(lds.r, lane, r);
+        in_order();
+        load_factors();
+        lds_here();
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
-            const f4 u = lower_product<G>(tf[tt], lds.r, lane) * sc[kUFit];
-            put_quarter(lds.w, wave * TT + tt, lane, u * fu[tt]);
+            const f4 u = lower_product<G>(tf[tt], r) * sc[kUFit];
+            put_quarter(lds.w, wave * TT + tt, lane, u * w_fit[tt]);
             put_quarter(lds.u, wave * TT + tt, lane, u);
         }
-        in_order();
-        load_matrix<TT, G>(p, next, 0, wave, lane, tf);
         lds_barrier();  // 3
 
         // S <- e^G_64 S + K^T W
-        f4 acc[2] = {zero, zero};
+        h8 w[2][2];
+        read_pairs<2>(lds.w, lane, w);
+        in_order();
+        load_t();
+        lds_here();
+        f4 acc[2] = {zero, zero}, acc_lo[2] = {zero, zero};
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            const h8 b_hi = lds.w[g][0][lane], b_lo = lds.w[g][1][lane];
+        for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                // elements 8 c + 4 t .. + 3 (c < 4) of four keys, alike
-                const _Float16 *const at = &lds.k[buf][wave][(32 * g + 8 * q + (m >> 2)) * 32 + 8 * ((m & 3) ^ q) + 4 * t];
-                const h4 x = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at));
-                const h4 y = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + 4 * 32)));
-                const h8 kt = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-                acc[t] = mfma16(kt, b_lo, mfma16(kt, b_hi, acc[t]));
+                acc[t] = mfma16(kt[g][t], w[g][0], acc[t]);
+                acc_lo[t] = mfma16(kt[g][t], w[g][1], acc_lo[t]);
             }
-        }
-        const float s_more = u_back * w_back;
+        in_order();
+        load_columns();
+        const float s_more = u_back * sc[kWBack];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) S[t][i] = __builtin_fmaf(acc[t][i], s_more, decay * S[t][i]);
+            for (int i = 0; i < 4; ++i) S[t][i] = __builtin_fmaf(acc[t][i] + acc_lo[t][i], s_more, sc[kDecay] * S[t][i]);
     }
     if (p.slot_out >= 0) {
 #pragma unroll
@@ -590,99 +701,97 @@ __device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &
 template <int KD, bool VEC, bool UPPER>
 __device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace &p, ScanLds<KD> &lds, int wave, int lane) {
     constexpr int NW = KD / 32, TT = 4 / NW, G = UPPER ? 2 : 1;
+    // known when compiled, so that the compiler can count the loads that are on their way
+    constexpr bool kValues = !UPPER || NW == 2;
     if (!p.n_chunks) return;
     const int m = lane & 15, q = lane >> 4;
-    uint32_t q_at[TT], k_at[4];
+    ChunkRows o_rows(a.out, p, p.head, 16 * p.slice, 16), v_rows(a.v, p, p.head, 16 * p.slice, 16);
+    // 16 rows of a tile, two lanes each.  The store is not left out by any lane or chunk (a place beyond the buffer is not
+    // written): where the compiler cannot count it, it waits for it together with the loads that it knows.
+    uint32_t o_at[TT];
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt)
-        q_at[tt] = (uint32_t)row_of(wave * TT + tt, m) * (uint32_t)(2 * a.q.token_stride) + 16 * q;
-    // keys: KD / 8 lanes a row, 64 / NW rows a wave in four loads
-    constexpr int L = KD / 8;
-    const int k_row = wave * (64 / NW) + lane / L, k_run = lane % L;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) k_at[j] = (uint32_t)(k_row + j * (64 / L)) * (uint32_t)(2 * a.k.token_stride) + 16 * k_run;
-    // values: two lanes a row of 16 columns, 32 rows in each of the first two waves
+        o_at[tt] = lane < 32 ? (uint32_t)(16 * (wave * TT + tt) + (lane >> 1)) * o_rows.row + 16 * (lane & 1) : 0xfffffff0u;
+    // values: two lanes a row of 16 columns, 32 rows a wave
     const int v_row = 32 * wave + (lane >> 1);
-    const uint32_t v_at = (uint32_t)v_row * (uint32_t)(2 * a.v.token_stride) + 16 * (lane & 1);
+    const uint32_t v_at = (uint32_t)v_row * v_rows.row + 16 * (lane & 1);
 
-    h8 qf[TT][NW], pf[TT][G][2], kr[4], vr;
-    f4 qs[TT], factors;
-    float scalar, o_back;
-    auto load_q = [&](int c) {
-        const Buffer b = chunk_rows(a.q, p, c, p.kh, 0, KD);
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-            for (int g = 0; g < NW; ++g) qf[tt][g] = load_run<VEC>(b, q_at[tt] + 64 * g);
+    h8 qf[TT][NW], pf[TT][G][2], vr;
+    f4 fq[TT], pu[TT] = {}, qs[TT] = {};
+    float o_back = 0.f, p_back;
+    Part queries(p.keys + (2 * NW * 4 + wave * TT * NW) * kFrag, key_bytes(KD), p.n_chunks),
+        factors(p.block + kRowFactors, kChunkBytes, p.n_chunks), p_part(p.block + kFrags * 2 * kFrag, kChunkBytes, p.n_chunks),
+        scalar(p.block + kScalars + 4 * kPBack, kChunkBytes, p.n_chunks);
+    auto load_p_back = [&]() {
+        p_back = *(const float *)scalar.at;
+        scalar.step();
         in_order();
     };
-    auto load_next = [&](int c) {  // what goes to LDS
-        const Buffer b = chunk_rows(a.k, p, c, p.kh, 0, KD);
+    auto load_q = [&]() {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) kr[j] = load_run<VEC>(b, k_at[j]);
-        if (wave < 2) vr = load_run<VEC>(chunk_rows(a.v, p, c, p.head, 16 * p.slice, 16), v_at);
-        if (wave == 0) {
-            const char *const f = p.block0 + c * p.step + kRowFactors;
-            factors = ((const f4 *)f)[lane];
-            scalar = ((const float *)(f + 4 * kChunk * 4))[lane & 7];
+        for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+            for (int g = 0; g < NW; ++g) qf[tt][g] = ((const h8 *)queries.at)[64 * (tt * NW + g) + lane];
+            fq[tt] = ((const f4 *)factors.at)[kChunk / 4 + 4 * (wave * TT + tt) + q];
         }
+        queries.step();
+        factors.step();
         in_order();
     };
-    auto put_next = [&](int buf) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int row = k_row + j * (64 / L);
-            *(h8 *)&lds.k[buf][k_run >> 2][row * 32 + 8 * ((k_run ^ (row >> 3)) & 3)] = kr[j];
-        }
-        if (wave < 2) {  // V's rows and the largest of them
+    auto load_p = [&]() {
+        load_matrix<TT, G>(p_part.at, wave, lane, pf);
+        p_part.step();
+        in_order();
+    };
+    auto load_v = [&]() {  // zeros behind the last chunk
+        if (kValues) vr = load_run<VEC>(v_rows.buffer(), v_at);
+        v_rows.step();
+        in_order();
+    };
+    h2 top = {};
+    auto put_v = [&]() {
+        if (kValues) {
             *(h8 *)&lds.v[v_row][8 * (lane & 1)] = vr;
-            float top = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf((float)vr[e]));
-            lds.v_top[wave] = wave_max(top);
-        }
-        if (wave == 0) {
-            (&lds.factor[buf][0][0])[lane] = factors;
-            lds.scalar[buf][lane & 7] = scalar;
+            const u4 x = bitcast<u4>(vr) & 0x7fff7fffu;
+            top = larger(larger(bitcast<h2>(x.x), bitcast<h2>(x.y)), larger(bitcast<h2>(x.z), bitcast<h2>(x.w)));
         }
     };
-    auto put_out = [&](int c) {  // e^G Q S + P U
-        const Buffer b = chunk_rows(a.out, p, c, p.head, 16 * p.slice, 16);
+    auto put_top = [&]() {  // the largest |V| of the wave's rows
+        if (kValues) {
+            const float x = max_lanes(fmaxf((float)top[0], (float)top[1]));
+            if (lane == 0) lds.v_top[wave] = x;
+        }
+    };
+    auto put_out = [&](Buffer b) {  // e^G Q S + P U
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
             const int t = wave * TT + tt;
-            const f4 x = lower_product<G>(pf[tt], lds.u, lane);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                lds.o[16 * t + 4 * q + i][m] = (_Float16)__builtin_fmaf(x[i], o_back, qs[tt][i]);
-            // 16 rows, two lanes each
-            const uint32_t at = (uint32_t)row_of(t, (lane >> 1) & 15) * (uint32_t)(2 * a.out.token_stride) + 16 * (lane & 1);
+                lds.o[16 * t + 4 * q + i][m] = (_Float16)__builtin_fmaf(pu[tt][i], o_back, qs[tt][i]);
             const h8 o = *(const h8 *)&lds.o[16 * t + ((lane >> 1) & 15)][8 * (lane & 1)];
-            if (lane < 32) {
-                if constexpr (VEC) {
-                    __builtin_amdgcn_raw_buffer_store_b128(bitcast<u4>(o), b, at, 0, 0);
-                } else {
+            if constexpr (VEC) {
+                __builtin_amdgcn_raw_buffer_store_b128(bitcast<u4>(o), b, o_at[tt], 0, 0);
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        __builtin_amdgcn_raw_buffer_store_b16(bitcast<uint16_t>((_Float16)o[e]), b, at + 2 * e, 0, 0);
-                }
+                for (int e = 0; e < 8; ++e)
+                    __builtin_amdgcn_raw_buffer_store_b16(bitcast<uint16_t>((_Float16)o[e]), b, o_at[tt] + 2 * e, 0, 0);
             }
         }
         in_order();
     };
-    if (NW > 2 && wave >= 2) lds.v_top[wave] = 0.f;
-    load_next(0);
-    load_q(0);
-    put_next(0);
+    load_v();
+    put_v();
+    put_top();
     in_order();
-    load_next(min(1, p.n_chunks - 1));
+    load_q();
+    load_v();
+    load_p_back();
+    load_p();
     lds_barrier();
+    Buffer before = __builtin_amdgcn_make_buffer_rsrc(o_rows.base, 0, 0, 0x00020000);  // nothing ahead of the first chunk
     for (int c = 0; c < p.n_chunks; ++c) {
-        const int next = min(c + 1, p.n_chunks - 1), after = min(c + 2, p.n_chunks - 1), buf = c & 1;
         lds_barrier();  // 1
-        if (c) put_out(c - 1);
-        load_matrix<TT, G>(p, c, 1, wave, lane, pf);
-        lds_barrier();  // 2
         h8 s_hi[NW], s_lo[NW];
         float back[NW];
 #pragma unroll
@@ -691,18 +800,35 @@ __device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace 
             s_lo[g] = lds.s[g][1][lane];
             back[g] = lds.back[g][m];
         }
-        o_back = lds.u_back[m] * lds.scalar[buf][kPBack];
+        lds_here();
+        f4 qs_now[TT];
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-            qs[tt] = state_product<NW>(qf[tt], s_hi, s_lo, back) * lds.factor[buf][1][row_of(wave * TT + tt, 4 * q) / 4];
+        for (int tt = 0; tt < TT; ++tt) qs_now[tt] = state_product<NW>(qf[tt], s_hi, s_lo, back) * fq[tt];
         in_order();
-        load_q(next);
-        put_next(buf ^ 1);
+        load_q();
+        lds_barrier();  // 2
+        put_out(before);
+        put_v();
         in_order();
-        load_next(after);
+        load_v();
+        o_back = lds.u_back[m] * p_back;
+        in_order();
+        load_p_back();
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) qs[tt] = qs_now[tt];
+        before = o_rows.buffer();
+        o_rows.step();
         lds_barrier();  // 3
+        h8 u[G][2];
+        read_pairs<G>(lds.u, lane, u);
+        lds_here();
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) pu[tt] = lower_product<G>(pf[tt], u);
+        in_order();
+        load_p();
+        put_top();
     }
-    put_out(p.n_chunks - 1);
+    put_out(before);
 }
 
 template <int KD, bool VEC>
@@ -719,7 +845,7 @@ __global__ __launch_bounds__(4 * KD) void delta_scan_kernel(DeltaArgs a, const c
     ScanPlace p;
     p.slice = at_xcd % slices;
     p.head = unit - s * heads;
-    p.kh = p.head / (heads / a.k.heads);
+    const int kh = p.head / (heads / a.k.heads);
     const Rows rows = rows_of(a.s, s);
     p.rows = {uniform(rows.first), uniform(rows.count)};
     p.slot_in = uniform(slot_in(a.s, s));
@@ -727,8 +853,8 @@ __global__ __launch_bounds__(4 * KD) void delta_scan_kernel(DeltaArgs a, const c
     const size_t tile0 = uniform(tiles_before(a.s, s, lane));
     // starts that overlap have more chunks than the workspace holds: those are left out
     p.n_chunks = (int)min((size_t)(p.rows.count + kChunk - 1) / kChunk, tiles - min(tiles, tile0));
-    p.block0 = chunks + (tile0 * heads + p.head) * kChunkBytes;
-    p.step = (size_t)heads * kChunkBytes;
+    p.block = chunks + (p.head * tiles + tile0) * kChunkBytes;
+    p.keys = chunks + heads * tiles * kChunkBytes + (kh * tiles + tile0) * key_bytes(KD);
     if (wave < NW / 2) state_wave<KD, false>(a, p, lds, wave, lane);
     else if (wave < NW) state_wave<KD, true>(a, p, lds, wave, lane);
     else if (wave < NW + NW / 2) output_wave<KD, VEC, false>(a, p, lds, wave - NW, lane);
@@ -741,7 +867,7 @@ hipError_t launch_kd(const DeltaArgs &a, char *chunks, hipStream_t stream) {
     delta_prepare_kernel<KD><<<dim3((unsigned)(tiles * a.v.heads)), dim3(256), 0, stream>>>(a, chunks);
     const int units = a.s.sequences * a.v.heads, slices = a.value_dim / 16;
     const dim3 blocks((unsigned)((units + 7) / 8 * 8 * slices));
-    if (a.q.vec && a.k.vec && a.v.vec && a.out.vec)
+    if (a.v.vec && a.out.vec)
         delta_scan_kernel<KD, true><<<blocks, dim3(4 * KD), 0, stream>>>(a, chunks, tiles, units, slices);
     else
         delta_scan_kernel<KD, false><<<blocks, dim3(4 * KD), 0, stream>>>(a, chunks, tiles, units, slices);
@@ -752,13 +878,13 @@ hipError_t launch_kd(const DeltaArgs &a, char *chunks, hipStream_t stream) {
 
 bool delta_prompt_serves(const DeltaArgs &a) {
     const size_t most = (size_t)1 << 24;
-    return a.q.token_stride <= most && a.k.token_stride <= most && a.v.token_stride <= most &&
-           a.out.token_stride <= most;
+    return a.v.token_stride <= most && a.out.token_stride <= most;
 }
 
-size_t delta_prompt_bytes(size_t heads, size_t sequences, size_t tokens) {
+size_t delta_prompt_bytes(size_t heads, int key_dim, size_t sequences, size_t tokens) {
     if (tokens < kDeltaPromptRows * sequences) return 0;
-    return kSharedPrefixBytes + (tokens / kChunk + sequences) * heads * kChunkBytes;
+    // as many key heads as value heads
+    return kSharedPrefixBytes + (tokens / kChunk + sequences) * heads * (kChunkBytes + key_bytes(key_dim));
 }
 
 hipError_t launch_delta_prompt(const DeltaArgs &a, void *workspace, hipStream_t stream) {

@@ -54,7 +54,7 @@ hipError_t launch_delta_step(const DeltaArgs &a, hipStream_t stream);
 // rows a sequence from which on the chunks take over
 constexpr size_t kDeltaPromptRows = 16;
 // 0: the call goes row by row and takes no workspace
-size_t delta_prompt_bytes(size_t heads, size_t sequences, size_t tokens);
+size_t delta_prompt_bytes(size_t heads, int key_dim, size_t sequences, size_t tokens);
 // whether a chunk's rows are within 32-bit byte offsets of its first
 bool delta_prompt_serves(const DeltaArgs &a);
 hipError_t launch_delta_prompt(const DeltaArgs &a, void *workspace, hipStream_t stream);

@@ -116,7 +116,7 @@ size_t exl3_hip_delta_rule_workspace_bytes(size_t v_heads, size_t key_dim, size_
                                            size_t tokens) {
     if (!delta_dims(v_heads, key_dim, value_dim) || sequences > kMaxSequences || tokens > kMaxTokens || !sequences)
         return 0;
-    return delta_prompt_bytes(v_heads, sequences, tokens);
+    return delta_prompt_bytes(v_heads, (int)key_dim, sequences, tokens);
 }
 
 exl3_status exl3_hip_delta_rule(const exl3_head_view *q, const exl3_head_view *k, const exl3_head_view *v,
@@ -153,7 +153,7 @@ exl3_status exl3_hip_delta_rule(const exl3_head_view *q, const exl3_head_view *k
     a.value_dim = (int)value_dim;
     a.scale = scale;
     a.eps = qk_eps;
-    const size_t need = delta_prompt_bytes(v->heads, sequences, tokens);
+    const size_t need = delta_prompt_bytes(v->heads, a.key_dim, sequences, tokens);
     if (!need || !delta_prompt_serves(a)) return from_hip(launch_delta_step(a, stream));
     WorkspaceLease lease;
     const exl3_status st = take_workspace(need, stream, &lease, &workspace, &workspace_bytes);
