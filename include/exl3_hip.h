@@ -571,7 +571,7 @@ exl3_status exl3_hip_short_conv(const void *x, exl3_dtype xt, size_t x_row_strid
  * States and sums in fp32.  From 16 rows a sequence on (tokens / sequences), rows are taken 64 at a
  * time, their products as fp16 pairs (high and low part, 22 bits), and an element that is not finite makes NaN of
  * its sequence and head from the first of its 64 rows on (from its own row on else).  The same inputs give the same bits on every call.  EXL3_NO_SUPPORT where (tokens / 64 +
- * sequences) * v heads * ceil(value_dim / 16) reaches 2^23.  sequences = 0 is a no-op. */
+ * sequences) * v heads * ceil(value_dim / 16) reaches 2^22.  sequences = 0 is a no-op. */
 exl3_status exl3_hip_delta_rule(const exl3_head_view *q, const exl3_head_view *k, const exl3_head_view *v,
                                 const float *g, const float *beta, size_t gate_stride, const float *a_log,
                                 const float *dt_bias, const exl3_head_view *out, size_t key_dim, size_t value_dim,

@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
         *(h8 *)(q_lds + query_at<KD>(r, c)) = y;
     }
     Gates gt{0.f, 0.f};
-    if (lane < count) gt = gates_of(a, first + lane, head);
+    if (lane < count) gt = gates_of(a, head_gates(a, head), load_gates(a, first + lane, head));
     double G = gt.g;  // 64 bits: differences of long sums are the exponents
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {

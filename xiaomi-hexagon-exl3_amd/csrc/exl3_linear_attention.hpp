@@ -51,7 +51,8 @@ struct DeltaArgs {
     float scale, eps;  // eps < 0: q and k as they are
 };
 hipError_t launch_delta_step(const DeltaArgs &a, hipStream_t stream);
-// rows a sequence from which on the chunks take over
+// Rows a sequence from which on the chunks take over.  16 heads of 128 x 128, row by row and in chunks: one sequence
+// of 8 rows 12 and 15.6 us, of 16 rows 20 and 15.3 us; 16 sequences of 12 rows 28 and 34.5 us, of 24 rows 48 and 35 us.
 constexpr size_t kDeltaPromptRows = 16;
 // 0: the call goes row by row and takes no workspace
 size_t delta_prompt_bytes(size_t heads, int key_dim, size_t sequences, size_t tokens);

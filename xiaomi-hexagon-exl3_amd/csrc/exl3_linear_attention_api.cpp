@@ -142,7 +142,7 @@ exl3_status exl3_hip_delta_rule(const exl3_head_view *q, const exl3_head_view *k
     if (!a_log != !dt_bias || !aligned(a_log, 4) || !aligned(dt_bias, 4)) return EXL3_INVAL_PARAMS;
     if (!std::isfinite(scale) || !std::isfinite(qk_eps)) return EXL3_INVAL_PARAMS;
     if (!sequences) return EXL3_OK;
-    if ((tokens / 64 + sequences) * v->heads * ((value_dim + 15) / 16) >= ((size_t)1 << 23)) return EXL3_NO_SUPPORT;
+    if ((tokens / 64 + sequences) * v->heads * (value_dim / 16) >= ((size_t)1 << 22)) return EXL3_NO_SUPPORT;
     a.g = g;
     a.beta = beta;
     a.a_log = a_log;
