@@ -1,8 +1,11 @@
 // exl3_short_conv.hip -- causal depthwise convolution of packed sequences, with their states.
 //
-// Bound by the rows' bytes.  A thread takes C channels of a tile of rows of one sequence and keeps the last
-// W - 1 rows in registers.  The rows ahead of a sequence's first come from its state, and only the
+// y_i = silu(bias + sum_j w_j x_(i - W + 1 + j)).  Bound by the rows' bytes.  A thread takes C channels of a tile of
+// rows of one sequence and keeps the last W - 1 rows in registers; four rows are on their way while the four ahead of
+// them are worked on.  The rows ahead of a sequence's first come from its state, and only the
 // threads of its first tile read that state: they also write the one that it leaves, so a slot may be both.
+// 8192 rows of 6144 fp16 channels, W = 4 with silu: 45 us, 4.5 TB/s (without the four rows ahead 46 us, with a
+// branch for silu at each element 47 us).  Eight rows of eight sequences: 4.9 us, a launch's.
 #include "exl3_activation.hpp"
 #include "exl3_head_rows.hpp"
 #include "exl3_packed_rows.hpp"
@@ -25,6 +28,19 @@ __device__ __forceinline__ void store_channels(void *p, size_t at, const float (
     else ((float *)p)[at] = v[0];
 }
 
+// A row's channels as loaded
+template <int F16, int C>
+struct Loaded {
+    typedef typename std::conditional<F16, _Float16, float>::type T;
+    typedef T V __attribute__((ext_vector_type(C)));
+    V v;
+    __device__ __forceinline__ void load(const void *p, size_t at) { v = *(const V *)((const T *)p + at); }
+    __device__ __forceinline__ void to(float (&x)[C]) const {
+#pragma unroll
+        for (int e = 0; e < C; ++e) x[e] = (float)v[e];
+    }
+};
+
 // blockIdx.x = tile * channel blocks + channel block; `per` rows a tile, at least W - 1
 template <int W, int C, int XF16, int YF16>
 __global__ __launch_bounds__(kConvThreads) void short_conv_kernel(ConvArgs a, int per, unsigned channel_blocks) {
@@ -46,7 +62,8 @@ __global__ __launch_bounds__(kConvThreads) void short_conv_kernel(ConvArgs a, in
         for (int j = 0; j < W; ++j) w[0][j] = a.weight[(size_t)c * W + j];
     }
 #pragma unroll
-    for (int e = 0; e < C; ++e) bias[e] = a.bias ? a.bias[c + e] : 0.f;
+    for (int e = 0; e < C; ++e) bias[e] = 0.f;
+    if (a.bias) load_channels<0, C>(a.bias, c, bias);
 
     float last[W - 1][C];  // the rows ahead of the next one, the oldest first
     const size_t first = t.rows.first;
@@ -82,37 +99,65 @@ __global__ __launch_bounds__(kConvThreads) void short_conv_kernel(ConvArgs a, in
             load_channels<XF16, C>(a.x, (first + t.row0 - (W - 1) + j) * a.x_stride + c, last[j]);
     }
 
+    const auto step = [&](int row, const Loaded<XF16, C> &loaded) {
+        float x[C];
+        loaded.to(x);
+        float y[C];
+#pragma unroll
+        for (int e = 0; e < C; ++e) {
+            y[e] = bias[e];
+#pragma unroll
+            for (int j = 0; j < W - 1; ++j) y[e] = __builtin_fmaf(w[e][j], last[j][e], y[e]);
+            y[e] = __builtin_fmaf(w[e][W - 1], x[e], y[e]);
+#pragma unroll
+            for (int j = 0; j + 1 < W - 1; ++j) last[j][e] = last[j + 1][e];
+            last[W - 2][e] = x[e];
+        }
+        if (a.silu) {  // one branch a row: eight chains of instructions side by side
+#pragma unroll
+            for (int e = 0; e < C; ++e) y[e] = silu_f32(y[e]);
+        }
+        store_channels<YF16, C>(a.y, (first + row) * a.y_stride + c, y);
+    };
     constexpr int U = 4;  // rows whose loads are on the way at once
     const int end = min(t.row0 + per, t.rows.count);
-    for (int row = t.row0; row < end; row += U) {
-        float x[U][C];
+    int row = t.row0;
+    if (row + U <= end) {
+        Loaded<XF16, C> x[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            load_channels<XF16, C>(a.x, (first + min(row + u, end - 1)) * a.x_stride + c, x[u]);
+        for (int u = 0; u < U; ++u) x[u].load(a.x, (first + row + u) * a.x_stride + c);
+        for (; row + 2 * U <= end; row += U) {
+            Loaded<XF16, C> next[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float y[C];
+            for (int u = 0; u < U; ++u) next[u].load(a.x, (first + row + U + u) * a.x_stride + c);
 #pragma unroll
-            for (int e = 0; e < C; ++e) {
-                y[e] = bias[e];
+            for (int u = 0; u < U; ++u) step(row + u, x[u]);
 #pragma unroll
-                for (int j = 0; j < W - 1; ++j) y[e] = __builtin_fmaf(w[e][j], last[j][e], y[e]);
-                y[e] = __builtin_fmaf(w[e][W - 1], x[u][e], y[e]);
-                if (a.silu) y[e] = silu_f32(y[e]);
-#pragma unroll
-                for (int j = 0; j + 1 < W - 1; ++j) last[j][e] = last[j + 1][e];
-                last[W - 2][e] = x[u][e];
-            }
-            if (row + u < end) store_channels<YF16, C>(a.y, (first + row + u) * a.y_stride + c, y);
+            for (int u = 0; u < U; ++u) x[u] = next[u];
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) step(row + u, x[u]);
+        row += U;
+    }
+    if (row < end) {
+        Loaded<XF16, C> x[U - 1];
+#pragma unroll
+        for (int u = 0; u < U - 1; ++u)
+            if (row + u < end) x[u].load(a.x, (first + row + u) * a.x_stride + c);
+#pragma unroll
+        for (int u = 0; u < U - 1; ++u)
+            if (row + u < end) step(row + u, x[u]);
     }
 }
 
 template <int W, int C, int XF16, int YF16>
 hipError_t launch_tiles(const ConvArgs &a, hipStream_t stream) {
     const unsigned channel_blocks = (a.channels + kConvThreads * C - 1) / (kConvThreads * C);
+    // Long tiles read their W - 1 rows ahead less often, short ones fill the card: three workgroups a CU where a thread
+    // has eight channels (6144 channels: 8192 rows in tiles of 16, 32, 64 47, 45, 48 us; 2048 rows in tiles of 4,
+    // 8, 16 16.0, 14.0, 16.0 us), eight where it has one (3,800 rows of 1531: tiles of 4, 8, 16 8.3, 7.6, 8.2 us).
     int per = 32;
-    while (per > 4 && tile_count(a.s, per) * channel_blocks < 2048) per /= 2;
+    while (per > 4 && tile_count(a.s, per) * channel_blocks < (C == 8 ? 768 : 2048)) per /= 2;
     const size_t blocks = tile_count(a.s, per) * channel_blocks;
     short_conv_kernel<W, C, XF16, YF16><<<dim3((unsigned)blocks), dim3(kConvThreads), 0, stream>>>(a, per, channel_blocks);
     return hipGetLastError();
