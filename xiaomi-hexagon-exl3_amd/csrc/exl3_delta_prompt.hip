@@ -159,23 +159,29 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
     // Rows are loaded whole, KD / 8 lanes each, and get into the operands' order through LDS (see output_wave): the
     // keys where T will be, the queries where the wave's own rows of A will be.  Rows beyond the last: zeros, decay 1,
     // beta 0.
-    constexpr int L = KD / 8;
+    constexpr int L = KD / 8, NR = 16 * L / 64;
     const int row = 16 * wave + m;
     _Float16 *const k_lds = (_Float16 *)T, *const q_lds = (_Float16 *)(A + 16 * wave * kRowFloats);
+    // all loads are on their way at once: rows beyond the last are the last one's until they are in registers
+    h8 kx[NR], qx[NR];
 #pragma unroll
-    for (int j = 0; j < 16 * L / 64; ++j) {
-        const int r = 64 / L * j + lane / L, c = lane % L;
-        h8 x{}, y{};
-        if (16 * wave + r < count) {
-            const size_t at = first + 16 * wave + r;
-            x = load_h8((const _Float16 *)a.k.data + at * a.k.token_stride + kh * a.k.head_stride + 8 * c, a.k.vec);
-            y = load_h8((const _Float16 *)a.q.data + at * a.q.token_stride + kh * a.q.head_stride + 8 * c, a.q.vec);
-        }
-        *(h8 *)(k_lds + query_at<KD>(16 * wave + r, c)) = x;
-        *(h8 *)(q_lds + query_at<KD>(r, c)) = y;
+    for (int j = 0; j < NR; ++j) {
+        const int r = 16 * wave + 64 / L * j + lane / L, c = lane % L;
+        const size_t at = first + min(r, count - 1);
+        kx[j] = load_h8((const _Float16 *)a.k.data + at * a.k.token_stride + kh * a.k.head_stride + 8 * c, a.k.vec);
+        qx[j] = load_h8((const _Float16 *)a.q.data + at * a.q.token_stride + kh * a.q.head_stride + 8 * c, a.q.vec);
     }
-    Gates gt{0.f, 0.f};
-    if (lane < count) gt = gates_of(a, head_gates(a, head), load_gates(a, first + lane, head));
+    const HeadGates hg = head_gates(a, head);
+    Gates gt = load_gates(a, first + min(lane, count - 1), head);
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+        const int r = 64 / L * j + lane / L, c = lane % L;
+        if (16 * wave + r >= count) kx[j] = qx[j] = h8{};
+        *(h8 *)(k_lds + query_at<KD>(16 * wave + r, c)) = kx[j];
+        *(h8 *)(q_lds + query_at<KD>(r, c)) = qx[j];
+    }
+    gt = gates_of(a, hg, gt);
+    if (lane >= count) gt = Gates{0.f, 0.f};
     double G = gt.g;  // 64 bits: differences of long sums are the exponents
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
