@@ -57,7 +57,7 @@ def call(amd, d, lens, states=None, sin=None, sout=None, norm=True, packed=True,
     want, after, bound, off = ref.delta_rule(
         f["q"], f["k"], f["v"], f["g"], f["beta"], lens, float(np.float32(scale)),
         None if states is None else states.astype(np.float64), sin, sout, f["a_log"], f["dt_bias"],
-        None if eps is None else float(np.float32(eps)), chunk=64 if n >= 16 * len(lens) else None)
+        None if eps is None else float(np.float32(eps)), chunk=64 if n >= max(16, (2 if packed and len(lens) > 1 else 16) * len(lens)) else None)
     assert bool((out[n:] == 9).all())
     got = out[:n].cpu().numpy().astype(np.float64)
     assert np.array_equal(np.isnan(got), np.isnan(want))
@@ -107,6 +107,17 @@ def test_packed_prompts(amd, lens, dk, dv, hk, hv):
         states = draw(77, (len(lens) + 1, hv, dk, dv), 0.5)
         slots = np.random.default_rng(2).permutation(len(lens) + 1)[:len(lens)].astype(np.int32)
         call(amd, d, lens, states, slots if prior else None, slots, norm, behind=3)
+
+
+@pytest.mark.parametrize("lens", [[1, 1, 1, 40, 0, 3, 90, 7, 8, 15, 16], [1] * 20 + [130], [2, 2, 2, 2], [9, 7], [64, 1],
+                                  [16, 1, 1, 1, 1, 1, 1, 1, 1]], ids=str)
+@pytest.mark.parametrize("dk,dv,hk,hv", [(128, 128, 1, 2), (64, 48, 2, 2)])
+def test_short_and_long_sequences_together(amd, lens, dk, dv, hk, hv):
+    d = inputs(21, sum(lens), hk, hv, dk, dv)
+    states = draw(79, (len(lens) + 2, hv, dk, dv), 0.5)
+    slots = np.random.default_rng(4).permutation(len(lens) + 2)[:len(lens)].astype(np.int32)
+    call(amd, d, lens, states, slots, slots, behind=5)
+    call(amd, d, lens, states, None, slots)
 
 
 @pytest.mark.parametrize("lens", [[1, 2, 1, 0, 1], [70, 2, 90, 0, 64]], ids=str)

@@ -104,6 +104,10 @@ def test_delta_rule(L):
         assert delta(L, v=x) == INVAL
     for out in (view(None), view(Q, heads=4), view(Q, head=64), view(P), view(Q, token=100)):
         assert delta(L, out=out) == INVAL
+    big = dict(starts=P, gs=16, q=view(heads=16, token=2048), k=view(heads=16, token=2048),
+               v=view(heads=16, token=2048), out=view(Q, heads=16, token=2048))
+    assert delta(L, **big, tokens=1 << 21) == NO_SUPPORT  # 2^15 chunks of 2^7 slices
+    assert delta(L, **big, tokens=64, sequences=1 << 15) == NO_SUPPORT
     assert delta(L, starts=P, tokens=1 << 29, q=view(heads=1), k=view(heads=1), v=view(heads=1), out=view(Q, heads=1),
                  states=None, sin=None, sout=None) == NO_SUPPORT
 
@@ -113,6 +117,10 @@ def test_delta_rule_workspace(L):
     for bad in ((0, 128, 128, 1, 64), (1025, 128, 128, 1, 64), (4, 96, 128, 1, 64), (4, 128, 24, 1, 64),
                 (4, 128, 128, 65537, 64), (4, 128, 128, 1, 1 << 31), (4, 128, 128, 0, 4096), (4, 128, 128, 8, 8)):
         assert f(*bad) == 0, bad
+    for few in ((4, 128, 128, 1, 15), (4, 128, 128, 9, 17)):
+        assert f(*few) == 0, few
+    sizes = [f(4, 128, 128, s, n) for s, n in ((1, 16), (8, 16), (8, 128), (1, 4096), (8, 4096))]
+    assert sizes[0] > 0 and sizes == sorted(sizes)
 
 
 def test_exports(L):

@@ -18,14 +18,12 @@
 // D leaves lane 16 q + n with column n of rows 4 q + i (i < 4), and B wants rows 8 q + j (j < 8) of column n there.
 // So a 32-row operand is two tiles whose rows 4 q + i stand for rows 8 q + i and 8 q + 4 + i: the second
 // product's operand is the first one's result, lane for lane.
-#include "exl3_delta_gates.hpp"
-#include "exl3_head_rows.hpp"
+#include "exl3_delta_step.hpp"
 
 namespace exl3k {
 
 namespace {
 
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
 
@@ -136,8 +134,10 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 constexpr int kRowFloats = kChunk + 4;  // of a matrix in LDS
 
 // One chunk of one value head: wave w has rows 16 w .. 16 w + 15 of the products and column block w of T.
+// Workgroups behind those of all tiles and heads take the sequences of fewer than `limit` rows, row by row.
 template <int KD>
-__global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *chunks) {
+__global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *chunks, size_t tiles, int limit, size_t units,
+                                                            int slices) {
     constexpr int NK = KD / 32;
     constexpr int kMatrix = kChunk * kRowFloats;
     __shared__ __attribute__((aligned(16))) float lds[3 * kMatrix];  // A, P, T
@@ -147,10 +147,17 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
     static_assert(kChunk * KD * 2 <= kMatrix * 4, "the keys fit");
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int heads = a.v.heads, tile = blockIdx.x / heads, head = blockIdx.x - tile * heads;
+    const int heads = a.v.heads;
+    if (blockIdx.x >= tiles * heads) {
+        static_assert(kStepWaves == 4, "a workgroup is a step's");
+        const size_t unit = (blockIdx.x - tiles * heads) * kStepWaves + wave;
+        if (unit < units) delta_step<KD>(a, unit, slices, limit);
+        return;  // the whole workgroup
+    }
+    const int tile = blockIdx.x / heads, head = blockIdx.x - tile * heads;
     const int m = lane & 15, q = lane >> 4;
     const Tile t = find_tile(a.s, tile, kChunk, lane);
-    if (t.s < 0) return;  // the whole workgroup
+    if (t.s < 0 || t.rows.count < limit) return;  // the whole workgroup
     const int count = min(kChunk, t.rows.count - t.row0);
     if (count <= 0) return;
     const size_t first = (size_t)t.rows.first + t.row0;
@@ -219,7 +226,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
     __syncthreads();
 
     if (head == kh * (heads / a.k.heads)) {  // one value head of the key head's
-        char *const keys = chunks + gridDim.x * (size_t)kChunkBytes + ((size_t)kh * (gridDim.x / heads) + tile) * key_bytes(KD);
+        char *const keys = chunks + tiles * heads * (size_t)kChunkBytes + (kh * tiles + tile) * key_bytes(KD);
         h8 *const rows = (h8 *)keys + lane, *const columns = rows + NK * kKeyFrags * 64, *const queries = columns + NK * kKeyFrags * 64;
 #pragma unroll
         for (int s = 0; s < NK; ++s) {
@@ -233,7 +240,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
         }
     }
     // a head's chunks next to each other: the walk over them stays in few pages
-    char *const block = chunks + ((size_t)head * (gridDim.x / heads) + tile) * kChunkBytes;
+    char *const block = chunks + (head * tiles + tile) * kChunkBytes;
     f4 kk_acc[4], qk_acc[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -839,7 +846,7 @@ __device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace 
 
 template <int KD, bool VEC>
 __global__ __launch_bounds__(4 * KD) void delta_scan_kernel(DeltaArgs a, const char *chunks, size_t tiles, int units,
-                                                            int slices) {
+                                                            int slices, int limit) {
     constexpr int NW = KD / 32;
     __shared__ __attribute__((aligned(16))) ScanLds<KD> lds;
     // the slices of a head on one XCD, whose L2 then holds what they share
@@ -854,6 +861,7 @@ __global__ __launch_bounds__(4 * KD) void delta_scan_kernel(DeltaArgs a, const c
     const int kh = p.head / (heads / a.k.heads);
     const Rows rows = rows_of(a.s, s);
     p.rows = {uniform(rows.first), uniform(rows.count)};
+    if (p.rows.count < limit) return;  // the whole workgroup
     p.slot_in = uniform(slot_in(a.s, s));
     p.slot_out = uniform(slot_out(a.s, s));
     const size_t tile0 = uniform(tiles_before(a.s, s, lane));
@@ -869,14 +877,17 @@ __global__ __launch_bounds__(4 * KD) void delta_scan_kernel(DeltaArgs a, const c
 
 template <int KD>
 hipError_t launch_kd(const DeltaArgs &a, char *chunks, hipStream_t stream) {
-    const size_t tiles = tile_count(a.s, kChunk);
-    delta_prepare_kernel<KD><<<dim3((unsigned)(tiles * a.v.heads)), dim3(256), 0, stream>>>(a, chunks);
-    const int units = a.s.sequences * a.v.heads, slices = a.value_dim / 16;
+    const size_t tiles = tile_count(a.s, kChunk), heads = a.v.heads, slices = a.value_dim / 16;
+    // sequences of one length are all long ones; one alone goes in chunks whatever its length
+    const int limit = a.s.starts && a.s.sequences > 1 ? (int)kDeltaShortRows : 0;
+    const size_t units = a.s.sequences * heads, steps = limit ? units * slices : 0;
+    delta_prepare_kernel<KD><<<dim3((unsigned)(tiles * heads + (steps + kStepWaves - 1) / kStepWaves)), dim3(256), 0, stream>>>(
+        a, chunks, tiles, limit, steps, (int)slices);
     const dim3 blocks((unsigned)((units + 7) / 8 * 8 * slices));
     if (a.v.vec && a.out.vec)
-        delta_scan_kernel<KD, true><<<blocks, dim3(4 * KD), 0, stream>>>(a, chunks, tiles, units, slices);
+        delta_scan_kernel<KD, true><<<blocks, dim3(4 * KD), 0, stream>>>(a, chunks, tiles, (int)units, (int)slices, limit);
     else
-        delta_scan_kernel<KD, false><<<blocks, dim3(4 * KD), 0, stream>>>(a, chunks, tiles, units, slices);
+        delta_scan_kernel<KD, false><<<blocks, dim3(4 * KD), 0, stream>>>(a, chunks, tiles, (int)units, (int)slices, limit);
     return hipGetLastError();
 }
 
@@ -884,11 +895,11 @@ hipError_t launch_kd(const DeltaArgs &a, char *chunks, hipStream_t stream) {
 
 bool delta_prompt_serves(const DeltaArgs &a) {
     const size_t most = (size_t)1 << 24;
-    return a.v.token_stride <= most && a.out.token_stride <= most;
+    return (a.s.starts || a.s.tokens >= kDeltaPromptRows * a.s.sequences) && a.v.token_stride <= most && a.out.token_stride <= most;
 }
 
 size_t delta_prompt_bytes(size_t heads, int key_dim, size_t sequences, size_t tokens) {
-    if (tokens < kDeltaPromptRows * sequences) return 0;
+    if (tokens < kDeltaPromptRows || tokens < kDeltaMixedRows * sequences) return 0;
     // as many key heads as value heads
     return kSharedPrefixBytes + (tokens / kChunk + sequences) * heads * (kChunkBytes + key_bytes(key_dim));
 }

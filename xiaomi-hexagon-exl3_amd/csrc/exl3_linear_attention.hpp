@@ -54,9 +54,15 @@ hipError_t launch_delta_step(const DeltaArgs &a, hipStream_t stream);
 // Rows a sequence from which on the chunks take over.  16 heads of 128 x 128, row by row and in chunks: one sequence
 // of 8 rows 12 and 15.6 us, of 16 rows 20 and 15.3 us; 16 sequences of 12 rows 28 and 34.5 us, of 24 rows 48 and 35 us.
 constexpr size_t kDeltaPromptRows = 16;
-// 0: the call goes row by row and takes no workspace
+// Packed sequences' lengths are on the device, and a call of few rows a sequence can have a long one among them: from
+// kDeltaMixedRows a sequence on, those shorter than kDeltaShortRows go row by row beside the preparation of the others'
+// chunks, which takes about as long.  (Five sequences of up to 39 rows, 6 heads of 128 x 256: 23 us, row by row 44 us; two
+// sequences of up to 222 rows, one of them short: 20 us, and 26 us where short is fewer than 16 rows.)
+constexpr size_t kDeltaMixedRows = 2, kDeltaShortRows = 8;
+// 0: such calls go row by row and take no workspace
 size_t delta_prompt_bytes(size_t heads, int key_dim, size_t sequences, size_t tokens);
-// whether a chunk's rows are within 32-bit byte offsets of its first
+// Whether this call has chunks: sequences of one known length that is long enough, or packed ones; and a chunk's rows are
+// within 32-bit byte offsets of its first
 bool delta_prompt_serves(const DeltaArgs &a);
 hipError_t launch_delta_prompt(const DeltaArgs &a, void *workspace, hipStream_t stream);
 
