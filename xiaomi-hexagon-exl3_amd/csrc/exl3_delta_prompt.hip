@@ -5,15 +5,23 @@
 //   U   = T diag(beta) (V - diag(e^G) K S),             (row i of U is the recurrence's u)
 //   out = scale (diag(e^G) Q S + P U),                  P_ij = e^(G_i - G_j) q_i . k_j  (j <= i),
 //   S  <- e^G_64 S + (diag(e^(G_64 - G)) K)^T U.
-// delta_prepare_kernel works out what needs no state for all chunks at once: T by blocks of 16, P, and the
-// factors of the rows.  delta_scan_kernel walks a sequence's chunks: a workgroup has 16 columns of one head's state
-// in the registers of its waves, 32 rows each, and three exchanges through LDS a chunk.
+// delta_prepare_kernel works out what needs no state for all chunks at once: T by blocks of 16, P, the factors of
+// the rows, and lays K and Q out as operands.  delta_scan_kernel walks a sequence's chunks: a workgroup has 16
+// columns of one head's state in the registers of its waves, 32 rows each, and three exchanges through LDS a chunk.
+//
+// Bound by the chain from chunk to chunk, three exchanges of about 1000 cycles (read, products of a few hundred cycles, write,
+// barrier), and by the preparation's writes.  8192 rows, 16 heads of 128: preparation 50 us (0.2 GB, 4.4 TB/s) and walk
+// 168 us, 1.3 us a chunk; 2048 rows 17 and 42.5 us; 16 sequences of 2048 rows 176 and 443 us.  Half the waves
+// carry the state and half make the output, so that the chain has only what the next chunk waits for (both on every
+// wave: 400 us in all at 8192 rows).  16 columns a workgroup: one long sequence of 16 heads has 128 workgroups, and
+// more columns would be fewer of them and longer chunks.  Where operands lie as lanes want them a load is 1 KB of
+// consecutive bytes; 16 rows by 64 bytes a load is four times as slow.
 //
 // The products run on mfma_f32_16x16x32_f16.  K and Q are fp16 as given (their lengths are factors of rows
 // applied afterwards); every other operand x is two fp16 numbers, hi = fp16(x) and lo = fp16(x - hi), 22 bits
 // together, after a power of two has taken a bound on its column (or matrix) to 2^15; below 2^-29 of that bound
-// they are steps of 2^-40 of it.  Products of two such pairs leave out lo lo.  One fp16 number in the state's place would lose what the recurrence in binary32 keeps
-// (2^-11 of S in every chunk).
+// they are steps of 2^-40 of it.  Products of two such pairs leave out lo lo.  One fp16 number in the state's place would
+// lose what the recurrence in binary32 keeps (2^-11 of S in every chunk).
 //
 // D leaves lane 16 q + n with column n of rows 4 q + i (i < 4), and B wants rows 8 q + j (j < 8) of column n there.
 // So a 32-row operand is two tiles whose rows 4 q + i stand for rows 8 q + i and 8 q + 4 + i: the second
