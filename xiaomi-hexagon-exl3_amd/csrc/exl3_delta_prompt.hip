@@ -615,7 +615,6 @@ __device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &
         load_rows();
         load_factors();
         load_t();
-        load_columns();
         lds_barrier();
     }
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -636,11 +635,13 @@ __device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &
         for (int t = 0; t < 4; ++t) x[t] = mfma16(kf[t], hi, zero);
 #pragma unroll
         for (int t = 0; t < 4; ++t) x[t] = mfma16(kf[t], lo, x[t]);
+        in_order();
+        load_columns();
         lds.s[wave][0][lane] = hi;
         lds.s[wave][1][lane] = lo;
         if (q == 0) lds.back[wave][m] = sf.back;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) lds.ks[wave][t][lane] = x[t] * sf.back;
+        for (int t = 0; t < 4; ++t) lds.ks[wave][t][lane] = x[t];
         lds_barrier();  // 1
 
         // R = beta (V - e^G K S), |R| <= r_value |V| + r_state |S|
@@ -651,9 +652,12 @@ __device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &
             for (int g = 0; g < NW; ++g) ks[tt][g] = lds.ks[g][wave * TT + tt][lane];
         in_order();  // loads are issued while LDS answers
         load_rows();
-        float s_back = 0.f;
+        float back[NW], s_back = 0.f;
 #pragma unroll
-        for (int g = 0; g < NW; ++g) s_back = fmaxf(s_back, lds.back[g][m]);
+        for (int g = 0; g < NW; ++g) {
+            back[g] = lds.back[g][m];
+            s_back = fmaxf(s_back, back[g]);
+        }
         const Fit rf = fit_of(__builtin_fmaf(sc[kRState] * 32768.f, s_back, sc[kRValue] * fmaxf(lds.v_top[0], lds.v_top[1])));
         const float u_back = rf.back * sc[kUBack];
         f4 w_fit[TT];
@@ -663,9 +667,13 @@ __device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &
             // 16 lanes read four rows of V: lane m gets column m of them
             const h4 v = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (lds_s4 *)&lds.v[row_of(t, 4 * q) + (m >> 2)][4 * (m & 3)]));
-            f4 y = ks[tt][0], r;
+            f4 y, r;
 #pragma unroll
-            for (int g = 1; g < NW; ++g) y += ks[tt][g];
+            for (int i = 0; i < 4; ++i) {
+                y[i] = ks[tt][0][i] * back[0];
+#pragma unroll
+                for (int g = 1; g < NW; ++g) y[i] = __builtin_fmaf(ks[tt][g][i], back[g], y[i]);
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[i] = fb[tt][i] * rf.to * __builtin_fmaf(-fk[tt][i], y[i], (float)v[i]);
             put_quarter(lds.r, t, lane, r);
@@ -686,13 +694,13 @@ __device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &
             put_quarter(lds.w, wave * TT + tt, lane, u * w_fit[tt]);
             put_quarter(lds.u, wave * TT + tt, lane, u);
         }
+        in_order();
+        load_t();
         lds_barrier();  // 3
 
         // S <- e^G_64 S + K^T W
         h8 w[2][2];
         read_pairs<2>(lds.w, lane, w);
-        in_order();
-        load_t();
         lds_here();
         f4 acc[2] = {zero, zero}, acc_lo[2] = {zero, zero};
 #pragma unroll
@@ -702,8 +710,6 @@ __device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &
                 acc[t] = mfma16(kt[g][t], w[g][0], acc[t]);
                 acc_lo[t] = mfma16(kt[g][t], w[g][1], acc_lo[t]);
             }
-        in_order();
-        load_columns();
         const float s_more = u_back * sc[kWBack];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
