@@ -120,6 +120,25 @@ def test_short_and_long_sequences_together(amd, lens, dk, dv, hk, hv):
     call(amd, d, lens, states, None, slots)
 
 
+@pytest.mark.parametrize("dk,dv,hk,hv,seqs", [(128, 256, 4, 16, 4), (64, 256, 16, 16, 4), (128, 160, 26, 26, 4),
+                                               (128, 32, 64, 64, 8), (64, 48, 32, 64, 6)])
+def test_many_columns(amd, dk, dv, hk, hv, seqs):
+    """1024 groups of 16 columns and more, in pairs where value_dim has them"""
+    import torch
+    lens = [70, 1, 9, 16, 64, 8, 0, 33][:seqs]
+    d = inputs(22, sum(lens), hk, hv, dk, dv)
+    states = draw(80, (seqs, hv, dk, dv), 0.5)
+    slots = np.arange(seqs, dtype=np.int32)[::-1].copy()
+    want, _ = call(amd, d, lens, states, slots, slots, behind=2)
+    t = {k: cuda(x) for k, x in d.items()}
+    wide = torch.zeros(sum(lens), hv, dv + 1, dtype=torch.float16, device="cuda")  # rows at no 16-byte places
+    wide[..., 1:] = t["v"]
+    out = torch.full_like(wide, 5)
+    amd.delta_rule(t["q"], t["k"], wide[..., 1:], t["g"], t["beta"], t["a_log"], t["dt_bias"], starts=starts_of(lens),
+                   states=cuda(states), slots_in=cuda(slots), qk_eps=1e-6, out=out[..., 1:])
+    assert torch.equal(out[..., 1:], want[:sum(lens)]) and bool((out[..., 0] == 5).all())
+
+
 @pytest.mark.parametrize("lens", [[1, 2, 1, 0, 1], [70, 2, 90, 0, 64]], ids=str)
 def test_slots_that_are_none_or_beyond_the_pool(amd, lens):
     d = inputs(6, sum(lens), 2, 4, 128, 64)

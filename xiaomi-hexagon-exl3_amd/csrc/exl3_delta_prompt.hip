@@ -6,15 +6,14 @@
 //   out = scale (diag(e^G) Q S + P U),                  P_ij = e^(G_i - G_j) q_i . k_j  (j <= i),
 //   S  <- e^G_64 S + (diag(e^(G_64 - G)) K)^T U.
 // delta_prepare_kernel works out what needs no state for all chunks at once: T by blocks of 16, P, the factors of
-// the rows, and lays K and Q out as operands.  delta_scan_kernel walks a sequence's chunks: a workgroup has 16
-// columns of one head's state in the registers of its waves, 32 rows each, and three exchanges through LDS a chunk.
+// the rows, and lays K and Q out as operands.  delta_scan_kernel walks a sequence's chunks: a workgroup has 16 or
+// 32 columns of one head's state in the registers of its waves, 32 rows each, and three exchanges through LDS a chunk.
 //
-// Bound by the chain from chunk to chunk, three exchanges of about 1000 cycles (read, products of a few hundred cycles, write,
-// barrier), and by the preparation's writes.  8192 rows, 16 heads of 128: preparation 50 us (0.2 GB, 4.4 TB/s) and walk
-// 168 us, 1.3 us a chunk; 2048 rows 17 and 42.5 us; 16 sequences of 2048 rows 176 and 443 us.  Half the waves
+// Bound by the chain from chunk to chunk, three exchanges of about 900 cycles (read, products, write, barrier), in
+// which a SIMD has 1500 cycles of instructions of its two waves, and by the preparation's writes.  8192 rows, 16 heads of 128: preparation 51 us (0.2 GB, 4.4 TB/s) and walk
+// 160 us, 1.25 us a chunk; 2048 rows 17 and 40 us; 16 sequences of 2048 rows 167 and 367 us.  Half the waves
 // carry the state and half make the output, so that the chain has only what the next chunk waits for (both on every
-// wave: 400 us in all at 8192 rows).  16 columns a workgroup: one long sequence of 16 heads has 128 workgroups, and
-// more columns would be fewer of them and longer chunks.  Where operands lie as lanes want them a load is 1 KB of
+// wave: 400 us in all at 8192 rows).  Where operands lie as lanes want them a load is 1 KB of
 // consecutive bytes; 16 rows by 64 bytes a load is four times as slow.
 //
 // The products run on mfma_f32_16x16x32_f16.  K and Q are fp16 as given (their lengths are factors of rows
@@ -436,23 +435,24 @@ __device__ __forceinline__ size_t uniform(size_t v) {
     return (uint32_t)uniform((int)(uint32_t)v) | (size_t)(uint32_t)uniform((int)(uint32_t)(v >> 32)) << 32;
 }
 
-// A workgroup has columns 16 slice .. of one head's state, and two kinds of waves, KD / 32 of each.  State wave w has
+// A workgroup has columns 16 NC slice .. of one head's state, NC tiles of them, and two kinds of waves, KD / 32 of each.  State wave w has
 // rows 32 w .. 32 w + 31 of the state, as two tiles, and TT of the chunk's four row tiles of R and U: what the next chunk
-// waits for.  Output wave w has Q S, P U and out of TT row tiles, and the first two bring V into LDS.  Everything else is
+// waits for.  Output wave w has Q S, P U and out of TT row tiles, and the first two (all where NC is 2) bring V into LDS.  Everything else is
 // read as operands, straight from the workspace.  VEC: 16 bytes of a row of v and out are one access.
 //
 // LDS, by the barrier (1 to 3 of a chunk) that its writes are ahead of and the one that its reads are ahead of:
 // s, back, ks: 1, 2;  v: 3 of the chunk before, 2;  v_top: 1, 2;  r, u_back: 2, 3;  u, w: 3, 1 of the next.  A buffer is
 // written again only past the barrier that its reads are ahead of.  o is a wave's own.
-template <int KD>
+template <int KD, int NC>
 struct ScanLds {
     static constexpr int NW = KD / 32;
-    h8 s[NW][2][64];                  // the state's operand: 32 rows, high and low
-    f4 ks[NW][4][64];                 // K S of those rows alone, the chunk's row tiles
-    h8 r[2][2][64];                   // R's, 32 rows each
-    h8 u[2][2][64], w[2][2][64];
-    _Float16 v[kChunk][16], o[kChunk][16];
-    float back[NW][16], u_back[16], v_top[2];
+    static constexpr int kValueWaves = NC == 1 ? 2 : NW;  // output waves that bring V
+    h8 s[NC][NW][2][64];              // the state's operand: 32 rows, high and low
+    f4 ks[NC][NW][4][64];             // K S of those rows alone, the chunk's row tiles
+    h8 r[NC][2][2][64];               // R's, 32 rows each
+    h8 u[NC][2][2][64], w[NC][2][2][64];
+    _Float16 v[kChunk][16 * NC], o[kChunk][16 * NC];
+    float back[NC][NW][16], u_back[NC][16], v_top[kValueWaves];
 };
 
 struct ScanPlace {
@@ -558,20 +558,26 @@ __device__ __forceinline__ f4 state_product(const h8 (&rows)[NW], const h8 (&hi)
 }
 
 // UPPER: the wave's row tiles are those of rows 32 .. 63, with two fragments of T or P each
-template <int KD, bool UPPER>
-__device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &p, ScanLds<KD> &lds, int wave, int lane) {
+template <int KD, int NC, bool UPPER>
+__device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &p, ScanLds<KD, NC> &lds, int wave, int lane) {
     constexpr int NW = KD / 32, TT = 4 / NW, G = UPPER ? 2 : 1;
     const int m = lane & 15, q = lane >> 4;
     const size_t state_size = (size_t)a.v.heads * KD * a.value_dim;
-    const size_t state_at = ((size_t)p.head * KD + 32 * wave + 8 * q) * a.value_dim + 16 * p.slice + m;
-    f4 S[2];
+    const size_t state_at = ((size_t)p.head * KD + 32 * wave + 8 * q) * a.value_dim + 16 * NC * p.slice + m;
+    f4 S[NC][2];
     const float start = p.slot_in == kBadState ? __builtin_nanf("") : 0.f;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int n = 0; n < NC; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            S[t][i] = p.slot_in >= 0 ? a.states[p.slot_in * state_size + state_at + (size_t)(4 * t + i) * a.value_dim] : start;
-    asm volatile("" : "+v"(S[0]), "+v"(S[1]));  // waited for here: in the loop it would be a wait for all loads
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                S[n][t][i] = p.slot_in >= 0
+                                 ? a.states[p.slot_in * state_size + state_at + (size_t)(4 * t + i) * a.value_dim + 16 * n]
+                                 : start;
+#pragma unroll
+    for (int n = 0; n < NC; ++n)  // waited for here: in the loop it would be a wait for all loads
+        asm volatile("" : "+v"(S[n][0]), "+v"(S[n][1]));
 
     // the keys' 32 elements of the wave, as rows of the chunk's tiles and as columns
     h8 kf[4], kt[2][2], tf[TT][G][2];
@@ -622,130 +628,169 @@ __device__ __forceinline__ void state_wave(const DeltaArgs &a, const ScanPlace &
 #pragma unroll
         for (int i = 0; i < 7; ++i) sc[i] = next_sc[i];
         // the state as an operand, each wave's rows by their own power of two a column
-        float top = 0.f;
+        h8 hi[NC], lo[NC];
+        float s_fit[NC];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int n = 0; n < NC; ++n) {
+            float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fabsf(S[t][i]));
-        const Fit sf = fit_of(max_quarters(top));
-        h8 hi, lo;
-        split8(S[0] * sf.to, S[1] * sf.to, hi, lo);
-        f4 x[4];
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] = mfma16(kf[t], hi, zero);
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fabsf(S[n][t][i]));
+            const Fit sf = fit_of(max_quarters(top));
+            split8(S[n][0] * sf.to, S[n][1] * sf.to, hi[n], lo[n]);
+            s_fit[n] = sf.back;
+        }
+        f4 x[NC][4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] = mfma16(kf[t], lo, x[t]);
+        for (int n = 0; n < NC; ++n) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) x[n][t] = mfma16(kf[t], hi[n], zero);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) x[n][t] = mfma16(kf[t], lo[n], x[n][t]);
+        }
         in_order();
         load_columns();
-        lds.s[wave][0][lane] = hi;
-        lds.s[wave][1][lane] = lo;
-        if (q == 0) lds.back[wave][m] = sf.back;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) lds.ks[wave][t][lane] = x[t];
+        for (int n = 0; n < NC; ++n) {
+            lds.s[n][wave][0][lane] = hi[n];
+            lds.s[n][wave][1][lane] = lo[n];
+            if (q == 0) lds.back[n][wave][m] = s_fit[n];
+        }
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) lds.ks[n][wave][t][lane] = x[n][t];
         lds_barrier();  // 1
 
         // R = beta (V - e^G K S), |R| <= r_value |V| + r_state |S|
-        f4 ks[TT][NW];
+        f4 ks[NC][TT][NW];
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
+        for (int n = 0; n < NC; ++n)
 #pragma unroll
-            for (int g = 0; g < NW; ++g) ks[tt][g] = lds.ks[g][wave * TT + tt][lane];
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (int g = 0; g < NW; ++g) ks[n][tt][g] = lds.ks[n][g][wave * TT + tt][lane];
         in_order();  // loads are issued while LDS answers
         load_rows();
-        float back[NW], s_back = 0.f;
+        float v_top = lds.v_top[0];
 #pragma unroll
-        for (int g = 0; g < NW; ++g) {
-            back[g] = lds.back[g][m];
-            s_back = fmaxf(s_back, back[g]);
-        }
-        const Fit rf = fit_of(__builtin_fmaf(sc[kRState] * 32768.f, s_back, sc[kRValue] * fmaxf(lds.v_top[0], lds.v_top[1])));
-        const float u_back = rf.back * sc[kUBack];
+        for (int i = 1; i < ScanLds<KD, NC>::kValueWaves; ++i) v_top = fmaxf(v_top, lds.v_top[i]);
+        float u_back[NC];
         f4 w_fit[TT];
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            const int t = wave * TT + tt;
-            // 16 lanes read four rows of V: lane m gets column m of them
-            const h4 v = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_s4 *)&lds.v[row_of(t, 4 * q) + (m >> 2)][4 * (m & 3)]));
-            f4 y, r;
+        for (int n = 0; n < NC; ++n) {
+            float back[NW], s_back = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                y[i] = ks[tt][0][i] * back[0];
-#pragma unroll
-                for (int g = 1; g < NW; ++g) y[i] = __builtin_fmaf(ks[tt][g][i], back[g], y[i]);
+            for (int g = 0; g < NW; ++g) {
+                back[g] = lds.back[n][g][m];
+                s_back = fmaxf(s_back, back[g]);
             }
+            const Fit rf = fit_of(__builtin_fmaf(sc[kRState] * 32768.f, s_back, sc[kRValue] * v_top));
+            u_back[n] = rf.back * sc[kUBack];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = fb[tt][i] * rf.to * __builtin_fmaf(-fk[tt][i], y[i], (float)v[i]);
-            put_quarter(lds.r, t, lane, r);
-            w_fit[tt] = fu[tt];
+            for (int tt = 0; tt < TT; ++tt) {
+                const int t = wave * TT + tt;
+                // 16 lanes read four rows of V: lane m gets column m of them
+                const h4 v = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_s4 *)&lds.v[row_of(t, 4 * q) + (m >> 2)][16 * n + 4 * (m & 3)]));
+                f4 y, r;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    y[i] = ks[n][tt][0][i] * back[0];
+#pragma unroll
+                    for (int g = 1; g < NW; ++g) y[i] = __builtin_fmaf(ks[n][tt][g][i], back[g], y[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[i] = fb[tt][i] * rf.to * __builtin_fmaf(-fk[tt][i], y[i], (float)v[i]);
+                put_quarter(lds.r[n], t, lane, r);
+            }
+            if (wave == 0 && q == 0) lds.u_back[n][m] = u_back[n];
         }
-        if (wave == 0 && q == 0) lds.u_back[m] = u_back;
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) w_fit[tt] = fu[tt];
         lds_barrier();  // 2
 
         // U = T R, and W = e^(G_64 - G) U for the state
-        h8 r[G][2];
-        read_pairs<G>(lds.r, lane, r);
+        h8 r[NC][G][2];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) read_pairs<G>(lds.r[n], lane, r[n]);
         in_order();
         load_factors();
         lds_here();
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            const f4 u = lower_product<G>(tf[tt], r) * sc[kUFit];
-            put_quarter(lds.w, wave * TT + tt, lane, u * w_fit[tt]);
-            put_quarter(lds.u, wave * TT + tt, lane, u);
-        }
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) {
+                const f4 u = lower_product<G>(tf[tt], r[n]) * sc[kUFit];
+                put_quarter(lds.w[n], wave * TT + tt, lane, u * w_fit[tt]);
+                put_quarter(lds.u[n], wave * TT + tt, lane, u);
+            }
         in_order();
         load_t();
         lds_barrier();  // 3
 
         // S <- e^G_64 S + K^T W
-        h8 w[2][2];
-        read_pairs<2>(lds.w, lane, w);
+        h8 w[NC][2][2];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) read_pairs<2>(lds.w[n], lane, w[n]);
         lds_here();
-        f4 acc[2] = {zero, zero}, acc_lo[2] = {zero, zero};
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+        for (int n = 0; n < NC; ++n) {
+            f4 acc[2] = {zero, zero}, acc_lo[2] = {zero, zero};
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                acc[t] = mfma16(kt[g][t], w[g][0], acc[t]);
-                acc_lo[t] = mfma16(kt[g][t], w[g][1], acc_lo[t]);
-            }
-        const float s_more = u_back * sc[kWBack];
+            for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < 2; ++t) {
+                    acc[t] = mfma16(kt[g][t], w[n][g][0], acc[t]);
+                    acc_lo[t] = mfma16(kt[g][t], w[n][g][1], acc_lo[t]);
+                }
+            const float s_more = u_back[n] * sc[kWBack];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) S[t][i] = __builtin_fmaf(acc[t][i] + acc_lo[t][i], s_more, sc[kDecay] * S[t][i]);
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    S[n][t][i] = __builtin_fmaf(acc[t][i] + acc_lo[t][i], s_more, sc[kDecay] * S[n][t][i]);
+        }
     }
     if (p.slot_out >= 0) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int n = 0; n < NC; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                a.states[p.slot_out * state_size + state_at + (size_t)(4 * t + i) * a.value_dim] = S[t][i];
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    a.states[p.slot_out * state_size + state_at + (size_t)(4 * t + i) * a.value_dim + 16 * n] = S[n][t][i];
     }
 }
 
-template <int KD, bool VEC, bool UPPER>
-__device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace &p, ScanLds<KD> &lds, int wave, int lane) {
+template <int KD, int NC, bool VEC, bool UPPER>
+__device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace &p, ScanLds<KD, NC> &lds, int wave, int lane) {
     constexpr int NW = KD / 32, TT = 4 / NW, G = UPPER ? 2 : 1;
     // known when compiled, so that the compiler can count the loads that are on their way
-    constexpr bool kValues = !UPPER || NW == 2;
+    constexpr bool kValues = NC == 2 || !UPPER || NW == 2;
+    constexpr int PR = 2 * NC, VL = NC * 2 / ScanLds<KD, NC>::kValueWaves;  // 16-byte pieces a row, loads of V a lane
     if (!p.n_chunks) return;
     const int m = lane & 15, q = lane >> 4;
-    ChunkRows o_rows(a.out, p, p.head, 16 * p.slice, 16), v_rows(a.v, p, p.head, 16 * p.slice, 16);
-    // 16 rows of a tile, two lanes each.  The store is not left out by any lane or chunk (a place beyond the buffer is not
+    ChunkRows o_rows(a.out, p, p.head, 16 * NC * p.slice, 16 * NC), v_rows(a.v, p, p.head, 16 * NC * p.slice, 16 * NC);
+    // 16 rows of a tile, PR lanes each.  The store is not left out by any lane or chunk (a place beyond the buffer is not
     // written): where the compiler cannot count it, it waits for it together with the loads that it knows.
     uint32_t o_at[TT];
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt)
-        o_at[tt] = lane < 32 ? (uint32_t)(16 * (wave * TT + tt) + (lane >> 1)) * o_rows.row + 16 * (lane & 1) : 0xfffffff0u;
-    // values: two lanes a row of 16 columns, 32 rows a wave
-    const int v_row = 32 * wave + (lane >> 1);
-    const uint32_t v_at = (uint32_t)v_row * v_rows.row + 16 * (lane & 1);
+        o_at[tt] = lane < 16 * PR ? (uint32_t)(16 * (wave * TT + tt) + lane / PR) * o_rows.row + 16 * (lane % PR) : 0xfffffff0u;
+    // values: 64 / PR rows a load
+    int v_row[VL];
+    uint32_t v_at[VL];
+#pragma unroll
+    for (int j = 0; j < VL; ++j) {
+        v_row[j] = 64 / PR * (wave * VL + j) + lane / PR;
+        v_at[j] = (uint32_t)v_row[j] * v_rows.row + 16 * (lane % PR);
+    }
 
-    h8 qf[TT][NW], pf[TT][G][2], vr;
-    f4 fq[TT], pu[TT] = {}, qs[TT] = {};
-    float o_back = 0.f, p_back;
+    h8 qf[TT][NW], pf[TT][G][2], vr[VL];
+    f4 fq[TT], pu[NC][TT] = {}, qs[NC][TT] = {};
+    float o_back[NC] = {}, p_back;
     Part queries(p.keys + (2 * NW * 4 + wave * TT * NW) * kFrag, key_bytes(KD), p.n_chunks),
         factors(p.block + kRowFactors, kChunkBytes, p.n_chunks), p_part(p.block + kFrags * 2 * kFrag, kChunkBytes, p.n_chunks),
         scalar(p.block + kScalars + 4 * kPBack, kChunkBytes, p.n_chunks);
@@ -771,16 +816,23 @@ __device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace 
         in_order();
     };
     auto load_v = [&]() {  // zeros behind the last chunk
-        if (kValues) vr = load_run<VEC>(v_rows.buffer(), v_at);
+        if (kValues) {
+#pragma unroll
+            for (int j = 0; j < VL; ++j) vr[j] = load_run<VEC>(v_rows.buffer(), v_at[j]);
+        }
         v_rows.step();
         in_order();
     };
     h2 top = {};
     auto put_v = [&]() {
         if (kValues) {
-            *(h8 *)&lds.v[v_row][8 * (lane & 1)] = vr;
-            const u4 x = bitcast<u4>(vr) & 0x7fff7fffu;
-            top = larger(larger(bitcast<h2>(x.x), bitcast<h2>(x.y)), larger(bitcast<h2>(x.z), bitcast<h2>(x.w)));
+#pragma unroll
+            for (int j = 0; j < VL; ++j) {
+                *(h8 *)&lds.v[v_row[j]][8 * (lane % PR)] = vr[j];
+                const u4 x = bitcast<u4>(vr[j]) & 0x7fff7fffu;
+                const h2 y = larger(larger(bitcast<h2>(x.x), bitcast<h2>(x.y)), larger(bitcast<h2>(x.z), bitcast<h2>(x.w)));
+                top = j ? larger(top, y) : y;
+            }
         }
     };
     auto put_top = [&]() {  // the largest |V| of the wave's rows
@@ -794,9 +846,11 @@ __device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace 
         for (int tt = 0; tt < TT; ++tt) {
             const int t = wave * TT + tt;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                lds.o[16 * t + 4 * q + i][m] = (_Float16)__builtin_fmaf(pu[tt][i], o_back, qs[tt][i]);
-            const h8 o = *(const h8 *)&lds.o[16 * t + ((lane >> 1) & 15)][8 * (lane & 1)];
+            for (int n = 0; n < NC; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    lds.o[16 * t + 4 * q + i][16 * n + m] = (_Float16)__builtin_fmaf(pu[n][tt][i], o_back[n], qs[n][tt][i]);
+            const h8 o = *(const h8 *)&lds.o[16 * t + (lane / PR & 15)][8 * (lane % PR)];
             if constexpr (VEC) {
                 __builtin_amdgcn_raw_buffer_store_b128(bitcast<u4>(o), b, o_at[tt], 0, 0);
             } else {
@@ -819,18 +873,21 @@ __device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace 
     Buffer before = __builtin_amdgcn_make_buffer_rsrc(o_rows.base, 0, 0, 0x00020000);  // nothing ahead of the first chunk
     for (int c = 0; c < p.n_chunks; ++c) {
         lds_barrier();  // 1
-        h8 s_hi[NW], s_lo[NW];
-        float back[NW];
+        f4 qs_now[NC][TT];
 #pragma unroll
-        for (int g = 0; g < NW; ++g) {
-            s_hi[g] = lds.s[g][0][lane];
-            s_lo[g] = lds.s[g][1][lane];
-            back[g] = lds.back[g][m];
+        for (int n = 0; n < NC; ++n) {
+            h8 s_hi[NW], s_lo[NW];
+            float back[NW];
+#pragma unroll
+            for (int g = 0; g < NW; ++g) {
+                s_hi[g] = lds.s[n][g][0][lane];
+                s_lo[g] = lds.s[n][g][1][lane];
+                back[g] = lds.back[n][g][m];
+            }
+            lds_here();
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) qs_now[n][tt] = state_product<NW>(qf[tt], s_hi, s_lo, back) * fq[tt];
         }
-        lds_here();
-        f4 qs_now[TT];
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) qs_now[tt] = state_product<NW>(qf[tt], s_hi, s_lo, back) * fq[tt];
         in_order();
         load_q();
         lds_barrier();  // 2
@@ -838,19 +895,25 @@ __device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace 
         put_v();
         in_order();
         load_v();
-        o_back = lds.u_back[m] * p_back;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) o_back[n] = lds.u_back[n][m] * p_back;
         in_order();
         load_p_back();
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) qs[tt] = qs_now[tt];
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) qs[n][tt] = qs_now[n][tt];
         before = o_rows.buffer();
         o_rows.step();
         lds_barrier();  // 3
-        h8 u[G][2];
-        read_pairs<G>(lds.u, lane, u);
+        h8 u[NC][G][2];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) read_pairs<G>(lds.u[n], lane, u[n]);
         lds_here();
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) pu[tt] = lower_product<G>(pf[tt], u);
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) pu[n][tt] = lower_product<G>(pf[tt], u[n]);
         in_order();
         load_p();
         put_top();
@@ -858,11 +921,11 @@ __device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace 
     put_out(before);
 }
 
-template <int KD, bool VEC>
+template <int KD, int NC, bool VEC>
 __global__ __launch_bounds__(4 * KD) void delta_scan_kernel(DeltaArgs a, const char *chunks, size_t tiles, int units,
                                                             int slices, int limit) {
     constexpr int NW = KD / 32;
-    __shared__ __attribute__((aligned(16))) ScanLds<KD> lds;
+    __shared__ __attribute__((aligned(16))) ScanLds<KD, NC> lds;
     // the slices of a head on one XCD, whose L2 then holds what they share
     const int id = blockIdx.x, at_xcd = id >> 3;
     const int unit = at_xcd / slices * 8 + (id & 7);
@@ -883,10 +946,26 @@ __global__ __launch_bounds__(4 * KD) void delta_scan_kernel(DeltaArgs a, const c
     p.n_chunks = (int)min((size_t)(p.rows.count + kChunk - 1) / kChunk, tiles - min(tiles, tile0));
     p.block = chunks + (p.head * tiles + tile0) * kChunkBytes;
     p.keys = chunks + heads * tiles * kChunkBytes + (kh * tiles + tile0) * key_bytes(KD);
-    if (wave < NW / 2) state_wave<KD, false>(a, p, lds, wave, lane);
-    else if (wave < NW) state_wave<KD, true>(a, p, lds, wave, lane);
-    else if (wave < NW + NW / 2) output_wave<KD, VEC, false>(a, p, lds, wave - NW, lane);
-    else output_wave<KD, VEC, true>(a, p, lds, wave - NW, lane);
+    if (wave < NW / 2) state_wave<KD, NC, false>(a, p, lds, wave, lane);
+    else if (wave < NW) state_wave<KD, NC, true>(a, p, lds, wave, lane);
+    else if (wave < NW + NW / 2) output_wave<KD, NC, VEC, false>(a, p, lds, wave - NW, lane);
+    else output_wave<KD, NC, VEC, true>(a, p, lds, wave - NW, lane);
+}
+
+// Parts of 16 columns of all sequences and heads from which on a workgroup takes 32 of them: their operands are
+// loaded once and the longer chain is hidden by nothing, but the card is full either way.  16 heads of 128, sequences of 2048
+// rows, walk alone, 16 and 32 columns: 2 sequences (256 parts) 44 and 75 us, 4: 89 and 83, 6: 174 and 176, 8: 226 and 188,
+// 16: 430 and 367 us.
+constexpr size_t kWideParts = 1024;
+
+template <int KD, int NC>
+void launch_scan(const DeltaArgs &a, const char *chunks, size_t tiles, int limit, hipStream_t stream) {
+    const int units = a.s.sequences * a.v.heads, slices = a.value_dim / (16 * NC);
+    const dim3 blocks((unsigned)((units + 7) / 8 * 8 * slices));
+    if (a.v.vec && a.out.vec)
+        delta_scan_kernel<KD, NC, true><<<blocks, dim3(4 * KD), 0, stream>>>(a, chunks, tiles, units, slices, limit);
+    else
+        delta_scan_kernel<KD, NC, false><<<blocks, dim3(4 * KD), 0, stream>>>(a, chunks, tiles, units, slices, limit);
 }
 
 template <int KD>
@@ -894,14 +973,11 @@ hipError_t launch_kd(const DeltaArgs &a, char *chunks, hipStream_t stream) {
     const size_t tiles = tile_count(a.s, kChunk), heads = a.v.heads, slices = a.value_dim / 16;
     // sequences of one length are all long ones; one alone goes in chunks whatever its length
     const int limit = a.s.starts && a.s.sequences > 1 ? (int)kDeltaShortRows : 0;
-    const size_t units = a.s.sequences * heads, steps = limit ? units * slices : 0;
+    const size_t parts = a.s.sequences * heads * slices, steps = limit ? parts : 0;
     delta_prepare_kernel<KD><<<dim3((unsigned)(tiles * heads + (steps + kStepWaves - 1) / kStepWaves)), dim3(256), 0, stream>>>(
         a, chunks, tiles, limit, steps, (int)slices);
-    const dim3 blocks((unsigned)((units + 7) / 8 * 8 * slices));
-    if (a.v.vec && a.out.vec)
-        delta_scan_kernel<KD, true><<<blocks, dim3(4 * KD), 0, stream>>>(a, chunks, tiles, (int)units, (int)slices, limit);
-    else
-        delta_scan_kernel<KD, false><<<blocks, dim3(4 * KD), 0, stream>>>(a, chunks, tiles, (int)units, (int)slices, limit);
+    if (parts >= kWideParts && slices % 2 == 0) launch_scan<KD, 2>(a, chunks, tiles, limit, stream);
+    else launch_scan<KD, 1>(a, chunks, tiles, limit, stream);
     return hipGetLastError();
 }
 
