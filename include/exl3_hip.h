@@ -570,10 +570,11 @@ exl3_status exl3_hip_short_conv(const void *x, exl3_dtype xt, size_t x_row_strid
  *              not 0; it may be one that other calls use too.  NULL: the internal one of this stream
  * States and sums in fp32.  Long sequences' rows are taken 64 at a time, their products as fp16 pairs (high
  * and low part, 22 bits), and an element that is not finite makes NaN of its sequence and head from the first of its
- * 64 rows on (from its own row on else).  Long ones are those of 16 rows and more where starts is NULL, and of 8
- * and more where it is given and tokens / sequences is at least 2 (one alone: where tokens is at least 16).
- * The same inputs give the same bits on every call.  EXL3_NO_SUPPORT where (tokens / 64 + sequences) *
- * v heads * ceil(value_dim / 16) reaches 2^22.  sequences = 0 is a no-op. */
+ * 64 rows on (from its own row on else).  Long ones are those of 16 rows and more (24 where sequences * v heads *
+ * value_dim / 16 reaches 512) where starts is NULL, and of 8 and more where it is given, tokens is at least 16 and
+ * tokens / sequences at least 2 (every one alone of at least 16 tokens).  The same inputs give the same bits on every
+ * call.  EXL3_NO_SUPPORT where (tokens / 64 + sequences) * v heads * value_dim / 16 reaches 2^22.  sequences = 0 is a
+ * no-op. */
 exl3_status exl3_hip_delta_rule(const exl3_head_view *q, const exl3_head_view *k, const exl3_head_view *v,
                                 const float *g, const float *beta, size_t gate_stride, const float *a_log,
                                 const float *dt_bias, const exl3_head_view *out, size_t key_dim, size_t value_dim,

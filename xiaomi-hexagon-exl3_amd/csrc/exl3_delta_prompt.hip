@@ -31,6 +31,7 @@ namespace exl3k {
 
 namespace {
 
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
 
@@ -984,8 +985,9 @@ hipError_t launch_kd(const DeltaArgs &a, char *chunks, hipStream_t stream) {
 }  // namespace
 
 bool delta_prompt_serves(const DeltaArgs &a) {
-    const size_t most = (size_t)1 << 24;
-    return (a.s.starts || a.s.tokens >= kDeltaPromptRows * a.s.sequences) && a.v.token_stride <= most && a.out.token_stride <= most;
+    const size_t most = (size_t)1 << 24, parts = (size_t)a.s.sequences * a.v.heads * (a.value_dim / 16);
+    const size_t rows = parts < kDeltaManyParts ? kDeltaPromptRows : kDeltaPromptRowsOfMany;
+    return (a.s.starts || a.s.tokens >= rows * a.s.sequences) && a.v.token_stride <= most && a.out.token_stride <= most;
 }
 
 size_t delta_prompt_bytes(size_t heads, int key_dim, size_t sequences, size_t tokens) {
