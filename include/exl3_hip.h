@@ -572,7 +572,7 @@ exl3_status exl3_hip_short_conv(const void *x, exl3_dtype xt, size_t x_row_strid
  * and low part, 22 bits), and an element that is not finite makes NaN of its sequence and head from the first of its
  * 64 rows on (from its own row on else).  Long ones are those of 16 rows and more (24 where sequences * v heads *
  * value_dim / 16 reaches 512) where starts is NULL, and of 8 and more where it is given, tokens is at least 16 and
- * tokens / sequences at least 2 (every one alone of at least 16 tokens).  The same inputs give the same bits on every
+ * tokens / sequences at least 2 (a sequence alone: where tokens is at least 16).  The same inputs give the same bits on every
  * call.  EXL3_NO_SUPPORT where (tokens / 64 + sequences) * v heads * value_dim / 16 reaches 2^22.  sequences = 0 is a
  * no-op. */
 exl3_status exl3_hip_delta_rule(const exl3_head_view *q, const exl3_head_view *k, const exl3_head_view *v,
