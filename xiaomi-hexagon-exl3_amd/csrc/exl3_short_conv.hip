@@ -153,11 +153,11 @@ __global__ __launch_bounds__(kConvThreads) void short_conv_kernel(ConvArgs a, in
 template <int W, int C, int XF16, int YF16>
 hipError_t launch_tiles(const ConvArgs &a, hipStream_t stream) {
     const unsigned channel_blocks = (a.channels + kConvThreads * C - 1) / (kConvThreads * C);
-    // Long tiles read their W - 1 rows ahead less often, short ones fill the card: three workgroups a CU where a thread
-    // has eight channels (6144 channels: 8192 rows in tiles of 16, 32, 64 47, 45, 48 us; 2048 rows in tiles of 4,
-    // 8, 16 16.0, 14.0, 16.0 us), eight where it has one (3,800 rows of 1531: tiles of 4, 8, 16 8.3, 7.6, 8.2 us).
+    // Long tiles read their W - 1 rows ahead less often, short ones fill the card: 640 workgroups, 2.5 a CU (8192 rows of
+    // 6144 channels in tiles of 16, 32, 64: 47, 45, 48 us; 2048 rows in tiles of 4, 8, 16: 16.0, 14.0, 16.0 us; 1760
+    // rows of 1531 channels, one a thread, in tiles of 4, 8, 16, 32: 8.0, 6.9, 6.7, 7.2 us).
     int per = 32;
-    while (per > 4 && tile_count(a.s, per) * channel_blocks < (C == 8 ? 768 : 2048)) per /= 2;
+    while (per > 4 && tile_count(a.s, per) * channel_blocks < 640) per /= 2;
     const size_t blocks = tile_count(a.s, per) * channel_blocks;
     short_conv_kernel<W, C, XF16, YF16><<<dim3((unsigned)blocks), dim3(kConvThreads), 0, stream>>>(a, per, channel_blocks);
     return hipGetLastError();
