@@ -4,8 +4,8 @@
 // rows of one sequence and keeps the last W - 1 rows in registers; four rows are on their way while the four ahead of
 // them are worked on.  The rows ahead of a sequence's first come from its state, and only the
 // threads of its first tile read that state: they also write the one that it leaves, so a slot may be both.
-// 8192 rows of 6144 fp16 channels, W = 4 with silu: 45 us, 4.5 TB/s (without the four rows ahead 46 us, with a
-// branch for silu at each element 47 us).  Eight rows of eight sequences: 4.9 us, a launch's.
+// 8192 rows of 6144 fp16 channels, W = 4 with silu: 44.4 us, 4.5 TB/s (without the four rows ahead 46 us, with a
+// branch for silu at each element 47 us).  Eight rows of eight sequences: 4.2 us (weights not through LDS: 4.9 us).
 #include "exl3_activation.hpp"
 #include "exl3_head_rows.hpp"
 #include "exl3_packed_rows.hpp"
@@ -28,6 +28,12 @@ __device__ __forceinline__ void store_channels(void *p, size_t at, const float (
     else ((float *)p)[at] = v[0];
 }
 
+// Where piece p is: eight lanes' reads of their piece i (p = 2 W lane + i) would meet in the same banks where 2 W is 8.
+template <int W>
+__device__ __forceinline__ int piece_at(int p) {
+    return W == 4 ? p ^ (p >> 3 & 7) : p;
+}
+
 // A row's channels as loaded
 template <int F16, int C>
 struct Loaded {
@@ -47,17 +53,29 @@ __global__ __launch_bounds__(kConvThreads) void short_conv_kernel(ConvArgs a, in
     const unsigned tile = blockIdx.x / channel_blocks;
     const int c = (int)((blockIdx.x - tile * channel_blocks) * kConvThreads + threadIdx.x) * C;
     const Tile t = find_tile(a.s, (int)tile, per, threadIdx.x & 63);
-    if (t.s < 0 || c >= a.channels) return;
+    if (t.s < 0) return;
     float w[C][W], bias[C];
     if constexpr (C == 8) {
-        float flat[8 * W];
+        // A wave's weights are one run of memory: they are loaded as such, and LDS gives each lane its 2 W pieces of 16
+        // bytes (loaded by the lanes that need them, a load touches 64 lines).  Lanes behind the last channel take the last piece.
+        __shared__ __attribute__((aligned(16))) f4 pieces[kConvThreads / 64][64 * 2 * W];
+        const int lane = threadIdx.x & 63, most = a.channels / 4 * W - 1, first_piece = (c - 8 * lane) / 4 * W;
+        f4 *const own = pieces[threadIdx.x >> 6];
+        f4 x[2 * W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) load_run8<0>(a.weight, (size_t)c * W + 8 * i, 1, *(float(*)[8]) & flat[8 * i]);
+        for (int i = 0; i < 2 * W; ++i) x[i] = ((const f4 *)a.weight)[min(first_piece + 64 * i + lane, most)];
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) own[piece_at<W>(64 * i + lane)] = x[i];
+        asm volatile("" ::: "memory");  // the wave's own
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) x[i] = own[piece_at<W>(2 * W * lane + i)];
+        if (c >= a.channels) return;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
-            for (int j = 0; j < W; ++j) w[e][j] = flat[e * W + j];
+            for (int j = 0; j < W; ++j) w[e][j] = x[(e * W + j) / 4][(e * W + j) % 4];
     } else {
+        if (c >= a.channels) return;
 #pragma unroll
         for (int j = 0; j < W; ++j) w[0][j] = a.weight[(size_t)c * W + j];
     }
