@@ -10,7 +10,7 @@
 // 32 columns of one head's state in the registers of its waves, 32 rows each, and three exchanges through LDS a chunk.
 //
 // Bound by the chain from chunk to chunk, three exchanges of about 900 cycles (read, products, write, barrier), in
-// which a SIMD has 1500 cycles of instructions of its two waves, and by the preparation's writes.  8192 rows, 16 heads of 128: preparation 51 us (0.2 GB, 4.4 TB/s) and walk
+// which a SIMD has 1500 cycles of instructions of its two waves, and by the preparation's writes.  8192 rows, 16 heads of 128: preparation 48 us (0.2 GB, 4.6 TB/s) and walk
 // 160 us, 1.25 us a chunk; 2048 rows 17 and 40 us; 16 sequences of 2048 rows 167 and 367 us.  Half the waves
 // carry the state and half make the output, so that the chain has only what the next chunk waits for (both on every
 // wave: 400 us in all at 8192 rows).  Where operands lie as lanes want them a load is 1 KB of
@@ -178,6 +178,9 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
     const int row = 16 * wave + m;
     _Float16 *const k_lds = (_Float16 *)T, *const q_lds = (_Float16 *)(A + 16 * wave * kRowFloats);
     // all loads are on their way at once: rows beyond the last are the last one's until they are in registers
+    const HeadGates hg = head_gates(a, head);
+    Gates gt = load_gates(a, first + min(lane, count - 1), head);
+    in_order();
     h8 kx[NR], qx[NR];
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
@@ -186,15 +189,8 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
         kx[j] = load_h8((const _Float16 *)a.k.data + at * a.k.token_stride + kh * a.k.head_stride + 8 * c, a.k.vec);
         qx[j] = load_h8((const _Float16 *)a.q.data + at * a.q.token_stride + kh * a.q.head_stride + 8 * c, a.q.vec);
     }
-    const HeadGates hg = head_gates(a, head);
-    Gates gt = load_gates(a, first + min(lane, count - 1), head);
-#pragma unroll
-    for (int j = 0; j < NR; ++j) {
-        const int r = 64 / L * j + lane / L, c = lane % L;
-        if (16 * wave + r >= count) kx[j] = qx[j] = h8{};
-        *(h8 *)(k_lds + query_at<KD>(16 * wave + r, c)) = kx[j];
-        *(h8 *)(q_lds + query_at<KD>(r, c)) = qx[j];
-    }
+    in_order();
+    // the gates while the rows are on their way
     gt = gates_of(a, hg, gt);
     if (lane >= count) gt = Gates{0.f, 0.f};
     double G = gt.g;  // 64 bits: differences of long sums are the exponents
@@ -203,6 +199,15 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
         const double o = __shfl_up(G, d);
         G += lane >= d ? o : 0.0;
     }
+    in_order();
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+        const int r = 64 / L * j + lane / L, c = lane % L;
+        if (16 * wave + r >= count) kx[j] = qx[j] = h8{};
+        *(h8 *)(k_lds + query_at<KD>(16 * wave + r, c)) = kx[j];
+        *(h8 *)(q_lds + query_at<KD>(r, c)) = qx[j];
+    }
+    in_order();  // a wave's own rows
     float kk = 0.f, qq = 0.f, k1 = 0.f;
     h8 kf[NK], qf[NK];
 #pragma unroll
