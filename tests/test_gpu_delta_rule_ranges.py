@@ -1,0 +1,58 @@
+"""exl3_hip_delta_rule against its recurrence in 64 bits where rows, gates and epsilons differ widely within 64 rows."""
+import numpy as np
+import pytest
+
+import linear_attention_ref as ref
+from test_gpu_delta_rule import cuda, draw, inputs, starts_of
+
+pytestmark = pytest.mark.gpu
+
+
+def compare(amd, d, lens, states, eps, packed=True, chunk=64, scale=None, **kw):
+    """out and states of a call that goes on from every state, in place, against the recurrence's; `chunk` None: a call
+    that goes row by row"""
+    f = {k: None if x is None else x.astype(np.float64) for k, x in d.items()}
+    scale = d["q"].shape[2] ** -0.5 if scale is None else scale
+    slots = np.arange(len(lens), dtype=np.int32)[::-1].copy()
+    want, after, bound, off = ref.delta_rule(f["q"], f["k"], f["v"], f["g"], f["beta"], lens, float(np.float32(scale)),
+                                             states.astype(np.float64), slots, slots, f["a_log"], f["dt_bias"],
+                                             None if eps is None else float(np.float32(eps)), chunk=chunk)
+    t, pool = {k: cuda(x) for k, x in d.items()}, cuda(states)
+    where = dict(starts=starts_of(lens)) if packed else dict(sequences=len(lens))
+    got = amd.delta_rule(t["q"], t["k"], t["v"], t["g"], t["beta"], t["a_log"], t["dt_bias"], states=pool,
+                         slots_in=cuda(slots), slots_out=cuda(slots), scale=scale, qk_eps=eps, **where, **kw)
+    for name, x, w, top in (("out", got.cpu().numpy().astype(np.float64), want,
+                             bound + ref.rounded(np.abs(want) + bound, "float16")),
+                            ("states", pool.cpu().numpy().astype(np.float64), after, off + ref.E32 * np.abs(after))):
+        assert np.all(np.isfinite(x)), name
+        err = np.abs(x - w)
+        print(f"  {name}: largest error {err.max(initial=0):.2e} of {np.abs(w).max(initial=0):.2e}, "
+              f"{np.max(err / top, initial=0):.2f} of its bound")
+        assert np.all(err <= top), name
+
+
+# A key of length |k| has 1 / |k| among the factors of its row: they spread as the lengths do.
+@pytest.mark.parametrize("eps", [1e-6, 1e-12, 1e-16, 1e-24, 1e-36])
+@pytest.mark.parametrize("n", [14, 64, 150])
+@pytest.mark.parametrize("dk,dv", [(128, 16), (64, 48)])
+def test_rows_of_zeros(amd, dk, dv, n, eps):
+    """keys and queries of nothing, as padding rows give: they leave the state as it is"""
+    d = inputs(31, n, 2, 2, dk, dv)
+    d["k"][[3, 5, n - 1]] = 0
+    d["q"][[4, 5]] = 0
+    compare(amd, d, [n], draw(32, (1, 2, dk, dv), 0.5), eps, chunk=64 if n >= 16 else None)
+
+
+@pytest.mark.parametrize("eps", [1e-6, 1e-12, 0.0])
+@pytest.mark.parametrize("least,most", [(-12, 10), (-20, 12)])
+@pytest.mark.parametrize("n", [14, 64, 150])
+@pytest.mark.parametrize("dk,dv", [(128, 16), (64, 48)])
+def test_rows_of_many_lengths(amd, dk, dv, n, least, most, eps):
+    d = inputs(33, n, 2, 2, dk, dv)
+    rng = np.random.default_rng(5)
+    for name in ("q", "k"):
+        by = 2.0 ** rng.integers(least, most + 1, (n, 2, 1))
+        x = (d[name].astype(np.float64) * by).astype(np.float16)
+        x[..., 0] = np.where(np.any(x, -1), x[..., 0], np.float16(2.0 ** -24))  # no row is empty
+        d[name] = x
+    compare(amd, d, [n], draw(34, (1, 2, dk, dv), 0.5), eps, chunk=64 if n >= 16 else None)

@@ -17,7 +17,7 @@
 // consecutive bytes; 16 rows by 64 bytes a load is four times as slow.
 //
 // The products run on mfma_f32_16x16x32_f16.  K and Q are fp16 as given (their lengths are factors of rows
-// applied afterwards); every other operand x is two fp16 numbers, hi = fp16(x) and lo = fp16(x - hi), 22 bits
+// applied afterwards; K's columns have a power of two a row); every other operand x is two fp16 numbers, hi = fp16(x) and lo = fp16(x - hi), 22 bits
 // together, after a power of two has taken a bound on its column (or matrix) to 2^15; below 2^-29 of that bound
 // they are steps of 2^-40 of it.  Products of two such pairs leave out lo lo.  One fp16 number in the state's place would
 // lose what the recurrence in binary32 keeps (2^-11 of S in every chunk).
@@ -151,6 +151,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
     __shared__ __attribute__((aligned(16))) float lds[3 * kMatrix];  // A, P, T
     __shared__ double sum_lds[kChunk];
     __shared__ float kr_lds[kChunk], qr_lds[kChunk], most_lds[4], l1_lds[4], sum_T_lds[4];
+    __shared__ __attribute__((aligned(16))) int shift_lds[kChunk];
     float *const A = lds, *const Pm = lds + kMatrix, *const T = lds + 2 * kMatrix;
     static_assert(kChunk * KD * 2 <= kMatrix * 4, "the keys fit");
 
@@ -231,10 +232,16 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
         rq = inverse_length(qq, a.eps);
     }
     if (row >= count) rk = rq = 0.f;  // 1 / sqrt(0) where eps is 0
+    // The keys' columns are laid out with a power of two a row that takes |k| to 2^14 .. 2^15, and its inverse is in the
+    // row's factor of W: one scale serves W's 64 rows, and 1 / |k| there would let the shortest key set it (with a row of
+    // zeros and eps = 1e-24 the others' W fell below fp16's steps, and the whole chunk's update was lost).  A row of zeros
+    // has none.
+    const int shift = kk > 0.f ? 15 - ((__builtin_amdgcn_frexp_expf(kk) + 1) >> 1) : 1000;
     if (wave == 0) sum_lds[lane] = G;
     if (q == 0) {
         kr_lds[row] = rk;
         qr_lds[row] = rq * a.scale;
+        shift_lds[row] = shift;
     }
     __syncthreads();
 
@@ -249,7 +256,10 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
             const int k = wave >> 1, t = wave & 1, r = 32 * k + 8 * q + (m >> 2), c = 4 * s + (m & 3);
             const h4 x = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(k_lds + query_at<KD>(r, c) + 4 * t)));
             const h4 y = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(k_lds + query_at<KD>(r + 4, c) + 4 * t)));
-            columns[(s * 4 + wave) * 64] = (h8){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            h8 z;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] = __builtin_amdgcn_ldexph(j < 4 ? x[j & 3] : y[j & 3], shift_lds[32 * k + 8 * q + j]);
+            columns[(s * 4 + wave) * 64] = z;
         }
     }
     // a head's chunks next to each other: the walk over them stays in few pages
@@ -393,7 +403,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
     __syncthreads();
     if (wave == 0) {  // lane = row
         const float r = kr_lds[lane], e = decay_of((float)G);
-        const float until = decay_of((float)(G_end - G)) * r;
+        const float until = __builtin_amdgcn_ldexpf(decay_of((float)(G_end - G)) * r, -shift_lds[lane]);
         int e_w = __builtin_amdgcn_frexp_expf(max_lanes(__builtin_fabsf(until)));
         e_w = e_w < -110 ? -110 : e_w;
         float *const f = (float *)(block + kRowFactors);
