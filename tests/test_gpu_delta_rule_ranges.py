@@ -56,3 +56,13 @@ def test_rows_of_many_lengths(amd, dk, dv, n, least, most, eps):
         x[..., 0] = np.where(np.any(x, -1), x[..., 0], np.float16(2.0 ** -24))  # no row is empty
         d[name] = x
     compare(amd, d, [n], draw(34, (1, 2, dk, dv), 0.5), eps, chunk=64 if n >= 16 else None)
+
+
+@pytest.mark.parametrize("eps", [1e-38, 1e-40, 2e-45])
+@pytest.mark.parametrize("n", [14, 150])
+def test_epsilons_at_the_end_of_their_type(amd, n, eps):
+    """1 / sqrt(eps) is finite and its square is not"""
+    d = inputs(35, n, 2, 2, 64, 32)
+    d["k"][[3, 5, 6, n - 1]] = 0
+    d["q"][[4, 5, 7]] = 0
+    compare(amd, d, [n], draw(36, (1, 2, 64, 32), 0.5), eps, chunk=64 if n >= 16 else None)

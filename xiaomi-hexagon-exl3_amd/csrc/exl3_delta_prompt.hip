@@ -303,9 +303,10 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
             const int i = 16 * wave + 4 * q + r;
             float av = 0.f, pv = 0.f;
             if (i >= c) {
+                // a row's factor meets the product ahead of the other row's: 1 / |k| of two rows of zeros may be 2^74 each
                 const float fall = decay_of((float)(Gr[r] - Gc)) * kc;
-                pv = qr[r] * fall * qk_acc[j][r];
-                if (i > c) av = brk[r] * fall * kk_acc[j][r];
+                pv = qr[r] * qk_acc[j][r] * fall;
+                if (i > c) av = brk[r] * kk_acc[j][r] * fall;
             }
             A[i * kRowFloats + c] = av;
             Pm[i * kRowFloats + c] = pv;
