@@ -569,9 +569,12 @@ exl3_status exl3_hip_short_conv(const void *x, exl3_dtype xt, size_t x_row_strid
  *   workspace  device, 256-byte aligned, >= exl3_hip_delta_rule_workspace_bytes() where that is
  *              not 0; it may be one that other calls use too.  NULL: the internal one of this stream
  * States and sums in fp32.  Long sequences' rows are taken 64 at a time, their products as fp16 pairs (high
- * and low part, 22 bits), and an element that is not finite makes NaN of its sequence and head from the first of its
- * 64 rows on (from its own row on else).  Long ones are those of 16 rows and more (24 where sequences * v heads *
- * value_dim / 16 reaches 512) where starts is NULL, and of 8 and more where it is given, tokens is at least 16 and
+ * and low part, 22 bits).
+ * An element that is not finite leaves other sequences, other heads and the rows ahead of its 64 as they are.  One of v
+ * or of a state reaches its own column alone (v counts as 65,504 in the bits of the others), one of k, g or beta its
+ * heads: infinite or NaN from its row on, and where rows are taken 64 at a time the rows ahead of it among them may be
+ * NaN as well.  One of q makes NaN of its row's outputs, there perhaps of others of the 64 too, and reaches no state.
+ * Long sequences are those of 16 rows and more (24 where sequences * v heads * value_dim / 16 reaches 512) where starts is NULL, and of 8 and more where it is given, tokens is at least 16 and
  * tokens / sequences at least 2 (a sequence alone: where tokens is at least 16).  The same inputs give the same bits on every
  * call.  EXL3_NO_SUPPORT where (tokens / 64 + sequences) * v heads * value_dim / 16 reaches 2^22.  sequences = 0 is a
  * no-op. */

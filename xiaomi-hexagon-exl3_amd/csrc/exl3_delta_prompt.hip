@@ -852,9 +852,9 @@ __device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace 
             }
         }
     };
-    auto put_top = [&]() {  // the largest |V| of the wave's rows
+    auto put_top = [&]() {  // the largest |V| of the wave's rows; infinities and NaN count as fp16's largest, for the other columns
         if (kValues) {
-            const float x = max_lanes(fmaxf((float)top[0], (float)top[1]));
+            const float x = fminf(max_lanes(fmaxf((float)top[0], (float)top[1])), 65504.f);
             if (lane == 0) lds.v_top[wave] = x;
         }
     };
