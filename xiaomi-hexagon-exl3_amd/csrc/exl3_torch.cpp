@@ -400,7 +400,7 @@ PyObject *delta_rule(PyObject *const *a) {
     const at::Tensor &g = c.tensor(a[3], "g is a tensor"), &beta = c.tensor(a[4], "beta is a tensor");
     need(g.scalar_type() == at::kFloat && beta.scalar_type() == at::kFloat && g.dim() == 2 && g.size(0) == n &&
              g.size(1) == h && same_shape(g, beta) && (h == 1 || !n || (g.stride(1) == 1 && beta.stride(1) == 1)) &&
-             row_stride(g) == row_stride(beta),
+             (n <= 1 || row_stride(g) == row_stride(beta)),
          "g and beta: float32 [tokens, v heads] with the same row stride, dense rows");
     const void *al = c.dense(a[5], at::kFloat, h, "a_log: dense float32 [v heads]", true);
     const void *dt = c.dense(a[6], at::kFloat, h, "dt_bias: dense float32 [v heads]", true);
@@ -412,7 +412,7 @@ PyObject *delta_rule(PyObject *const *a) {
     size_t ws_bytes;
     void *const ws = c.workspace(a[15], &ws_bytes);
     return one(exl3_hip_delta_rule(&qv, &kv, &vv, (const float *)g.data_ptr(), (const float *)beta.data_ptr(),
-                                   row_stride(g), (const float *)al, (const float *)dt, &ov, (size_t)dk, (size_t)dv,
+                                   std::max(row_stride(g), row_stride(beta)), (const float *)al, (const float *)dt, &ov, (size_t)dk, (size_t)dv,
                                    p.starts, p.sequences, (size_t)n, (float *)p.states, p.slots, p.in, p.out,
                                    scale_of(a[12], dk), given(a[13]) ? real_of(a[13]) : -1.f, ws, ws_bytes, c.stream),
                out);

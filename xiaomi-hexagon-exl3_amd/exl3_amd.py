@@ -680,10 +680,10 @@ def delta_rule_workspace_bytes(v_heads, key_dim, value_dim, sequences, tokens):
 def delta_rule(q, k, v, g, beta, a_log=None, dt_bias=None, starts=None, sequences=1, states=None, slots_in=None,
                slots_out=None, scale=None, qk_eps=None, out=None, workspace=None, stream=None):
     """The gated delta rule over packed rows, all fp16: q and k [tokens, k_heads, key_dim], v [tokens, v_heads,
-    value_dim] -> [tokens, v_heads, value_dim].  g (log decay) and beta fp32 [tokens, v_heads]; with a_log and
-    dt_bias (fp32 [v_heads]) they are -exp(a_log) softplus(g + dt_bias) and sigmoid(beta).  qk_eps: q and k are
-    divided by sqrt(sum of squares + qk_eps) (None: as they are); scale: 1 / sqrt(key_dim) unless given.
-    states: fp32 [slots, v_heads, key_dim, value_dim]."""
+    value_dim] -> [tokens, v_heads, value_dim].  g (log decay) and beta fp32 [tokens, v_heads], dense rows that lie as
+    far apart in both (columns of one matrix, or both contiguous); with a_log and dt_bias (fp32 [v_heads]) they are
+    -exp(a_log) softplus(g + dt_bias) and sigmoid(beta).  qk_eps: q and k are divided by sqrt(sum of squares + qk_eps)
+    (None: as they are); scale: 1 / sqrt(key_dim) unless given.  states: fp32 [slots, v_heads, key_dim, value_dim]."""
     return _taken((_TORCH or _torch_module()).delta_rule(
         q, k, v, g, beta, a_log, dt_bias, starts, sequences, states, slots_in, slots_out, scale, qk_eps, out, workspace,
         stream), "delta_rule")
