@@ -18,3 +18,17 @@ def test_one_row_of_gates_has_any_stride(amd):
     two = [t.repeat(2, *[1] * (t.dim() - 1)) for t in (q, k, v, wide, beta)]
     with pytest.raises(AssertionError, match="row stride"):
         amd.delta_rule(*two[:3], two[3][:, 2:6], two[4])
+
+
+@pytest.mark.parametrize("off", [4, 8, 12, 1])
+def test_fp32_rows_at_places_of_16_bytes(amd, off):
+    """eight channels at a time lie at 16-byte places that are none of 32"""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(2)
+    base = torch.randn(off + 37 * 80, generator=g, device="cuda")
+    x, w = base[off:].view(37, 80)[:, :40], torch.randn(40, 4, generator=g, device="cuda")
+    dense = x.contiguous()
+    out = torch.zeros(off + 37 * 48, device="cuda")[off:].view(37, 48)
+    amd.short_conv(x, w, bias=w[:, 0].contiguous(), sequences=1, out=out[:, :40])
+    assert torch.equal(out[:, :40], amd.short_conv(dense, w, bias=w[:, 0].contiguous()))
+    assert bool((out[:, 40:] == 0).all())

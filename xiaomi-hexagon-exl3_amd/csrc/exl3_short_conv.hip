@@ -34,11 +34,11 @@ __device__ __forceinline__ int piece_at(int p) {
     return W == 4 ? p ^ (p >> 3 & 7) : p;
 }
 
-// A row's channels as loaded
+// A row's channels as loaded; eight of fp32 are at 16-byte places, not at the 32 of their type
 template <int F16, int C>
 struct Loaded {
     typedef typename std::conditional<F16, _Float16, float>::type T;
-    typedef T V __attribute__((ext_vector_type(C)));
+    typedef T V __attribute__((ext_vector_type(C), aligned(C == 8 ? 16 : sizeof(T))));
     V v;
     __device__ __forceinline__ void load(const void *p, size_t at) { v = *(const V *)((const T *)p + at); }
     __device__ __forceinline__ void to(float (&x)[C]) const {
