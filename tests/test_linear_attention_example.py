@@ -35,3 +35,31 @@ def test_a_sequence_named_twice_takes_nothing(block):
     with pytest.raises(RuntimeError, match="no free state"):
         block.rows(None, None, list("abcd"), [1] * 4)
     assert (block.free, block.slot) == ([2, 1, 0], {})
+
+
+def test_a_call_that_fails_takes_nothing(block):
+    """a new sequence whose rows() failed would go on from whatever its slot held"""
+    torch = pytest.importorskip("torch")
+    assert block._take(["old"]) == ([-1], [0])
+    x = torch.zeros(3, 8)
+    for seqs, lens in ((["a"], [2]), (["a"], [4]), (["a", "b"], [3]), (["a"], [1, 2]), (["a", "b"], [4, -1]), ([], [3])):
+        with pytest.raises(ValueError, match="lengths"):
+            block.rows(x, x, seqs, lens)
+        assert (block.free, block.slot) == ([2, 1], {"old": 0}), (seqs, lens)
+
+    def fails(*_):
+        raise RuntimeError("refused")
+
+    block._block, block.workspace, block.max_rows = fails, None, 32
+    with pytest.raises(Exception):
+        block.rows(x, x, ["old", "a", "b"], [1, 1, 1])
+    assert (block.free, block.slot) == ([2, 1], {"old": 0})
+
+
+def test_a_plan_names_a_sequence_once(block):
+    """two sequences in one slot would race for its state"""
+    block._take(["a", "b"])
+    with pytest.raises(ValueError, match="twice"):
+        block.plan(["a", "b", "a"])
+    with pytest.raises(KeyError):
+        block.plan(["c"])

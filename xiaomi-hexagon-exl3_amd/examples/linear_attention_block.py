@@ -92,17 +92,28 @@ class LinearAttentionBlock:
 
     def rows(self, x, residual, seqs, lengths):
         """x, residual fp32 [sum of lengths, hidden]: lengths[i] rows of each sequence, one after the other -> (the
-        block's output, x + residual), both [rows, hidden].  The layers take up to 65,536 rows in a call."""
+        block's output, x + residual), both [rows, hidden].  The layers take up to 65,536 rows in a call.  Where it fails,
+        new sequences stay new: their slots hold states of others."""
         starts = [0]
         for n in lengths:
             starts.append(starts[-1] + n)
         from_, to = self._take(seqs)
-        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
-        where = dict(starts=i32(starts), sequences=len(seqs), slots_in=i32(from_), slots_out=i32(to))
-        return self._block(x, residual, where, self.workspace if starts[-1] <= self.max_rows else None)
+        try:
+            if len(lengths) != len(seqs) or min(lengths, default=0) < 0 or starts[-1] != x.shape[0]:
+                raise ValueError("lengths: one a sequence, together the rows of x")
+            i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+            where = dict(starts=i32(starts), sequences=len(seqs), slots_in=i32(from_), slots_out=i32(to))
+            return self._block(x, residual, where, self.workspace if starts[-1] <= self.max_rows else None)
+        except BaseException:
+            for s, was in reversed(list(zip(seqs, from_))):
+                if was < 0:
+                    self.release(s)
+            raise
 
     def plan(self, seqs):
         """for step(): the slots of sequences that rows() has started, on the GPU"""
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence is named twice")
         return torch.tensor([self.slot[s] for s in seqs], dtype=torch.int32, device="cuda")
 
     def step(self, x, residual, plan, tokens=1):
