@@ -66,3 +66,13 @@ def test_epsilons_at_the_end_of_their_type(amd, n, eps):
     d["k"][[3, 5, 6, n - 1]] = 0
     d["q"][[4, 5, 7]] = 0
     compare(amd, d, [n], draw(36, (1, 2, 64, 32), 0.5), eps, chunk=64 if n >= 16 else None)
+
+
+@pytest.mark.parametrize("size", [1.0, 300.0, 3e4, 3e6, 3e8])
+@pytest.mark.parametrize("n", [14, 64, 100])
+def test_states_emptied_on_the_way(amd, n, size):
+    """a gate of -inf: 14 rows go row by row and keep binary32's bits, 64 together the steps of the state ahead of them"""
+    d = inputs(37, n, 2, 2, 128, 32, raw=False)
+    d["g"][n // 2] = -np.inf
+    d["v"][:n // 2] = 0
+    compare(amd, d, [n], draw(38, (1, 2, 128, 32)) * np.float32(size), 1e-6, chunk=64 if n >= 16 else None, scale=1e-9)
