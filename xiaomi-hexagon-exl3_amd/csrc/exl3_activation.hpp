@@ -1,4 +1,4 @@
-// exl3_activation.hpp -- device exponentials and sigmoids in binary32.
+// exl3_activation.hpp -- device exponentials, sigmoids and inverse roots in binary32.
 #pragma once
 
 #include "exl3_device.hpp"
@@ -20,5 +20,11 @@ __device__ __forceinline__ float exp_f32(float x) {
 // 1 / (1 + exp(-z)); a NaN stays one in silu by its factor
 __device__ __forceinline__ float sigmoid_f32(float z) { return __builtin_amdgcn_rcpf(1.f + exp_f32(-z)); }
 __device__ __forceinline__ float silu_f32(float z) { return z * sigmoid_f32(z); }
+
+// 1 / sqrt(x): v_rsq_f32 is good to 1 ulp, of normal numbers
+__device__ __forceinline__ float inverse_root(float x) {
+    const bool tiny = x < 0x1p-100f;
+    return __builtin_amdgcn_rsqf(tiny ? x * 0x1p64f : x) * (tiny ? 0x1p32f : 1.f);
+}
 
 }  // namespace exl3k

@@ -1,4 +1,4 @@
-// exl3_delta_gates.hpp -- device helpers of the delta rule's kernels: gates and inverse lengths.
+// exl3_delta_gates.hpp -- device helpers of the delta rule's kernels: gates.
 #pragma once
 
 #include <math.h>
@@ -37,12 +37,5 @@ __device__ __forceinline__ Gates gates_of(const DeltaArgs &a, const HeadGates &h
 }
 // exp of a log decay (or a sum of them); NaN stays one
 __device__ __forceinline__ float decay_of(float g) { return g == g ? exp_f32(g) : g; }
-
-// 1 / sqrt(sum of squares + eps), to 1 ulp
-__device__ __forceinline__ float inverse_length(float squares, float eps) {
-    const float s = squares + eps;
-    const bool tiny = s < 0x1p-100f;
-    return __builtin_amdgcn_rsqf(tiny ? s * 0x1p64f : s) * (tiny ? 0x1p32f : 1.f);
-}
 
 }  // namespace exl3k

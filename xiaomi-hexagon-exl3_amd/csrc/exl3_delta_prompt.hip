@@ -116,14 +116,6 @@ __device__ __forceinline__ float sum_quarters(float v) {
     return __int_as_float(b[0]) + __int_as_float(b[1]);
 }
 
-__device__ __forceinline__ h8 load_h8(const _Float16 *p, int vec) {
-    if (vec) return *(const h8 *)p;
-    h8 t;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) t[e] = p[e];
-    return t;
-}
-
 // Where 16-byte run c of row r of rows of KD elements in LDS is: 16 rows' runs c lie in all banks, as do a row's runs.
 template <int KD>
 __device__ __forceinline__ int query_at(int r, int c) {
@@ -187,8 +179,8 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
     for (int j = 0; j < NR; ++j) {
         const int r = 16 * wave + 64 / L * j + lane / L, c = lane % L;
         const size_t at = first + min(r, count - 1);
-        kx[j] = load_h8((const _Float16 *)a.k.data + at * a.k.token_stride + kh * a.k.head_stride + 8 * c, a.k.vec);
-        qx[j] = load_h8((const _Float16 *)a.q.data + at * a.q.token_stride + kh * a.q.head_stride + 8 * c, a.q.vec);
+        kx[j] = load_halves<8>((const _Float16 *)a.k.data + at * a.k.token_stride + kh * a.k.head_stride + 8 * c, a.k.vec);
+        qx[j] = load_halves<8>((const _Float16 *)a.q.data + at * a.q.token_stride + kh * a.q.head_stride + 8 * c, a.q.vec);
     }
     in_order();
     // the gates while the rows are on their way
@@ -228,8 +220,8 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
     k1 = sum_quarters(k1);
     float rk = 1.f, rq = 1.f;
     if (a.eps >= 0.f) {
-        rk = inverse_length(kk, a.eps);
-        rq = inverse_length(qq, a.eps);
+        rk = inverse_root(kk + a.eps);
+        rq = inverse_root(qq + a.eps);
     }
     if (row >= count) rk = rq = 0.f;  // 1 / sqrt(0) where eps is 0
     // The keys' columns are laid out with a power of two a row that takes |k| to 2^14 .. 2^15, and its inverse is in the

@@ -9,8 +9,9 @@
 //   out = scale (e^g S^T q + (k . q) u).
 // The sums over r of two and four numbers are exchanged together (sums_in_rows), and a row of 16 lanes works out u and out
 // of one of the four columns.
-// 16 heads of 128 x 128, one row each: 4.9 us of one sequence, of 64 sequences 24 us, 5.6 TB/s.  With each number
-// summed by itself a further row of one sequence took 1.0 us, now 0.73 us, about 1750 cycles from k and q to the state.
+// 16 heads of 128 x 128, one row each: 4.8 us of one sequence, of 64 sequences 24 us, 5.6 TB/s.  With each number
+// summed by itself a further row of one sequence took 1.0 us, summed together 0.77 us, and with a row's halves kept in
+// pairs, as they were loaded, 0.60 us, about 1450 cycles from k and q to the state.
 // Waves of 32 columns were slower (7.3 and 29 us: too few on the card to hide their loads), waves of 8 columns
 // too (5.0 and 29 us: 64 bytes of a state's row at a time); loading four rows ahead instead of one changed nothing.
 #pragma once
@@ -21,7 +22,6 @@
 namespace exl3k {
 
 namespace {
-
 
 constexpr int kStepWaves = 4;  // of a workgroup; nothing is shared
 
@@ -61,33 +61,33 @@ __device__ __forceinline__ float lane_value(float v, int t) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), t & 63));
 }
 
+// N consecutive elements, at a place of their size where `vec`
 template <int N>
-__device__ __forceinline__ void load_halves(const _Float16 *p, bool vec, _Float16 (&to)[N]) {
-    typedef _Float16 hv __attribute__((ext_vector_type(N < 8 ? N : 8)));
-    if (vec) {
+struct Halves {
+    typedef _Float16 V __attribute__((ext_vector_type(N)));
+};
+template <int N>
+__device__ __forceinline__ typename Halves<N>::V load_halves(const _Float16 *p, int vec) {
+    typedef typename Halves<N>::V V;
+    if (vec) return *(const V *)p;
+    V t;
 #pragma unroll
-        for (int i = 0; i < N; i += 8) {
-            const hv t = *(const hv *)(p + i);
-#pragma unroll
-            for (int e = 0; e < (N < 8 ? N : 8); ++e) to[i + e] = t[e];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) to[i] = p[i];
-    }
+    for (int e = 0; e < N; ++e) t[e] = p[e];
+    return t;
 }
 
 // One row's inputs as a lane needs them: its R elements of k and q, one of v.
 template <int R>
 struct StepRow {
-    _Float16 k[R], q[R], v;
+    typename Halves<R>::V k, q;
+    _Float16 v;
 };
 template <int R>
 __device__ __forceinline__ void load_row(const DeltaArgs &a, size_t row, int head, int kr, int col,
                                          StepRow<R> &x) {
     const int kh = head / (a.v.heads / a.k.heads);
-    load_halves((const _Float16 *)a.k.data + row * a.k.token_stride + kh * a.k.head_stride + kr, a.k.vec, x.k);
-    load_halves((const _Float16 *)a.q.data + row * a.q.token_stride + kh * a.q.head_stride + kr, a.q.vec, x.q);
+    x.k = load_halves<R>((const _Float16 *)a.k.data + row * a.k.token_stride + kh * a.k.head_stride + kr, a.k.vec);
+    x.q = load_halves<R>((const _Float16 *)a.q.data + row * a.q.token_stride + kh * a.q.head_stride + kr, a.q.vec);
     x.v = ((const _Float16 *)a.v.data)[row * a.v.token_stride + head * a.v.head_stride + col];
 }
 
@@ -144,7 +144,7 @@ __device__ __forceinline__ void delta_step(const DeltaArgs &a, size_t unit, int 
         kq = row_value(sums, 1);
         float rk = 1.f, rq = 1.f;
         if (a.eps >= 0.f) {
-            const float inverse = inverse_length(sums, a.eps);
+            const float inverse = inverse_root(sums + a.eps);
             rk = row_value(inverse, 0);
             rq = row_value(inverse, 2);
         }

@@ -14,12 +14,6 @@ namespace {
 
 constexpr int kNormThreads = 256;
 
-// 1 / sqrt(mean): v_rsq_f32 is good to 1 ulp, of normal numbers
-__device__ __forceinline__ float inverse_root(float mean) {
-    const bool tiny = mean < 0x1p-100f;
-    return __builtin_amdgcn_rsqf(tiny ? mean * 0x1p64f : mean) * (tiny ? 0x1p32f : 1.f);
-}
-
 // Eight elements as loaded, one or two 16-byte words.
 struct Run {
     u4 a, b;
