@@ -76,3 +76,26 @@ def test_states_emptied_on_the_way(amd, n, size):
     d["g"][n // 2] = -np.inf
     d["v"][:n // 2] = 0
     compare(amd, d, [n], draw(38, (1, 2, 128, 32)) * np.float32(size), 1e-6, chunk=64 if n >= 16 else None, scale=1e-9)
+
+
+@pytest.mark.parametrize("n", [14, 64, 150])
+@pytest.mark.parametrize("least,most", [(-6, 6), (-13, 13)])
+@pytest.mark.parametrize("dk,dv", [(128, 32), (64, 48)])
+def test_queries_of_many_lengths_as_they_are(amd, dk, dv, n, least, most):
+    """without the norm: rows of P differ as the queries do"""
+    d = inputs(39, n, 2, 2, dk, dv, norm=False)
+    by = 2.0 ** np.random.default_rng(6).integers(least, most + 1, (n, 2, 1))
+    d["q"] = (d["q"].astype(np.float64) * by).astype(np.float16)
+    compare(amd, d, [n], draw(40, (1, 2, dk, dv), 0.5), None, chunk=64 if n >= 16 else None, scale=1.0)
+
+
+@pytest.mark.parametrize("n", [14, 64, 150])
+@pytest.mark.parametrize("least,most", [(-3, 3), (-8, 6)])
+@pytest.mark.parametrize("dk,dv", [(128, 32), (64, 48)])
+def test_keys_of_many_lengths_as_they_are(amd, dk, dv, n, least, most):
+    """without the norm: beta |k|^2 is at most 1, as where the recurrence is a contraction"""
+    d = inputs(41, n, 2, 2, dk, dv, raw=False, norm=False)
+    by = 2.0 ** np.random.default_rng(7).integers(least, most + 1, (n, 2))
+    d["k"] = (d["k"].astype(np.float64) * by[..., None]).astype(np.float16)
+    d["beta"] = (d["beta"] / np.maximum(1, by * by)).astype(np.float32)
+    compare(amd, d, [n], draw(42, (1, 2, dk, dv), 0.5), None, chunk=64 if n >= 16 else None)

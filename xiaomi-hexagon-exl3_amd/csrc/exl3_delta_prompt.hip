@@ -10,17 +10,18 @@
 // 32 columns of one head's state in the registers of its waves, 32 rows each, and three exchanges through LDS a chunk.
 //
 // Bound by the chain from chunk to chunk, three exchanges of about 900 cycles (read, products, write, barrier), in
-// which a SIMD has 1500 cycles of instructions of its two waves, and by the preparation's writes.  8192 rows, 16 heads of 128: preparation 48 us (0.2 GB, 4.6 TB/s) and walk
-// 160 us, 1.25 us a chunk; 2048 rows 17 and 40 us; 16 sequences of 2048 rows 167 and 367 us.  Half the waves
-// carry the state and half make the output, so that the chain has only what the next chunk waits for (both on every
-// wave: 400 us in all at 8192 rows).  Where operands lie as lanes want them a load is 1 KB of
-// consecutive bytes; 16 rows by 64 bytes a load is four times as slow.
+// which a SIMD has 1500 cycles of instructions of its two waves, and by the preparation's writes.  8192 rows, 16 heads
+// of 128: preparation 48 us (0.2 GB, 4.6 TB/s) and walk 158 us, 1.25 us a chunk; 2048 rows 17 and 40 us; 16 sequences
+// of 2048 rows 167 and 366 us.  Half the waves carry the state and half make the output, so that the chain has only
+// what the next chunk waits for (both on every wave: 400 us in all at 8192 rows).  Where operands lie as lanes want
+// them a load is 1 KB of consecutive bytes; 16 rows by 64 bytes a load is four times as slow.
 //
-// The products run on mfma_f32_16x16x32_f16.  K and Q are fp16 as given (their lengths are factors of rows
-// applied afterwards; K's columns have a power of two a row); every other operand x is two fp16 numbers, hi = fp16(x) and lo = fp16(x - hi), 22 bits
-// together, after a power of two has taken a bound on its column (or matrix) to 2^15; below 2^-29 of that bound
-// they are steps of 2^-40 of it.  Products of two such pairs leave out lo lo.  One fp16 number in the state's place would
-// lose what the recurrence in binary32 keeps (2^-11 of S in every chunk).
+// The products run on mfma_f32_16x16x32_f16.  K and Q are fp16 as given (their lengths are factors of rows applied
+// afterwards; K's columns have a power of two a row); every other operand x is two fp16 numbers, hi = fp16(x) and
+// lo = fp16(x - hi), 22 bits together, after a power of two has taken a bound on its column (or matrix) to 2^15; below
+// 2^-29 of that bound they are steps of 2^-40 of it.  Products of two such pairs leave out lo lo.  One fp16 number in
+// the state's place would lose what the recurrence in binary32 keeps (2^-11 of S in every chunk).
+// (P's one power of two serves rows of any |q|: outputs are fp16, and queries 2^26 apart in length lose none of their bits.)
 //
 // D leaves lane 16 q + n with column n of rows 4 q + i (i < 4), and B wants rows 8 q + j (j < 8) of column n there.
 // So a 32-row operand is two tiles whose rows 4 q + i stand for rows 8 q + i and 8 q + 4 + i: the second
@@ -250,7 +251,8 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaArgs a, char *c
             const h4 y = bitcast<h4>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(k_lds + query_at<KD>(r + 4, c) + 4 * t)));
             h8 z;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] = __builtin_amdgcn_ldexph(j < 4 ? x[j & 3] : y[j & 3], shift_lds[32 * k + 8 * q + j]);
+            for (int j = 0; j < 8; ++j)
+                z[j] = __builtin_amdgcn_ldexph(j < 4 ? x[j & 3] : y[j & 3], shift_lds[32 * k + 8 * q + j]);
             columns[(s * 4 + wave) * 64] = z;
         }
     }
@@ -444,10 +446,11 @@ __device__ __forceinline__ size_t uniform(size_t v) {
     return (uint32_t)uniform((int)(uint32_t)v) | (size_t)(uint32_t)uniform((int)(uint32_t)(v >> 32)) << 32;
 }
 
-// A workgroup has columns 16 NC slice .. of one head's state, NC tiles of them, and two kinds of waves, KD / 32 of each.  State wave w has
-// rows 32 w .. 32 w + 31 of the state, as two tiles, and TT of the chunk's four row tiles of R and U: what the next chunk
-// waits for.  Output wave w has Q S, P U and out of TT row tiles, and the first two (all where NC is 2) bring V into LDS.  Everything else is
-// read as operands, straight from the workspace.  VEC: 16 bytes of a row of v and out are one access.
+// A workgroup has columns 16 NC slice .. of one head's state, NC tiles of them, and two kinds of waves, KD / 32 of
+// each.  State wave w has rows 32 w .. 32 w + 31 of the state, as two tiles, and TT of the chunk's four row tiles of R
+// and U: what the next chunk waits for.  Output wave w has Q S, P U and out of TT row tiles, and the first two (all
+// where NC is 2) bring V into LDS.  Everything else is read as operands, straight from the workspace.  VEC: 16 bytes of
+// a row of v and out are one access.
 //
 // LDS, by the barrier (1 to 3 of a chunk) that its writes are ahead of and the one that its reads are ahead of:
 // s, back, ks: 1, 2;  v: 3 of the chunk before, 2;  v_top: 1, 2;  r, u_back: 2, 3;  u, w: 3, 1 of the next.  A buffer is
@@ -844,7 +847,8 @@ __device__ __forceinline__ void output_wave(const DeltaArgs &a, const ScanPlace 
             }
         }
     };
-    auto put_top = [&]() {  // the largest |V| of the wave's rows; infinities and NaN count as fp16's largest, for the other columns
+    // the largest |V| of the wave's rows; infinities and NaN count as fp16's largest, for the other columns
+    auto put_top = [&]() {
         if (kValues) {
             const float x = fminf(max_lanes(fmaxf((float)top[0], (float)top[1])), 65504.f);
             if (lane == 0) lds.v_top[wave] = x;
@@ -962,9 +966,11 @@ __global__ __launch_bounds__(4 * KD) void delta_scan_kernel(DeltaArgs a, const c
 }
 
 // Parts of 16 columns of all sequences and heads from which on a workgroup takes 32 of them: their operands are
-// loaded once and the longer chain is hidden by nothing, but the card is full either way.  16 heads of 128, sequences of 2048
-// rows, walk alone, 16 and 32 columns: 2 sequences (256 parts) 44 and 75 us, 4: 89 and 83, 6: 174 and 176, 8: 226 and 188,
-// 16: 430 and 367 us.
+// loaded once and the longer chain is hidden by nothing, but the card is full either way.  16 heads of 128, sequences of
+// 2048 rows, walk alone, 16 and 32 columns: 2 sequences (256 parts) 41 and 70 us, 4: 87 and 79, 6: 171 and 173, 8: 219 and
+// 182, 16: 423 and 354 us.  16 heads with keys of 64, where the wide kernel has one workgroup a CU and the narrow one two:
+// values of 128, 4 sequences (512 parts) 66 and 74 us, 6: 118 and 149, 8: 163 and 161, 16: 325 and 324; values of 64, 16
+// sequences (1024 parts) 196 and 174 us.
 constexpr size_t kWideParts = 1024;
 
 template <int KD, int NC>

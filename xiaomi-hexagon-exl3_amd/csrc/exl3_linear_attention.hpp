@@ -52,15 +52,16 @@ struct DeltaArgs {
 };
 hipError_t launch_delta_step(const DeltaArgs &a, hipStream_t stream);
 // Rows a sequence from which on the chunks take over, and from which on where the sequences, their heads and groups of 16
-// columns are kDeltaManyParts or more.  16 heads of 128 x 128, row by row and in chunks: one sequence of 12 rows 13.0 and
-// 14.9 us, of 16 rows 16.2 and 14.9 us; 16 sequences of 15 rows 24.5 and 35.7 us; 64 of 15 rows 74 and 108 us,
-// of 24 rows (3 us a row) 101 and 108 us.
+// columns are kDeltaManyParts or more.  16 heads of 128 x 128: one sequence of 12 rows row by row 11.6 us, of 15 rows
+// 13.4 us, of 16 to 24 rows in chunks 15.2 us; 16 sequences of 23 rows 31.4 us row by row, of 24 rows 35.5 us in chunks;
+// 64 of 23 rows 96 us, of 24 rows 106 us.
 constexpr size_t kDeltaPromptRows = 16, kDeltaPromptRowsOfMany = 24, kDeltaManyParts = 512;
 // Packed sequences' lengths are on the device, and a call of few rows a sequence can have a long one among them: from
 // kDeltaMixedRows a sequence on, those shorter than kDeltaShortRows go row by row beside the preparation of the others'
-// chunks, which takes about as long.  (Five sequences of up to 39 rows, 6 heads of 128 x 256: 18 us, and 23 us where short is
-// fewer than 16 rows.  31 single rows and a prompt of 60, 16 heads: 25 us, row by row more than 60; 64 sequences of three rows,
-// whose lengths the device alone knows: 39 and 30 us.)
+// chunks, which takes about as long.  (Five sequences of up to 39 rows, 6 heads of 128 x 256: 18 us, and 23 us where
+// short is fewer than 16 rows.  63 single rows and a prompt of 150, 16 heads: 45 us; with a prompt of 60, fewer than two
+// rows a sequence, row by row 60 us; 64 sequences of three rows, whose lengths the device alone knows: 39 us, row by row
+// 30 us.)
 constexpr size_t kDeltaMixedRows = 2, kDeltaShortRows = 8;
 // 0: such calls go row by row and take no workspace
 size_t delta_prompt_bytes(size_t heads, int key_dim, size_t sequences, size_t tokens);

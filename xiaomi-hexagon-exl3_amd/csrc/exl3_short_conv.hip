@@ -5,7 +5,7 @@
 // them are worked on.  The rows ahead of a sequence's first come from its state, and only the
 // threads of its first tile read that state: they also write the one that it leaves, so a slot may be both.
 // 8192 rows of 6144 fp16 channels, W = 4 with silu: 44.4 us, 4.5 TB/s (without the four rows ahead 46 us, with a
-// branch for silu at each element 47 us).  Eight rows of eight sequences: 4.2 us (weights not through LDS: 4.9 us).
+// branch for silu at each element 47 us).  A row each of eight sequences: 4.2 to 4.7 us (weights not through LDS: 4.9 us).
 #include "exl3_activation.hpp"
 #include "exl3_head_rows.hpp"
 #include "exl3_packed_rows.hpp"
@@ -171,9 +171,11 @@ __global__ __launch_bounds__(kConvThreads) void short_conv_kernel(ConvArgs a, in
 template <int W, int C, int XF16, int YF16>
 hipError_t launch_tiles(const ConvArgs &a, hipStream_t stream) {
     const unsigned channel_blocks = (a.channels + kConvThreads * C - 1) / (kConvThreads * C);
-    // Long tiles read their W - 1 rows ahead less often, short ones fill the card: 640 workgroups, 2.5 a CU (8192 rows of
-    // 6144 channels in tiles of 16, 32, 64: 47, 45, 48 us; 2048 rows in tiles of 4, 8, 16: 16.0, 14.0, 16.0 us; 1760
-    // rows of 1531 channels, one a thread, in tiles of 4, 8, 16, 32: 8.0, 6.9, 6.7, 7.2 us).
+    // Long tiles read their W - 1 rows ahead less often, short ones fill the card: 640 workgroups, 2.5 a CU.  fp16 in
+    // tiles of 4, 8, 16, 32, the rule's first: 8192 rows of 6144 channels 36.6 us (50.8, 42.8, 39.9, 36.4), 2000 rows
+    // 14.2 us (15.5, 14.0, 15.0, 15.4); of 1531 channels, one a thread, 1760 rows 5.6 us (6.6, 6.0, 5.6, 6.5), 3800
+    // rows 8.5 us (11.1, 9.4, 8.3, 8.5), 8000 rows 12.5 us (19.7, 15.9, 12.9, 12.5).  fp32: 3800 rows of 1531 9.8 us
+    // (11.9, 10.8, 9.9, 9.8); the rule loses most at 3800 rows of 1536, 12.5 us (12.6, 11.5, 10.8, 14.6).
     int per = 32;
     while (per > 4 && tile_count(a.s, per) * channel_blocks < 640) per /= 2;
     const size_t blocks = tile_count(a.s, per) * channel_blocks;

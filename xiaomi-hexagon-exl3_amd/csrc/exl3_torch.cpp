@@ -102,7 +102,7 @@ struct Call {
     }
 };
 
-// rows of heads [tokens, heads, head_dim], F16 or F32, a head's elements dense
+// rows of heads [tokens, heads, head_dim], F16 or F32, a head's elements dense (of no elements, any strides)
 exl3_head_view heads(const at::Tensor &t) {
     need(t.dim() == 3, "rows of heads are [tokens, heads, head_dim]");
     need(t.size(2) <= 1 || t.stride(2) == 1 || !t.numel(), "the elements of a head must be dense");
