@@ -524,7 +524,8 @@ size_t exl3_hip_attention_prompt_workspace_bytes(size_t q_heads, size_t head_dim
  *   h = x + residual                                   (residual NULL: h = x)
  *   out = h / sqrt(mean(h^2) + eps) * weight * silu(gate)   (weight NULL: 1; gate NULL: no factor)
  *   residual_out = h                                   (NULL: not kept; needs a residual)
- * with silu(z) = z / (1 + exp(-z)).  Computed in fp32 from h as summed, each output rounded once.
+ * with silu(z) = z / (1 + exp(-z)).  Computed in fp32 from h as summed, each output rounded once; the squares are fp32's
+ * too (|h| beyond 1.8e19 / sqrt(width) makes their sum infinite and the row 0).
  *   x, gate    xt rows; all views have x's heads, each head `width` elements, 1 .. 65536
  *   residual, residual_out   rt rows
  *   weight     device fp32[width] or NULL, shared by the heads

@@ -11,8 +11,8 @@
 //
 // Bound by the chain from chunk to chunk, three exchanges of about 900 cycles (read, products, write, barrier), in
 // which a SIMD has 1500 cycles of instructions of its two waves, and by the preparation's writes.  8192 rows, 16 heads
-// of 128: preparation 48 us (0.2 GB, 4.6 TB/s) and walk 158 us, 1.25 us a chunk; 2048 rows 17 and 40 us; 16 sequences
-// of 2048 rows 167 and 366 us.  Half the waves carry the state and half make the output, so that the chain has only
+// of 128: preparation 48 us (0.2 GB, 4.6 TB/s) and walk 159 us, 1.25 us a chunk; 2048 rows 17 and 40 us; 16 sequences
+// of 2048 rows 168 and 370 us.  Half the waves carry the state and half make the output, so that the chain has only
 // what the next chunk waits for (both on every wave: 400 us in all at 8192 rows).  Where operands lie as lanes want
 // them a load is 1 KB of consecutive bytes; 16 rows by 64 bytes a load is four times as slow.
 //
