@@ -42,3 +42,30 @@ def test_packed_sequences(amd, lens, chunks):
     d = inputs(53, sum(lens), 1, 2, 64, 32)
     assert goes_in_chunks(amd, d, lens, True) == chunks
     compare(amd, d, lens, draw(54, (len(lens), 2, 64, 32), 0.5), 1e-6, chunk=64 if chunks else None)
+
+
+@pytest.mark.parametrize("seqs,n", [(65536, 1), (65536, 2), (9000, 9)])
+def test_as_many_sequences_as_there_may_be(amd, seqs, n):
+    """packed ones, whose places every workgroup looks for, and the same without starts, bit for bit; states at their ends"""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(3)
+    draw = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    starts = torch.arange(seqs + 1, device="cuda", dtype=torch.int32) * n
+    slots = torch.randperm(seqs, generator=g, device="cuda").to(torch.int32)
+    x, w, old = draw(seqs * n, 8).half(), draw(8, 4), draw(seqs, 3, 8).half()
+    a, b = old.clone(), old.clone()
+    got = amd.short_conv(x, w, starts=starts, states=a, slots_in=slots, slots_out=slots)
+    want = amd.short_conv(x, w, sequences=seqs, states=b, slots_in=slots, slots_out=slots)
+    assert torch.equal(got, want) and torch.equal(a, b)
+    q, k, v = (draw(seqs * n, 1, d).half() for d in (64, 64, 16))
+    gates, old = draw(seqs * n, 2), draw(seqs, 1, 64, 16)
+    a, b = old.clone(), old.clone()
+    decay, beta = -gates[:, :1].abs(), gates[:, 1:].sigmoid()
+    got = amd.delta_rule(q, k, v, decay, beta, starts=starts, states=a, slots_in=slots, slots_out=slots, qk_eps=1e-6)
+    if n < 8:  # row by row both
+        want = amd.delta_rule(q, k, v, decay, beta, sequences=seqs, states=b, slots_in=slots, slots_out=slots, qk_eps=1e-6)
+    else:  # in chunks, a thousand sequences a call
+        want = torch.cat([amd.delta_rule(*(t[i * n:(i + 1000) * n] for t in (q, k, v, decay, beta)), starts=starts[:1001],
+                                         states=b, slots_in=slots[i:i + 1000], slots_out=slots[i:i + 1000], qk_eps=1e-6)
+                          for i in range(0, seqs, 1000)])
+    assert torch.equal(got, want) and torch.equal(a, b)
